@@ -344,6 +344,81 @@ int trs_pointwise_plan_access(int n_inputs, const void *const *inputs, const trs
                               const int *elem_bytes, const float *out, const trs_layout *lo, int cu_count, int roles,
                               int *vector, int *through_lds);
 
+/* ---- the attention block's operators (new; no counterpart in the reference) */
+
+/* Dropout with a mask that a counter gives and nothing stores.  Element i of x
+ * in row-major order is kept where word i % 4 of Philox4x32-10 (Salmon, Moraes,
+ * Dror, Shaw, SC'11) at counter offset + i/4 (mod 2^64; words 0 and 1 of the
+ * counter, low half first) and key `seed` (low half first) is at least
+ * floor(p * 2^32 + 1/2):
+ *     out[i] = kept ? x[i] * f32(1/(1-p)) : +0.0
+ * whatever a dropped element holds.  The mask depends on (seed, offset, p) and
+ * the shape, not on strides or launches; a call uses ceil(n/4) counters, so the
+ * next call's offset is that much further on.  The gradient is the same call
+ * on the upstream gradient.  p outside [0, 1] is TRS_E_INVALID_ARGUMENT; `out`
+ * may be x's own view (in place). */
+int trs_dropout_f32(const float *x, const trs_layout *lx, double p, uint64_t seed, uint64_t offset, float *out,
+                    const trs_layout *lo);
+
+/* The norm of every head's vector with the rotation by its position, of n = 1
+ * or 2 tensors (queries, and keys) [batch, head, token, dim] in one launch; they
+ * share batch, tokens and dim.  Per row x of dim entries:
+ *     y = R(position) (x * r * weight),  r = 1 / sqrt(mean(x^2) + eps)
+ * R turns the pairs (i, i + rot/2) of the first `rot` entries or, interleaved,
+ * (2i, 2i+1), by the angle whose cosine and sine stand in entry i of the tables'
+ * row `position`: (u, w) -> (u cos - w sin, w cos + u sin).  The tables are
+ * [rows, rot/2] with the layout ltab and a unit stride along a row; rot <= dim,
+ * and entries from rot on are not rotated.  The position of token t is
+ * positions[batch][token] (int32 on the device, contiguous), or start + t where
+ * positions is null; start + t has to lie in the tables
+ * (TRS_E_INVALID_ARGUMENT), and a row whose own position does not is NaN.
+ * weight: n pointers to dim floats each, any of them (or the array) null for
+ * ones.  dim is at most 1024.  Inputs may have any strides; outputs share no
+ * memory with inputs. */
+int trs_head_norm_rope_f32(int n, const float *const *x, const trs_layout *lx, const float *const *weight, float eps,
+                           const float *cos, const float *sin, const trs_layout *ltab, int interleaved,
+                           const int32_t *positions, int64_t start, float *const *out, const trs_layout *lo);
+/* Its gradients: dx (n tensors, layouts ldx) and dweight (n pointers to dim
+ * floats, any of them or the array null: not wanted).  The rows' shares of
+ * dweight are added in a fixed order, in a workspace from the block cache of at
+ * most 4 * dim floats per CU and tensor. */
+int trs_head_norm_rope_backward_f32(int n, const float *const *x, const trs_layout *lx, const float *const *weight,
+                                    float eps, const float *cos, const float *sin, const trs_layout *ltab,
+                                    int interleaved, const int32_t *positions, int64_t start, const float *const *up,
+                                    const trs_layout *lup, float *const *dx, const trs_layout *ldx,
+                                    float *const *dweight);
+
+/* Causal attention with a sliding window and first tokens that stay visible.
+ * q [batch, heads, Sq, dim], k and v [batch, key heads, Sk, dim], dim at most
+ * 256; head h reads key head h / (heads / key heads).  A sequence has n keys,
+ * lengths[batch] (int32 on the device, taken into [0, Sk]) or Sk where lengths
+ * is null; query i stands at place p = n - Sq + i, so that the last query is the
+ * last key's, and sees key j where
+ *     j <= p  and  (p - j < window  or  j < sinks).
+ *     out = sum over the keys it sees of softmax(scale q k) v
+ * A query that sees nothing (p < 0) gives 0.  Keys and values that no query
+ * sees are not read, and what stands in one that a query does not see, NaN
+ * included, does not reach that query.  window >= 1 (INT64_MAX: no window);
+ * sinks >= 0.  lse (or null) receives log(sum(exp(scale q k))) as
+ * [batch, heads, Sq], -inf where nothing is seen.  Products and sums are fp32
+ * throughout; the order of the sums is fixed.  Inputs may have any strides (one
+ * with no unit stride along dim is copied first, into the block cache); outputs
+ * need a unit stride along dim and share no memory with inputs.  Few rows over
+ * many keys are split over the keys, into a workspace from the block cache. */
+int trs_window_attention_f32(const float *q, const trs_layout *lq, const float *k, const trs_layout *lk,
+                             const float *v, const trs_layout *lv, const int32_t *lengths, int64_t window,
+                             int64_t sinks, float scale, float *out, const trs_layout *lo, float *lse);
+/* Its gradients, from the forward call's arguments, out and lse, and the
+ * upstream gradient of out; those of a shared key head are summed over its query
+ * heads, and keys that no query sees get 0.  No atomic adds: the result is the
+ * same bits each time.  Takes a workspace from the block cache. */
+int trs_window_attention_backward_f32(const float *q, const trs_layout *lq, const float *k, const trs_layout *lk,
+                                      const float *v, const trs_layout *lv, const int32_t *lengths, int64_t window,
+                                      int64_t sinks, float scale, const float *out, const trs_layout *lo,
+                                      const float *lse, const float *up, const trs_layout *lup, float *dq,
+                                      const trs_layout *ldq, float *dk, const trs_layout *ldk, float *dv,
+                                      const trs_layout *ldv);
+
 /* ---- pointwise fusion compiler (new; no counterpart in the reference) */
 
 /* Compile a pointwise IR program to a gfx950 kernel with hipRTC (-O3,

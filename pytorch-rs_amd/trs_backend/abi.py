@@ -95,6 +95,7 @@ class PwPlanInfo(ctypes.Structure):
 
 _LP = POINTER(Layout)
 _FP = POINTER(c_float)
+_PP = POINTER(c_void_p)
 
 _SIGNATURES = {
     "trs_init": ([], c_int),
@@ -133,6 +134,16 @@ _SIGNATURES = {
     "trs_matmul_f32": ([c_void_p, _LP, c_void_p, _LP, c_void_p, _LP], c_int),
     "trs_matmul_plan_f32": ([c_void_p, _LP, c_void_p, _LP, c_void_p, _LP, POINTER(c_int), POINTER(c_int),
                              POINTER(c_int), POINTER(ctypes.c_int64), POINTER(ctypes.c_int64)], c_int),
+    "trs_dropout_f32": ([c_void_p, _LP, c_double, c_uint64, c_uint64, c_void_p, _LP], c_int),
+    "trs_head_norm_rope_f32": ([c_int, _PP, _LP, _PP, c_float, c_void_p, c_void_p, _LP, c_int, c_void_p, c_int64, _PP, _LP],
+                               c_int),
+    "trs_head_norm_rope_backward_f32": ([c_int, _PP, _LP, _PP, c_float, c_void_p, c_void_p, _LP, c_int, c_void_p, c_int64,
+                                         _PP, _LP, _PP, _LP, _PP], c_int),
+    "trs_window_attention_f32": ([c_void_p, _LP, c_void_p, _LP, c_void_p, _LP, c_void_p, c_int64, c_int64, c_float,
+                                  c_void_p, _LP, c_void_p], c_int),
+    "trs_window_attention_backward_f32": ([c_void_p, _LP, c_void_p, _LP, c_void_p, _LP, c_void_p, c_int64, c_int64, c_float,
+                                           c_void_p, _LP, c_void_p, c_void_p, _LP, c_void_p, _LP, c_void_p, _LP,
+                                           c_void_p, _LP], c_int),
     "trs_pointwise_plan": ([c_int, POINTER(c_void_p), POINTER(_LP), POINTER(c_int), c_void_p, _LP, c_int, c_int,
                             POINTER(PwPlanInfo)], c_int),
     "trs_pointwise_plan_access": ([c_int, POINTER(c_void_p), POINTER(_LP), POINTER(c_int), c_void_p, _LP, c_int, c_int,
