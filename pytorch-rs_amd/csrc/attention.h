@@ -206,6 +206,8 @@ struct Notices {
     uint32_t word[2][4];
 };
 
+// Few rows a key head (attention_few.hip): row_tiles of 16 rows, `splits` parts.
+int launch_attention_few(const AttnArgs &a, hipStream_t s);
 int attention_forward(AttnArgs a, hipStream_t s, int cu_count);
 int attention_backward(AttnArgs a, hipStream_t s, int cu_count);
 

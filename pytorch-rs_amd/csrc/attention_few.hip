@@ -1,0 +1,234 @@
+// attention_few.hip -- attention.h's attention for few rows a key head: single
+// tokens over a cache.
+//
+// Bound by reading the keys and values once.  A wave takes 16 rows (the query
+// heads that share the key head, and the few tokens) and streams its share of
+// the keys 16 at a time, straight from memory into the registers that
+// v_mfma_f32_16x16x4_f32 takes them from: no LDS, no barrier, nothing that waits
+// for another wave.  Lane l holds of an operand row (column) l % 16 at k = l / 16,
+// of a result column l % 16, register i row 4 (l/16) + i.
+//   S^T = K Q^T: k runs over the dims 16 j + 4 (l/16) + e, so that a lane's four
+//     steps are 16 bytes of its key.
+//   O^T += V^T P^T: k runs over the keys 4 (l/16) + i, where the lane has P as a
+//     result; a lane reads W consecutive dims of its key at once, which go to W
+//     result tiles: tile u W + w holds in its row rho dim 16 W u + W rho + w.
+// The waves of a block join their maxima and sums in LDS, blocks in a second
+// pass.
+#include <hip/hip_runtime.h>
+
+#include "attention.h"
+
+namespace trs {
+
+namespace {
+
+typedef float at_f2 __attribute__((ext_vector_type(2)));
+
+// N floats of a row from column c on; columns from D on are 0.  MODE 0: D is the
+// padded width; 1: D is a multiple of 4; 2: any D.  No branch around a load:
+// what lies past the row's end is read at its start.
+template <int N, int MODE>
+__device__ __forceinline__ void take(float *v, const float *row, int c, int D) {
+    typedef float Vec __attribute__((ext_vector_type(N), aligned(4)));
+    if constexpr (MODE == 2) {
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            const float x = row[c + e < D ? c + e : 0];
+            v[e] = c + e < D ? x : 0.f;
+        }
+    } else {
+        const bool in = MODE == 0 || c < D;
+        const Vec x = *(const Vec *)(row + (in ? c : 0));
+#pragma unroll
+        for (int e = 0; e < N; e++) v[e] = in ? x[e] : 0.f;
+    }
+}
+
+// DP: the width, a multiple of 32.  NW waves a block.
+template <int DP, int NW, int MODE>
+__global__ void __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) attn_few(AttnArgs a) {
+    constexpr int KJ = DP / 16, W = DP % 64 == 0 ? 4 : 2, VU = DP / (16 * W), TO = DP / 16;
+    __shared__ float out_o[NW][16][DP + 4];
+    __shared__ float out_ml[NW][16][2];
+    const int lane = (int)threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    uint32_t id = blockIdx.x;
+    const int part = (int)(id % (uint32_t)a.splits);
+    id /= (uint32_t)a.splits;
+    const int tile = (int)(id % (uint32_t)a.row_tiles);
+    id /= (uint32_t)a.row_tiles;
+    const int hk = (int)(id % (uint32_t)a.kv_heads), b = (int)(id / (uint32_t)a.kv_heads);
+
+    const Sequence seq = sequence_of(a, b);
+    const int r0 = tile * 16, r1 = min(r0 + 16, a.rows), row = min(r0 + col, a.rows - 1);
+    const int i = (int)a.by_group.divide((uint32_t)row), g = row - i * a.group;
+    const int place = r0 + col < a.rows ? seq.first + i : -1;
+    const int lo = seq.first + (int)a.by_group.divide((uint32_t)r0), hi = seq.first + (int)a.by_group.divide((uint32_t)(r1 - 1));
+    const int key_lo = max(0, lo - a.window + 1), key_hi = hi;
+    const int sinks = min(a.sinks, key_hi + 1);
+    const int first = key_lo >> 4;
+    const int nsink = key_hi < 0 ? 0 : min((sinks + 15) >> 4, first);
+    const int tiles = key_hi < 0 ? 0 : nsink + (key_hi >> 4) - first + 1;
+    const int waves = a.splits * NW, mine = part * NW + wave;
+    const int t0 = (int)((int64_t)tiles * mine / waves), t1 = (int)((int64_t)tiles * (mine + 1) / waves);
+    const auto first_key = [&](int t) { return (t < nsink ? t : first + t - nsink) << 4; };
+    // A key that no row of the block sees is not read: the last one that is seen stands for it.
+    const auto read_key = [&](int j) { return j <= key_hi && (j >= key_lo || j < sinks) ? j : key_hi; };
+
+    const float *kb = a.k + b * a.ks.b + hk * a.ks.h, *vb = a.v + b * a.vs.b + hk * a.vs.h;
+    const float *qrow = a.q + b * a.qs.b + (int64_t)(hk * a.group + g) * a.qs.h + (int64_t)i * a.qs.s;
+    float q[KJ][4], k[KJ][4], v[4][VU][W];
+    const auto load_k = [&](int t) {
+        const float *p = kb + (int64_t)read_key(first_key(t) + col) * a.ks.s;
+#pragma unroll
+        for (int j = 0; j < KJ; j++) take<4, MODE>(k[j], p, 16 * j + 4 * quarter, a.D);
+    };
+    const auto load_v = [&](int t) {
+        const int j0 = first_key(t) + 4 * quarter;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float *p = vb + (int64_t)read_key(j0 + e) * a.vs.s;
+#pragma unroll
+            for (int u = 0; u < VU; u++) take<W, MODE>(v[e][u], p, 16 * W * u + W * col, a.D);
+        }
+    };
+    at_f4 acc[TO];
+#pragma unroll
+    for (int t = 0; t < TO; t++) acc[t] = (at_f4)(0.f);
+    float most = -__builtin_inff(), sum = 0.f;
+    if (t0 < t1) {
+        load_k(t0);
+        load_v(t0);
+#pragma unroll
+        for (int j = 0; j < KJ; j++) {
+            take<4, MODE>(q[j], qrow, 16 * j + 4 * quarter, a.D);
+#pragma unroll
+            for (int e = 0; e < 4; e++) q[j][e] *= a.scale2;
+        }
+    }
+    for (int t = t0; t < t1; t++) {
+        const int j0 = first_key(t), next = t + 1 < t1 ? t + 1 : t;  // the last tile's loads repeat it
+        at_f4 s = (at_f4)(0.f);
+#pragma unroll
+        for (int j = 0; j < KJ; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[j][e], q[j][e], s, 0, 0, 0);
+        load_k(next);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (!sees(a, place, j0 + 4 * quarter + e)) s[e] = -__builtin_inff();
+        float m = __builtin_fmaxf(__builtin_fmaxf(s[0], s[1]), __builtin_fmaxf(s[2], s[3]));
+        m = __builtin_fmaxf(m, __shfl_xor(m, 16));
+        m = __builtin_fmaxf(m, __shfl_xor(m, 32));
+        const float now = __builtin_fmaxf(most, m), base = now == -__builtin_inff() ? 0.f : now;
+        const float keep = __builtin_amdgcn_exp2f(most - base);
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[e] = __builtin_amdgcn_exp2f(s[e] - base);
+        sum = sum * keep + ((s[0] + s[1]) + (s[2] + s[3]));
+        most = now;
+        if (__builtin_amdgcn_ballot_w64(keep != 1.f)) {
+#pragma unroll
+            for (int c = 0; c < TO; c++) acc[c] *= keep;
+        }
+        float bad = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int u = 0; u < VU; u++)
+#pragma unroll
+                for (int w = 0; w < W; w++) bad += v[e][u][w] * 0.f;
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(bad != 0.f) == 0, 1)) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int u = 0; u < VU; u++)
+#pragma unroll
+                    for (int w = 0; w < W; w++)
+                        acc[u * W + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[e][u][w], s[e], acc[u * W + w], 0, 0, 0);
+        } else {
+            // Infinities or NaN: a pair that does not see each other adds nothing.
+#pragma unroll 1
+            for (int n = 0; n < 16; n++) {
+                float p = 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; e++) p = (n & 3) == e ? s[e] : p;
+                p = __shfl(p, col + 16 * (n >> 2));
+                if (!sees(a, place, j0 + n)) continue;
+                const float *x = vb + (int64_t)(j0 + n) * a.vs.s;
+#pragma unroll
+                for (int c = 0; c < TO; c++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int d = 16 * W * (c / W) + W * (4 * quarter + e) + c % W;
+                        if (d < a.D) acc[c][e] += p * x[d];
+                    }
+            }
+        }
+        load_v(next);
+    }
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+#pragma unroll
+    for (int c = 0; c < TO; c++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) out_o[wave][col][16 * W * (c / W) + W * (4 * quarter + e) + c % W] = acc[c][e];
+    if (quarter == 0) out_ml[wave][col][0] = most, out_ml[wave][col][1] = sum;
+    __syncthreads();
+    // The waves' shares of row r, and the row's place in the output.
+    for (int x = (int)threadIdx.x; x < 16 * (DP / 4); x += 64 * NW) {
+        const int r = x / (DP / 4), d = x % (DP / 4) * 4, at_row = r0 + r;
+        if (at_row >= a.rows || d >= a.D) continue;
+        float top = -__builtin_inff(), total = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) top = __builtin_fmaxf(top, out_ml[w][r][0]);
+        const float base = top == -__builtin_inff() ? 0.f : top;
+        at_f4 o = (at_f4)(0.f);
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const float f = __builtin_amdgcn_exp2f(out_ml[w][r][0] - base);
+            total += out_ml[w][r][1] * f;
+            o += *(const at_f4 *)&out_o[w][r][d] * f;
+        }
+        const int at_i = (int)a.by_group.divide((uint32_t)at_row);
+        const int64_t h = (int64_t)hk * a.group + at_row - at_i * a.group;
+        const int64_t head = (int64_t)b * a.kv_heads + hk;
+        float *p;
+        if (a.splits > 1) {
+            const int64_t at = ((int64_t)part * a.batch * a.kv_heads + head) * a.rows + at_row;
+            p = a.part_o + at * a.D + d;
+            if (d == 0) a.part_ml[2 * at] = top, a.part_ml[2 * at + 1] = total;
+        } else {
+            o *= total == 0.f ? 0.f : 1.f / total;
+            p = a.out + b * a.os.b + h * a.os.h + (int64_t)at_i * a.os.s + d;
+            if (a.lse && d == 0) a.lse[((int64_t)b * a.heads + h) * a.Sq + at_i] = (top + __builtin_amdgcn_logf(total)) * kLn2;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (d + e < a.D) p[e] = o[e];
+    }
+}
+
+template <int DP, int NW>
+void launch(const AttnArgs &a, dim3 grid, hipStream_t s) {
+    if (a.D == DP) hipLaunchKernelGGL((attn_few<DP, NW, 0>), grid, dim3(64 * NW), 0, s, a);
+    else if (a.D % 4 == 0) hipLaunchKernelGGL((attn_few<DP, NW, 1>), grid, dim3(64 * NW), 0, s, a);
+    else hipLaunchKernelGGL((attn_few<DP, NW, 2>), grid, dim3(64 * NW), 0, s, a);
+}
+
+}  // namespace
+
+int launch_attention_few(const AttnArgs &a, hipStream_t s) {
+    const int64_t blocks = (int64_t)a.batch * a.kv_heads * a.row_tiles * a.splits;
+    if (blocks >> 31) return set_error(TRS_E_INVALID_ARGUMENT, "attention over %lld blocks of rows", (long long)blocks);
+    const dim3 grid((unsigned)blocks);
+    if (a.D <= 32) launch<32, 4>(a, grid, s);
+    else if (a.D <= 64) launch<64, 4>(a, grid, s);
+    else if (a.D <= 96) launch<96, 4>(a, grid, s);
+    else if (a.D <= 128) launch<128, 4>(a, grid, s);
+    else if (a.D <= 192) launch<192, 4>(a, grid, s);
+    else launch<256, 4>(a, grid, s);
+    TRS_LAUNCH_CHECK("attention launch");
+    return TRS_OK;
+}
+
+}  // namespace trs

@@ -7,6 +7,9 @@ namespace trs {
 
 namespace {
 
+constexpr int kFewRows = 32;   // rows a key head that attn_few takes
+constexpr int kPartTiles = 2;  // the least key tiles of a part, a wave
+
 // 128 rows of one key head, 32 a wave, over key tiles that the block stages in
 // LDS, two buffers in turn.  S^T = K Q^T puts a row of the softmax in a lane
 // (and its other half): the running maximum and sum are per lane, and P^T is
@@ -160,19 +163,40 @@ __global__ void __launch_bounds__(256) attn_join(AttnArgs a) {
 }  // namespace
 
 int attention_forward(AttnArgs a, hipStream_t s, int cu_count) {
-    (void)cu_count;
-    a.row_tiles = (a.rows + kRowsBlock - 1) / kRowsBlock;
-    a.splits = 1;
-    const int64_t blocks = (int64_t)a.batch * a.kv_heads * a.row_tiles * a.splits;
-    if (blocks >> 31) return set_error(TRS_E_INVALID_ARGUMENT, "attention over %lld blocks of rows", (long long)blocks);
-    const dim3 grid((unsigned)blocks);
-    if (a.D <= 32) hipLaunchKernelGGL(attn_rows<1>, grid, dim3(256), 0, s, a);
-    else if (a.D <= 64) hipLaunchKernelGGL(attn_rows<2>, grid, dim3(256), 0, s, a);
-    else if (a.D <= 96) hipLaunchKernelGGL(attn_rows<3>, grid, dim3(256), 0, s, a);
-    else if (a.D <= 128) hipLaunchKernelGGL(attn_rows<4>, grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL(attn_rows<8>, grid, dim3(256), 0, s, a);
-    TRS_LAUNCH_CHECK("attention launch");
-    return TRS_OK;
+    const int64_t heads = (int64_t)a.batch * a.kv_heads;
+    const bool few = a.rows <= kFewRows;
+    const int rows_block = few ? 16 : kRowsBlock, tile = few ? 16 : kTile, waves = few ? 4 : 1;
+    a.row_tiles = (a.rows + rows_block - 1) / rows_block;
+    // The keys in parts where the rows' blocks are fewer than the device takes.
+    const int64_t blocks = heads * a.row_tiles, keys = std::min<int64_t>(a.Sk, (int64_t)a.window + a.sinks + rows_block / std::max(a.group, 1));
+    const int64_t most = std::max<int64_t>(1, keys / tile / waves / kPartTiles);
+    a.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({most, (4 * (int64_t)cu_count + blocks - 1) / blocks, 64}));
+    if ((blocks * a.splits) >> 31) return set_error(TRS_E_INVALID_ARGUMENT, "attention over %lld blocks of rows", (long long)blocks);
+    void *ws = nullptr;
+    if (a.splits > 1) {
+        const int64_t parts = a.splits * heads * a.rows;
+        const int rc = trs_alloc((size_t)(parts * (a.D + 2)) * sizeof(float), &ws);
+        if (rc == TRS_E_ALLOCATION_FAILED) a.splits = 1;  // the parts are for speed alone
+        else if (rc) return rc;
+        a.part_ml = (float *)ws, a.part_o = a.part_ml + 2 * parts;
+    }
+    const auto launch = [&]() -> int {
+        const dim3 grid((unsigned)(blocks * a.splits));
+        if (few) TRS_CHECK(launch_attention_few(a, s));
+        else if (a.D <= 32) hipLaunchKernelGGL(attn_rows<1>, grid, dim3(256), 0, s, a);
+        else if (a.D <= 64) hipLaunchKernelGGL(attn_rows<2>, grid, dim3(256), 0, s, a);
+        else if (a.D <= 96) hipLaunchKernelGGL(attn_rows<3>, grid, dim3(256), 0, s, a);
+        else if (a.D <= 128) hipLaunchKernelGGL(attn_rows<4>, grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL(attn_rows<8>, grid, dim3(256), 0, s, a);
+        TRS_LAUNCH_CHECK("attention launch");
+        if (a.splits > 1) {
+            hipLaunchKernelGGL(attn_join, dim3((unsigned)((heads * a.rows + 3) / 4)), dim3(256), 0, s, a);
+            TRS_LAUNCH_CHECK("attention join launch");
+        }
+        return TRS_OK;
+    };
+    const int rc = launch(), frc = ws ? trs_free(ws) : TRS_OK;
+    return rc ? rc : frc;
 }
 
 }  // namespace trs
