@@ -431,6 +431,9 @@ const char *node_name(Node n) {
     case Node::SqueezeDimensions: return "SqueezeBackward2";
     case Node::Unsqueeze: return "UnsqueezeBackward0";
     case Node::Fused: return "FusedBackward0";
+    case Node::Dropout: return "DropoutBackward0";
+    case Node::HeadNormRope: return "HeadNormRopeBackward0";
+    case Node::WindowAttention: return "WindowAttentionBackward0";
     }
     return "UnknownBackward";
 }
@@ -1168,6 +1171,124 @@ Tensor mask_apply(const Tensor &h, const BytePtr &maskp, float scale) {
     return out;
 }
 
+Tensor dropout_counter(const Tensor &x, const DropoutSpec &spec) {
+    x.require_cuda("dropout");
+    Tensor out = empty_like_layout(x.device(), x.shape, layout::unary_output_strides(x.shape, x.strides, x.numel));
+    const trs_layout lx = x.abi_layout(), lo = out.abi_layout();
+    check(trs_dropout_f32(x.storage->dptr, &lx, spec.p, spec.seed, spec.offset, out.storage->dptr, &lo));
+    if (records(x)) {
+        auto fn = std::make_unique<GradFn>();
+        fn->kind = GradKind::Dropout;
+        fn->node = Node::Dropout;
+        fn->dropout = spec;
+        fn->inputs.push_back(save(x, false));
+        attach(out, std::move(fn));
+    }
+    return out;
+}
+
+static void require_same_device(const Tensor &a, const Tensor &b) {
+    if (!(a.device() == b.device()))
+        throw TensorError("Expected all tensors to be on the same device, but found at least two devices, " +
+                          a.device().str() + " and " + b.device().str() + "!");
+}
+
+// An output of x's shape in the order of x's memory where that leaves the last dim
+// a unit stride, else contiguous.
+static Tensor empty_rows_like(const Tensor &x) {
+    Dims st = layout::unary_output_strides(x.shape, x.strides, x.numel);
+    if (!st.empty() && st.back() != 1) st = layout::contiguous_strides(x.shape);
+    return empty_like_layout(x.device(), x.shape, st);
+}
+
+std::vector<Tensor> head_norm_rope(const std::vector<Tensor> &xs, const std::vector<Tensor> &weights, const Tensor &cos,
+                                   const Tensor &sin, RotationSpec spec) {
+    if (xs.empty() || xs.size() > 2 || weights.size() != xs.size()) throw TensorError("head_norm_rope takes one or two tensors");
+    std::vector<Tensor> w;
+    std::vector<const float *> px, pw;
+    std::vector<float *> po;
+    std::vector<trs_layout> lx, lo;
+    std::vector<Tensor> outs;
+    for (size_t i = 0; i < xs.size(); i++) {
+        const Tensor &x = xs[i];
+        x.require_cuda("head_norm_rope");
+        require_same_device(xs[0], x);
+        if (x.shape.size() != 4)
+            throw TensorError("head_norm_rope takes tensors of 4 dims (batch, head, token, dim), got " + dims_str(x.shape));
+        if (!weights[i].shape.empty()) {
+            require_same_device(x, weights[i]);
+            if (weights[i].shape != Dims{x.shape[3]})
+                throw TensorError("head_norm_rope weight has shape " + dims_str(weights[i].shape) + ", expected " +
+                                  dims_str(Dims{x.shape[3]}));
+            w.push_back(weights[i].contiguous());
+        } else {
+            w.push_back(Tensor{});
+        }
+        outs.push_back(empty_rows_like(x));
+        px.push_back(x.storage->dptr);
+        pw.push_back(w[i].storage ? w[i].storage->dptr + w[i].offset : nullptr);
+        po.push_back(outs[i].storage->dptr);
+        lx.push_back(x.abi_layout());
+        lo.push_back(outs[i].abi_layout());
+    }
+    require_same_device(xs[0], cos);
+    require_same_device(xs[0], sin);
+    if (cos.shape.size() != 2 || cos.shape != sin.shape)
+        throw TensorError("head_norm_rope tables have shapes " + dims_str(cos.shape) + " and " + dims_str(sin.shape) +
+                          ", expected two of (positions, pairs)");
+    if (cos.requires_grad() || sin.requires_grad()) throw TensorError("head_norm_rope records no gradient of its tables");
+    const Tensor c = cos.contiguous(), s = sin.contiguous();
+    const IndexPtr &pos = spec.positions;
+    if (pos && (!(pos->device == xs[0].device()) || pos->shape != Dims{xs[0].shape[0], xs[0].shape[2]}))
+        throw TensorError("head_norm_rope positions have shape " + dims_str(pos->shape) + ", expected (batch, tokens) on the tensors' device");
+    // The contiguous tables start at their own offset.
+    const trs_layout lt = abi_layout_of(c.shape, layout::contiguous_strides(c.shape), 0);
+    check(trs_head_norm_rope_f32((int)xs.size(), px.data(), lx.data(), pw.data(), spec.eps, c.storage->dptr + c.offset,
+                                 s.storage->dptr + s.offset, &lt, spec.interleaved, pos ? pos->dptr : nullptr, spec.start,
+                                 po.data(), lo.data()));
+    for (size_t i = 0; i < xs.size(); i++) {
+        if (!is_grad_enabled() || !(xs[i].requires_grad() || w[i].requires_grad())) continue;
+        auto fn = std::make_unique<GradFn>();
+        fn->kind = GradKind::HeadNormRope;
+        fn->node = Node::HeadNormRope;
+        fn->rotation = spec;
+        fn->rotation.tables = {save(c, true), save(s, true)};
+        fn->inputs.push_back(save(xs[i], true));
+        fn->inputs.push_back(w[i].storage ? save(w[i], true) : SavedTensor{});
+        attach(outs[i], std::move(fn));
+    }
+    return outs;
+}
+
+Tensor window_attention(const Tensor &q, const Tensor &k, const Tensor &v, AttentionSpec spec) {
+    for (const Tensor *t : {&q, &k, &v}) {
+        t->require_cuda("window_attention");
+        require_same_device(q, *t);
+        if (t->shape.size() != 4)
+            throw TensorError("window_attention takes tensors of 4 dims (batch, head, token, dim), got " + dims_str(t->shape));
+    }
+    const IndexPtr &len = spec.lengths;
+    if (len && (!(len->device == q.device()) || len->shape != Dims{q.shape[0]}))
+        throw TensorError("window_attention key lengths have shape " + dims_str(len->shape) + ", expected (batch) on the tensors' device");
+    const bool grad = is_grad_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
+    Tensor out = empty_rows_like(q);
+    if (grad) spec.lse = Storage::allocate(q.device(), q.shape[0] * q.shape[1] * q.shape[2]);
+    const trs_layout lq = q.abi_layout(), lk = k.abi_layout(), lv = v.abi_layout(), lo = out.abi_layout();
+    check(trs_window_attention_f32(q.storage->dptr, &lq, k.storage->dptr, &lk, v.storage->dptr, &lv, len ? len->dptr : nullptr,
+                                   spec.window, spec.sinks, spec.scale, out.storage->dptr, &lo, grad ? spec.lse->dptr : nullptr));
+    if (grad) {
+        auto fn = std::make_unique<GradFn>();
+        fn->kind = GradKind::WindowAttention;
+        fn->node = Node::WindowAttention;
+        fn->attention = std::move(spec);
+        for (const Tensor *t : {&q, &k, &v}) fn->inputs.push_back(save(*t, true));
+        fn->output = save(out, true);
+        fn->output.autograd.reset();
+        attach(out, std::move(fn));
+    }
+    return out;
+}
+
 float Tensor::item() const {
     if (numel != 1)
         throw TensorError("a Tensor with " + std::to_string(numel) + " elements cannot be converted to Scalar");
@@ -1235,6 +1356,12 @@ void validate(const GradFn &fn) {
     case GradKind::MaskApply:
         if (!fn.mask) throw TensorError(kGraphFreed);
         break;
+    case GradKind::HeadNormRope:
+        if (!fn.inputs[0].values) throw TensorError(kGraphFreed);
+        break;
+    case GradKind::WindowAttention:
+        if (!fn.attention.lse) throw TensorError(kGraphFreed);
+        break;
     case GradKind::Fused:
         for (int a : fn.fused.args) {
             if (a < 0) continue;
@@ -1260,6 +1387,17 @@ void consume(GradFn &fn) {
     case GradKind::Relu: fn.inputs[0].values.reset(); break;
     case GradKind::Exp: fn.output.values.reset(); break;
     case GradKind::MaskApply: fn.mask.reset(); break;
+    case GradKind::HeadNormRope:
+        for (auto &in : fn.inputs) in.values.reset();
+        fn.rotation.tables.clear();
+        fn.rotation.positions.reset();
+        break;
+    case GradKind::WindowAttention:
+        for (auto &in : fn.inputs) in.values.reset();
+        fn.output.values.reset();
+        fn.attention.lse.reset();
+        fn.attention.lengths.reset();
+        break;
     case GradKind::Fused:
         for (auto &in : fn.inputs) in.values.reset();
         for (auto &b : fn.fused_bytes) b.reset();
@@ -1371,6 +1509,49 @@ void apply_grad_fn(const GradFn &fn, Grad up, Device dev, std::map<GradKey, Grad
         const trs_layout lg = abi_layout_of(in.shape, layout::contiguous_strides(in.shape), 0);
         if (in.numel) check(trs_mask_backward_f32(up.st->dptr, &lg, fn.mask->dptr, &lg, fn.scalar, g.st->dptr, &lg));
         add_gradient(grads, in.autograd, in.output_nr, std::move(g));
+        return;
+    }
+    case GradKind::Dropout: {  // the same mask on the upstream
+        const SavedTensor &in = fn.inputs[0];
+        if (!in.autograd) return;
+        Grad g = new_grad(dev, in.shape);
+        check(trs_dropout_f32(up.st->dptr, &lup, fn.dropout.p, fn.dropout.seed, fn.dropout.offset, g.st->dptr, &lup));
+        add_gradient(grads, in.autograd, in.output_nr, std::move(g));
+        return;
+    }
+    case GradKind::HeadNormRope: {
+        const SavedTensor &in = fn.inputs[0], &w = fn.inputs[1];
+        const RotationSpec &r = fn.rotation;
+        Grad dx = new_grad(dev, in.shape), dw;
+        if (w.autograd) dw = new_grad(dev, w.shape);
+        const trs_layout lx = saved_layout(in), lt = abi_layout_of(r.tables[0].shape, layout::contiguous_strides(r.tables[0].shape), 0);
+        const float *px = in.values->dptr, *pw = w.values ? w.values->dptr + w.offset : nullptr, *pu = up.st->dptr;
+        float *pdx = dx.st->dptr, *pdw = w.autograd ? dw.st->dptr : nullptr;
+        check(trs_head_norm_rope_backward_f32(1, &px, &lx, &pw, r.eps, r.tables[0].values->dptr + r.tables[0].offset,
+                                              r.tables[1].values->dptr + r.tables[1].offset, &lt, r.interleaved,
+                                              r.positions ? r.positions->dptr : nullptr, r.start, &pu, &lup, &pdx, &lup, &pdw));
+        if (in.autograd) add_gradient(grads, in.autograd, in.output_nr, std::move(dx));
+        if (w.autograd) add_gradient(grads, w.autograd, w.output_nr, std::move(dw));
+        return;
+    }
+    case GradKind::WindowAttention: {
+        const SavedTensor &q = fn.inputs[0], &k = fn.inputs[1], &v = fn.inputs[2];
+        const AttentionSpec &a = fn.attention;
+        Grad g[3];
+        trs_layout lin[3], lg[3];
+        for (int i = 0; i < 3; i++) {
+            const SavedTensor &in = fn.inputs[i];
+            g[i] = new_grad(dev, in.shape);
+            lin[i] = saved_layout(in);
+            lg[i] = abi_layout_of(in.shape, layout::contiguous_strides(in.shape), 0);
+        }
+        const trs_layout lo = saved_layout(fn.output);
+        check(trs_window_attention_backward_f32(q.values->dptr, &lin[0], k.values->dptr, &lin[1], v.values->dptr, &lin[2],
+                                                a.lengths ? a.lengths->dptr : nullptr, a.window, a.sinks, a.scale,
+                                                fn.output.values->dptr, &lo, a.lse->dptr, up.st->dptr, &lup, g[0].st->dptr, &lg[0],
+                                                g[1].st->dptr, &lg[1], g[2].st->dptr, &lg[2]));
+        for (int i = 0; i < 3; i++)
+            if (fn.inputs[i].autograd) add_gradient(grads, fn.inputs[i].autograd, fn.inputs[i].output_nr, std::move(g[i]));
         return;
     }
     case GradKind::Multiply: {  // src/tensor.rs:3031-3097
@@ -1610,6 +1791,30 @@ std::shared_ptr<ByteBuffer> ByteBuffer::from_host(const uint8_t *data, const Dim
         if (rc != TRS_OK) throw TensorError("failed to allocate storage for " + std::to_string(b->numel) + " elements");
         b->dptr = (uint8_t *)p;
         check(trs_memcpy_h2d(b->dptr, data, (size_t)b->numel));
+    }
+    return b;
+}
+
+IndexBuffer::~IndexBuffer() {
+    if (dptr) {
+        select_device_quietly(device);
+        (void)trs_free(dptr);
+    }
+}
+
+std::shared_ptr<IndexBuffer> IndexBuffer::from_host(const int32_t *data, const Dims &shape, Device device) {
+    if (!device.is_cuda()) throw TensorError("index buffers live on the device");
+    select_device(device);
+    auto b = std::make_shared<IndexBuffer>();
+    b->device = device;
+    b->shape = shape;
+    b->numel = layout::numel_of(shape);
+    if (b->numel > 0) {
+        void *p = nullptr;
+        const size_t bytes = (size_t)b->numel * sizeof(int32_t);
+        if (trs_alloc(bytes, &p) != TRS_OK) throw TensorError("failed to allocate storage for " + std::to_string(b->numel) + " elements");
+        b->dptr = (int32_t *)p;
+        check(trs_memcpy_h2d(b->dptr, data, bytes));
     }
     return b;
 }

@@ -85,7 +85,7 @@ using MetaPtr = std::shared_ptr<AutogradMeta>;
 enum class Node {
     Add, Alias, Clone, Multiply, Negate, Permute, Relu, ReflectedSubtract, Subtract, Sum, MatrixTranspose,
     Transpose, View, Select, Exp, Mm, Bmm, AddTensor, SubTensor, Squeeze, SqueezeDimension, SqueezeDimensions,
-    Unsqueeze, Fused
+    Unsqueeze, Fused, Dropout, HeadNormRope, WindowAttention
 };
 const char *node_name(Node n);
 
@@ -100,7 +100,7 @@ struct SavedTensor {
 
 enum class GradKind {
     Multiply, MultiplyScalar, Negate, Relu, Sum, Identity, Permute, Index, AddTensor, SubTensor, Matmul, Exp,
-    MaskApply, Transfer, Fused
+    MaskApply, Transfer, Fused, Dropout, HeadNormRope, WindowAttention
 };
 
 // The backward of a fused node: one compiled pointwise program whose
@@ -124,6 +124,36 @@ struct ByteBuffer {
 };
 using BytePtr = std::shared_ptr<ByteBuffer>;
 
+// 32-bit integers in HBM (positions, the key lengths of a batch).
+struct IndexBuffer {
+    Device device;
+    Dims shape;
+    int64_t numel = 0;
+    int32_t *dptr = nullptr;
+    ~IndexBuffer();
+    static std::shared_ptr<IndexBuffer> from_host(const int32_t *data, const Dims &shape, Device device);
+};
+using IndexPtr = std::shared_ptr<IndexBuffer>;
+
+// What the attention block's nodes keep beside their inputs.
+struct DropoutSpec {
+    double p = 0.0;
+    uint64_t seed = 0, offset = 0;
+};
+struct RotationSpec {
+    float eps = 0.0f;
+    bool interleaved = false;
+    int64_t start = 0;
+    IndexPtr positions;
+    std::vector<SavedTensor> tables;  // cosines, sines
+};
+struct AttentionSpec {
+    int64_t window = 0, sinks = 0;
+    float scale = 0.0f;
+    IndexPtr lengths;
+    StoragePtr lse;
+};
+
 struct GradFn {
     GradKind kind;
     Node node;
@@ -137,6 +167,9 @@ struct GradFn {
     BytePtr mask;         // mask-apply: the keep-mask
     FusedBackward fused;  // fused: the gradient program
     std::vector<BytePtr> fused_bytes;  // fused: byte-buffer inputs by position (null for tensors)
+    DropoutSpec dropout;
+    RotationSpec rotation;    // head norm: inputs are x and its weight
+    AttentionSpec attention;  // window attention: inputs are q, k, v; `output` its output
 };
 
 struct AutogradMeta {
@@ -227,6 +260,18 @@ private:
 
 // Dropout-apply with a precomputed keep-mask: (h * mask) * scale.
 Tensor mask_apply(const Tensor &h, const BytePtr &mask, float scale);
+
+// Dropout whose mask a counter gives (trs_dropout_f32); nothing but the spec is
+// saved for backward.
+Tensor dropout_counter(const Tensor &x, const DropoutSpec &spec);
+// The norm of every head's vector with the rotation by its position, of one or
+// two tensors [batch, head, token, dim] in one launch (trs_head_norm_rope_f32).
+// A weight of rank 0 stands for none.
+std::vector<Tensor> head_norm_rope(const std::vector<Tensor> &xs, const std::vector<Tensor> &weights, const Tensor &cos,
+                                   const Tensor &sin, RotationSpec spec);
+// Causal attention with a sliding window and first tokens that stay visible
+// (trs_window_attention_f32).
+Tensor window_attention(const Tensor &q, const Tensor &k, const Tensor &v, AttentionSpec spec);
 
 // Thread-local no-grad depth (src/grad_mode.rs:5-38).
 void enter_no_grad();

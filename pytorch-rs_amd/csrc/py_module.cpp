@@ -210,6 +210,14 @@ PYBIND11_MODULE(_trs_native, m) {
         .def_property_readonly("shape", [](const ByteBuffer &b) { return to_tuple(b.shape); })
         .def_property_readonly("device", [](const ByteBuffer &b) { return b.device.str(); });
 
+    py::class_<IndexBuffer, std::shared_ptr<IndexBuffer>>(m, "IndexBuffer")
+        .def_property_readonly("shape", [](const IndexBuffer &b) { return to_tuple(b.shape); })
+        .def_property_readonly("device", [](const IndexBuffer &b) { return b.device.str(); });
+    m.def("indices_from_numpy", [](py::array_t<int32_t, py::array::c_style> arr, const std::string &device) {
+        Dims shape(arr.shape(), arr.shape() + arr.ndim());
+        return IndexBuffer::from_host(arr.data(), shape, Device::parse(device));
+    });
+
     m.def("empty_pinned", &empty_pinned, py::arg("shape"), py::arg("dtype") = "float32");
     m.def("copy_into", &copy_into, py::arg("tensor"), py::arg("out"));
     m.def("bytes_from_numpy",
@@ -312,6 +320,22 @@ PYBIND11_MODULE(_trs_native, m) {
         return Tensor::full(shape, v, Device::parse(dev));
     });
     m.def("mask_apply", &mask_apply);
+    m.def("dropout_counter", [](const Tensor &x, double p, uint64_t seed, uint64_t offset) {
+        return dropout_counter(x, DropoutSpec{p, seed, offset});
+    });
+    m.def("head_norm_rope",
+          [](const std::vector<Tensor> &xs, const std::vector<py::object> &weights, const Tensor &cos, const Tensor &sin,
+             float eps, bool interleaved, int64_t start, IndexPtr positions) {
+              std::vector<Tensor> w;
+              for (const py::object &o : weights) w.push_back(o.is_none() ? Tensor{} : o.cast<Tensor>());
+              RotationSpec spec;
+              spec.eps = eps, spec.interleaved = interleaved, spec.start = start, spec.positions = std::move(positions);
+              return head_norm_rope(xs, w, cos, sin, std::move(spec));
+          });
+    m.def("window_attention", [](const Tensor &q, const Tensor &k, const Tensor &v, int64_t window, int64_t sinks, float scale,
+                                 IndexPtr lengths) {
+        return window_attention(q, k, v, AttentionSpec{window, sinks, scale, std::move(lengths), nullptr});
+    });
     m.def("enter_no_grad", &enter_no_grad);
     m.def("exit_no_grad", &exit_no_grad);
     m.def("is_grad_enabled", &is_grad_enabled);

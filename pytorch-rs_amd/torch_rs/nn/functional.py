@@ -105,7 +105,7 @@ def _float_like(p, op):
     raise TypeError(f"{op}(): argument 'p' (position 2) must be float, not {_type_name(p)}")
 
 
-def _dropout_bridge(kind, input, p, training, inplace, mask=None):
+def _dropout_bridge(kind, input, p, training, inplace, mask=None, counter=None):
     """_nn_functional_dropout (src/python_nn_functional.rs:117-200): schema
     checks, then identity when not training, p == 0 or the input is empty;
     ``input * 0.0`` for p == 1 where the kind allows it; sampling is
@@ -137,6 +137,10 @@ def _dropout_bridge(kind, input, p, training, inplace, mask=None):
         # PyTorch runs an unbatched input through unsqueeze(0) and squeeze(0),
         # so even the identity returns a new view with a SqueezeBackward1 edge.
         return input._unsqueeze_front().squeeze(0) if unbatched_1d else input
+    if counter is not None:
+        if inplace:
+            raise NotImplementedError(f"torch_rs.nn.functional.{kind} does not support inplace=True")
+        return _C.dropout_counter(input, prob, *counter)
     if mask is not None:
         if inplace:
             raise NotImplementedError(f"torch_rs.nn.functional.{kind} does not support inplace=True")
@@ -148,7 +152,16 @@ def _dropout_bridge(kind, input, p, training, inplace, mask=None):
     raise NotImplementedError(f"torch_rs.nn.functional.{kind} does not support sampling")
 
 
-def dropout(input, p: float = 0.5, training: bool = True, inplace: bool = False, *, mask=None):
+def _word64(name, value) -> int:
+    """An int taken modulo nothing: it has to fit an unsigned 64-bit word."""
+    if isinstance(value, bool) or not isinstance(value, (int, _np.integer)):
+        raise TypeError(f"dropout(): argument '{name}' must be int, not {_type_name(value)}")
+    if not 0 <= int(value) < 1 << 64:
+        raise ValueError(f"dropout {name} has to be between 0 and 2**64 - 1, but got {int(value)}")
+    return int(value)
+
+
+def dropout(input, p: float = 0.5, training: bool = True, inplace: bool = False, *, mask=None, seed=None, offset: int = 0):
     """The reference's dropout (python/torch_rs/nn/functional.py:14-31, 121-143):
     the Python range check, then the native bridge.
 
@@ -156,9 +169,20 @@ def dropout(input, p: float = 0.5, training: bool = True, inplace: bool = False,
     array (or a device byte buffer from ``keep_mask``) of the input's shape
     with 1 = keep -- applied as ``(input * mask) * f32(1/(1-p))``, the
     reference composition ``mul`` then ``mul_scalar``, with the mask read as
-    one byte per element."""
+    one byte per element.
+
+    ``seed`` (this backend's addition) samples on the device instead, from a
+    counter-based generator (``trs_dropout_f32``): element i in row-major order is
+    kept by word i % 4 of counter ``offset + i // 4``, and nothing is stored for
+    backward.  A call uses ``ceil(numel / 4)`` counters: advance ``offset`` by that
+    much, or change the seed, for another mask."""
     _validate_probability(p)
-    return _dropout_bridge("dropout", input, p, training, inplace, mask)
+    counter = None
+    if seed is not None:
+        if mask is not None:
+            raise ValueError("dropout takes a mask or a seed, not both")
+        counter = _word64("seed", seed), _word64("offset", offset)
+    return _dropout_bridge("dropout", input, p, training, inplace, mask, counter)
 
 
 def dropout1d(input, p: float = 0.5, training: bool = True, inplace: bool = False):
@@ -205,3 +229,74 @@ def keep_mask(mask, device="cuda"):
     from .. import _device_str
     arr = _np.asarray(mask, dtype=_np.uint8, order="C")
     return _C.bytes_from_numpy(arr, _device_str(device, "keep_mask"))
+
+
+def index_buffer(values, device="cuda"):
+    """Upload integers (positions, key lengths) to the device once, as int32, for reuse across calls."""
+    from .. import _device_str
+    arr = _np.asarray(values)
+    if arr.size and arr.dtype.kind not in "iu":
+        raise TypeError(f"index_buffer(): values must be integers, not {arr.dtype}")
+    if arr.size and (arr.min() < -(1 << 31) or arr.max() >= 1 << 31):
+        raise ValueError("index_buffer(): values must fit 32 bits")
+    return _C.indices_from_numpy(_np.ascontiguousarray(arr, dtype=_np.int32).reshape(arr.shape), _device_str(device, "index_buffer"))
+
+
+def _indices(values, like):
+    if values is None or isinstance(values, _C.IndexBuffer):
+        return values
+    return index_buffer(values, like.device)
+
+
+def _tensor_arguments(op, **tensors):
+    for name, t in tensors.items():
+        if not isinstance(t, _C.Tensor):
+            raise TypeError(f"{op}(): argument '{name}' must be Tensor, not {_type_name(t)}")
+
+
+def head_norm_rope(query, key, query_weight, key_weight, cos, sin, *, eps: float = 1e-6, start: int = 0, positions=None,
+                   interleaved: bool = False):
+    """The norm of every head's vector with the rotation by its position, of
+    queries and keys [batch, head, token, dim] in one launch; returns both.
+
+    Per row: ``y = R(position) (x * weight / sqrt(mean(x**2) + eps))``.  ``cos`` and
+    ``sin`` are tables [positions, pairs]: row t turns the pairs (i, i + pairs) or,
+    ``interleaved``, (2i, 2i + 1) of the first 2 * pairs entries.  Token t stands at
+    ``start + t``, or where ``positions`` ([batch, token] integers, or an
+    ``index_buffer``) says.  A weight may be None (ones); ``key`` may be None, and the
+    query alone is returned then.  Gradients reach queries, keys and weights."""
+    _tensor_arguments("head_norm_rope", query=query, cos=cos, sin=sin)
+    xs, ws = [query], [query_weight]
+    if key is not None:
+        _tensor_arguments("head_norm_rope", key=key)
+        xs.append(key)
+        ws.append(key_weight)
+    for name, w in zip(("query_weight", "key_weight"), ws):
+        if w is not None:
+            _tensor_arguments("head_norm_rope", **{name: w})
+            if len(w.shape) != 1:
+                raise RuntimeError(f"head_norm_rope weight has {len(w.shape)} dims, expected 1")
+    out = _C.head_norm_rope(xs, ws, cos, sin, float(eps), bool(interleaved), int(start), _indices(positions, query))
+    return out[0] if key is None else tuple(out)
+
+
+def window_attention(query, key, value, *, window=None, sinks: int = 0, scale=None, key_lengths=None):
+    """Causal attention with a sliding window and first tokens that stay visible.
+
+    ``query`` [batch, heads, tokens, dim], ``key`` and ``value`` [batch, key heads,
+    keys, dim]; each key head serves heads / key heads consecutive query heads.
+    The last query stands at the last key's place, and a query at place p sees key
+    j where ``j <= p and (p - j < window or j < sinks)`` (``window`` None: all up to
+    p).  ``scale`` is 1/sqrt(dim) by default.  ``key_lengths`` ([batch] integers, or
+    an ``index_buffer``) are the keys that each sequence of a cache has.  A query
+    that sees nothing gives 0.  Gradients reach queries, keys and values."""
+    _tensor_arguments("window_attention", query=query, key=key, value=value)
+    if window is not None and int(window) < 1:
+        raise ValueError(f"window_attention window has to be at least 1, but got {window}")
+    if int(sinks) < 0:
+        raise ValueError(f"window_attention sinks have to be at least 0, but got {sinks}")
+    if scale is None:
+        scale = 1.0 / math.sqrt(query.shape[-1]) if len(query.shape) and query.shape[-1] else 1.0
+    every = (1 << 63) - 1
+    return _C.window_attention(query, key, value, every if window is None else min(int(window), every), min(int(sinks), every),
+                               float(scale), _indices(key_lengths, query))
