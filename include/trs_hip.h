@@ -396,13 +396,14 @@ int trs_head_norm_rope_backward_f32(int n, const float *const *x, const trs_layo
  * last key's, and sees key j where
  *     j <= p  and  (p - j < window  or  j < sinks).
  *     out = sum over the keys it sees of softmax(scale q k) v
- * A query that sees nothing (p < 0) gives 0.  Keys and values that no query
- * sees are not read, and what stands in one that a query does not see, NaN
- * included, does not reach that query.  window >= 1 (INT64_MAX: no window);
+ * A query that sees nothing (p < 0) gives 0.  Keys and values behind a
+ * sequence's last are not read, and what stands in one that a query does not see,
+ * NaN included, does not reach that query.  window >= 1 (INT64_MAX: no window);
  * sinks >= 0.  lse (or null) receives log(sum(exp(scale q k))) as
- * [batch, heads, Sq], -inf where nothing is seen.  Products and sums are fp32
- * throughout; the order of the sums is fixed.  Inputs may have any strides (one
- * with no unit stride along dim is copied first, into the block cache); outputs
+ * [batch, heads, Sq], -inf where nothing is seen.  Sums are fp32, products
+ * fp32 or exact in pieces (trs_matmul_f32); the order of the sums is fixed.  Inputs may have any strides (one
+ * with no unit stride along dim, or 2^24 elements or more from token to token, is
+ * copied first, into the block cache); outputs
  * need a unit stride along dim and share no memory with inputs.  Few rows over
  * many keys are split over the keys, into a workspace from the block cache. */
 int trs_window_attention_f32(const float *q, const trs_layout *lq, const float *k, const trs_layout *lk,

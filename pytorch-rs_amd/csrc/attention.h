@@ -17,6 +17,7 @@
 // other operand read at row 8 (i/4) + 4 (l/32) + i%4.
 #pragma once
 
+#include "gemm_tile.h"
 #include "op_checks.h"
 
 namespace trs {
@@ -45,8 +46,8 @@ struct AttnArgs {
     float scale, scale2;  // scale2 = scale * log2(e)
     SmallDivisor by_group;
     // Work split over the keys (forward): the parts, their unnormalised
-    // outputs [part][batch, key head, row][D], and (maximum, sum).
-    int32_t splits, row_tiles;
+    // outputs [part][batch, key head, row][part_width], and (maximum, sum).
+    int32_t splits, row_tiles, part_width;
     float *part_o, *part_ml;
     // Work split over the rows (backward).
     int32_t key_tiles, row_splits, sink_tiles, sink_splits;
@@ -86,24 +87,25 @@ __device__ __forceinline__ int result_row(int i, int half) { return 8 * (i >> 2)
 
 // A tile of kTile rows by 32 NT floats in LDS.  The pitch puts rows 4 banks
 // apart, so that 8 lanes reading 16 bytes each at one column cover 32 banks.
-template <int NT>
+template <int NT, int LANES = 256>
 struct Tile {
     static constexpr int kCols = 32 * NT, kPitch = kCols + 4, kFloats = kTile * kPitch;
-    static constexpr int kChunks = kTile * kCols / 4 / 256;  // 16-byte chunks a lane of 256 moves
+    static constexpr int kAll = kTile * kCols / 4, kChunks = (kAll + LANES - 1) / LANES;  // 16-byte chunks, and a lane's
     // Columns a lane reads at once in a product over the tile's rows, and so the
     // result tiles whose rows interleave: result tile u * W + w holds in its row
     // rho the tile's column 32 W u + W rho + w.
     static constexpr int W = NT % 4 == 0 ? 4 : NT % 2 == 0 ? 2 : 1;
     typedef at_f4 Regs[kChunks];
 
-    __device__ __forceinline__ static int row_of(int q) { return ((int)threadIdx.x + q * 256) / (kCols / 4); }
-    __device__ __forceinline__ static int col_of(int q) { return ((int)threadIdx.x + q * 256) % (kCols / 4) * 4; }
+    __device__ __forceinline__ static int row_of(int q) { return ((int)threadIdx.x + q * LANES) / (kCols / 4); }
+    __device__ __forceinline__ static int col_of(int q) { return ((int)threadIdx.x + q * LANES) % (kCols / 4) * 4; }
+    __device__ __forceinline__ static bool has(int q) { return kAll % LANES == 0 || (int)threadIdx.x + q * LANES < kAll; }
     // row(r): the tile's row r in memory, or null for a row of zeros.
     template <class Row>
     __device__ __forceinline__ static void load(Regs &v, int D, Row &&row) {
 #pragma unroll
         for (int q = 0; q < kChunks; q++) {
-            const float *p = row(row_of(q));
+            const float *p = has(q) ? row(row_of(q)) : nullptr;
             v[q] = p ? row_chunk(p, col_of(q), D) : at_f4{0.f, 0.f, 0.f, 0.f};
         }
     }
@@ -112,7 +114,7 @@ struct Tile {
         float s = 0.f;
 #pragma unroll
         for (int q = 0; q < kChunks; q++) {
-            *(at_f4 *)(lds + row_of(q) * kPitch + col_of(q)) = v[q];
+            if (has(q)) *(at_f4 *)(lds + row_of(q) * kPitch + col_of(q)) = v[q];
             s += v[q][0] * 0.f + v[q][1] * 0.f + v[q][2] * 0.f + v[q][3] * 0.f;
         }
         return s != 0.f;
@@ -136,6 +138,20 @@ struct Tile {
             const at_f4 x = *(const at_f4 *)(p + 8 * j);
 #pragma unroll
             for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], f[j][e], c, 0, 0, 0);
+        }
+        return c;
+    }
+    // The same with the lane's row (null: zeros) read as it goes, for few registers.
+    __device__ __forceinline__ static at_f16 times_row(const float *lds, const float *row, int D, float scale, int lane) {
+        at_f16 c = (at_f16)(0.f);
+        const float *p = lds + (lane & 31) * kPitch + 4 * (lane >> 5);
+#pragma unroll 1
+        for (int j = 0; j < NT * 4; j++) {
+            const at_f4 x = *(const at_f4 *)(p + 8 * j);
+            at_f4 y = {0.f, 0.f, 0.f, 0.f};
+            if (row) y = row_chunk(row, 8 * j + 4 * (lane >> 5), D);
+#pragma unroll
+            for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e] * scale, c, 0, 0, 0);
         }
         return c;
     }
@@ -201,9 +217,198 @@ struct Tile {
     }
 };
 
+// The same products on the bf16 matrix cores: every float as the exact sum of
+// three bf16 pieces and six of their nine products, as in gemm_tile.h, at 3/8 of
+// the fp32 instruction's time.  Values are taken times 2^40 and results times the
+// inverse, powers of two that cost no rounding: so the third piece of any float,
+// subnormals included, stands above bf16's least value and nothing is lost.
+// An infinity, a NaN or a value (or sum) beyond what is left of the range, 2^87 and
+// 2^47, shows as a result that is not finite; the block then does its rows again on
+// the fp32 instruction.
+constexpr float kUp = 0x1p40f, kDown = 0x1p-40f, kDown2 = 0x1p-80f;
+
+struct Pieces {
+    gt_bf8 p[3];  // h, m, l of eight values
+};
+__device__ __forceinline__ Pieces split8(const float (&v)[8]) {
+    typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+    U4 h, m, l;
+    uint32_t lost = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        uint32_t x, y, z;
+        split_pair(v[2 * e], v[2 * e + 1], x, y, z, lost);
+        h[e] = x, m[e] = y, l[e] = z;
+    }
+    return Pieces{{__builtin_bit_cast(gt_bf8, h), __builtin_bit_cast(gt_bf8, m), __builtin_bit_cast(gt_bf8, l)}};
+}
+__device__ __forceinline__ void mfma_pieces(at_f16 &c, const Pieces &a, const Pieces &b) {
+    constexpr int PA[6] = {2, 1, 1, 0, 0, 0}, PB[6] = {0, 0, 1, 1, 2, 0};
+#pragma unroll
+    for (int i = 0; i < 6; i++) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[PA[i]], b.p[PB[i]], c, 0, 0, 0);
+}
+
+// A tile of kTile rows by 32 NT columns of one tensor, or of two, as pieces in LDS.
+// A unit is 1 KiB of each piece, an operand fragment of 32 by 16 in lane order (lane
+// l holds row or column l % 32 at k 8 (l/32) to 8 (l/32) + 7), loaded, split and
+// stored by one wave:
+//   along: k runs along the tile's columns; unit u holds columns 16 u on.
+//   across: k runs across its rows, in the order in which a result holds them:
+//     place 8 h + e of slot s is row 16 s + 8 (e/4) + 4 h + e%4.  Unit 2 t + s
+//     holds columns 32 t on.
+// FULL: D is the tile's width.  Else columns from D on are 0.
+//
+// A tile's rows lie `stride` bytes apart from a base that is the same in all
+// lanes; past `last` the last one stands in, so that no branch stands around a
+// load.  Offsets in a tile take 32 bits (the host copies what is spread wider).
+struct TileRows {
+    const float *base;
+    uint32_t stride;
+    int last;
+    __device__ __forceinline__ float at(uint32_t offset) const {
+        return *(gt_global)((gt_global_bytes)base + offset);
+    }
+    __device__ __forceinline__ f4u four(uint32_t offset) const {
+        typedef const f4u __attribute__((address_space(1))) *Ptr;
+        return *(Ptr)((gt_global_bytes)base + offset);
+    }
+};
+template <int NT, bool FULL>
+struct Unit {
+    float v[8];
+    __device__ __forceinline__ void load_along(const TileRows &t, int u, int D, int lane) {
+        const int c = 16 * u + 8 * (lane >> 5);
+        const uint32_t row = (uint32_t)min(lane & 31, t.last) * t.stride;
+        if constexpr (FULL) {
+            const f4u x = t.four(row + 4 * c), y = t.four(row + 4 * c + 16);
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = x[e], v[4 + e] = y[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float x = t.at(row + (c + e < D ? 4 * (c + e) : 0));
+                v[e] = c + e < D ? x : 0.f;
+            }
+        }
+    }
+    __device__ __forceinline__ void load_across(const TileRows &t, int u, int D, int lane) {
+        const int c = 32 * (u >> 1) + (lane & 31);
+        const bool in = FULL || c < D;
+        const uint32_t column = in ? 4 * c : 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int k = 16 * (u & 1) + 8 * (e >> 2) + (e & 3);
+            const uint32_t lo = (uint32_t)min(k, t.last) * t.stride, hi = (uint32_t)min(k + 4, t.last) * t.stride;
+            const float x = t.at((lane & 32 ? hi : lo) + column);
+            v[e] = in ? x : 0.f;
+        }
+    }
+    // A row of the lane's own, as an operand held in registers.
+    __device__ __forceinline__ void load_row(const float *row, int u, int D, int lane) {
+        const int c = 16 * u + 8 * (lane >> 5);
+        const at_f4 x = row_chunk(row, c, D), y = row_chunk(row, c + 4, D);
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = x[e], v[4 + e] = y[e];
+    }
+    __device__ __forceinline__ Pieces split(float scale) const {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = v[e] * scale;
+        return split8(x);
+    }
+    // UNITS: units of a piece in the buffer.
+    template <int UNITS>
+    __device__ __forceinline__ void store(char *lds, int u, int lane) const {
+        const Pieces x = split(kUp);
+#pragma unroll
+        for (int p = 0; p < 3; p++) *(gt_bf8 *)(lds + (p * UNITS + u) * 1024 + lane * 16) = x.p[p];
+    }
+};
+template <int UNITS>
+__device__ __forceinline__ Pieces fragment(const char *lds, int u, int lane) {
+    Pieces x;
+#pragma unroll
+    for (int p = 0; p < 3; p++) x.p[p] = *(const gt_bf8 *)(lds + (p * UNITS + u) * 1024 + lane * 16);
+    return x;
+}
+// The result's columns that register r of result tile t holds.
+__device__ __forceinline__ int across_column(int t, int r, int half) { return 32 * t + result_row(r, half); }
+
+// Whether a value is an infinity or NaN in any lane of the wave.
+template <int N>
+__device__ __forceinline__ bool not_finite(const at_f16 (&acc)[N], float more) {
+    float s = more * 0.f;
+#pragma unroll
+    for (int t = 0; t < N; t++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) s += acc[t][r] * 0.f;
+    return __builtin_amdgcn_ballot_w64(s != 0.f) != 0;
+}
+
+// What a block of 32 rows a wave works on: its rows, their places, and the key
+// tiles that they see, the sinks' first and then the window's.
+template <int NW>
+struct RowBlock {
+    int lane, half, wave;
+    int hk, b, row, i, g;  // the lane's row: query i of head hk * group + g
+    int place;             // below 0: sees nothing
+    int wave_lo, wave_hi;  // places of the wave's rows
+    bool whole;            // the wave has 32 rows
+    int key_lo, key_hi, sinks, first, nsink, tiles;
+
+    // id: over tiles of 32 NW rows, key heads and batches.
+    __device__ __forceinline__ RowBlock(const AttnArgs &a, uint32_t id) {
+        lane = (int)threadIdx.x & 63, half = lane >> 5;
+        wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+        const int tile = (int)(id % (uint32_t)a.row_tiles);
+        id /= (uint32_t)a.row_tiles;
+        hk = (int)(id % (uint32_t)a.kv_heads), b = (int)(id / (uint32_t)a.kv_heads);
+        const Sequence seq = sequence_of(a, b);
+        const auto place_of = [&](int r) { return seq.first + (int)a.by_group.divide((uint32_t)r); };
+        const int r0 = tile * 32 * NW, r1 = min(r0 + 32 * NW, a.rows), last = a.rows - 1;
+        const int w0 = r0 + wave * 32, w1 = min(w0 + 32, a.rows);
+        row = w0 + (lane & 31);
+        i = (int)a.by_group.divide((uint32_t)min(row, last)), g = min(row, last) - i * a.group;
+        place = row < a.rows ? max(seq.first + i, -1) : -1;
+        wave_lo = place_of(min(w0, last));
+        wave_hi = w0 < w1 ? place_of(w1 - 1) : -1;
+        whole = w1 - w0 == 32;
+        key_hi = place_of(r1 - 1), key_lo = max(0, place_of(r0) - a.window + 1);
+        sinks = min(a.sinks, key_hi + 1);
+        first = key_lo / kTile;
+        nsink = key_hi < 0 ? 0 : min((sinks + kTile - 1) / kTile, first);
+        tiles = key_hi < 0 ? 0 : nsink + key_hi / kTile - first + 1;
+    }
+    __device__ __forceinline__ int first_key(int t) const { return (t < nsink ? t : first + t - nsink) * kTile; }
+    // Whether a row of the block sees key j.
+    __device__ __forceinline__ bool read(int j) const { return j <= key_hi && (j >= key_lo || j < sinks); }
+    // Whether a row of the wave sees a key of the tile at j0, and whether all see all.
+    __device__ __forceinline__ bool any(const AttnArgs &a, int j0) const {
+        return j0 <= wave_hi && (wave_lo - (j0 + kTile - 1) < a.window || j0 < a.sinks);
+    }
+    __device__ __forceinline__ bool all(const AttnArgs &a, int j0) const {
+        return whole && j0 + kTile - 1 <= wave_lo && (wave_hi - j0 < a.window || j0 + kTile <= a.sinks);
+    }
+    // The row's place in a [batch, head, token, dim] view.
+    __device__ __forceinline__ int64_t at(const AttnArgs &a, const AttnView &v) const {
+        return b * v.b + (int64_t)(hk * a.group + g) * v.h + (int64_t)i * v.s;
+    }
+    // And in [batch, head, token].
+    __device__ __forceinline__ int64_t index(const AttnArgs &a) const {
+        return ((int64_t)b * a.heads + hk * a.group + g) * a.Sq + i;
+    }
+};
+
 // Words that the waves of a block tell one another ahead of a barrier.
+template <int NW>
 struct Notices {
-    uint32_t word[2][4];
+    uint32_t word[2][NW];
+    __device__ __forceinline__ bool any(int n) const {
+        uint32_t x = 0;
+#pragma unroll
+        for (int w = 0; w < NW; w++) x |= word[n][w];
+        return __builtin_amdgcn_readfirstlane(x) != 0;
+    }
 };
 
 // Few rows a key head (attention_few.hip): row_tiles of 16 rows, `splits` parts.

@@ -47,7 +47,7 @@ template <int NT, int NA>
 __global__ void __launch_bounds__(256, NT <= 2 ? 2 : 1) attn_grad_rows(AttnArgs a) {
     using T = Tile<NT>;
     __shared__ __attribute__((aligned(16))) float lds[2][2][T::kFloats];
-    __shared__ Notices notices;
+    __shared__ Notices<4> notices;
     const int lane = (int)threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     uint32_t id = blockIdx.x;
     const int c0 = (int)(id % (NT / NA)) * 32 * NA;

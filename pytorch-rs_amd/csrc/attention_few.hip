@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) attn_few(AttnArgs 
         float *p;
         if (a.splits > 1) {
             const int64_t at = ((int64_t)part * a.batch * a.kv_heads + head) * a.rows + at_row;
-            p = a.part_o + at * a.D + d;
+            p = a.part_o + at * a.part_width + d;
             if (d == 0) a.part_ml[2 * at] = top, a.part_ml[2 * at + 1] = total;
         } else {
             o *= total == 0.f ? 0.f : 1.f / total;

@@ -10,154 +10,271 @@ namespace {
 constexpr int kFewRows = 32;   // rows a key head that attn_few takes
 constexpr int kPartTiles = 2;  // the least key tiles of a part, a wave
 
-// 128 rows of one key head, 32 a wave, over key tiles that the block stages in
-// LDS, two buffers in turn.  S^T = K Q^T puts a row of the softmax in a lane
-// (and its other half): the running maximum and sum are per lane, and P^T is
-// the operand of O^T += V^T P^T as it stands.  The maximum and sum are of
-// base-2 exponents, log2(e) going into the queries with the scale.
+// A row of the softmax so far: maximum and sum are of base-2 exponents, log2(e)
+// going into the queries with the scale.  A lane holds its row's sum over half of
+// the keys (its other half the rest).
 template <int NT>
-__global__ void __launch_bounds__(256, NT <= 4 ? 2 : 1) attn_rows(AttnArgs a) {
-    using T = Tile<NT>;
-    __shared__ __attribute__((aligned(16))) float lds[2][2][T::kFloats];
-    __shared__ Notices notices;
-    const int lane = (int)threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    uint32_t id = blockIdx.x;
-    const int part = (int)(id % (uint32_t)a.splits);
-    id /= (uint32_t)a.splits;
-    const int tile = (int)(id % (uint32_t)a.row_tiles);
-    id /= (uint32_t)a.row_tiles;
-    const int hk = (int)(id % (uint32_t)a.kv_heads), b = (int)(id / (uint32_t)a.kv_heads);
-
-    const Sequence seq = sequence_of(a, b);
-    const int r0 = tile * kRowsBlock, r1 = min(r0 + kRowsBlock, a.rows);
-    const int row = r0 + wave * 32 + (lane & 31);
-    const bool live = row < a.rows;
-    const int i = (int)a.by_group.divide((uint32_t)min(row, a.rows - 1)), g = min(row, a.rows - 1) - i * a.group;
-    const int place = live ? seq.first + i : -1;
-    // Places of the block's and of the wave's rows.
-    const int block_lo = seq.first + (int)a.by_group.divide((uint32_t)r0);
-    const int block_hi = seq.first + (int)a.by_group.divide((uint32_t)(r1 - 1));
-    const int w0 = r0 + wave * 32, w1 = min(w0 + 32, a.rows);
-    const int wave_lo = seq.first + (int)a.by_group.divide((uint32_t)min(w0, a.rows - 1));
-    const int wave_hi = w0 < w1 ? seq.first + (int)a.by_group.divide((uint32_t)(w1 - 1)) : -1;
-    // Key tiles: those of the sinks, then the window's.
-    const int key_hi = block_hi, key_lo = max(0, block_lo - a.window + 1);
-    const int sinks = min(a.sinks, key_hi + 1);
-    const int first = key_lo / kTile;
-    const int nsink = key_hi < 0 ? 0 : min((sinks + kTile - 1) / kTile, first);
-    const int tiles = key_hi < 0 ? 0 : nsink + key_hi / kTile - first + 1;
-    const int t0 = (int)((int64_t)tiles * part / a.splits), t1 = (int)((int64_t)tiles * (part + 1) / a.splits);
-    const auto first_key = [&](int t) { return (t < nsink ? t : first + t - nsink) * kTile; };
-
-    const float *kb = a.k + b * a.ks.b + hk * a.ks.h, *vb = a.v + b * a.vs.b + hk * a.vs.h;
-    typename T::Regs kr, vr;
-    const auto load = [&](int t) {
-        const int j0 = first_key(t);
-        // A key that no row of the block sees is not read.
-        const auto seen = [&](int r) { return j0 + r <= key_hi && (j0 + r >= key_lo || j0 + r < sinks); };
-        T::load(kr, a.D, [&](int r) { return seen(r) ? kb + (int64_t)(j0 + r) * a.ks.s : nullptr; });
-        T::load(vr, a.D, [&](int r) { return seen(r) ? vb + (int64_t)(j0 + r) * a.vs.s : nullptr; });
-    };
-    const auto store = [&](int buf) {
-        T::store(kr, lds[buf][0]);
-        const bool bad = T::store(vr, lds[buf][1]);
-        notices.word[buf][wave] = __builtin_amdgcn_ballot_w64(bad) != 0;
-    };
-
-    if (t0 < t1) load(t0);
-    at_f4 qf[NT * 4];
-    T::hold(qf, live ? a.q + b * a.qs.b + (int64_t)(hk * a.group + g) * a.qs.h + (int64_t)i * a.qs.s : nullptr, a.D, half, a.scale2);
+struct RowState {
     at_f16 acc[NT];
+    float most, sum;
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int t = 0; t < NT; t++) acc[t] = (at_f16)(0.f);
-    float most = -__builtin_inff(), sum = 0.f;
-    if (t0 < t1) store(0);
-    __syncthreads();
-    for (int t = t0; t < t1; t++) {
-        const int buf = (t - t0) & 1, j0 = first_key(t);
-        if (t + 1 < t1) load(t + 1);
-        // Whether a row of the wave sees a key of the tile, and whether all see all.
-        const bool any = j0 <= wave_hi && (wave_lo - (j0 + kTile - 1) < a.window || j0 < a.sinks);
-        if (any) {
-            at_f16 s = T::times_held(lds[buf][0], qf, lane);
-            const bool all = j0 + kTile - 1 <= wave_lo && (wave_hi - j0 < a.window || j0 + kTile <= a.sinks) && w1 - w0 == 32;
-            if (!all) {
+        for (int t = 0; t < NT; t++) acc[t] = (at_f16)(0.f);
+        most = -__builtin_inff(), sum = 0.f;
+    }
+    // A tile's scores become its weights: s is S^T / unit, -inf where hidden.  The
+    // maximum is kept in the units of s.
+    __device__ __forceinline__ void weigh(at_f16 &s, float unit) {
+        float m = s[0];
 #pragma unroll
-                for (int e = 0; e < 16; e++)
-                    if (!sees(a, place, j0 + result_row(e, half))) s[e] = -__builtin_inff();
-            }
-            float m = s[0];
+        for (int e = 1; e < 16; e++) m = __builtin_fmaxf(m, s[e]);
+        m = __builtin_fmaxf(m, __shfl_xor(m, 32));
+        const float now = __builtin_fmaxf(most, m);
+        const float base = now == -__builtin_inff() ? 0.f : now;  // a row that sees nothing so far
+        const float keep = __builtin_amdgcn_exp2f((most - base) * unit);
+        float add[2] = {0.f, 0.f};
 #pragma unroll
-            for (int e = 1; e < 16; e++) m = __builtin_fmaxf(m, s[e]);
-            m = __builtin_fmaxf(m, __shfl_xor(m, 32));
-            const float now = __builtin_fmaxf(most, m);
-            const float base = now == -__builtin_inff() ? 0.f : now;  // a row that sees nothing so far
-            const float keep = __builtin_amdgcn_exp2f(most - base);
-            float add = 0.f;
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                s[e] = __builtin_amdgcn_exp2f(s[e] - base);
-                add += s[e];
-            }
-            sum = sum * keep + add;
-            most = now;
-            if (__builtin_amdgcn_ballot_w64(keep != 1.f)) {
-#pragma unroll
-                for (int c = 0; c < NT; c++) acc[c] *= keep;
-            }
-            const uint32_t bad = notices.word[buf][0] | notices.word[buf][1] | notices.word[buf][2] | notices.word[buf][3];
-            if (__builtin_expect(__builtin_amdgcn_readfirstlane(bad) == 0, 1))
-                T::add_product(acc, 0, lds[buf][1], s, lane);
-            else
-                T::add_product_seen(acc, 0, lds[buf][1], s, lane, [&](int k) { return sees(a, place, j0 + k); });
+        for (int e = 0; e < 16; e++) {
+            s[e] = __builtin_amdgcn_exp2f((s[e] - base) * unit);
+            add[e & 1] += s[e];
         }
-        if (t + 1 < t1) store(buf ^ 1);
+        sum = sum * keep + (add[0] + add[1]);
+        most = now;
+        if (__builtin_amdgcn_ballot_w64(keep != 1.f)) {
+#pragma unroll
+            for (int c = 0; c < NT; c++) acc[c] *= keep;
+        }
+    }
+};
+
+// The rows of a block over its key tiles t0 to t1 on the fp32 matrix instruction,
+// whatever the values: tiles staged in LDS.  S^T = K Q^T puts a row of the softmax in
+// a lane (and its other half), and P^T is the operand of O^T += V^T P^T as it
+// stands.  FAST: queries held in registers and the next tile loaded ahead; else
+// neither, for few registers.
+template <int NT, int NW, bool FAST>
+__device__ __forceinline__ void rows_fp32(const AttnArgs &a, const RowBlock<NW> &r, int t0, int t1, float *lds,
+                                          Notices<NW> &notices, RowState<NT> &state) {
+    using T = Tile<NT, 64 * NW>;
+    const auto buffer = [&](int n, int which) { return lds + (2 * n + which) * T::kFloats; };
+    const float *kb = a.k + r.b * a.ks.b + r.hk * a.ks.h, *vb = a.v + r.b * a.vs.b + r.hk * a.vs.h;
+    const float *q = r.place >= 0 ? a.q + r.at(a, a.qs) : nullptr;
+    typename T::Regs kr, vr;
+    // A key that no row of the block sees is not read.
+    const auto load = [&](int t, typename T::Regs &x, const float *p, int64_t stride) {
+        const int j0 = r.first_key(t);
+        T::load(x, a.D, [&](int k) { return r.read(j0 + k) ? p + (int64_t)(j0 + k) * stride : nullptr; });
+    };
+    const auto store = [&](int n, bool bad) { notices.word[n][r.wave] = __builtin_amdgcn_ballot_w64(bad) != 0; };
+    state.clear();
+    at_f4 qf[FAST ? NT * 4 : 1];
+    if constexpr (FAST) {
+        if (t0 < t1) load(t0, kr, kb, a.ks.s), load(t0, vr, vb, a.vs.s);
+        T::hold(qf, q, a.D, r.half, a.scale2);
+        if (t0 < t1) T::store(kr, buffer(0, 0)), store(0, T::store(vr, buffer(0, 1)));
         __syncthreads();
     }
-    sum += __shfl_xor(sum, 32);
-    if (!live) return;
-    const int64_t head = (int64_t)b * a.kv_heads + hk;
+#pragma unroll 1
+    for (int t = t0; t < t1; t++) {
+        const int n = FAST ? (t - t0) & 1 : 0, j0 = r.first_key(t);
+        if constexpr (FAST) {
+            if (t + 1 < t1) load(t + 1, kr, kb, a.ks.s), load(t + 1, vr, vb, a.vs.s);
+        } else {
+            load(t, kr, kb, a.ks.s);
+            T::store(kr, buffer(0, 0));
+            load(t, kr, vb, a.vs.s);
+            store(0, T::store(kr, buffer(0, 1)));
+            __syncthreads();
+        }
+        if (r.any(a, j0)) {
+            at_f16 s;
+            if constexpr (FAST) s = T::times_held(buffer(n, 0), qf, r.lane);
+            else s = T::times_row(buffer(n, 0), q, a.D, a.scale2, r.lane);
+            if (!r.all(a, j0)) {
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    if (!sees(a, r.place, j0 + result_row(e, r.half))) s[e] = -__builtin_inff();
+            }
+            state.weigh(s, 1.f);
+            if (FAST && __builtin_expect(!notices.any(n), 1)) T::add_product(state.acc, 0, buffer(n, 1), s, r.lane);
+            else T::add_product_seen(state.acc, 0, buffer(n, 1), s, r.lane, [&](int k) { return sees(a, r.place, j0 + k); });
+        }
+        if constexpr (FAST) {
+            if (t + 1 < t1) T::store(kr, buffer(n ^ 1, 0)), store(n ^ 1, T::store(vr, buffer(n ^ 1, 1)));
+        }
+        __syncthreads();
+    }
+}
+
+// The rows' outputs, or the part's.  `unit`: of the maximum; `up`: acc is that many
+// times the output's.
+template <int NT, int NW, class Column>
+__device__ __forceinline__ void write_rows(const AttnArgs &a, const RowBlock<NW> &r, int part, RowState<NT> &state, float unit,
+                                           float down, Column &&write) {
+    const float sum = state.sum + __shfl_xor(state.sum, 32), most = state.most * unit;
+    if (r.row >= a.rows) return;
     if (a.splits > 1) {
-        const int64_t at = ((int64_t)part * a.batch * a.kv_heads + head) * a.rows + row;
-        T::write(acc, 0, a.part_o + at * a.D, 1.f, a.D, half);
-        if (half == 0) a.part_ml[2 * at] = most, a.part_ml[2 * at + 1] = sum;
+        const int64_t at = (((int64_t)part * a.batch + r.b) * a.kv_heads + r.hk) * a.rows + r.row;
+        write(a.part_o + at * a.part_width, down);
+        if (r.half == 0) a.part_ml[2 * at] = most, a.part_ml[2 * at + 1] = sum;
         return;
     }
     // A row that sees nothing gives 0 and a logarithm of -inf.
-    const float f = sum == 0.f ? 0.f : 1.f / sum;
-    const int64_t h = (int64_t)hk * a.group + g;
-    T::write(acc, 0, a.out + b * a.os.b + h * a.os.h + (int64_t)i * a.os.s, f, a.D, half);
-    if (a.lse && half == 0) a.lse[((int64_t)b * a.heads + h) * a.Sq + i] = (most + __builtin_amdgcn_logf(sum)) * kLn2;
+    write(a.out + r.at(a, a.os), sum == 0.f ? 0.f : down / sum);
+    if (a.lse && r.half == 0) a.lse[r.index(a)] = (most + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-// The parts of a row, joined: a wave a row.
+template <int NT, int NW>
+__global__ void __launch_bounds__(64 * NW, 1) attn_rows_fp32(AttnArgs a) {
+    using T = Tile<NT, 64 * NW>;
+    __shared__ __attribute__((aligned(16))) float lds[4 * T::kFloats];
+    __shared__ Notices<NW> notices;
+    const int part = (int)(blockIdx.x % (uint32_t)a.splits);
+    const RowBlock<NW> r(a, blockIdx.x / (uint32_t)a.splits);
+    RowState<NT> state;
+    rows_fp32<NT, NW, true>(a, r, (int)((int64_t)r.tiles * part / a.splits), (int)((int64_t)r.tiles * (part + 1) / a.splits), lds, notices, state);
+    write_rows(a, r, part, state, 1.f, 1.f, [&](float *p, float f) { T::write(state.acc, 0, p, f, a.D, r.half); });
+}
+
+// The same on the bf16 matrix cores, in pieces: the block splits a key tile once for
+// its waves, into one of two LDS buffers, while it computes from the other.
+template <int NT, int NW, bool FULL>
+__global__ void __launch_bounds__(64 * NW, 2) attn_rows(AttnArgs a) {
+    using T = Tile<NT, 64 * NW>;
+    constexpr int UNITS = 4 * NT, ROUNDS = (UNITS + NW - 1) / NW;  // of K and V; of a wave
+    constexpr int kBuffer = 3 * UNITS * 1024, kBytes = 2 * kBuffer > 16 * T::kFloats ? 2 * kBuffer : 16 * T::kFloats;
+    __shared__ __attribute__((aligned(1024))) char lds[kBytes];
+    __shared__ Notices<NW> notices;
+    const int part = (int)(blockIdx.x % (uint32_t)a.splits);
+    const RowBlock<NW> r(a, blockIdx.x / (uint32_t)a.splits);
+    const int t0 = (int)((int64_t)r.tiles * part / a.splits), t1 = (int)((int64_t)r.tiles * (part + 1) / a.splits);
+    const float *kb = a.k + r.b * a.ks.b + r.hk * a.ks.h, *vb = a.v + r.b * a.vs.b + r.hk * a.vs.h;
+    Unit<NT, FULL> in[ROUNDS];
+    const auto load = [&](int t) {
+        const int j0 = r.first_key(t);
+        const int last = r.key_hi - j0;
+        const TileRows kt = {kb + (int64_t)j0 * a.ks.s, 4 * (uint32_t)a.ks.s, last}, vt = {vb + (int64_t)j0 * a.vs.s, 4 * (uint32_t)a.vs.s, last};
+#pragma unroll
+        for (int q = 0; q < ROUNDS; q++) {
+            const int u = r.wave + q * NW;
+            if (u < UNITS / 2) in[q].load_along(kt, u, a.D, r.lane);
+            else if (u < UNITS) in[q].load_across(vt, u - UNITS / 2, a.D, r.lane);
+        }
+    };
+    const auto store = [&](int n) {
+#pragma unroll
+        for (int q = 0; q < ROUNDS; q++) {
+            const int u = r.wave + q * NW;
+            if (u < UNITS) in[q].template store<UNITS>(lds + n * kBuffer, u, r.lane);
+        }
+    };
+    RowState<NT> state;
+    state.clear();
+    if (t0 < t1) {
+        load(t0);
+        Pieces q[2 * NT];
+#pragma unroll
+        for (int s = 0; s < 2 * NT; s++) {
+            Unit<NT, FULL> x;
+            x.load_row(a.q + r.at(a, a.qs), s, a.D, r.lane);
+            q[s] = x.split(r.place >= 0 ? a.scale2 * kUp : 0.f);
+        }
+        store(0);
+        __syncthreads();
+        for (int t = t0; t < t1; t++) {
+            const int n = (t - t0) & 1, j0 = r.first_key(t);
+            const char *buf = lds + n * kBuffer;
+            if (t + 1 < t1) load(t + 1);
+            if (r.any(a, j0)) {
+                at_f16 s = (at_f16)(0.f);
+#pragma unroll
+                for (int u = 0; u < 2 * NT; u++) mfma_pieces(s, fragment<UNITS>(buf, u, r.lane), q[u]);
+                if (!r.all(a, j0)) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        if (!sees(a, r.place, j0 + result_row(e, r.half))) s[e] = -__builtin_inff();
+                }
+                state.weigh(s, kDown2);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float p[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) p[e] = s[8 * h + e];
+                    const Pieces w = split8(p);
+#pragma unroll
+                    for (int c = 0; c < NT; c++) mfma_pieces(state.acc[c], fragment<UNITS>(buf, 2 * NT + 2 * c + h, r.lane), w);
+                }
+            }
+            if (t + 1 < t1) store(n ^ 1);
+            __syncthreads();
+        }
+        notices.word[0][r.wave] = not_finite(state.acc, state.sum);
+        __syncthreads();
+        if (__builtin_expect(notices.any(0), 0)) {
+            __syncthreads();
+            rows_fp32<NT, NW, false>(a, r, t0, t1, (float *)lds, notices, state);
+            write_rows(a, r, part, state, 1.f, 1.f, [&](float *p, float f) { T::write(state.acc, 0, p, f, a.D, r.half); });
+            return;
+        }
+    }
+    write_rows(a, r, part, state, kDown2, kDown, [&](float *p, float f) {
+#pragma unroll
+        for (int c = 0; c < NT; c++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int d = across_column(c, e, r.half);
+                if (FULL || d < a.D) p[d] = state.acc[c][e] * f;
+            }
+    });
+}
+
+// The parts of a row, joined: four columns a lane.  Every part is read before the
+// first is added, up to eight: one memory latency, not one a part.
 __global__ void __launch_bounds__(256) attn_join(AttnArgs a) {
-    const int lane = (int)threadIdx.x & 63;
     const int64_t rows = (int64_t)a.batch * a.kv_heads * a.rows;
-    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const uint32_t quads = (uint32_t)a.part_width / 4;
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, r = e / quads;
     if (r >= rows) return;
+    const int d = (int)(e - r * quads) * 4;
     const int64_t head = r / a.rows;
     const int row = (int)(r - head * a.rows), b = (int)(head / a.kv_heads), hk = (int)(head - (int64_t)b * a.kv_heads);
     const int i = (int)a.by_group.divide((uint32_t)row);
     const int64_t h = (int64_t)hk * a.group + row - i * a.group;
     float most = -__builtin_inff(), sum = 0.f;
-    for (int p = 0; p < a.splits; p++) most = __builtin_fmaxf(most, a.part_ml[2 * (p * rows + r)]);
-    const float base = most == -__builtin_inff() ? 0.f : most;
-    for (int p = 0; p < a.splits; p++) {
-        const float *ml = a.part_ml + 2 * (p * rows + r);
-        sum += ml[1] * __builtin_amdgcn_exp2f(ml[0] - base);
-    }
-    const float f = sum == 0.f ? 0.f : 1.f / sum;
-    float *o = a.out + b * a.os.b + h * a.os.h + (int64_t)i * a.os.s;
-    for (int d = lane; d < a.D; d += 64) {
-        float v = 0.f;
-        for (int p = 0; p < a.splits; p++) {
-            const int64_t at = p * rows + r;
-            v += a.part_o[at * a.D + d] * __builtin_amdgcn_exp2f(a.part_ml[2 * at] - base);
+    at_f4 o = (at_f4)(0.f);
+    for (int p0 = 0; p0 < a.splits; p0 += 8) {
+        float m[8], l[8];
+        at_f4 x[8];
+#pragma unroll
+        for (int p = 0; p < 8; p++) {
+            const int64_t at = min(p0 + p, a.splits - 1) * rows + r;
+            m[p] = a.part_ml[2 * at], l[p] = a.part_ml[2 * at + 1];
+            x[p] = *(const at_f4 *)(a.part_o + at * a.part_width + d);
         }
-        o[d] = v * f;
+        float now = most;
+#pragma unroll
+        for (int p = 0; p < 8; p++) now = __builtin_fmaxf(now, m[p]);
+        const float base = now == -__builtin_inff() ? 0.f : now, keep = __builtin_amdgcn_exp2f(most - base);
+        sum *= keep, o *= keep, most = now;
+#pragma unroll
+        for (int p = 0; p < 8; p++) {
+            if (p0 + p >= a.splits) break;
+            const float f = __builtin_amdgcn_exp2f(m[p] - base);
+            sum += l[p] * f, o += x[p] * f;
+        }
     }
-    if (a.lse && lane == 0) a.lse[((int64_t)b * a.heads + h) * a.Sq + i] = (most + __builtin_amdgcn_logf(sum)) * kLn2;
+    o *= sum == 0.f ? 0.f : 1.f / sum;
+    float *out = a.out + b * a.os.b + h * a.os.h + (int64_t)i * a.os.s + d;
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+        if (d + q < a.D) out[q] = o[q];
+    if (a.lse && d == 0) a.lse[((int64_t)b * a.heads + h) * a.Sq + i] = (most + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+template <int NT>
+void launch_rows(const AttnArgs &a, dim3 grid, hipStream_t s) {
+    if (a.D == 32 * NT) hipLaunchKernelGGL((attn_rows<NT, 8, true>), grid, dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((attn_rows<NT, 8, false>), grid, dim3(512), 0, s, a);
 }
 
 }  // namespace
@@ -165,32 +282,35 @@ __global__ void __launch_bounds__(256) attn_join(AttnArgs a) {
 int attention_forward(AttnArgs a, hipStream_t s, int cu_count) {
     const int64_t heads = (int64_t)a.batch * a.kv_heads;
     const bool few = a.rows <= kFewRows;
-    const int rows_block = few ? 16 : kRowsBlock, tile = few ? 16 : kTile, waves = few ? 4 : 1;
+    // 8 waves a block share a key tile's splitting, 4 where the width leaves a wave no half of the registers.
+    const int rows_block = few ? 16 : a.D <= 128 ? 256 : 128, tile = few ? 16 : kTile, waves = few ? 4 : 1;
     a.row_tiles = (a.rows + rows_block - 1) / rows_block;
-    // The keys in parts where the rows' blocks are fewer than the device takes.
+    // The keys in parts where the rows' blocks leave CUs without one.
     const int64_t blocks = heads * a.row_tiles, keys = std::min<int64_t>(a.Sk, (int64_t)a.window + a.sinks + rows_block / std::max(a.group, 1));
-    const int64_t most = std::max<int64_t>(1, keys / tile / waves / kPartTiles);
-    a.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({most, (4 * (int64_t)cu_count + blocks - 1) / blocks, 64}));
+    const int64_t most = std::max<int64_t>(1, keys / tile / waves / kPartTiles), want = (few ? 4 : 1) * (int64_t)cu_count;
+    a.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({most, want / blocks, 64}));
     if ((blocks * a.splits) >> 31) return set_error(TRS_E_INVALID_ARGUMENT, "attention over %lld blocks of rows", (long long)blocks);
+    a.part_width = (a.D + 3) / 4 * 4;
+    const int64_t parts = a.splits * heads * a.rows, join_blocks = (heads * a.rows * (a.part_width / 4) + 255) / 256;
     void *ws = nullptr;
+    if (a.splits > 1 && join_blocks >> 31) a.splits = 1;
     if (a.splits > 1) {
-        const int64_t parts = a.splits * heads * a.rows;
-        const int rc = trs_alloc((size_t)(parts * (a.D + 2)) * sizeof(float), &ws);
+        const int rc = trs_alloc((size_t)(parts * (a.part_width + 2)) * sizeof(float), &ws);
         if (rc == TRS_E_ALLOCATION_FAILED) a.splits = 1;  // the parts are for speed alone
         else if (rc) return rc;
-        a.part_ml = (float *)ws, a.part_o = a.part_ml + 2 * parts;
+        a.part_o = (float *)ws, a.part_ml = a.part_o + parts * a.part_width;
     }
     const auto launch = [&]() -> int {
         const dim3 grid((unsigned)(blocks * a.splits));
         if (few) TRS_CHECK(launch_attention_few(a, s));
-        else if (a.D <= 32) hipLaunchKernelGGL(attn_rows<1>, grid, dim3(256), 0, s, a);
-        else if (a.D <= 64) hipLaunchKernelGGL(attn_rows<2>, grid, dim3(256), 0, s, a);
-        else if (a.D <= 96) hipLaunchKernelGGL(attn_rows<3>, grid, dim3(256), 0, s, a);
-        else if (a.D <= 128) hipLaunchKernelGGL(attn_rows<4>, grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL(attn_rows<8>, grid, dim3(256), 0, s, a);
+        else if (a.D <= 32) launch_rows<1>(a, grid, s);
+        else if (a.D <= 64) launch_rows<2>(a, grid, s);
+        else if (a.D <= 96) launch_rows<3>(a, grid, s);
+        else if (a.D <= 128) launch_rows<4>(a, grid, s);
+        else hipLaunchKernelGGL((attn_rows_fp32<8, 4>), grid, dim3(256), 0, s, a);
         TRS_LAUNCH_CHECK("attention launch");
         if (a.splits > 1) {
-            hipLaunchKernelGGL(attn_join, dim3((unsigned)((heads * a.rows + 3) / 4)), dim3(256), 0, s, a);
+            hipLaunchKernelGGL(attn_join, dim3((unsigned)join_blocks), dim3(256), 0, s, a);
             TRS_LAUNCH_CHECK("attention join launch");
         }
         return TRS_OK;
