@@ -41,7 +41,8 @@ HIP_FLAGS = [
 # parallel (one file held every instantiation and took about 3 minutes).
 HIP_SOURCES = ["pw_binary.hip", "pw_binary_muldiv.hip", "pw_scalar.hip", "pw_unary.hip", "pw_mask.hip",
                "pointwise.hip", "runtime.hip", "transfer.hip", "gemm.hip", "gemm_skinny.hip", "fusion.hip",
-               "dropout.hip", "head_norm.hip", "attention.hip", "attention_forward.hip", "attention_few.hip", "attention_backward.hip"]
+               "dropout.hip", "head_norm.hip", "attention.hip", "attention_forward.hip", "attention_few.hip", "attention_backward.hip",
+               "attention_backward_split.hip"]
 ENGINE_SOURCES = ["engine.cpp", "py_module.cpp"]
 
 

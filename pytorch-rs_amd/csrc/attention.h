@@ -310,6 +310,32 @@ struct Unit {
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = x[e], v[4 + e] = y[e];
     }
+    // The same with the columns' guard of load_along.
+    __device__ __forceinline__ void load_row_full(const float *row, int u, int D, int lane) {
+        const int c = 16 * u + 8 * (lane >> 5);
+        if constexpr (FULL) {
+            const f4u x = *(const f4u *)(row + c), y = *(const f4u *)(row + c + 4);
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = x[e], v[4 + e] = y[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float x = row[c + e < D ? c + e : 0];
+                v[e] = c + e < D ? x : 0.f;
+            }
+        }
+    }
+    // Across the tile whose row k lies rows[k] floats from base.
+    __device__ __forceinline__ void load_across_rows(const float *base, const int64_t *rows, int u, int D, int lane) {
+        const int c = 32 * (u >> 1) + (lane & 31);
+        const bool in = FULL || c < D;
+        const float *p = base + (in ? c : 0);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float x = p[rows[16 * (u & 1) + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)]];
+            v[e] = in ? x : 0.f;
+        }
+    }
     __device__ __forceinline__ Pieces split(float scale) const {
         float x[8];
 #pragma unroll
@@ -413,6 +439,10 @@ struct Notices {
 
 // Few rows a key head (attention_few.hip): row_tiles of 16 rows, `splits` parts.
 int launch_attention_few(const AttnArgs &a, hipStream_t s);
+// The gradients' kernels in pieces, for D up to 128: blocks of 128 rows, and of 128
+// keys over their windows' rows.
+void launch_grad_rows(const AttnArgs &a, unsigned blocks, hipStream_t s);
+void launch_grad_keys(const AttnArgs &a, unsigned blocks, hipStream_t s);
 int attention_forward(AttnArgs a, hipStream_t s, int cu_count);
 int attention_backward(AttnArgs a, hipStream_t s, int cu_count);
 

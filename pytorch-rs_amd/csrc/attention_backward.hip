@@ -20,6 +20,8 @@ namespace trs {
 
 namespace {
 
+constexpr int kPartTiles = 8;  // the least row tiles of a part
+
 // delta of every row: 16 lanes a row.
 __global__ void __launch_bounds__(256) attn_delta(AttnArgs a, float *delta) {
     const int64_t rows = (int64_t)a.batch * a.heads * a.Sq;
@@ -44,7 +46,7 @@ __global__ void __launch_bounds__(256) attn_delta(AttnArgs a, float *delta) {
 // NA result tiles a block: those of one half of the columns where all would not
 // fit the registers.
 template <int NT, int NA>
-__global__ void __launch_bounds__(256, NT <= 2 ? 2 : 1) attn_grad_rows(AttnArgs a) {
+__global__ void __launch_bounds__(256, NT <= 2 ? 2 : 1) attn_grad_rows_fp32(AttnArgs a) {
     using T = Tile<NT>;
     __shared__ __attribute__((aligned(16))) float lds[2][2][T::kFloats];
     __shared__ Notices<4> notices;
@@ -131,7 +133,7 @@ __global__ void __launch_bounds__(256, NT <= 2 ? 2 : 1) attn_grad_rows(AttnArgs 
 // of the sinks' pairs holds 32 keys and walks groups of SLOTS row tiles, one a
 // wave.
 template <int NT, int NA>
-__global__ void __launch_bounds__(256, NT <= 2 ? 2 : 1) attn_grad_keys(AttnArgs a) {
+__global__ void __launch_bounds__(256, NT <= 2 ? 2 : 1) attn_grad_keys_fp32(AttnArgs a) {
     using T = Tile<NT>;
     constexpr int SLOTS = NT <= 4 ? 4 : 2;
     __shared__ __attribute__((aligned(16))) float lds[SLOTS][2][T::kFloats];
@@ -312,18 +314,24 @@ __global__ void __launch_bounds__(256) attn_reduce(AttnArgs a, int count, int sl
 }
 
 template <int NT, int NA>
-int run(AttnArgs a, hipStream_t s) {
+int run(AttnArgs a, hipStream_t s, int cu_count) {
     const int64_t heads = (int64_t)a.batch * a.kv_heads;
     const int slots = NT <= 4 ? 4 : 2;
     a.row_tiles = (a.rows + kRowsBlock - 1) / kRowsBlock;
     a.key_tiles = (a.Sk + kRowsBlock - 1) / kRowsBlock;
+    constexpr bool pieces = NT <= 4;
+    // The rows that see a key tile in parts where the tiles are few for the CUs.
+    const int64_t near_tiles = std::max<int64_t>(1, std::min<int64_t>(a.rows, ((int64_t)a.window + kRowsBlock) * a.group) / kTile);
     a.row_splits = 1;
+    if (pieces && a.key_tiles)
+        a.row_splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({2 * (int64_t)cu_count / (heads * a.key_tiles), near_tiles / kPartTiles, 16}));
     // Rows beyond a window see sinks alone.
     a.sink_tiles = a.window < a.Sk ? (std::min(a.sinks, a.Sk) + kTile - 1) / kTile : 0;
     a.sink_splits = 1;
     if (a.sink_tiles) {
-        const int64_t far_tiles = a.rows / kTile / slots, near_tiles = ((int64_t)a.window + kRowsBlock) * a.group / kTile;
-        a.sink_splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(64, far_tiles / std::max<int64_t>(1, near_tiles)));
+        // In parts that fill the device; a part's waves take whole groups of row tiles.
+        const int64_t groups = (a.rows / kTile + slots - 1) / slots;
+        a.sink_splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({64, groups, (pieces ? 1 : 2) * (int64_t)cu_count / (heads * a.sink_tiles)}));
     }
     const int64_t row_blocks = heads * a.row_tiles * (NT / NA);
     const int64_t key_blocks = heads * (a.sink_tiles * a.sink_splits + (int64_t)a.key_tiles * a.row_splits) * (NT / NA);
@@ -343,10 +351,23 @@ int run(AttnArgs a, hipStream_t s) {
         // No rows: the keys' gradients are 0.  No keys: the rows' are.
         if (delta_blocks) hipLaunchKernelGGL(attn_delta, dim3((unsigned)delta_blocks), dim3(256), 0, s, a, delta);
         TRS_LAUNCH_CHECK("attention gradient launch");
-        if (key_blocks) hipLaunchKernelGGL((attn_grad_keys<NT, NA>), dim3((unsigned)key_blocks), dim3(256), 0, s, a);
-        TRS_LAUNCH_CHECK("attention gradient launch");
-        if (row_blocks) hipLaunchKernelGGL((attn_grad_rows<NT, NA>), dim3((unsigned)row_blocks), dim3(256), 0, s, a);
-        TRS_LAUNCH_CHECK("attention gradient launch");
+        if constexpr (pieces) {
+            if (a.key_tiles) launch_grad_keys(a, (unsigned)(heads * a.key_tiles * a.row_splits), s);
+            TRS_LAUNCH_CHECK("attention gradient launch");
+            if (a.sink_tiles) {
+                AttnArgs far = a;
+                far.key_tiles = 0;
+                hipLaunchKernelGGL((attn_grad_keys_fp32<NT, NA>), dim3((unsigned)(heads * a.sink_tiles * a.sink_splits)), dim3(256), 0, s, far);
+                TRS_LAUNCH_CHECK("attention gradient launch");
+            }
+            if (row_blocks) launch_grad_rows(a, (unsigned)row_blocks, s);
+            TRS_LAUNCH_CHECK("attention gradient launch");
+        } else {
+            if (key_blocks) hipLaunchKernelGGL((attn_grad_keys_fp32<NT, NA>), dim3((unsigned)key_blocks), dim3(256), 0, s, a);
+            TRS_LAUNCH_CHECK("attention gradient launch");
+            if (row_blocks) hipLaunchKernelGGL((attn_grad_rows_fp32<NT, NA>), dim3((unsigned)row_blocks), dim3(256), 0, s, a);
+            TRS_LAUNCH_CHECK("attention gradient launch");
+        }
         const int count = a.row_splits > 1 ? a.Sk : std::min(a.sink_tiles * kTile, a.Sk);
         if (count) {
             const int64_t n = heads * count * a.D;
@@ -362,12 +383,11 @@ int run(AttnArgs a, hipStream_t s) {
 }  // namespace
 
 int attention_backward(AttnArgs a, hipStream_t s, int cu_count) {
-    (void)cu_count;
-    if (a.D <= 32) return run<1, 1>(a, s);
-    if (a.D <= 64) return run<2, 2>(a, s);
-    if (a.D <= 96) return run<3, 3>(a, s);
-    if (a.D <= 128) return run<4, 4>(a, s);
-    return run<8, 4>(a, s);
+    if (a.D <= 32) return run<1, 1>(a, s, cu_count);
+    if (a.D <= 64) return run<2, 2>(a, s, cu_count);
+    if (a.D <= 96) return run<3, 3>(a, s, cu_count);
+    if (a.D <= 128) return run<4, 4>(a, s, cu_count);
+    return run<8, 4>(a, s, cu_count);
 }
 
 }  // namespace trs

@@ -1,0 +1,479 @@
+// attention_backward_split.hip -- the gradients of attention_backward.hip on the
+// bf16 matrix cores, in pieces (attention.h), for dims up to 128.
+//
+// A tile is needed twice: along its columns for the scores and dO V^T, across its
+// rows for the gradients.  Both forms have one LDS buffer.  A tile is computed in two
+// phases, and while one form is read the other one is written: the second form of
+// this tile during the first phase, the first form of the next tile during the
+// second.  Two barriers a tile; the loads from memory are a phase ahead.
+//
+// Queries, keys, values and upstream rows are taken times 2^40, and P as 2^40 P, so
+// that no piece of a value or weight is lost.  A block whose sums are not finite does its work again on
+// the fp32 instruction, pair by pair where a tile holds infinities or NaN.
+#include <hip/hip_runtime.h>
+
+#include "attention.h"
+
+namespace trs {
+
+namespace {
+
+// 2^40 2^x.  The exponential gives 0 for subnormal results, and a key may have no
+// larger weight: below 2^-126 it is taken of x + 64.  (Adding 40 to x would cost the
+// low bits of x.)
+__device__ __forceinline__ float up_exp2(float x) {
+    const bool low = x < -126.f;
+    return __builtin_amdgcn_exp2f(x + (low ? 64.f : 0.f)) * (low ? 0x1p-24f : kUp);
+}
+
+// The eight weights of a lane in k order of slot h, as an operand.
+__device__ __forceinline__ Pieces weights(const at_f16 &w, int h) {
+    float p[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) p[e] = w[8 * h + e];
+    return split8(p);
+}
+
+// acc[c] += across-units from u0 on (2 c + slot), times the weights.
+template <int UNITS, int NT>
+__device__ __forceinline__ void add_across(at_f16 (&acc)[NT], const char *lds, int u0, const at_f16 &w, int lane) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const Pieces x = weights(w, h);
+#pragma unroll
+        for (int c = 0; c < NT; c++) mfma_pieces(acc[c], fragment<UNITS>(lds, u0 + 2 * c + h, lane), x);
+    }
+}
+
+template <int NT, bool FULL>
+__device__ __forceinline__ void write_across(const at_f16 (&acc)[NT], float *p, float f, int D, int half) {
+#pragma unroll
+    for (int c = 0; c < NT; c++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const int d = across_column(c, e, half);
+            if (FULL || d < D) p[d] = acc[c][e] * kDown2 * f;
+        }
+}
+
+// ---- dQ -----------------------------------------------------------------------
+
+// The block's rows on the fp32 instruction, whatever the values.
+template <int NT, int NW>
+__device__ __forceinline__ void grad_rows_fp32(const AttnArgs &a, const RowBlock<NW> &r, float lse, float delta, float *lds,
+                                               Notices<NW> &notices, at_f16 (&acc)[NT]) {
+    using T = Tile<NT, 64 * NW>;
+    const float *kb = a.k + r.b * a.ks.b + r.hk * a.ks.h, *vb = a.v + r.b * a.vs.b + r.hk * a.vs.h;
+    const float *q = r.place >= 0 ? a.q + r.at(a, a.qs) : nullptr, *u = r.place >= 0 ? a.up + r.at(a, a.us) : nullptr;
+#pragma unroll
+    for (int t = 0; t < NT; t++) acc[t] = (at_f16)(0.f);
+#pragma unroll 1
+    for (int t = 0; t < r.tiles; t++) {
+        const int j0 = r.first_key(t);
+        typename T::Regs x;
+        T::load(x, a.D, [&](int k) { return r.read(j0 + k) ? kb + (int64_t)(j0 + k) * a.ks.s : nullptr; });
+        notices.word[0][r.wave] = __builtin_amdgcn_ballot_w64(T::store(x, lds)) != 0;
+        T::load(x, a.D, [&](int k) { return r.read(j0 + k) ? vb + (int64_t)(j0 + k) * a.vs.s : nullptr; });
+        T::store(x, lds + T::kFloats);
+        __syncthreads();
+        if (r.any(a, j0)) {
+            at_f16 s = T::times_row(lds, q, a.D, a.scale2, r.lane);
+            const at_f16 d = T::times_row(lds + T::kFloats, u, a.D, 1.f, r.lane);
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                s[e] = __builtin_amdgcn_exp2f(s[e] - lse) * (d[e] - delta);
+                if (!sees(a, r.place, j0 + result_row(e, r.half))) s[e] = 0.f;
+            }
+            T::add_product_seen(acc, 0, lds, s, r.lane, [&](int k) { return sees(a, r.place, j0 + k); });
+        }
+        __syncthreads();
+    }
+}
+
+template <int NT, int NW, bool FULL>
+__global__ void __launch_bounds__(64 * NW, NT <= 2 ? 2 : 1) attn_grad_rows(AttnArgs a) {
+    using T = Tile<NT, 64 * NW>;
+    constexpr int ALONG = 4 * NT, ACROSS = 2 * NT;  // units: K and V; K
+    constexpr int RA = (ALONG + NW - 1) / NW, RC = (ACROSS + NW - 1) / NW;
+    constexpr int kAlong = 3 * ALONG * 1024, kBytes = kAlong + 3 * ACROSS * 1024;
+    static_assert(kBytes >= 8 * T::kFloats, "the fp32 tiles fit the pieces' LDS");
+    __shared__ __attribute__((aligned(1024))) char lds[kBytes];
+    __shared__ Notices<NW> notices;
+    const RowBlock<NW> r(a, blockIdx.x);
+    char *const along = lds, *const across = lds + kAlong;
+    const float *kb = a.k + r.b * a.ks.b + r.hk * a.ks.h, *vb = a.v + r.b * a.vs.b + r.hk * a.vs.h;
+    Unit<NT, FULL> in[RA], in2[RC];
+    const auto rows_of = [&](const float *p, int64_t stride, int t) {
+        const int j0 = r.first_key(t);
+        return TileRows{p + (int64_t)j0 * stride, 4 * (uint32_t)stride, r.key_hi - j0};
+    };
+    const auto load_along = [&](int t) {
+        const TileRows kt = rows_of(kb, a.ks.s, t), vt = rows_of(vb, a.vs.s, t);
+#pragma unroll
+        for (int q = 0; q < RA; q++) {
+            const int u = r.wave + q * NW;
+            if (u < ALONG) in[q].load_along(u < ALONG / 2 ? kt : vt, u < ALONG / 2 ? u : u - ALONG / 2, a.D, r.lane);
+        }
+    };
+    const auto load_across = [&](int t) {
+        const TileRows kt = rows_of(kb, a.ks.s, t);
+#pragma unroll
+        for (int q = 0; q < RC; q++)
+            if (r.wave + q * NW < ACROSS) in2[q].load_across(kt, r.wave + q * NW, a.D, r.lane);
+    };
+    const auto store_along = [&]() {
+#pragma unroll
+        for (int q = 0; q < RA; q++)
+            if (r.wave + q * NW < ALONG) in[q].template store<ALONG>(along, r.wave + q * NW, r.lane);
+    };
+    const auto store_across = [&]() {
+#pragma unroll
+        for (int q = 0; q < RC; q++)
+            if (r.wave + q * NW < ACROSS) in2[q].template store<ACROSS>(across, r.wave + q * NW, r.lane);
+    };
+    const bool live = r.place >= 0;
+    const int64_t at = r.index(a);
+    const float lse = live ? a.lse[at] * kLog2e : 0.f, delta = live ? a.delta[at] : 0.f;
+    at_f16 acc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) acc[t] = (at_f16)(0.f);
+    if (r.tiles > 0) {
+        load_along(0);
+        load_across(0);
+        Pieces qp[2 * NT], up[2 * NT];
+#pragma unroll
+        for (int s = 0; s < 2 * NT; s++) {
+            Unit<NT, FULL> x;
+            x.load_row(a.q + r.at(a, a.qs), s, a.D, r.lane);
+            qp[s] = x.split(live ? a.scale2 * kUp : 0.f);
+            x.load_row(a.up + r.at(a, a.us), s, a.D, r.lane);
+            up[s] = x.split(live ? kUp : 0.f);
+        }
+        store_along();
+        for (int t = 0; t < r.tiles; t++) {
+            const int j0 = r.first_key(t);
+            const bool any = r.any(a, j0), more = t + 1 < r.tiles;
+            at_f16 s = (at_f16)(0.f), d = (at_f16)(0.f);
+            __syncthreads();
+            if (more) load_along(t + 1);
+            if (any) {
+#pragma unroll
+                for (int u = 0; u < 2 * NT; u++) {
+                    mfma_pieces(s, fragment<ALONG>(along, u, r.lane), qp[u]);
+                    mfma_pieces(d, fragment<ALONG>(along, 2 * NT + u, r.lane), up[u]);
+                }
+            }
+            store_across();
+            __syncthreads();
+            if (more) load_across(t + 1);
+            if (any) {
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], kDown2, -lse)) * __builtin_fmaf(d[e], kDown, -delta * kUp);
+                if (!r.all(a, j0)) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        if (!sees(a, r.place, j0 + result_row(e, r.half))) s[e] = 0.f;
+                }
+                add_across<ACROSS>(acc, across, 0, s, r.lane);
+            }
+            if (more) store_along();
+        }
+        __syncthreads();
+        notices.word[1][r.wave] = not_finite(acc, 0.f);
+        __syncthreads();
+        if (__builtin_expect(notices.any(1), 0)) {
+            grad_rows_fp32<NT, NW>(a, r, lse, delta, (float *)lds, notices, acc);
+            if (r.row < a.rows) T::write(acc, 0, a.dq + r.at(a, a.dqs), a.scale, a.D, r.half);
+            return;
+        }
+    }
+    if (r.row < a.rows) write_across<NT, FULL>(acc, a.dq + r.at(a, a.dqs), a.scale, a.D, r.half);
+}
+
+// ---- dK and dV ------------------------------------------------------------------
+
+// What a block of 128 keys works on: its keys, 32 a wave, and the rows whose window
+// holds them.
+struct KeyBlock {
+    int lane, half, wave;
+    int hk, b, head, key, keys;  // the lane's key; past the last key
+    int j0, j1;                  // the wave's keys
+    int part;
+    int first;          // place of query 0
+    int rlo, rhi;       // rows
+    int t0, t1;         // row tiles of the part, from rlo on
+    __device__ __forceinline__ KeyBlock(const AttnArgs &a, uint32_t id) {
+        lane = (int)threadIdx.x & 63, half = lane >> 5;
+        wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+        part = (int)(id % (uint32_t)a.row_splits);
+        id /= (uint32_t)a.row_splits;
+        const int tile = (int)(id % (uint32_t)a.key_tiles);
+        head = (int)(id / (uint32_t)a.key_tiles);
+        hk = head % a.kv_heads, b = head / a.kv_heads;
+        const Sequence seq = sequence_of(a, b);
+        first = seq.first, keys = seq.keys;
+        const int block_j0 = tile * kRowsBlock, block_j1 = min(block_j0 + kRowsBlock, keys);
+        j0 = block_j0 + wave * 32, j1 = min(j0 + 32, keys);
+        key = j0 + (lane & 31);
+        const int place_lo = max(block_j0, max(first, 0)), place_hi = min(keys - 1, block_j1 - 1 + a.window - 1);
+        rlo = rhi = 0;
+        int tiles = 0;
+        if (block_j0 < block_j1 && place_lo <= place_hi) {
+            rlo = (place_lo - first) * a.group, rhi = (place_hi - first + 1) * a.group;
+            tiles = (rhi - rlo + kTile - 1) / kTile;
+        }
+        t0 = (int)((int64_t)tiles * part / a.row_splits), t1 = (int)((int64_t)tiles * (part + 1) / a.row_splits);
+    }
+    // Whether a key of the wave is in the window of a row of tile t, and whether all are in all.
+    __device__ __forceinline__ void look(const AttnArgs &a, int t, bool &any, bool &all) const {
+        const int r0 = rlo + t * kTile, r1 = min(r0 + kTile, rhi);
+        const int lo = first + (int)a.by_group.divide((uint32_t)r0), hi = first + (int)a.by_group.divide((uint32_t)(r1 - 1));
+        any = j0 < j1 && j0 <= hi && lo - (j1 - 1) < a.window;
+        all = r1 - r0 == kTile && j1 - j0 == 32 && j1 - 1 <= lo && hi - j0 < a.window;
+    }
+    __device__ __forceinline__ bool pair(const AttnArgs &a, int place) const {
+        return key < keys && key <= place && place - key < a.window;
+    }
+};
+
+// A tile's rows, as the waves of a block share them; two tiles in turn.
+struct RowFacts {
+    int64_t q[2][kTile], u[2][kTile];  // offsets of the rows
+    float lse[2][kTile], delta[2][kTile];  // lse in base 2
+    int place[2][kTile];               // -1: past the last row
+};
+
+template <int NT>
+__device__ __forceinline__ void grad_keys_fp32(const AttnArgs &a, const KeyBlock &k, float *lds, RowFacts &facts,
+                                               Notices<4> &notices, at_f16 (&dk)[NT], at_f16 (&dv)[NT]) {
+    using T = Tile<NT, 256>;
+    const bool live = k.key < k.keys;
+    const float *kp = live ? a.k + k.b * a.ks.b + k.hk * a.ks.h + (int64_t)k.key * a.ks.s : nullptr;
+    const float *vp = live ? a.v + k.b * a.vs.b + k.hk * a.vs.h + (int64_t)k.key * a.vs.s : nullptr;
+#pragma unroll
+    for (int t = 0; t < NT; t++) dk[t] = dv[t] = (at_f16)(0.f);
+#pragma unroll 1
+    for (int t = k.t0; t < k.t1; t++) {
+        const int r0 = k.rlo + t * kTile;
+        const auto row_at = [&](const float *p, const AttnView &v, int r) -> const float * {
+            const int row = r0 + r;
+            if (row >= k.rhi) return nullptr;
+            const int i = (int)a.by_group.divide((uint32_t)row), g = row - i * a.group;
+            return p + k.b * v.b + (int64_t)(k.hk * a.group + g) * v.h + (int64_t)i * v.s;
+        };
+        typename T::Regs x;
+        T::load(x, a.D, [&](int r) { return row_at(a.q, a.qs, r); });
+        notices.word[0][k.wave] = __builtin_amdgcn_ballot_w64(T::store(x, lds)) != 0;
+        T::load(x, a.D, [&](int r) { return row_at(a.up, a.us, r); });
+        notices.word[1][k.wave] = __builtin_amdgcn_ballot_w64(T::store(x, lds + T::kFloats)) != 0;
+        if (threadIdx.x < kTile) {
+            const int row = r0 + (int)threadIdx.x;
+            float lse = 0.f, delta = 0.f;
+            int place = -1;
+            if (row < k.rhi) {
+                const int i = (int)a.by_group.divide((uint32_t)row), g = row - i * a.group;
+                const int64_t at = ((int64_t)k.b * a.heads + k.hk * a.group + g) * a.Sq + i;
+                lse = a.lse[at] * kLog2e, delta = a.delta[at], place = k.first + i;
+            }
+            facts.lse[0][threadIdx.x] = lse, facts.delta[0][threadIdx.x] = delta, facts.place[0][threadIdx.x] = place;
+        }
+        __syncthreads();
+        bool any, all;
+        k.look(a, t, any, all);
+        if (any) {
+            at_f16 p = T::times_row(lds, kp, a.D, a.scale2, k.lane);
+            at_f16 d = T::times_row(lds + T::kFloats, vp, a.D, 1.f, k.lane);
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int r = result_row(e, k.half);
+                p[e] = __builtin_exp2f(p[e] - facts.lse[0][r]);
+                d[e] = p[e] * (d[e] - facts.delta[0][r]);
+                if (!k.pair(a, facts.place[0][r])) p[e] = d[e] = 0.f;
+            }
+            const auto seen = [&](int r) { return k.pair(a, facts.place[0][r]); };
+            T::add_product_seen(dv, 0, lds + T::kFloats, p, k.lane, seen);
+            T::add_product_seen(dk, 0, lds, d, k.lane, seen);
+        }
+        __syncthreads();
+    }
+}
+
+template <int NT, bool FULL>
+__global__ void __launch_bounds__(256, NT <= 2 ? 2 : 1) attn_grad_keys(AttnArgs a) {
+    using T = Tile<NT, 256>;
+    constexpr int UNITS = 4 * NT, kForm = 3 * UNITS * 1024;  // of queries and upstream rows, in either form
+    static_assert(2 * kForm >= 8 * T::kFloats, "the fp32 tiles fit the pieces' LDS");
+    __shared__ __attribute__((aligned(1024))) char lds[2 * kForm];
+    __shared__ RowFacts facts;
+    __shared__ Notices<4> notices;
+    const KeyBlock k(a, blockIdx.x);
+    char *const along = lds, *const across = lds + kForm;
+    const float *qb = a.q + k.b * a.qs.b + (int64_t)k.hk * a.group * a.qs.h, *ub = a.up + k.b * a.us.b + (int64_t)k.hk * a.group * a.us.h;
+
+    // Rows past the last are read as the last.
+    const auto row_of = [&](int t, int r, int &i, int &g) {
+        const int row = min(k.rlo + t * kTile + r, k.rhi - 1);
+        i = (int)a.by_group.divide((uint32_t)row), g = row - i * a.group;
+    };
+    int64_t fact_q = 0, fact_u = 0;
+    float fact_lse = 0.f, fact_delta = 0.f;
+    int fact_place = -1;
+    const auto load_facts = [&](int t) {  // by the first lanes
+        if (threadIdx.x < kTile) {
+            int i, g;
+            row_of(t, (int)threadIdx.x, i, g);
+            fact_q = g * a.qs.h + i * a.qs.s, fact_u = g * a.us.h + i * a.us.s;
+            const int64_t at = ((int64_t)k.b * a.heads + k.hk * a.group + g) * a.Sq + i;
+            fact_lse = a.lse[at], fact_delta = a.delta[at];
+            fact_place = k.rlo + t * kTile + (int)threadIdx.x < k.rhi ? k.first + i : -1;
+        }
+    };
+    const auto store_facts = [&](int t) {
+        if (threadIdx.x < kTile) {
+            const int n = t & 1, r = (int)threadIdx.x;
+            facts.q[n][r] = fact_q, facts.u[n][r] = fact_u;
+            facts.lse[n][r] = fact_lse * kLog2e, facts.delta[n][r] = fact_delta, facts.place[n][r] = fact_place;
+        }
+    };
+    Unit<NT, FULL> in[NT], in2[NT];
+    const auto load_along = [&](int t) {
+        int i, g;
+        row_of(t, k.lane & 31, i, g);
+        const float *q = qb + (g * a.qs.h + i * a.qs.s), *u = ub + (g * a.us.h + i * a.us.s);
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const int unit = k.wave + 4 * n;
+            in[n].load_row_full(unit < 2 * NT ? q : u, unit < 2 * NT ? unit : unit - 2 * NT, a.D, k.lane);
+        }
+    };
+    const auto load_across = [&](int t) {
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const int unit = k.wave + 4 * n;
+            const bool mine = unit < 2 * NT;
+            in2[n].load_across_rows(mine ? qb : ub, mine ? facts.q[t & 1] : facts.u[t & 1], mine ? unit : unit - 2 * NT, a.D, k.lane);
+        }
+    };
+    const auto store_along = [&]() {
+#pragma unroll
+        for (int n = 0; n < NT; n++) in[n].template store<UNITS>(along, k.wave + 4 * n, k.lane);
+    };
+    const auto store_across = [&]() {
+#pragma unroll
+        for (int n = 0; n < NT; n++) in2[n].template store<UNITS>(across, k.wave + 4 * n, k.lane);
+    };
+    at_f16 dk[NT], dv[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) dk[t] = dv[t] = (at_f16)(0.f);
+    bool again = false;
+    if (k.t0 < k.t1) {
+        load_facts(k.t0);
+        store_facts(k.t0);
+        load_along(k.t0);
+        const bool live = k.key < k.keys;
+        const int key = live ? k.key : 0;
+        Pieces kp[2 * NT], vp[2 * NT];
+#pragma unroll
+        for (int s = 0; s < 2 * NT; s++) {
+            Unit<NT, FULL> x;
+            x.load_row_full(a.k + k.b * a.ks.b + k.hk * a.ks.h + (int64_t)key * a.ks.s, s, a.D, k.lane);
+            kp[s] = x.split(live ? a.scale2 * kUp : 0.f);
+            x.load_row_full(a.v + k.b * a.vs.b + k.hk * a.vs.h + (int64_t)key * a.vs.s, s, a.D, k.lane);
+            vp[s] = x.split(live ? kUp : 0.f);
+        }
+        __syncthreads();
+        load_across(k.t0);
+        store_along();
+        for (int t = k.t0; t < k.t1; t++) {
+            const bool more = t + 1 < k.t1;
+            bool any, all;
+            k.look(a, t, any, all);
+            at_f16 p = (at_f16)(0.f), d = (at_f16)(0.f);
+            if (more) load_facts(t + 1);
+            __syncthreads();
+            if (more) load_along(t + 1);
+            if (any) {
+#pragma unroll
+                for (int u = 0; u < 2 * NT; u++) {
+                    mfma_pieces(p, fragment<UNITS>(along, u, k.lane), kp[u]);
+                    mfma_pieces(d, fragment<UNITS>(along, 2 * NT + u, k.lane), vp[u]);
+                }
+            }
+            store_across();
+            if (more) store_facts(t + 1);
+            __syncthreads();
+            if (more) load_across(t + 1);
+            if (any) {
+                const int n = t & 1;
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int r = result_row(e, k.half);
+                    p[e] = up_exp2(__builtin_fmaf(p[e], kDown2, -facts.lse[n][r]));
+                    d[e] = p[e] * __builtin_fmaf(d[e], kDown2, -facts.delta[n][r]);
+                }
+                if (!all) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        if (!k.pair(a, facts.place[n][result_row(e, k.half)])) p[e] = d[e] = 0.f;
+                }
+                add_across<UNITS>(dv, across, 2 * NT, p, k.lane);
+                add_across<UNITS>(dk, across, 0, d, k.lane);
+            }
+            if (more) store_along();
+        }
+        __syncthreads();
+        notices.word[0][k.wave] = not_finite(dk, 0.f) || not_finite(dv, 0.f);
+        __syncthreads();
+        again = notices.any(0);
+        if (__builtin_expect(again, 0)) {
+            __syncthreads();
+            grad_keys_fp32<NT>(a, k, (float *)lds, facts, notices, dk, dv);
+        }
+    }
+    if (k.key >= a.Sk) return;
+    float *pk, *pv;
+    if (a.row_splits > 1) {
+        const int64_t at = ((int64_t)k.part * a.batch * a.kv_heads + k.head) * a.Sk + k.key;
+        pk = a.part_k + at * a.D, pv = a.part_v + at * a.D;
+    } else {
+        pk = a.dk + k.b * a.dks.b + k.hk * a.dks.h + (int64_t)k.key * a.dks.s;
+        pv = a.dv + k.b * a.dvs.b + k.hk * a.dvs.h + (int64_t)k.key * a.dvs.s;
+    }
+    if (again) {
+        T::write(dk, 0, pk, a.scale, a.D, k.half);
+        T::write(dv, 0, pv, 1.f, a.D, k.half);
+    } else {
+        write_across<NT, FULL>(dk, pk, a.scale, a.D, k.half);
+        write_across<NT, FULL>(dv, pv, 1.f, a.D, k.half);
+    }
+}
+
+template <int NT>
+void launch_rows(const AttnArgs &a, unsigned blocks, hipStream_t s) {
+    if (a.D == 32 * NT) hipLaunchKernelGGL((attn_grad_rows<NT, 4, true>), dim3(blocks), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attn_grad_rows<NT, 4, false>), dim3(blocks), dim3(256), 0, s, a);
+}
+template <int NT>
+void launch_keys(const AttnArgs &a, unsigned blocks, hipStream_t s) {
+    if (a.D == 32 * NT) hipLaunchKernelGGL((attn_grad_keys<NT, true>), dim3(blocks), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attn_grad_keys<NT, false>), dim3(blocks), dim3(256), 0, s, a);
+}
+
+}  // namespace
+
+void launch_grad_rows(const AttnArgs &a, unsigned blocks, hipStream_t s) {
+    if (a.D <= 32) launch_rows<1>(a, blocks, s);
+    else if (a.D <= 64) launch_rows<2>(a, blocks, s);
+    else if (a.D <= 96) launch_rows<3>(a, blocks, s);
+    else launch_rows<4>(a, blocks, s);
+}
+
+void launch_grad_keys(const AttnArgs &a, unsigned blocks, hipStream_t s) {
+    if (a.D <= 32) launch_keys<1>(a, blocks, s);
+    else if (a.D <= 64) launch_keys<2>(a, blocks, s);
+    else if (a.D <= 96) launch_keys<3>(a, blocks, s);
+    else launch_keys<4>(a, blocks, s);
+}
+
+}  // namespace trs
