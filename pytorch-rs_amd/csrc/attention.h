@@ -66,7 +66,7 @@ __device__ __forceinline__ Sequence sequence_of(const AttnArgs &a, int b) {
 }
 
 __device__ __forceinline__ bool sees(const AttnArgs &a, int place, int key) {
-    return key <= place && (place - key < a.window || key < a.sinks);
+    return (key <= place) & ((place - key < a.window) | (key < a.sinks));
 }
 
 // Four floats of a row from column c on, zero from the row's end on.
@@ -230,88 +230,40 @@ constexpr float kUp = 0x1p40f, kDown = 0x1p-40f, kDown2 = 0x1p-80f;
 struct Pieces {
     gt_bf8 p[3];  // h, m, l of eight values
 };
-__device__ __forceinline__ Pieces split8(const float (&v)[8]) {
-    typedef uint32_t U4 __attribute__((ext_vector_type(4)));
-    U4 h, m, l;
-    uint32_t lost = 0;
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-        uint32_t x, y, z;
-        split_pair(v[2 * e], v[2 * e + 1], x, y, z, lost);
-        h[e] = x, m[e] = y, l[e] = z;
+// Eight values split pair by pair, among matrix instructions.
+struct Splitting {
+    uint32_t h[4], m[4], l[4];
+    __device__ __forceinline__ void pair(int i, float a, float b) {
+        uint32_t lost = 0;
+        split_pair(a, b, h[i], m[i], l[i], lost);
     }
-    return Pieces{{__builtin_bit_cast(gt_bf8, h), __builtin_bit_cast(gt_bf8, m), __builtin_bit_cast(gt_bf8, l)}};
-}
+    __device__ __forceinline__ Pieces done() const {
+        typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+        const U4 x = {h[0], h[1], h[2], h[3]}, y = {m[0], m[1], m[2], m[3]}, z = {l[0], l[1], l[2], l[3]};
+        return Pieces{{__builtin_bit_cast(gt_bf8, x), __builtin_bit_cast(gt_bf8, y), __builtin_bit_cast(gt_bf8, z)}};
+    }
+};
 __device__ __forceinline__ void mfma_pieces(at_f16 &c, const Pieces &a, const Pieces &b) {
     constexpr int PA[6] = {2, 1, 1, 0, 0, 0}, PB[6] = {0, 0, 1, 1, 2, 0};
 #pragma unroll
     for (int i = 0; i < 6; i++) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[PA[i]], b.p[PB[i]], c, 0, 0, 0);
 }
 
-// A tile of kTile rows by 32 NT columns of one tensor, or of two, as pieces in LDS.
-// A unit is 1 KiB of each piece, an operand fragment of 32 by 16 in lane order (lane
-// l holds row or column l % 32 at k 8 (l/32) to 8 (l/32) + 7), loaded, split and
-// stored by one wave:
-//   along: k runs along the tile's columns; unit u holds columns 16 u on.
-//   across: k runs across its rows, in the order in which a result holds them:
-//     place 8 h + e of slot s is row 16 s + 8 (e/4) + 4 h + e%4.  Unit 2 t + s
-//     holds columns 32 t on.
-// FULL: D is the tile's width.  Else columns from D on are 0.
+// A tile of kTile rows by 32 NT columns of one tensor or of two, as pieces in LDS.  A
+// unit is 16 columns, 1 KiB of each piece, loaded, split and stored by one wave: (row,
+// column) at 512 (column/8) + 16 row + 2 (column%8), which is the order of a fragment
+// whose k runs along the columns (lane l: row l % 32 at columns 8 (l/32) on), free
+// of bank conflicts.  A fragment whose k runs across the rows is read from the same
+// bytes by the transposing load: 16 lanes ask for 4 rows by 16 columns, four columns of
+// a row each, and each gets its own column's four rows.
 //
-// A tile's rows lie `stride` bytes apart from a base that is the same in all
-// lanes; past `last` the last one stands in, so that no branch stands around a
-// load.  Offsets in a tile take 32 bits (the host copies what is spread wider).
-struct TileRows {
-    const float *base;
-    uint32_t stride;
-    int last;
-    __device__ __forceinline__ float at(uint32_t offset) const {
-        return *(gt_global)((gt_global_bytes)base + offset);
-    }
-    __device__ __forceinline__ f4u four(uint32_t offset) const {
-        typedef const f4u __attribute__((address_space(1))) *Ptr;
-        return *(Ptr)((gt_global_bytes)base + offset);
-    }
-};
+// FULL: D is the tile's width.  Else columns from D on are 0.  No branch stands around a
+// load, which would wait for all of them: what must not be read is read elsewhere in the
+// row and then 0.
 template <int NT, bool FULL>
 struct Unit {
     float v[8];
-    __device__ __forceinline__ void load_along(const TileRows &t, int u, int D, int lane) {
-        const int c = 16 * u + 8 * (lane >> 5);
-        const uint32_t row = (uint32_t)min(lane & 31, t.last) * t.stride;
-        if constexpr (FULL) {
-            const f4u x = t.four(row + 4 * c), y = t.four(row + 4 * c + 16);
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = x[e], v[4 + e] = y[e];
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float x = t.at(row + (c + e < D ? 4 * (c + e) : 0));
-                v[e] = c + e < D ? x : 0.f;
-            }
-        }
-    }
-    __device__ __forceinline__ void load_across(const TileRows &t, int u, int D, int lane) {
-        const int c = 32 * (u >> 1) + (lane & 31);
-        const bool in = FULL || c < D;
-        const uint32_t column = in ? 4 * c : 0;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int k = 16 * (u & 1) + 8 * (e >> 2) + (e & 3);
-            const uint32_t lo = (uint32_t)min(k, t.last) * t.stride, hi = (uint32_t)min(k + 4, t.last) * t.stride;
-            const float x = t.at((lane & 32 ? hi : lo) + column);
-            v[e] = in ? x : 0.f;
-        }
-    }
-    // A row of the lane's own, as an operand held in registers.
-    __device__ __forceinline__ void load_row(const float *row, int u, int D, int lane) {
-        const int c = 16 * u + 8 * (lane >> 5);
-        const at_f4 x = row_chunk(row, c, D), y = row_chunk(row, c + 4, D);
-#pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = x[e], v[4 + e] = y[e];
-    }
-    // The same with the columns' guard of load_along.
-    __device__ __forceinline__ void load_row_full(const float *row, int u, int D, int lane) {
+    __device__ __forceinline__ void load(const float *row, int u, int D, int lane) {
         const int c = 16 * u + 8 * (lane >> 5);
         if constexpr (FULL) {
             const f4u x = *(const f4u *)(row + c), y = *(const f4u *)(row + c + 4);
@@ -325,39 +277,87 @@ struct Unit {
             }
         }
     }
-    // Across the tile whose row k lies rows[k] floats from base.
-    __device__ __forceinline__ void load_across_rows(const float *base, const int64_t *rows, int u, int D, int lane) {
-        const int c = 32 * (u >> 1) + (lane & 31);
-        const bool in = FULL || c < D;
-        const float *p = base + (in ? c : 0);
+    __device__ __forceinline__ Pieces split(float scale) const {
+        Splitting x;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float x = p[rows[16 * (u & 1) + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)]];
-            v[e] = in ? x : 0.f;
+        for (int i = 0; i < 4; i++) x.pair(i, v[2 * i] * scale, v[2 * i + 1] * scale);
+        return x.done();
+    }
+    // Pair i of four; the last one stores the unit.  UNITS: units of a piece in the buffer.
+    template <int UNITS>
+    __device__ __forceinline__ void store_pair(Splitting &x, int i, char *lds, int u, int lane) const {
+        x.pair(i, v[2 * i] * kUp, v[2 * i + 1] * kUp);
+        if (i == 3) {
+            const Pieces y = x.done();
+#pragma unroll
+            for (int p = 0; p < 3; p++) *(gt_bf8 *)(lds + (p * UNITS + u) * 1024 + lane * 16) = y.p[p];
         }
     }
-    __device__ __forceinline__ Pieces split(float scale) const {
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = v[e] * scale;
-        return split8(x);
-    }
-    // UNITS: units of a piece in the buffer.
     template <int UNITS>
     __device__ __forceinline__ void store(char *lds, int u, int lane) const {
-        const Pieces x = split(kUp);
+        Splitting x;
 #pragma unroll
-        for (int p = 0; p < 3; p++) *(gt_bf8 *)(lds + (p * UNITS + u) * 1024 + lane * 16) = x.p[p];
+        for (int i = 0; i < 4; i++) store_pair<UNITS>(x, i, lds, u, lane);
     }
 };
+// Unit u: k runs along its columns.
 template <int UNITS>
-__device__ __forceinline__ Pieces fragment(const char *lds, int u, int lane) {
+__device__ __forceinline__ Pieces along(const char *lds, int u, int lane) {
     Pieces x;
 #pragma unroll
     for (int p = 0; p < 3; p++) x.p[p] = *(const gt_bf8 *)(lds + (p * UNITS + u) * 1024 + lane * 16);
     return x;
 }
-// The result's columns that register r of result tile t holds.
+// Units u and u + 1 as 32 columns: k runs across rows 16 slot to 16 slot + 15, in the
+// order in which a result holds them: place 8 h + e is row 8 (e/4) + 4 h + e%4.
+template <int UNITS>
+__device__ __forceinline__ Pieces across(const char *lds, int u, int slot, int lane) {
+    typedef short S4 __attribute__((ext_vector_type(4)));
+    typedef short S8 __attribute__((ext_vector_type(8)));
+    typedef S4 __attribute__((address_space(3))) *Lds;
+    const char *at = lds + (lane >> 4 & 1) * 1024 + (lane >> 1 & 1) * 512 + (4 * (lane >> 5) + (lane >> 2 & 3)) * 16 + (lane & 1) * 8;
+    Pieces x;
+#pragma unroll
+    for (int p = 0; p < 3; p++) {
+        const char *q = at + (p * UNITS + u) * 1024 + slot * 256;
+        const S4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)q), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(q + 128));
+        x.p[p] = __builtin_bit_cast(gt_bf8, (S8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+    }
+    return x;
+}
+// STEPS steps of six matrix instructions, in the order written: multiply(s, f) takes the
+// fragment that read(s) asked for a step earlier, and work(s) is other work for the
+// step's matrix instructions to run under (a wave issues in order, so it has to stand
+// among them).  `f` holds step 0's fragment; next(f) reads the one that follows the last
+// step's, with that step.
+#ifndef ATTN_V
+#define ATTN_V 8
+#endif
+template <int STEPS, class Read, class Multiply, class Work, class Next>
+__device__ __forceinline__ void steps(Pieces &f, Read &&read, Multiply &&multiply, Work &&work, Next &&next) {
+#pragma unroll
+    for (int s = 0; s < STEPS; s++) {
+        const Pieces now = f;
+        if (s + 1 < STEPS) f = read(s + 1);
+        else next(f);
+        multiply(s, now);
+        work(s);
+        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);  // LDS reads
+#pragma unroll
+        for (int i = 0; i < 6; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction
+            __builtin_amdgcn_sched_group_barrier(0x002, ATTN_V, 0);  // vector instructions
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+// Items first to last of `items` dealt evenly to `of` steps: those of step s.
+template <class F>
+__device__ __forceinline__ void dealt(int items, int s, int of, F &&item) {
+#pragma unroll
+    for (int i = s * items / of; i < (s + 1) * items / of; i++) item(i);
+}
+// The result's column that register r of result tile t holds.
 __device__ __forceinline__ int across_column(int t, int r, int half) { return 32 * t + result_row(r, half); }
 
 // Whether a value is an infinity or NaN in any lane of the wave.

@@ -1,15 +1,17 @@
 // attention_backward_split.hip -- the gradients of attention_backward.hip on the
 // bf16 matrix cores, in pieces (attention.h), for dims up to 128.
 //
-// A tile is needed twice: along its columns for the scores and dO V^T, across its
-// rows for the gradients.  Both forms have one LDS buffer.  A tile is computed in two
-// phases, and while one form is read the other one is written: the second form of
-// this tile during the first phase, the first form of the next tile during the
-// second.  Two barriers a tile; the loads from memory are a phase ahead.
+// A tile in LDS serves twice: along its columns for the scores and dO V^T, across its
+// rows for the gradients.  It is split into one of two buffers while the block
+// computes from the other, the loads from memory a tile further ahead: one barrier a
+// tile.  The block has a CU to itself (512 registers a lane) above dims of 64, and a
+// wave a SIMD nothing to run beside but its own instructions: so splitting and
+// exponentials stand among the matrix instructions (steps()).
 //
 // Queries, keys, values and upstream rows are taken times 2^40, and P as 2^40 P, so
-// that no piece of a value or weight is lost.  A block whose sums are not finite does its work again on
-// the fp32 instruction, pair by pair where a tile holds infinities or NaN.
+// that no piece of a value or weight is lost.  A block whose sums are not finite does
+// its work again on the fp32 instruction, pair by pair where a tile holds infinities or
+// NaN.
 #include <hip/hip_runtime.h>
 
 #include "attention.h"
@@ -24,25 +26,6 @@ namespace {
 __device__ __forceinline__ float up_exp2(float x) {
     const bool low = x < -126.f;
     return __builtin_amdgcn_exp2f(x + (low ? 64.f : 0.f)) * (low ? 0x1p-24f : kUp);
-}
-
-// The eight weights of a lane in k order of slot h, as an operand.
-__device__ __forceinline__ Pieces weights(const at_f16 &w, int h) {
-    float p[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) p[e] = w[8 * h + e];
-    return split8(p);
-}
-
-// acc[c] += across-units from u0 on (2 c + slot), times the weights.
-template <int UNITS, int NT>
-__device__ __forceinline__ void add_across(at_f16 (&acc)[NT], const char *lds, int u0, const at_f16 &w, int lane) {
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const Pieces x = weights(w, h);
-#pragma unroll
-        for (int c = 0; c < NT; c++) mfma_pieces(acc[c], fragment<UNITS>(lds, u0 + 2 * c + h, lane), x);
-    }
 }
 
 template <int NT, bool FULL>
@@ -93,43 +76,22 @@ __device__ __forceinline__ void grad_rows_fp32(const AttnArgs &a, const RowBlock
 template <int NT, int NW, bool FULL>
 __global__ void __launch_bounds__(64 * NW, NT <= 2 ? 2 : 1) attn_grad_rows(AttnArgs a) {
     using T = Tile<NT, 64 * NW>;
-    constexpr int ALONG = 4 * NT, ACROSS = 2 * NT;  // units: K and V; K
-    constexpr int RA = (ALONG + NW - 1) / NW, RC = (ACROSS + NW - 1) / NW;
-    constexpr int kAlong = 3 * ALONG * 1024, kBytes = kAlong + 3 * ACROSS * 1024;
-    static_assert(kBytes >= 8 * T::kFloats, "the fp32 tiles fit the pieces' LDS");
-    __shared__ __attribute__((aligned(1024))) char lds[kBytes];
+    constexpr int UNITS = 4 * NT, OWN = UNITS / NW;  // of keys and values; of a wave
+    constexpr int kBuffer = 3 * UNITS * 1024;
+    static_assert(UNITS % NW == 0 && 2 * kBuffer >= 8 * T::kFloats, "whole shares, and the fp32 tiles fit the pieces' LDS");
+    __shared__ __attribute__((aligned(1024))) char lds[2 * kBuffer];
     __shared__ Notices<NW> notices;
     const RowBlock<NW> r(a, blockIdx.x);
-    char *const along = lds, *const across = lds + kAlong;
     const float *kb = a.k + r.b * a.ks.b + r.hk * a.ks.h, *vb = a.v + r.b * a.vs.b + r.hk * a.vs.h;
-    Unit<NT, FULL> in[RA], in2[RC];
-    const auto rows_of = [&](const float *p, int64_t stride, int t) {
-        const int j0 = r.first_key(t);
-        return TileRows{p + (int64_t)j0 * stride, 4 * (uint32_t)stride, r.key_hi - j0};
-    };
-    const auto load_along = [&](int t) {
-        const TileRows kt = rows_of(kb, a.ks.s, t), vt = rows_of(vb, a.vs.s, t);
+    Unit<NT, FULL> in[OWN];
+    const auto load = [&](int t) {  // past the last tile: that one
+        const int j = min(r.first_key(min(t, r.tiles - 1)) + (r.lane & 31), r.key_hi);
+        const float *kp = kb + (int64_t)j * a.ks.s, *vp = vb + (int64_t)j * a.vs.s;
 #pragma unroll
-        for (int q = 0; q < RA; q++) {
+        for (int q = 0; q < OWN; q++) {
             const int u = r.wave + q * NW;
-            if (u < ALONG) in[q].load_along(u < ALONG / 2 ? kt : vt, u < ALONG / 2 ? u : u - ALONG / 2, a.D, r.lane);
+            in[q].load(u < UNITS / 2 ? kp : vp, u < UNITS / 2 ? u : u - UNITS / 2, a.D, r.lane);
         }
-    };
-    const auto load_across = [&](int t) {
-        const TileRows kt = rows_of(kb, a.ks.s, t);
-#pragma unroll
-        for (int q = 0; q < RC; q++)
-            if (r.wave + q * NW < ACROSS) in2[q].load_across(kt, r.wave + q * NW, a.D, r.lane);
-    };
-    const auto store_along = [&]() {
-#pragma unroll
-        for (int q = 0; q < RA; q++)
-            if (r.wave + q * NW < ALONG) in[q].template store<ALONG>(along, r.wave + q * NW, r.lane);
-    };
-    const auto store_across = [&]() {
-#pragma unroll
-        for (int q = 0; q < RC; q++)
-            if (r.wave + q * NW < ACROSS) in2[q].template store<ACROSS>(across, r.wave + q * NW, r.lane);
     };
     const bool live = r.place >= 0;
     const int64_t at = r.index(a);
@@ -138,46 +100,58 @@ __global__ void __launch_bounds__(64 * NW, NT <= 2 ? 2 : 1) attn_grad_rows(AttnA
 #pragma unroll
     for (int t = 0; t < NT; t++) acc[t] = (at_f16)(0.f);
     if (r.tiles > 0) {
-        load_along(0);
-        load_across(0);
+        load(0);
         Pieces qp[2 * NT], up[2 * NT];
 #pragma unroll
         for (int s = 0; s < 2 * NT; s++) {
             Unit<NT, FULL> x;
-            x.load_row(a.q + r.at(a, a.qs), s, a.D, r.lane);
+            x.load(a.q + r.at(a, a.qs), s, a.D, r.lane);
             qp[s] = x.split(live ? a.scale2 * kUp : 0.f);
-            x.load_row(a.up + r.at(a, a.us), s, a.D, r.lane);
+            x.load(a.up + r.at(a, a.us), s, a.D, r.lane);
             up[s] = x.split(live ? kUp : 0.f);
         }
-        store_along();
+#pragma unroll
+        for (int n = 0; n < OWN; n++) in[n].template store<UNITS>(lds, r.wave + n * NW, r.lane);
+        load(1);
+#pragma unroll 1
         for (int t = 0; t < r.tiles; t++) {
             const int j0 = r.first_key(t);
-            const bool any = r.any(a, j0), more = t + 1 < r.tiles;
+            char *const buf = lds + (t & 1) * kBuffer, *const other = lds + (t & 1 ? 0 : kBuffer);
+            __syncthreads();
             at_f16 s = (at_f16)(0.f), d = (at_f16)(0.f);
-            __syncthreads();
-            if (more) load_along(t + 1);
-            if (any) {
-#pragma unroll
-                for (int u = 0; u < 2 * NT; u++) {
-                    mfma_pieces(s, fragment<ALONG>(along, u, r.lane), qp[u]);
-                    mfma_pieces(d, fragment<ALONG>(along, 2 * NT + u, r.lane), up[u]);
-                }
+            Splitting x;
+            {
+                const auto read = [&](int n) { return along<UNITS>(buf, (n & 1) * 2 * NT + n / 2, r.lane); };
+                Pieces f = read(0);
+                steps<4 * NT>(
+                    f, read, [&](int n, const Pieces &now) { mfma_pieces(n & 1 ? d : s, now, n & 1 ? up[n / 2] : qp[n / 2]); },
+                    [&](int n) {
+                        dealt(4 * OWN, n, 4 * NT, [&](int i) { in[i / 4].template store_pair<UNITS>(x, i % 4, other, r.wave + i / 4 * NW, r.lane); });
+                    },
+                    [](Pieces &) {});
             }
-            store_across();
-            __syncthreads();
-            if (more) load_across(t + 1);
-            if (any) {
+            load(t + 2);
+            if (!r.all(a, j0)) {
 #pragma unroll
-                for (int e = 0; e < 16; e++)
-                    s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], kDown2, -lse)) * __builtin_fmaf(d[e], kDown, -delta * kUp);
-                if (!r.all(a, j0)) {
-#pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        if (!sees(a, r.place, j0 + result_row(e, r.half))) s[e] = 0.f;
-                }
-                add_across<ACROSS>(acc, across, 0, s, r.lane);
+                for (int e = 0; e < 16; e++) s[e] = sees(a, r.place, j0 + result_row(e, r.half)) ? s[e] : -__builtin_inff();
             }
-            if (more) store_along();
+            const auto weigh = [&](int e) {  // 2^40 dS
+                return __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], kDown2, -lse)) * __builtin_fmaf(d[e], kDown, -delta * kUp);
+            };
+            const auto read = [&](int n) { return across<UNITS>(buf, 2 * (n % NT), n / NT, r.lane); };
+            Pieces f = read(0);
+            Splitting w;
+#pragma unroll
+            for (int i = 0; i < 4; i++) w.pair(i, weigh(2 * i), weigh(2 * i + 1));
+            const Pieces p0 = w.done();
+            steps<NT>(
+                f, read, [&](int n, const Pieces &now) { mfma_pieces(acc[n], now, p0); },
+                [&](int n) { dealt(4, n, NT, [&](int i) { w.pair(i, weigh(8 + 2 * i), weigh(9 + 2 * i)); }); },
+                [&](Pieces &y) { y = read(NT); });
+            const Pieces p1 = w.done();
+            steps<NT>(
+                f, [&](int n) { return read(NT + n); }, [&](int n, const Pieces &now) { mfma_pieces(acc[n], now, p1); }, [](int) {},
+                [](Pieces &) {});
         }
         __syncthreads();
         notices.word[1][r.wave] = not_finite(acc, 0.f);
@@ -225,23 +199,21 @@ struct KeyBlock {
         }
         t0 = (int)((int64_t)tiles * part / a.row_splits), t1 = (int)((int64_t)tiles * (part + 1) / a.row_splits);
     }
-    // Whether a key of the wave is in the window of a row of tile t, and whether all are in all.
-    __device__ __forceinline__ void look(const AttnArgs &a, int t, bool &any, bool &all) const {
+    // Whether every key of the wave is in the window of every row of tile t.
+    __device__ __forceinline__ bool all(const AttnArgs &a, int t) const {
         const int r0 = rlo + t * kTile, r1 = min(r0 + kTile, rhi);
         const int lo = first + (int)a.by_group.divide((uint32_t)r0), hi = first + (int)a.by_group.divide((uint32_t)(r1 - 1));
-        any = j0 < j1 && j0 <= hi && lo - (j1 - 1) < a.window;
-        all = r1 - r0 == kTile && j1 - j0 == 32 && j1 - 1 <= lo && hi - j0 < a.window;
+        return r1 - r0 == kTile && j1 - j0 == 32 && j1 - 1 <= lo && hi - j0 < a.window;
     }
     __device__ __forceinline__ bool pair(const AttnArgs &a, int place) const {
-        return key < keys && key <= place && place - key < a.window;
+        return (key < keys) & (key <= place) & (place - key < a.window);
     }
 };
 
 // A tile's rows, as the waves of a block share them; two tiles in turn.
 struct RowFacts {
-    int64_t q[2][kTile], u[2][kTile];  // offsets of the rows
     float lse[2][kTile], delta[2][kTile];  // lse in base 2
-    int place[2][kTile];               // -1: past the last row
+    int place[2][kTile];                   // -1: past the last row
 };
 
 template <int NT>
@@ -279,9 +251,7 @@ __device__ __forceinline__ void grad_keys_fp32(const AttnArgs &a, const KeyBlock
             facts.lse[0][threadIdx.x] = lse, facts.delta[0][threadIdx.x] = delta, facts.place[0][threadIdx.x] = place;
         }
         __syncthreads();
-        bool any, all;
-        k.look(a, t, any, all);
-        if (any) {
+        {
             at_f16 p = T::times_row(lds, kp, a.D, a.scale2, k.lane);
             at_f16 d = T::times_row(lds + T::kFloats, vp, a.D, 1.f, k.lane);
 #pragma unroll
@@ -302,125 +272,105 @@ __device__ __forceinline__ void grad_keys_fp32(const AttnArgs &a, const KeyBlock
 template <int NT, bool FULL>
 __global__ void __launch_bounds__(256, NT <= 2 ? 2 : 1) attn_grad_keys(AttnArgs a) {
     using T = Tile<NT, 256>;
-    constexpr int UNITS = 4 * NT, kForm = 3 * UNITS * 1024;  // of queries and upstream rows, in either form
-    static_assert(2 * kForm >= 8 * T::kFloats, "the fp32 tiles fit the pieces' LDS");
-    __shared__ __attribute__((aligned(1024))) char lds[2 * kForm];
+    constexpr int UNITS = 4 * NT, kBuffer = 3 * UNITS * 1024;  // of queries and upstream rows
+    static_assert(2 * kBuffer >= 8 * T::kFloats, "the fp32 tiles fit the pieces' LDS");
+    __shared__ __attribute__((aligned(1024))) char lds[2 * kBuffer];
     __shared__ RowFacts facts;
     __shared__ Notices<4> notices;
     const KeyBlock k(a, blockIdx.x);
-    char *const along = lds, *const across = lds + kForm;
     const float *qb = a.q + k.b * a.qs.b + (int64_t)k.hk * a.group * a.qs.h, *ub = a.up + k.b * a.us.b + (int64_t)k.hk * a.group * a.us.h;
 
-    // Rows past the last are read as the last.
-    const auto row_of = [&](int t, int r, int &i, int &g) {
-        const int row = min(k.rlo + t * kTile + r, k.rhi - 1);
-        i = (int)a.by_group.divide((uint32_t)row), g = row - i * a.group;
-    };
-    int64_t fact_q = 0, fact_u = 0;
-    float fact_lse = 0.f, fact_delta = 0.f;
-    int fact_place = -1;
-    const auto load_facts = [&](int t) {  // by the first lanes
-        if (threadIdx.x < kTile) {
-            int i, g;
-            row_of(t, (int)threadIdx.x, i, g);
-            fact_q = g * a.qs.h + i * a.qs.s, fact_u = g * a.us.h + i * a.us.s;
-            const int64_t at = ((int64_t)k.b * a.heads + k.hk * a.group + g) * a.Sq + i;
-            fact_lse = a.lse[at], fact_delta = a.delta[at];
-            fact_place = k.rlo + t * kTile + (int)threadIdx.x < k.rhi ? k.first + i : -1;
-        }
-    };
-    const auto store_facts = [&](int t) {
-        if (threadIdx.x < kTile) {
-            const int n = t & 1, r = (int)threadIdx.x;
-            facts.q[n][r] = fact_q, facts.u[n][r] = fact_u;
-            facts.lse[n][r] = fact_lse * kLog2e, facts.delta[n][r] = fact_delta, facts.place[n][r] = fact_place;
-        }
-    };
-    Unit<NT, FULL> in[NT], in2[NT];
-    const auto load_along = [&](int t) {
-        int i, g;
-        row_of(t, k.lane & 31, i, g);
+    // A lane's row of a tile, and what the waves share of it.  Past the part's last tile
+    // that one is loaded, past the last row that one.
+    Unit<NT, FULL> in[NT];
+    float lse = 0.f, delta = 0.f;
+    int place = -1;
+    const auto load = [&](int t) {
+        const int at = k.rlo + min(t, k.t1 - 1) * kTile + (k.lane & 31), row = min(at, k.rhi - 1);
+        const int i = (int)a.by_group.divide((uint32_t)row), g = row - i * a.group;
         const float *q = qb + (g * a.qs.h + i * a.qs.s), *u = ub + (g * a.us.h + i * a.us.s);
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             const int unit = k.wave + 4 * n;
-            in[n].load_row_full(unit < 2 * NT ? q : u, unit < 2 * NT ? unit : unit - 2 * NT, a.D, k.lane);
+            in[n].load(unit < 2 * NT ? q : u, unit < 2 * NT ? unit : unit - 2 * NT, a.D, k.lane);
         }
+        const int64_t fact = ((int64_t)k.b * a.heads + k.hk * a.group + g) * a.Sq + i;
+        lse = a.lse[fact], delta = a.delta[fact];
+        place = at < k.rhi ? k.first + i : -1;
     };
-    const auto load_across = [&](int t) {
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const int unit = k.wave + 4 * n;
-            const bool mine = unit < 2 * NT;
-            in2[n].load_across_rows(mine ? qb : ub, mine ? facts.q[t & 1] : facts.u[t & 1], mine ? unit : unit - 2 * NT, a.D, k.lane);
-        }
-    };
-    const auto store_along = [&]() {
-#pragma unroll
-        for (int n = 0; n < NT; n++) in[n].template store<UNITS>(along, k.wave + 4 * n, k.lane);
-    };
-    const auto store_across = [&]() {
-#pragma unroll
-        for (int n = 0; n < NT; n++) in2[n].template store<UNITS>(across, k.wave + 4 * n, k.lane);
+    const auto store_facts = [&](int n) {
+        if (threadIdx.x < kTile) facts.lse[n][threadIdx.x] = lse * kLog2e, facts.delta[n][threadIdx.x] = delta, facts.place[n][threadIdx.x] = place;
     };
     at_f16 dk[NT], dv[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) dk[t] = dv[t] = (at_f16)(0.f);
     bool again = false;
     if (k.t0 < k.t1) {
-        load_facts(k.t0);
-        store_facts(k.t0);
-        load_along(k.t0);
+        load(k.t0);
         const bool live = k.key < k.keys;
         const int key = live ? k.key : 0;
         Pieces kp[2 * NT], vp[2 * NT];
 #pragma unroll
         for (int s = 0; s < 2 * NT; s++) {
             Unit<NT, FULL> x;
-            x.load_row_full(a.k + k.b * a.ks.b + k.hk * a.ks.h + (int64_t)key * a.ks.s, s, a.D, k.lane);
+            x.load(a.k + k.b * a.ks.b + k.hk * a.ks.h + (int64_t)key * a.ks.s, s, a.D, k.lane);
             kp[s] = x.split(live ? a.scale2 * kUp : 0.f);
-            x.load_row_full(a.v + k.b * a.vs.b + k.hk * a.vs.h + (int64_t)key * a.vs.s, s, a.D, k.lane);
+            x.load(a.v + k.b * a.vs.b + k.hk * a.vs.h + (int64_t)key * a.vs.s, s, a.D, k.lane);
             vp[s] = x.split(live ? kUp : 0.f);
         }
-        __syncthreads();
-        load_across(k.t0);
-        store_along();
+#pragma unroll
+        for (int n = 0; n < NT; n++) in[n].template store<UNITS>(lds, k.wave + 4 * n, k.lane);
+        store_facts(0);
+        load(k.t0 + 1);
+#pragma unroll 1
         for (int t = k.t0; t < k.t1; t++) {
-            const bool more = t + 1 < k.t1;
-            bool any, all;
-            k.look(a, t, any, all);
+            const int n2 = (t - k.t0) & 1;
+            char *const buf = lds + n2 * kBuffer, *const other = lds + (n2 ? 0 : kBuffer);
+            __syncthreads();
             at_f16 p = (at_f16)(0.f), d = (at_f16)(0.f);
-            if (more) load_facts(t + 1);
-            __syncthreads();
-            if (more) load_along(t + 1);
-            if (any) {
-#pragma unroll
-                for (int u = 0; u < 2 * NT; u++) {
-                    mfma_pieces(p, fragment<UNITS>(along, u, k.lane), kp[u]);
-                    mfma_pieces(d, fragment<UNITS>(along, 2 * NT + u, k.lane), vp[u]);
-                }
+            Splitting x, w;
+            {
+                const auto read = [&](int n) { return along<UNITS>(buf, (n & 1) * 2 * NT + n / 2, k.lane); };
+                Pieces f = read(0);
+                steps<4 * NT>(
+                    f, read, [&](int n, const Pieces &now) { mfma_pieces(n & 1 ? d : p, now, n & 1 ? vp[n / 2] : kp[n / 2]); },
+                    [&](int n) { in[n / 4].template store_pair<UNITS>(x, n % 4, other, k.wave + n / 4 * 4, k.lane); }, [](Pieces &) {});
             }
-            store_across();
-            if (more) store_facts(t + 1);
-            __syncthreads();
-            if (more) load_across(t + 1);
-            if (any) {
-                const int n = t & 1;
+            store_facts(n2 ^ 1);
+            load(t + 2);
+            if (!k.all(a, t)) {
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const int r = result_row(e, k.half);
-                    p[e] = up_exp2(__builtin_fmaf(p[e], kDown2, -facts.lse[n][r]));
-                    d[e] = p[e] * __builtin_fmaf(d[e], kDown2, -facts.delta[n][r]);
-                }
-                if (!all) {
-#pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        if (!k.pair(a, facts.place[n][result_row(e, k.half)])) p[e] = d[e] = 0.f;
-                }
-                add_across<UNITS>(dv, across, 2 * NT, p, k.lane);
-                add_across<UNITS>(dk, across, 0, d, k.lane);
+                for (int e = 0; e < 16; e++) p[e] = k.pair(a, facts.place[n2][result_row(e, k.half)]) ? p[e] : -__builtin_inff();
             }
-            if (more) store_along();
+            // 2^40 P and 2^40 dS come pair by pair, each eight of them ahead of the products that take them.
+            const auto pair_p = [&](int e) { return p[e] = up_exp2(__builtin_fmaf(p[e], kDown2, -facts.lse[n2][result_row(e, k.half)])); };
+            const auto pair_d = [&](int e) { return p[e] * __builtin_fmaf(d[e], kDown2, -facts.delta[n2][result_row(e, k.half)]); };
+            // dV's first 16 rows, its others, dK's first, its others.
+            const auto read = [&](int n) { return across<UNITS>(buf, (n < 2 * NT ? 2 * NT : 0) + 2 * (n % NT), n / NT % 2, k.lane); };
+            Pieces f = read(0);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float w0 = pair_p(2 * i), w1 = pair_p(2 * i + 1);
+                w.pair(i, w0, w1);
+            }
+            Pieces weights = w.done();
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                steps<NT>(
+                    f, [&](int n) { return read(g * NT + n); }, [&](int n, const Pieces &now) { mfma_pieces(g < 2 ? dv[n] : dk[n], now, weights); },
+                    [&](int n) {
+                        dealt(4, n, NT, [&](int i) {
+                            if (g == 3) return;
+                            const int e = (g == 1 ? 0 : 8) + 2 * i;
+                            const float w0 = g == 0 ? pair_p(e) : pair_d(e), w1 = g == 0 ? pair_p(e + 1) : pair_d(e + 1);
+                            w.pair(i, w0, w1);
+                        });
+                    },
+                    [&](Pieces &y) {
+                        if (g < 3) y = read((g + 1) * NT);
+                    });
+                if (g < 3) weights = w.done();
+            }
         }
         __syncthreads();
         notices.word[0][k.wave] = not_finite(dk, 0.f) || not_finite(dv, 0.f);

@@ -137,11 +137,12 @@ __global__ void __launch_bounds__(64 * NW, 1) attn_rows_fp32(AttnArgs a) {
 }
 
 // The same on the bf16 matrix cores, in pieces: the block splits a key tile once for
-// its waves, into one of two LDS buffers, while it computes from the other.
+// its waves, into one of two LDS buffers while it computes from the other; the loads from
+// memory are a tile further ahead.
 template <int NT, int NW, bool FULL>
 __global__ void __launch_bounds__(64 * NW, 2) attn_rows(AttnArgs a) {
     using T = Tile<NT, 64 * NW>;
-    constexpr int UNITS = 4 * NT, ROUNDS = (UNITS + NW - 1) / NW;  // of K and V; of a wave
+    constexpr int UNITS = 4 * NT, OWN = (UNITS + NW - 1) / NW;  // of keys and values; of a wave (some twice)
     constexpr int kBuffer = 3 * UNITS * 1024, kBytes = 2 * kBuffer > 16 * T::kFloats ? 2 * kBuffer : 16 * T::kFloats;
     __shared__ __attribute__((aligned(1024))) char lds[kBytes];
     __shared__ Notices<NW> notices;
@@ -149,23 +150,15 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_rows(AttnArgs a) {
     const RowBlock<NW> r(a, blockIdx.x / (uint32_t)a.splits);
     const int t0 = (int)((int64_t)r.tiles * part / a.splits), t1 = (int)((int64_t)r.tiles * (part + 1) / a.splits);
     const float *kb = a.k + r.b * a.ks.b + r.hk * a.ks.h, *vb = a.v + r.b * a.vs.b + r.hk * a.vs.h;
-    Unit<NT, FULL> in[ROUNDS];
-    const auto load = [&](int t) {
-        const int j0 = r.first_key(t);
-        const int last = r.key_hi - j0;
-        const TileRows kt = {kb + (int64_t)j0 * a.ks.s, 4 * (uint32_t)a.ks.s, last}, vt = {vb + (int64_t)j0 * a.vs.s, 4 * (uint32_t)a.vs.s, last};
+    Unit<NT, FULL> in[OWN];
+    const auto unit = [&](int q) { return min(r.wave + q * NW, UNITS - 1); };
+    const auto load = [&](int t) {  // past the part's last tile: that one
+        const int j = min(r.first_key(min(t, t1 - 1)) + (r.lane & 31), r.key_hi);
+        const float *kp = kb + (int64_t)j * a.ks.s, *vp = vb + (int64_t)j * a.vs.s;
 #pragma unroll
-        for (int q = 0; q < ROUNDS; q++) {
-            const int u = r.wave + q * NW;
-            if (u < UNITS / 2) in[q].load_along(kt, u, a.D, r.lane);
-            else if (u < UNITS) in[q].load_across(vt, u - UNITS / 2, a.D, r.lane);
-        }
-    };
-    const auto store = [&](int n) {
-#pragma unroll
-        for (int q = 0; q < ROUNDS; q++) {
-            const int u = r.wave + q * NW;
-            if (u < UNITS) in[q].template store<UNITS>(lds + n * kBuffer, u, r.lane);
+        for (int q = 0; q < OWN; q++) {
+            const bool key = unit(q) < UNITS / 2;
+            in[q].load(key ? kp : vp, key ? unit(q) : unit(q) - UNITS / 2, a.D, r.lane);
         }
     };
     RowState<NT> state;
@@ -176,38 +169,53 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_rows(AttnArgs a) {
 #pragma unroll
         for (int s = 0; s < 2 * NT; s++) {
             Unit<NT, FULL> x;
-            x.load_row(a.q + r.at(a, a.qs), s, a.D, r.lane);
+            x.load(a.q + r.at(a, a.qs), s, a.D, r.lane);
             q[s] = x.split(r.place >= 0 ? a.scale2 * kUp : 0.f);
         }
-        store(0);
-        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < OWN; n++) in[n].template store<UNITS>(lds, unit(n), r.lane);
+        load(t0 + 1);
+#pragma unroll 1
         for (int t = t0; t < t1; t++) {
-            const int n = (t - t0) & 1, j0 = r.first_key(t);
-            const char *buf = lds + n * kBuffer;
-            if (t + 1 < t1) load(t + 1);
-            if (r.any(a, j0)) {
-                at_f16 s = (at_f16)(0.f);
-#pragma unroll
-                for (int u = 0; u < 2 * NT; u++) mfma_pieces(s, fragment<UNITS>(buf, u, r.lane), q[u]);
-                if (!r.all(a, j0)) {
-#pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        if (!sees(a, r.place, j0 + result_row(e, r.half))) s[e] = -__builtin_inff();
-                }
-                state.weigh(s, kDown2);
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    float p[8];
-#pragma unroll
-                    for (int e = 0; e < 8; e++) p[e] = s[8 * h + e];
-                    const Pieces w = split8(p);
-#pragma unroll
-                    for (int c = 0; c < NT; c++) mfma_pieces(state.acc[c], fragment<UNITS>(buf, 2 * NT + 2 * c + h, r.lane), w);
-                }
-            }
-            if (t + 1 < t1) store(n ^ 1);
+            const int j0 = r.first_key(t);
+            char *const buf = lds + ((t - t0) & 1) * kBuffer, *const other = lds + ((t - t0) & 1 ? 0 : kBuffer);
             __syncthreads();
+            at_f16 s = (at_f16)(0.f);
+            Splitting x;
+            {
+                const auto read = [&](int n) { return along<UNITS>(buf, n, r.lane); };
+                Pieces f = read(0);
+                steps<2 * NT>(
+                    f, read, [&](int n, const Pieces &now) { mfma_pieces(s, now, q[n]); },
+                    [&](int n) {
+                        dealt(4 * OWN, n, 2 * NT, [&](int i) { in[i / 4].template store_pair<UNITS>(x, i % 4, other, unit(i / 4), r.lane); });
+                    },
+                    [](Pieces &) {});
+            }
+            load(t + 2);
+            if (!r.all(a, j0)) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[e] = sees(a, r.place, j0 + result_row(e, r.half)) ? s[e] : -__builtin_inff();
+            }
+            state.weigh(s, kDown2);
+            {
+                const auto read = [&](int n) { return across<UNITS>(buf, 2 * NT + 2 * (n % NT), n / NT, r.lane); };
+                Pieces f = read(0);
+                Splitting w;
+#pragma unroll
+                for (int i = 0; i < 4; i++) w.pair(i, s[2 * i], s[2 * i + 1]);
+                const Pieces p0 = w.done();
+                steps<NT>(
+                    f, read, [&](int n, const Pieces &now) { mfma_pieces(state.acc[n], now, p0); },
+                    [&](int n) { dealt(4, n, NT, [&](int i) { w.pair(i, s[8 + 2 * i], s[9 + 2 * i]); }); },
+                    [&](Pieces &y) { y = read(NT); });
+                const Pieces p1 = w.done();
+                steps<NT>(
+                    f, [&](int n) { return read(NT + n); }, [&](int n, const Pieces &now) { mfma_pieces(state.acc[n], now, p1); }, [](int) {},
+                    [](Pieces &) {});
+            }
         }
+        __syncthreads();
         notices.word[0][r.wave] = not_finite(state.acc, state.sum);
         __syncthreads();
         if (__builtin_expect(notices.any(0), 0)) {
