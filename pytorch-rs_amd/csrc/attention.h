@@ -225,7 +225,7 @@ struct Tile {
 // An infinity, a NaN or a value (or sum) beyond what is left of the range, 2^87 and
 // 2^47, shows as a result that is not finite; the block then does its rows again on
 // the fp32 instruction.
-constexpr float kUp = 0x1p40f, kDown = 0x1p-40f, kDown2 = 0x1p-80f;
+constexpr float kUp = 0x1p40f, kDown = 0x1p-40f, kUp2 = 0x1p80f, kDown2 = 0x1p-80f;
 
 struct Pieces {
     gt_bf8 p[3];  // h, m, l of eight values
@@ -439,10 +439,10 @@ struct Notices {
 
 // Few rows a key head (attention_few.hip): row_tiles of 16 rows, `splits` parts.
 int launch_attention_few(const AttnArgs &a, hipStream_t s);
-// The gradients' kernels in pieces, for D up to 128: blocks of 128 rows, and of 128
-// keys over their windows' rows.
-void launch_grad_rows(const AttnArgs &a, unsigned blocks, hipStream_t s);
-void launch_grad_keys(const AttnArgs &a, unsigned blocks, hipStream_t s);
+// The gradients' kernel in pieces, for D up to 128: blocks of 128 keys over their windows'
+// rows, or over the rows beyond the window of the sinks (sink_tiles of 128 keys), and of 128
+// rows.
+void launch_attention_grad(const AttnArgs &a, uint32_t key_blocks, uint32_t row_blocks, hipStream_t s);
 int attention_forward(AttnArgs a, hipStream_t s, int cu_count);
 int attention_backward(AttnArgs a, hipStream_t s, int cu_count);
 

@@ -283,10 +283,24 @@ __global__ void __launch_bounds__(256, NT <= 2 ? 2 : 1) attn_grad_keys_fp32(Attn
     }
 }
 
-// dk and dv of the first `count` keys: the parts over the rows, or what the one
-// part wrote, and the sinks' parts, in a fixed order.
-__global__ void __launch_bounds__(256) attn_reduce(AttnArgs a, int count, int slots) {
+// dk and dv of the first `count` keys: the parts over the rows, or what the one part
+// wrote, and the sinks' `far` parts of tiles of `tile` keys, in a fixed order.  Eight parts
+// are read at a time: one memory latency for all of them.
+__global__ void __launch_bounds__(256) attn_reduce(AttnArgs a, int count, int tile, int far) {
     const int64_t heads = (int64_t)a.batch * a.kv_heads, n = heads * count * a.D;
+    const auto add = [](float &x, float &y, const float *px, const float *py, int64_t step, int parts) {
+        for (int p = 0; p < parts; p += 8) {
+            float u[8], w[8];
+#pragma unroll
+            for (int q = 0; q < 8; q++) {
+                const int64_t at = min(p + q, parts - 1) * step;
+                u[q] = px[at], w[q] = py[at];
+            }
+#pragma unroll
+            for (int q = 0; q < 8; q++)
+                if (p + q < parts) x += u[q], y += w[q];
+        }
+    };
     for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n; e += (int64_t)gridDim.x * 256) {
         const int64_t row = e / a.D, head = row / count;
         const int d = (int)(e - row * a.D), key = (int)(row - head * count), hk = (int)(head % a.kv_heads);
@@ -295,19 +309,14 @@ __global__ void __launch_bounds__(256) attn_reduce(AttnArgs a, int count, int sl
         float *dv = a.dv + b * a.dvs.b + hk * a.dvs.h + (int64_t)key * a.dvs.s + d;
         float x = 0.f, y = 0.f;
         if (a.row_splits > 1) {
-            for (int p = 0; p < a.row_splits; p++) {
-                const int64_t at = ((p * heads + head) * a.Sk + key) * a.D + d;
-                x += a.part_k[at], y += a.part_v[at];
-            }
+            const int64_t at = (head * a.Sk + key) * a.D + d;
+            add(x, y, a.part_k + at, a.part_v + at, heads * a.Sk * a.D, a.row_splits);
         } else {
             x = *dk, y = *dv;
         }
-        if (key < a.sink_tiles * kTile) {
-            const int tile = key / kTile, from = a.sink_splits * slots;
-            for (int p = 0; p < from; p++) {
-                const int64_t at = (((head * a.sink_tiles + tile) * from + p) * kTile + key % kTile) * a.D + d;
-                x += a.sink_k[at], y += a.sink_v[at];
-            }
+        if (far && key < a.sinks) {
+            const int64_t at = (((head * a.sink_tiles + key / tile) * far) * tile + key % tile) * a.D + d;
+            add(x, y, a.sink_k + at, a.sink_v + at, (int64_t)tile * a.D, far);
         }
         *dk = x, *dv = y;
     }
@@ -315,31 +324,33 @@ __global__ void __launch_bounds__(256) attn_reduce(AttnArgs a, int count, int sl
 
 template <int NT, int NA>
 int run(AttnArgs a, hipStream_t s, int cu_count) {
+    constexpr bool pieces = NT <= 4;
     const int64_t heads = (int64_t)a.batch * a.kv_heads;
-    const int slots = NT <= 4 ? 4 : 2;
+    const int slots = NT <= 4 ? 4 : 2, sink_tile = pieces ? kRowsBlock : kTile;
     a.row_tiles = (a.rows + kRowsBlock - 1) / kRowsBlock;
     a.key_tiles = (a.Sk + kRowsBlock - 1) / kRowsBlock;
-    constexpr bool pieces = NT <= 4;
     // The rows that see a key tile in parts where the tiles are few for the CUs.
     const int64_t near_tiles = std::max<int64_t>(1, std::min<int64_t>(a.rows, ((int64_t)a.window + kRowsBlock) * a.group) / kTile);
     a.row_splits = 1;
     if (pieces && a.key_tiles)
         a.row_splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({2 * (int64_t)cu_count / (heads * a.key_tiles), near_tiles / kPartTiles, 16}));
-    // Rows beyond a window see sinks alone.
-    a.sink_tiles = a.window < a.Sk ? (std::min(a.sinks, a.Sk) + kTile - 1) / kTile : 0;
+    // Rows beyond a window see sinks alone: in parts of about as many row tiles as the others,
+    // or that fill the device.
+    a.sink_tiles = a.window < a.Sk ? (std::min(a.sinks, a.Sk) + sink_tile - 1) / sink_tile : 0;
     a.sink_splits = 1;
     if (a.sink_tiles) {
-        // In parts that fill the device; a part's waves take whole groups of row tiles.
-        const int64_t groups = (a.rows / kTile + slots - 1) / slots;
-        a.sink_splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({64, groups, (pieces ? 1 : 2) * (int64_t)cu_count / (heads * a.sink_tiles)}));
+        const int64_t far_tiles = std::max<int64_t>(1, a.rows / kTile);
+        const int64_t want = pieces ? far_tiles * a.row_splits / near_tiles : 2 * (int64_t)cu_count / (heads * a.sink_tiles);
+        a.sink_splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({64, (far_tiles + slots - 1) / slots, want}));
     }
+    const int far = a.sink_tiles ? a.sink_splits * (pieces ? 1 : slots) : 0;
     const int64_t row_blocks = heads * a.row_tiles * (NT / NA);
     const int64_t key_blocks = heads * (a.sink_tiles * a.sink_splits + (int64_t)a.key_tiles * a.row_splits) * (NT / NA);
     const int64_t delta_blocks = ((int64_t)a.batch * a.heads * a.Sq + 15) / 16;
-    if (row_blocks >> 31 || key_blocks >> 31 || delta_blocks >> 31)
+    if ((row_blocks + key_blocks) >> 31 || delta_blocks >> 31)
         return set_error(TRS_E_INVALID_ARGUMENT, "attention gradient over too many blocks");
     const int64_t deltas = ((int64_t)a.batch * a.heads * a.Sq + 63) / 64 * 64;
-    const int64_t sink_floats = heads * a.sink_tiles * a.sink_splits * slots * kTile * a.D;
+    const int64_t sink_floats = heads * a.sink_tiles * far * sink_tile * a.D;
     const int64_t part_floats = a.row_splits > 1 ? heads * a.row_splits * a.Sk * a.D : 0;
     void *ws = nullptr;
     TRS_CHECK(trs_alloc((size_t)(deltas + 2 * sink_floats + 2 * part_floats) * sizeof(float), &ws));
@@ -352,15 +363,7 @@ int run(AttnArgs a, hipStream_t s, int cu_count) {
         if (delta_blocks) hipLaunchKernelGGL(attn_delta, dim3((unsigned)delta_blocks), dim3(256), 0, s, a, delta);
         TRS_LAUNCH_CHECK("attention gradient launch");
         if constexpr (pieces) {
-            if (a.key_tiles) launch_grad_keys(a, (unsigned)(heads * a.key_tiles * a.row_splits), s);
-            TRS_LAUNCH_CHECK("attention gradient launch");
-            if (a.sink_tiles) {
-                AttnArgs far = a;
-                far.key_tiles = 0;
-                hipLaunchKernelGGL((attn_grad_keys_fp32<NT, NA>), dim3((unsigned)(heads * a.sink_tiles * a.sink_splits)), dim3(256), 0, s, far);
-                TRS_LAUNCH_CHECK("attention gradient launch");
-            }
-            if (row_blocks) launch_grad_rows(a, (unsigned)row_blocks, s);
+            if (key_blocks + row_blocks) launch_attention_grad(a, (uint32_t)key_blocks, (uint32_t)row_blocks, s);
             TRS_LAUNCH_CHECK("attention gradient launch");
         } else {
             if (key_blocks) hipLaunchKernelGGL((attn_grad_keys_fp32<NT, NA>), dim3((unsigned)key_blocks), dim3(256), 0, s, a);
@@ -368,10 +371,10 @@ int run(AttnArgs a, hipStream_t s, int cu_count) {
             if (row_blocks) hipLaunchKernelGGL((attn_grad_rows_fp32<NT, NA>), dim3((unsigned)row_blocks), dim3(256), 0, s, a);
             TRS_LAUNCH_CHECK("attention gradient launch");
         }
-        const int count = a.row_splits > 1 ? a.Sk : std::min(a.sink_tiles * kTile, a.Sk);
+        const int count = a.row_splits > 1 ? a.Sk : a.sink_tiles ? std::min(a.sinks, a.Sk) : 0;
         if (count) {
             const int64_t n = heads * count * a.D;
-            hipLaunchKernelGGL(attn_reduce, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 1 << 20)), dim3(256), 0, s, a, count, slots);
+            hipLaunchKernelGGL(attn_reduce, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 1 << 20)), dim3(256), 0, s, a, count, sink_tile, far);
             TRS_LAUNCH_CHECK("attention gradient launch");
         }
         return TRS_OK;

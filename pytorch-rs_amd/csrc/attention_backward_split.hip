@@ -73,15 +73,14 @@ __device__ __forceinline__ void grad_rows_fp32(const AttnArgs &a, const RowBlock
     }
 }
 
-template <int NT, int NW, bool FULL>
-__global__ void __launch_bounds__(64 * NW, NT <= 2 ? 2 : 1) attn_grad_rows(AttnArgs a) {
+// A block of 128 rows over their key tiles.
+template <int NT, bool FULL>
+__device__ __forceinline__ void rows_block(const AttnArgs &a, uint32_t id, char *lds, Notices<4> &notices) {
+    constexpr int NW = 4;
     using T = Tile<NT, 64 * NW>;
-    constexpr int UNITS = 4 * NT, OWN = UNITS / NW;  // of keys and values; of a wave
+    constexpr int UNITS = 4 * NT, OWN = NT;  // of keys and values; of a wave
     constexpr int kBuffer = 3 * UNITS * 1024;
-    static_assert(UNITS % NW == 0 && 2 * kBuffer >= 8 * T::kFloats, "whole shares, and the fp32 tiles fit the pieces' LDS");
-    __shared__ __attribute__((aligned(1024))) char lds[2 * kBuffer];
-    __shared__ Notices<NW> notices;
-    const RowBlock<NW> r(a, blockIdx.x);
+    const RowBlock<NW> r(a, id);
     const float *kb = a.k + r.b * a.ks.b + r.hk * a.ks.h, *vb = a.v + r.b * a.vs.b + r.hk * a.vs.h;
     Unit<NT, FULL> in[OWN];
     const auto load = [&](int t) {  // past the last tile: that one
@@ -118,7 +117,9 @@ __global__ void __launch_bounds__(64 * NW, NT <= 2 ? 2 : 1) attn_grad_rows(AttnA
             const int j0 = r.first_key(t);
             char *const buf = lds + (t & 1) * kBuffer, *const other = lds + (t & 1 ? 0 : kBuffer);
             __syncthreads();
-            at_f16 s = (at_f16)(0.f), d = (at_f16)(0.f);
+            // dO V^T - delta, times 2^80: the sum starts from -delta.  (The scores' does not start
+            // from -lse: it is the larger part, and every product would be rounded to it.)
+            at_f16 s = (at_f16)(0.f), d = (at_f16)(-delta * kUp2);
             Splitting x;
             {
                 const auto read = [&](int n) { return along<UNITS>(buf, (n & 1) * 2 * NT + n / 2, r.lane); };
@@ -136,7 +137,7 @@ __global__ void __launch_bounds__(64 * NW, NT <= 2 ? 2 : 1) attn_grad_rows(AttnA
                 for (int e = 0; e < 16; e++) s[e] = sees(a, r.place, j0 + result_row(e, r.half)) ? s[e] : -__builtin_inff();
             }
             const auto weigh = [&](int e) {  // 2^40 dS
-                return __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], kDown2, -lse)) * __builtin_fmaf(d[e], kDown, -delta * kUp);
+                return __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], kDown2, -lse)) * (d[e] * kDown);
             };
             const auto read = [&](int n) { return across<UNITS>(buf, 2 * (n % NT), n / NT, r.lane); };
             Pieces f = read(0);
@@ -168,52 +169,58 @@ __global__ void __launch_bounds__(64 * NW, NT <= 2 ? 2 : 1) attn_grad_rows(AttnA
 // ---- dK and dV ------------------------------------------------------------------
 
 // What a block of 128 keys works on: its keys, 32 a wave, and the rows whose window
-// holds them.
+// holds them; or, of the first keys, the rows beyond it, which the sinks alone see.
 struct KeyBlock {
+    bool far;
     int lane, half, wave;
     int hk, b, head, key, keys;  // the lane's key; past the last key
     int j0, j1;                  // the wave's keys
-    int part;
+    int tile, part;
     int first;          // place of query 0
     int rlo, rhi;       // rows
     int t0, t1;         // row tiles of the part, from rlo on
     __device__ __forceinline__ KeyBlock(const AttnArgs &a, uint32_t id) {
         lane = (int)threadIdx.x & 63, half = lane >> 5;
         wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-        part = (int)(id % (uint32_t)a.row_splits);
-        id /= (uint32_t)a.row_splits;
-        const int tile = (int)(id % (uint32_t)a.key_tiles);
-        head = (int)(id / (uint32_t)a.key_tiles);
+        const uint32_t far_units = (uint32_t)(a.sink_tiles * a.sink_splits), units = far_units + (uint32_t)(a.key_tiles * a.row_splits);
+        head = (int)(id / units);
+        id -= (uint32_t)head * units;
+        far = id < far_units;
+        const int parts = far ? a.sink_splits : a.row_splits;
+        if (!far) id -= far_units;
+        tile = (int)(id / (uint32_t)parts), part = (int)(id % (uint32_t)parts);
         hk = head % a.kv_heads, b = head / a.kv_heads;
         const Sequence seq = sequence_of(a, b);
-        first = seq.first, keys = seq.keys;
+        first = seq.first, keys = far ? min(a.sinks, seq.keys) : seq.keys;
         const int block_j0 = tile * kRowsBlock, block_j1 = min(block_j0 + kRowsBlock, keys);
         j0 = block_j0 + wave * 32, j1 = min(j0 + 32, keys);
         key = j0 + (lane & 31);
-        const int place_lo = max(block_j0, max(first, 0)), place_hi = min(keys - 1, block_j1 - 1 + a.window - 1);
+        const int place_lo = max(far ? block_j0 + a.window : block_j0, max(first, 0));
+        const int place_hi = far ? seq.keys - 1 : min(seq.keys - 1, block_j1 - 1 + a.window - 1);
         rlo = rhi = 0;
         int tiles = 0;
         if (block_j0 < block_j1 && place_lo <= place_hi) {
             rlo = (place_lo - first) * a.group, rhi = (place_hi - first + 1) * a.group;
             tiles = (rhi - rlo + kTile - 1) / kTile;
         }
-        t0 = (int)((int64_t)tiles * part / a.row_splits), t1 = (int)((int64_t)tiles * (part + 1) / a.row_splits);
+        t0 = (int)((int64_t)tiles * part / parts), t1 = (int)((int64_t)tiles * (part + 1) / parts);
     }
-    // Whether every key of the wave is in the window of every row of tile t.
+    // Whether every key of the wave makes a pair with every row of tile t.
     __device__ __forceinline__ bool all(const AttnArgs &a, int t) const {
         const int r0 = rlo + t * kTile, r1 = min(r0 + kTile, rhi);
         const int lo = first + (int)a.by_group.divide((uint32_t)r0), hi = first + (int)a.by_group.divide((uint32_t)(r1 - 1));
-        return r1 - r0 == kTile && j1 - j0 == 32 && j1 - 1 <= lo && hi - j0 < a.window;
+        return r1 - r0 == kTile && j1 - j0 == 32 && (far ? lo - (j1 - 1) >= a.window : j1 - 1 <= lo && hi - j0 < a.window);
     }
     __device__ __forceinline__ bool pair(const AttnArgs &a, int place) const {
-        return (key < keys) & (key <= place) & (place - key < a.window);
+        return (key < keys) & (key <= place) & ((place - key < a.window) != far);
     }
 };
 
 // A tile's rows, as the waves of a block share them; two tiles in turn.
 struct RowFacts {
-    float lse[2][kTile], delta[2][kTile];  // lse in base 2
-    int place[2][kTile];                   // -1: past the last row
+    float lse[2][kTile];    // in base 2
+    float delta[2][kTile];  // -2^80 delta, what the sum of dO V^T starts from
+    int place[2][kTile];    // -1: past the last row
 };
 
 template <int NT>
@@ -269,15 +276,12 @@ __device__ __forceinline__ void grad_keys_fp32(const AttnArgs &a, const KeyBlock
     }
 }
 
+// A block of 128 keys over the row tiles that make pairs with them.
 template <int NT, bool FULL>
-__global__ void __launch_bounds__(256, NT <= 2 ? 2 : 1) attn_grad_keys(AttnArgs a) {
+__device__ __forceinline__ void keys_block(const AttnArgs &a, uint32_t id, char *lds, RowFacts &facts, Notices<4> &notices) {
     using T = Tile<NT, 256>;
     constexpr int UNITS = 4 * NT, kBuffer = 3 * UNITS * 1024;  // of queries and upstream rows
-    static_assert(2 * kBuffer >= 8 * T::kFloats, "the fp32 tiles fit the pieces' LDS");
-    __shared__ __attribute__((aligned(1024))) char lds[2 * kBuffer];
-    __shared__ RowFacts facts;
-    __shared__ Notices<4> notices;
-    const KeyBlock k(a, blockIdx.x);
+    const KeyBlock k(a, id);
     const float *qb = a.q + k.b * a.qs.b + (int64_t)k.hk * a.group * a.qs.h, *ub = a.up + k.b * a.us.b + (int64_t)k.hk * a.group * a.us.h;
 
     // A lane's row of a tile, and what the waves share of it.  Past the part's last tile
@@ -299,7 +303,7 @@ __global__ void __launch_bounds__(256, NT <= 2 ? 2 : 1) attn_grad_keys(AttnArgs 
         place = at < k.rhi ? k.first + i : -1;
     };
     const auto store_facts = [&](int n) {
-        if (threadIdx.x < kTile) facts.lse[n][threadIdx.x] = lse * kLog2e, facts.delta[n][threadIdx.x] = delta, facts.place[n][threadIdx.x] = place;
+        if (threadIdx.x < kTile) facts.lse[n][threadIdx.x] = lse * kLog2e, facts.delta[n][threadIdx.x] = delta * -kUp2, facts.place[n][threadIdx.x] = place;
     };
     at_f16 dk[NT], dv[NT];
 #pragma unroll
@@ -327,7 +331,9 @@ __global__ void __launch_bounds__(256, NT <= 2 ? 2 : 1) attn_grad_keys(AttnArgs 
             const int n2 = (t - k.t0) & 1;
             char *const buf = lds + n2 * kBuffer, *const other = lds + (n2 ? 0 : kBuffer);
             __syncthreads();
-            at_f16 p = (at_f16)(0.f), d = (at_f16)(0.f);
+            at_f16 p, d;
+#pragma unroll
+            for (int e = 0; e < 16; e++) p[e] = 0.f, d[e] = facts.delta[n2][result_row(e, k.half)];
             Splitting x, w;
             {
                 const auto read = [&](int n) { return along<UNITS>(buf, (n & 1) * 2 * NT + n / 2, k.lane); };
@@ -336,15 +342,17 @@ __global__ void __launch_bounds__(256, NT <= 2 ? 2 : 1) attn_grad_keys(AttnArgs 
                     f, read, [&](int n, const Pieces &now) { mfma_pieces(n & 1 ? d : p, now, n & 1 ? vp[n / 2] : kp[n / 2]); },
                     [&](int n) { in[n / 4].template store_pair<UNITS>(x, n % 4, other, k.wave + n / 4 * 4, k.lane); }, [](Pieces &) {});
             }
+            at_f16 lse16;
+#pragma unroll
+            for (int e = 0; e < 16; e++) lse16[e] = facts.lse[n2][result_row(e, k.half)];
             store_facts(n2 ^ 1);
-            load(t + 2);
             if (!k.all(a, t)) {
 #pragma unroll
                 for (int e = 0; e < 16; e++) p[e] = k.pair(a, facts.place[n2][result_row(e, k.half)]) ? p[e] : -__builtin_inff();
             }
             // 2^40 P and 2^40 dS come pair by pair, each eight of them ahead of the products that take them.
-            const auto pair_p = [&](int e) { return p[e] = up_exp2(__builtin_fmaf(p[e], kDown2, -facts.lse[n2][result_row(e, k.half)])); };
-            const auto pair_d = [&](int e) { return p[e] * __builtin_fmaf(d[e], kDown2, -facts.delta[n2][result_row(e, k.half)]); };
+            const auto pair_p = [&](int e) { return p[e] = up_exp2(__builtin_fmaf(p[e], kDown2, -lse16[e])); };
+            const auto pair_d = [&](int e) { return p[e] * (d[e] * kDown2); };
             // dV's first 16 rows, its others, dK's first, its others.
             const auto read = [&](int n) { return across<UNITS>(buf, (n < 2 * NT ? 2 * NT : 0) + 2 * (n % NT), n / NT % 2, k.lane); };
             Pieces f = read(0);
@@ -370,6 +378,8 @@ __global__ void __launch_bounds__(256, NT <= 2 ? 2 : 1) attn_grad_keys(AttnArgs 
                         if (g < 3) y = read((g + 1) * NT);
                     });
                 if (g < 3) weights = w.done();
+                // Late, for few registers at a time: the first is wanted in the next tile's first step.
+                if (g == 2) load(t + 2);
             }
         }
         __syncthreads();
@@ -381,9 +391,12 @@ __global__ void __launch_bounds__(256, NT <= 2 ? 2 : 1) attn_grad_keys(AttnArgs 
             grad_keys_fp32<NT>(a, k, (float *)lds, facts, notices, dk, dv);
         }
     }
-    if (k.key >= a.Sk) return;
+    if (k.key >= (k.far ? a.sinks : a.Sk)) return;
     float *pk, *pv;
-    if (a.row_splits > 1) {
+    if (k.far) {
+        const int64_t at = (((int64_t)k.head * a.sink_tiles + k.tile) * a.sink_splits + k.part) * kRowsBlock + k.key % kRowsBlock;
+        pk = a.sink_k + at * a.D, pv = a.sink_v + at * a.D;
+    } else if (a.row_splits > 1) {
         const int64_t at = ((int64_t)k.part * a.batch * a.kv_heads + k.head) * a.Sk + k.key;
         pk = a.part_k + at * a.D, pv = a.part_v + at * a.D;
     } else {
@@ -399,31 +412,34 @@ __global__ void __launch_bounds__(256, NT <= 2 ? 2 : 1) attn_grad_keys(AttnArgs 
     }
 }
 
-template <int NT>
-void launch_rows(const AttnArgs &a, unsigned blocks, hipStream_t s) {
-    if (a.D == 32 * NT) hipLaunchKernelGGL((attn_grad_rows<NT, 4, true>), dim3(blocks), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((attn_grad_rows<NT, 4, false>), dim3(blocks), dim3(256), 0, s, a);
+// Both kinds of block in one launch, so that neither waits for the other's last: those
+// of the keys first, whose tiles take longer.
+template <int NT, bool FULL>
+__global__ void __launch_bounds__(256, NT <= 2 ? 2 : 1) attn_grad(AttnArgs a, uint32_t key_blocks) {
+    using T = Tile<NT, 256>;
+    constexpr int kBytes = 2 * 3 * 4 * NT * 1024;
+    static_assert(kBytes >= 8 * T::kFloats, "the fp32 tiles fit the pieces' LDS");
+    __shared__ __attribute__((aligned(1024))) char lds[kBytes];
+    __shared__ RowFacts facts;
+    __shared__ Notices<4> notices;
+    if (blockIdx.x < key_blocks) keys_block<NT, FULL>(a, blockIdx.x, lds, facts, notices);
+    else rows_block<NT, FULL>(a, blockIdx.x - key_blocks, lds, notices);
 }
+
 template <int NT>
-void launch_keys(const AttnArgs &a, unsigned blocks, hipStream_t s) {
-    if (a.D == 32 * NT) hipLaunchKernelGGL((attn_grad_keys<NT, true>), dim3(blocks), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((attn_grad_keys<NT, false>), dim3(blocks), dim3(256), 0, s, a);
+void launch(const AttnArgs &a, uint32_t key_blocks, uint32_t row_blocks, hipStream_t s) {
+    const dim3 grid(key_blocks + row_blocks);
+    if (a.D == 32 * NT) hipLaunchKernelGGL((attn_grad<NT, true>), grid, dim3(256), 0, s, a, key_blocks);
+    else hipLaunchKernelGGL((attn_grad<NT, false>), grid, dim3(256), 0, s, a, key_blocks);
 }
 
 }  // namespace
 
-void launch_grad_rows(const AttnArgs &a, unsigned blocks, hipStream_t s) {
-    if (a.D <= 32) launch_rows<1>(a, blocks, s);
-    else if (a.D <= 64) launch_rows<2>(a, blocks, s);
-    else if (a.D <= 96) launch_rows<3>(a, blocks, s);
-    else launch_rows<4>(a, blocks, s);
-}
-
-void launch_grad_keys(const AttnArgs &a, unsigned blocks, hipStream_t s) {
-    if (a.D <= 32) launch_keys<1>(a, blocks, s);
-    else if (a.D <= 64) launch_keys<2>(a, blocks, s);
-    else if (a.D <= 96) launch_keys<3>(a, blocks, s);
-    else launch_keys<4>(a, blocks, s);
+void launch_attention_grad(const AttnArgs &a, uint32_t key_blocks, uint32_t row_blocks, hipStream_t s) {
+    if (a.D <= 32) launch<1>(a, key_blocks, row_blocks, s);
+    else if (a.D <= 64) launch<2>(a, key_blocks, row_blocks, s);
+    else if (a.D <= 96) launch<3>(a, key_blocks, row_blocks, s);
+    else launch<4>(a, key_blocks, row_blocks, s);
 }
 
 }  // namespace trs
