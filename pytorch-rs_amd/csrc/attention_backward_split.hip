@@ -28,14 +28,14 @@ __device__ __forceinline__ float up_exp2(float x) {
     return __builtin_amdgcn_exp2f(x + (low ? 64.f : 0.f)) * (low ? 0x1p-24f : kUp);
 }
 
-template <int NT, bool FULL>
+template <int NT, int WIDTH>
 __device__ __forceinline__ void write_across(const at_f16 (&acc)[NT], float *p, float f, int D, int half) {
 #pragma unroll
     for (int c = 0; c < NT; c++)
 #pragma unroll
         for (int e = 0; e < 16; e++) {
             const int d = across_column(c, e, half);
-            if (FULL || d < D) p[d] = acc[c][e] * kDown2 * f;
+            if (WIDTH == 4 || d < D) p[d] = acc[c][e] * kDown2 * f;
         }
 }
 
@@ -74,7 +74,7 @@ __device__ __forceinline__ void grad_rows_fp32(const AttnArgs &a, const RowBlock
 }
 
 // A block of 128 rows over their key tiles.
-template <int NT, bool FULL>
+template <int NT, int WIDTH>
 __device__ __forceinline__ void rows_block(const AttnArgs &a, uint32_t id, char *lds, Notices<4> &notices) {
     constexpr int NW = 4;
     using T = Tile<NT, 64 * NW>;
@@ -82,7 +82,7 @@ __device__ __forceinline__ void rows_block(const AttnArgs &a, uint32_t id, char 
     constexpr int kBuffer = 3 * UNITS * 1024;
     const RowBlock<NW> r(a, id);
     const float *kb = a.k + r.b * a.ks.b + r.hk * a.ks.h, *vb = a.v + r.b * a.vs.b + r.hk * a.vs.h;
-    Unit<NT, FULL> in[OWN];
+    Unit<WIDTH> in[OWN];
     const auto load = [&](int t) {  // past the last tile: that one
         const int j = min(r.first_key(min(t, r.tiles - 1)) + (r.lane & 31), r.key_hi);
         const float *kp = kb + (int64_t)j * a.ks.s, *vp = vb + (int64_t)j * a.vs.s;
@@ -103,7 +103,7 @@ __device__ __forceinline__ void rows_block(const AttnArgs &a, uint32_t id, char 
         Pieces qp[2 * NT], up[2 * NT];
 #pragma unroll
         for (int s = 0; s < 2 * NT; s++) {
-            Unit<NT, FULL> x;
+            Unit<WIDTH> x;
             x.load(a.q + r.at(a, a.qs), s, a.D, r.lane);
             qp[s] = x.split(live ? a.scale2 * kUp : 0.f);
             x.load(a.up + r.at(a, a.us), s, a.D, r.lane);
@@ -163,7 +163,7 @@ __device__ __forceinline__ void rows_block(const AttnArgs &a, uint32_t id, char 
             return;
         }
     }
-    if (r.row < a.rows) write_across<NT, FULL>(acc, a.dq + r.at(a, a.dqs), a.scale, a.D, r.half);
+    if (r.row < a.rows) write_across<NT, WIDTH>(acc, a.dq + r.at(a, a.dqs), a.scale, a.D, r.half);
 }
 
 // ---- dK and dV ------------------------------------------------------------------
@@ -277,7 +277,7 @@ __device__ __forceinline__ void grad_keys_fp32(const AttnArgs &a, const KeyBlock
 }
 
 // A block of 128 keys over the row tiles that make pairs with them.
-template <int NT, bool FULL>
+template <int NT, int WIDTH>
 __device__ __forceinline__ void keys_block(const AttnArgs &a, uint32_t id, char *lds, RowFacts &facts, Notices<4> &notices) {
     using T = Tile<NT, 256>;
     constexpr int UNITS = 4 * NT, kBuffer = 3 * UNITS * 1024;  // of queries and upstream rows
@@ -286,7 +286,7 @@ __device__ __forceinline__ void keys_block(const AttnArgs &a, uint32_t id, char 
 
     // A lane's row of a tile, and what the waves share of it.  Past the part's last tile
     // that one is loaded, past the last row that one.
-    Unit<NT, FULL> in[NT];
+    Unit<WIDTH> in[NT];
     float lse = 0.f, delta = 0.f;
     int place = -1;
     const auto load = [&](int t) {
@@ -316,7 +316,7 @@ __device__ __forceinline__ void keys_block(const AttnArgs &a, uint32_t id, char 
         Pieces kp[2 * NT], vp[2 * NT];
 #pragma unroll
         for (int s = 0; s < 2 * NT; s++) {
-            Unit<NT, FULL> x;
+            Unit<WIDTH> x;
             x.load(a.k + k.b * a.ks.b + k.hk * a.ks.h + (int64_t)key * a.ks.s, s, a.D, k.lane);
             kp[s] = x.split(live ? a.scale2 * kUp : 0.f);
             x.load(a.v + k.b * a.vs.b + k.hk * a.vs.h + (int64_t)key * a.vs.s, s, a.D, k.lane);
@@ -407,14 +407,14 @@ __device__ __forceinline__ void keys_block(const AttnArgs &a, uint32_t id, char 
         T::write(dk, 0, pk, a.scale, a.D, k.half);
         T::write(dv, 0, pv, 1.f, a.D, k.half);
     } else {
-        write_across<NT, FULL>(dk, pk, a.scale, a.D, k.half);
-        write_across<NT, FULL>(dv, pv, 1.f, a.D, k.half);
+        write_across<NT, WIDTH>(dk, pk, a.scale, a.D, k.half);
+        write_across<NT, WIDTH>(dv, pv, 1.f, a.D, k.half);
     }
 }
 
 // Both kinds of block in one launch, so that neither waits for the other's last: those
 // of the keys first, whose tiles take longer.
-template <int NT, bool FULL>
+template <int NT, int WIDTH>
 __global__ void __launch_bounds__(256, NT <= 2 ? 2 : 1) attn_grad(AttnArgs a, uint32_t key_blocks) {
     using T = Tile<NT, 256>;
     constexpr int kBytes = 2 * 3 * 4 * NT * 1024;
@@ -422,15 +422,16 @@ __global__ void __launch_bounds__(256, NT <= 2 ? 2 : 1) attn_grad(AttnArgs a, ui
     __shared__ __attribute__((aligned(1024))) char lds[kBytes];
     __shared__ RowFacts facts;
     __shared__ Notices<4> notices;
-    if (blockIdx.x < key_blocks) keys_block<NT, FULL>(a, blockIdx.x, lds, facts, notices);
-    else rows_block<NT, FULL>(a, blockIdx.x - key_blocks, lds, notices);
+    if (blockIdx.x < key_blocks) keys_block<NT, WIDTH>(a, blockIdx.x, lds, facts, notices);
+    else rows_block<NT, WIDTH>(a, blockIdx.x - key_blocks, lds, notices);
 }
 
 template <int NT>
 void launch(const AttnArgs &a, uint32_t key_blocks, uint32_t row_blocks, hipStream_t s) {
     const dim3 grid(key_blocks + row_blocks);
-    if (a.D == 32 * NT) hipLaunchKernelGGL((attn_grad<NT, true>), grid, dim3(256), 0, s, a, key_blocks);
-    else hipLaunchKernelGGL((attn_grad<NT, false>), grid, dim3(256), 0, s, a, key_blocks);
+    if (a.D == 32 * NT) hipLaunchKernelGGL((attn_grad<NT, 4>), grid, dim3(256), 0, s, a, key_blocks);
+    else if (a.D % 4 == 0) hipLaunchKernelGGL((attn_grad<NT, 2>), grid, dim3(256), 0, s, a, key_blocks);
+    else hipLaunchKernelGGL((attn_grad<NT, 1>), grid, dim3(256), 0, s, a, key_blocks);
 }
 
 }  // namespace

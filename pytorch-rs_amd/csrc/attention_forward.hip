@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(64 * NW, 1) attn_rows_fp32(AttnArgs a) {
 // The same on the bf16 matrix cores, in pieces: the block splits a key tile once for
 // its waves, into one of two LDS buffers while it computes from the other; the loads from
 // memory are a tile further ahead.
-template <int NT, int NW, bool FULL>
+template <int NT, int NW, int WIDTH>
 __global__ void __launch_bounds__(64 * NW, 2) attn_rows(AttnArgs a) {
     using T = Tile<NT, 64 * NW>;
     constexpr int UNITS = 4 * NT, OWN = (UNITS + NW - 1) / NW;  // of keys and values; of a wave (some twice)
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_rows(AttnArgs a) {
     const RowBlock<NW> r(a, blockIdx.x / (uint32_t)a.splits);
     const int t0 = (int)((int64_t)r.tiles * part / a.splits), t1 = (int)((int64_t)r.tiles * (part + 1) / a.splits);
     const float *kb = a.k + r.b * a.ks.b + r.hk * a.ks.h, *vb = a.v + r.b * a.vs.b + r.hk * a.vs.h;
-    Unit<NT, FULL> in[OWN];
+    Unit<WIDTH> in[OWN];
     const auto unit = [&](int q) { return min(r.wave + q * NW, UNITS - 1); };
     const auto load = [&](int t) {  // past the part's last tile: that one
         const int j = min(r.first_key(min(t, t1 - 1)) + (r.lane & 31), r.key_hi);
@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_rows(AttnArgs a) {
         Pieces q[2 * NT];
 #pragma unroll
         for (int s = 0; s < 2 * NT; s++) {
-            Unit<NT, FULL> x;
+            Unit<WIDTH> x;
             x.load(a.q + r.at(a, a.qs), s, a.D, r.lane);
             q[s] = x.split(r.place >= 0 ? a.scale2 * kUp : 0.f);
         }
@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_rows(AttnArgs a) {
 #pragma unroll
             for (int e = 0; e < 16; e++) {
                 const int d = across_column(c, e, r.half);
-                if (FULL || d < a.D) p[d] = state.acc[c][e] * f;
+                if (WIDTH == 4 || d < a.D) p[d] = state.acc[c][e] * f;
             }
     });
 }
@@ -281,8 +281,9 @@ __global__ void __launch_bounds__(256) attn_join(AttnArgs a) {
 
 template <int NT>
 void launch_rows(const AttnArgs &a, dim3 grid, hipStream_t s) {
-    if (a.D == 32 * NT) hipLaunchKernelGGL((attn_rows<NT, 8, true>), grid, dim3(512), 0, s, a);
-    else hipLaunchKernelGGL((attn_rows<NT, 8, false>), grid, dim3(512), 0, s, a);
+    if (a.D == 32 * NT) hipLaunchKernelGGL((attn_rows<NT, 8, 4>), grid, dim3(512), 0, s, a);
+    else if (a.D % 4 == 0) hipLaunchKernelGGL((attn_rows<NT, 8, 2>), grid, dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((attn_rows<NT, 8, 1>), grid, dim3(512), 0, s, a);
 }
 
 }  // namespace
