@@ -359,8 +359,25 @@ __device__ __forceinline__ void dealt(int items, int s, int of, F &&item) {
 #pragma unroll
     for (int i = s * items / of; i < (s + 1) * items / of; i++) item(i);
 }
-// The result's column that register r of result tile t holds.
-__device__ __forceinline__ int across_column(int t, int r, int half) { return 32 * t + result_row(r, half); }
+// Writes unit * f * acc^T: the lane's column of acc is the row at p.  Registers 4 i to 4 i + 3 are
+// consecutive columns, 16 bytes; two halves of a wave write 32 of a row.
+template <int WIDTH, int NT>
+__device__ __forceinline__ void write_row(const at_f16 (&acc)[NT], float *p, float unit, float f, int D, int half) {
+#pragma unroll
+    for (int c = 0; c < NT; c++)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int d = 32 * c + result_row(e, half);
+            const f4u x = {acc[c][e] * unit * f, acc[c][e + 1] * unit * f, acc[c][e + 2] * unit * f, acc[c][e + 3] * unit * f};
+            if (WIDTH == 4 || (WIDTH == 2 && d < D)) {
+                *(f4u *)(p + d) = x;
+            } else if (WIDTH == 1) {
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+                    if (d + q < D) p[d + q] = x[q];
+            }
+        }
+}
 
 // Whether a value is an infinity or NaN in any lane of the wave.
 template <int N>

@@ -20,7 +20,9 @@ namespace trs {
 
 namespace {
 
-constexpr int kPartTiles = 8;  // the least row tiles of a part
+// The least row tiles of a part: 333 tokens, 4 heads of 32 57.8 us with 8, 34.5 with 4, 33.2 with 2
+// (2 x 2048 tokens, whose parts are longer, alike).
+constexpr int kPartTiles = 2;
 
 // delta of every row: 16 lanes a row.
 __global__ void __launch_bounds__(256) attn_delta(AttnArgs a, float *delta) {

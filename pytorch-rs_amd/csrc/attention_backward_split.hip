@@ -28,17 +28,6 @@ __device__ __forceinline__ float up_exp2(float x) {
     return __builtin_amdgcn_exp2f(x + (low ? 64.f : 0.f)) * (low ? 0x1p-24f : kUp);
 }
 
-template <int NT, int WIDTH>
-__device__ __forceinline__ void write_across(const at_f16 (&acc)[NT], float *p, float f, int D, int half) {
-#pragma unroll
-    for (int c = 0; c < NT; c++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const int d = across_column(c, e, half);
-            if (WIDTH == 4 || d < D) p[d] = acc[c][e] * kDown2 * f;
-        }
-}
-
 // ---- dQ -----------------------------------------------------------------------
 
 // The block's rows on the fp32 instruction, whatever the values.
@@ -163,7 +152,7 @@ __device__ __forceinline__ void rows_block(const AttnArgs &a, uint32_t id, char 
             return;
         }
     }
-    if (r.row < a.rows) write_across<NT, WIDTH>(acc, a.dq + r.at(a, a.dqs), a.scale, a.D, r.half);
+    if (r.row < a.rows) write_row<WIDTH>(acc, a.dq + r.at(a, a.dqs), kDown2, a.scale, a.D, r.half);
 }
 
 // ---- dK and dV ------------------------------------------------------------------
@@ -407,8 +396,8 @@ __device__ __forceinline__ void keys_block(const AttnArgs &a, uint32_t id, char 
         T::write(dk, 0, pk, a.scale, a.D, k.half);
         T::write(dv, 0, pv, 1.f, a.D, k.half);
     } else {
-        write_across<NT, WIDTH>(dk, pk, a.scale, a.D, k.half);
-        write_across<NT, WIDTH>(dv, pv, 1.f, a.D, k.half);
+        write_row<WIDTH>(dk, pk, kDown2, a.scale, a.D, k.half);
+        write_row<WIDTH>(dv, pv, kDown2, 1.f, a.D, k.half);
     }
 }
 

@@ -106,21 +106,20 @@ __device__ __forceinline__ void rows_fp32(const AttnArgs &a, const RowBlock<NW> 
     }
 }
 
-// The rows' outputs, or the part's.  `unit`: of the maximum; `up`: acc is that many
-// times the output's.
-template <int NT, int NW, class Column>
+// The rows' outputs, or the part's, through write(row, factor).  `unit`: of the maximum.
+template <int NT, int NW, class Write>
 __device__ __forceinline__ void write_rows(const AttnArgs &a, const RowBlock<NW> &r, int part, RowState<NT> &state, float unit,
-                                           float down, Column &&write) {
+                                           Write &&write) {
     const float sum = state.sum + __shfl_xor(state.sum, 32), most = state.most * unit;
     if (r.row >= a.rows) return;
     if (a.splits > 1) {
         const int64_t at = (((int64_t)part * a.batch + r.b) * a.kv_heads + r.hk) * a.rows + r.row;
-        write(a.part_o + at * a.part_width, down);
+        write(a.part_o + at * a.part_width, 1.f);
         if (r.half == 0) a.part_ml[2 * at] = most, a.part_ml[2 * at + 1] = sum;
         return;
     }
     // A row that sees nothing gives 0 and a logarithm of -inf.
-    write(a.out + r.at(a, a.os), sum == 0.f ? 0.f : down / sum);
+    write(a.out + r.at(a, a.os), sum == 0.f ? 0.f : 1.f / sum);
     if (a.lse && r.half == 0) a.lse[r.index(a)] = (most + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
@@ -133,7 +132,7 @@ __global__ void __launch_bounds__(64 * NW, 1) attn_rows_fp32(AttnArgs a) {
     const RowBlock<NW> r(a, blockIdx.x / (uint32_t)a.splits);
     RowState<NT> state;
     rows_fp32<NT, NW, true>(a, r, (int)((int64_t)r.tiles * part / a.splits), (int)((int64_t)r.tiles * (part + 1) / a.splits), lds, notices, state);
-    write_rows(a, r, part, state, 1.f, 1.f, [&](float *p, float f) { T::write(state.acc, 0, p, f, a.D, r.half); });
+    write_rows(a, r, part, state, 1.f, [&](float *p, float f) { T::write(state.acc, 0, p, f, a.D, r.half); });
 }
 
 // The same on the bf16 matrix cores, in pieces: the block splits a key tile once for
@@ -221,19 +220,11 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_rows(AttnArgs a) {
         if (__builtin_expect(notices.any(0), 0)) {
             __syncthreads();
             rows_fp32<NT, NW, false>(a, r, t0, t1, (float *)lds, notices, state);
-            write_rows(a, r, part, state, 1.f, 1.f, [&](float *p, float f) { T::write(state.acc, 0, p, f, a.D, r.half); });
+            write_rows(a, r, part, state, 1.f, [&](float *p, float f) { T::write(state.acc, 0, p, f, a.D, r.half); });
             return;
         }
     }
-    write_rows(a, r, part, state, kDown2, kDown, [&](float *p, float f) {
-#pragma unroll
-        for (int c = 0; c < NT; c++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int d = across_column(c, e, r.half);
-                if (WIDTH == 4 || d < a.D) p[d] = state.acc[c][e] * f;
-            }
-    });
+    write_rows(a, r, part, state, kDown2, [&](float *p, float f) { write_row<WIDTH>(state.acc, p, kDown, f, a.D, r.half); });
 }
 
 // The parts of a row, joined: four columns a lane.  Every part is read before the
