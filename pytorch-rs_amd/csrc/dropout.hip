@@ -52,48 +52,40 @@ __device__ __forceinline__ float kept(float x, uint32_t word, const DropoutArgs 
     return a.any && word >= a.least ? x * a.scale : 0.f;
 }
 
-constexpr int kGroups = 4;  // groups of four elements per lane
+// Blocks of one wave, a group of four a lane, in one go over the tensor: the DRAM pages in
+// use stay few.  Forward and gradient of 8192 x 4096 83.2 us (6.5 TB/s; a copy's rate is 6.7),
+// 87.0 with blocks of 256 lanes, 94.5 with four groups a lane and through the caches.  The
+// words cost about 150 instructions a group, under the loads' latency.
+constexpr int kGroupLanes = 64;
 
 // Unit strides along the last dim, whose length is a multiple of four unless it
 // is the only one: a lane's four elements share a generator block and are 16
 // bytes of a row.
 template <bool FLAT>
-__global__ void __launch_bounds__(256) dropout_groups(DropoutArgs a) {
+__global__ void __launch_bounds__(kGroupLanes) dropout_groups(DropoutArgs a) {
     const int64_t groups = (a.n + 3) / 4;
-    const int64_t step = (int64_t)gridDim.x * 256 * kGroups;
-    for (int64_t g0 = (int64_t)blockIdx.x * 256 * kGroups + threadIdx.x; g0 < groups; g0 += step) {
-        int64_t xo[kGroups], yo[kGroups];
-        f4u v[kGroups];
-#pragma unroll
-        for (int u = 0; u < kGroups; u++) {
-            const int64_t g = g0 + u * 256;
-            if (g >= groups) break;
-            int64_t i = g * 4;
-            xo[u] = yo[u] = i;
-            if constexpr (!FLAT) {
-                xo[u] = yo[u] = 0;
-                for (int d = 0; d < a.rank; d++) {
-                    const int64_t at = (a.n >> 32) ? i / a.ls[d] : (int64_t)((uint32_t)i / (uint32_t)a.ls[d]);
-                    i -= at * a.ls[d];
-                    xo[u] += at * a.xs[d], yo[u] += at * a.ys[d];
-                }
+    for (int64_t g = (int64_t)blockIdx.x * kGroupLanes + threadIdx.x; g < groups; g += (int64_t)gridDim.x * kGroupLanes) {
+        int64_t i = g * 4, xo = i, yo = i;
+        if constexpr (!FLAT) {
+            xo = yo = 0;
+            for (int d = 0; d < a.rank; d++) {
+                const int64_t at = (a.n >> 32) ? i / a.ls[d] : (int64_t)((uint32_t)i / (uint32_t)a.ls[d]);
+                i -= at * a.ls[d];
+                xo += at * a.xs[d], yo += at * a.ys[d];
             }
-            if (g * 4 + 4 <= a.n) v[u] = *(const f4u *)(a.x + xo[u]);
-            else
-                for (int e = 0; e < 4; e++) v[u][e] = g * 4 + e < a.n ? a.x[xo[u] + e] : 0.f;
         }
+        const bool whole = g * 4 + 4 <= a.n;
+        f4u v;
+        if (whole) v = __builtin_nontemporal_load((const f4u *)(a.x + xo));
+        else
+            for (int e = 0; e < 4; e++) v[e] = g * 4 + e < a.n ? a.x[xo + e] : 0.f;
+        const Words w = philox(a.offset + (uint64_t)g, a.seed);
 #pragma unroll
-        for (int u = 0; u < kGroups; u++) {
-            const int64_t g = g0 + u * 256;
-            if (g >= groups) break;
-            const Words w = philox(a.offset + (uint64_t)g, a.seed);
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[u][e] = kept(v[u][e], w.w[e], a);
-            if (g * 4 + 4 <= a.n) *(f4u *)(a.y + yo[u]) = v[u];
-            else
-                for (int e = 0; e < 4; e++)
-                    if (g * 4 + e < a.n) a.y[yo[u] + e] = v[u][e];
-        }
+        for (int e = 0; e < 4; e++) v[e] = kept(v[e], w.w[e], a);
+        if (whole) __builtin_nontemporal_store(v, (f4u *)(a.y + yo));
+        else
+            for (int e = 0; e < 4; e++)
+                if (g * 4 + e < a.n) a.y[yo + e] = v[e];
     }
 }
 
@@ -164,10 +156,10 @@ int run_dropout(const float *x, const trs_layout *lx, double p, uint64_t seed, u
         const int d = r - 1 - i;
         a.size[d] = size[order[i]], a.xs[d] = xs[order[i]], a.ys[d] = ys[order[i]], a.ls[d] = ls[order[i]];
     }
-    const int64_t lanes = groups ? (a.n + 3) / 4 : a.n, block = groups ? 256 * kGroups : 256;
+    const int64_t lanes = groups ? (a.n + 3) / 4 : a.n, block = groups ? kGroupLanes : 256;
     const dim3 grid((unsigned)std::min<int64_t>((lanes + block - 1) / block, 1 << 22));
-    if (groups && r == 1) hipLaunchKernelGGL(dropout_groups<true>, grid, dim3(256), 0, dev->stream, a);
-    else if (groups) hipLaunchKernelGGL(dropout_groups<false>, grid, dim3(256), 0, dev->stream, a);
+    if (groups && r == 1) hipLaunchKernelGGL(dropout_groups<true>, grid, dim3(kGroupLanes), 0, dev->stream, a);
+    else if (groups) hipLaunchKernelGGL(dropout_groups<false>, grid, dim3(kGroupLanes), 0, dev->stream, a);
     else hipLaunchKernelGGL(dropout_elements, grid, dim3(256), 0, dev->stream, a);
     TRS_LAUNCH_CHECK("dropout launch");
     return TRS_OK;
