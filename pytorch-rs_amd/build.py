@@ -42,11 +42,11 @@ HIP_FLAGS = [
 HIP_SOURCES = ["pw_binary.hip", "pw_binary_muldiv.hip", "pw_scalar.hip", "pw_unary.hip", "pw_mask.hip",
                "pointwise.hip", "runtime.hip", "transfer.hip", "gemm.hip", "gemm_skinny.hip", "fusion.hip",
                "dropout.hip", "head_norm.hip", "attention.hip", "attention_forward.hip", "attention_few.hip", "attention_backward.hip",
-               "attention_backward_split.hip"]
+               "attention_backward_split.hip", "attention_backward_wide.hip"]
 # Flags of one source.  The attention gradients hold over 256 registers a lane: with the matrix
 # results in the vector registers, and not the accumulation ones, nothing spills (47 registers did
 # at a head dim of 128, 1.72 ms where the kernel now takes 1.29).
-SOURCE_FLAGS = {"attention_backward_split.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+SOURCE_FLAGS = {f"attention_backward_{kind}.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for kind in ("split", "wide")}
 ENGINE_SOURCES = ["engine.cpp", "py_module.cpp"]
 
 
@@ -87,7 +87,7 @@ def build_hip(jobs: int, if_stale: bool) -> Path:
     BUILD.mkdir(parents=True, exist_ok=True)
     LIB.mkdir(parents=True, exist_ok=True)
     gen_embedded_source()
-    headers = [CSRC / h for h in ("pw_core.h", "pw_host.h", "pw_ops.h", "trs_internal.h", "gemm_skinny.h", "gemm_tile.h", "lds_dma.h", "op_checks.h", "attention.h")] + [INCLUDE / "trs_hip.h",
+    headers = [CSRC / h for h in ("pw_core.h", "pw_host.h", "pw_ops.h", "trs_internal.h", "gemm_skinny.h", "gemm_tile.h", "lds_dma.h", "op_checks.h", "attention.h", "attention_wide.h")] + [INCLUDE / "trs_hip.h",
                                                                                  GEN / "pw_core_src.inc"]
     objs = []
     todo = []

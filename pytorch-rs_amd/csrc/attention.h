@@ -8,13 +8,14 @@
 // numbered r = i * group + (head within the group), so that a tile of rows
 // reads its keys and values once for all of them and spans few places.
 //
-// Products run on the fp32 matrix instruction v_mfma_f32_32x32x2_f32.  Lane l of
-// a wave holds of its operands row (or column) l % 32 at k = l / 32, and of
-// its result column l % 32, register i row  8 (i/4) + 4 (l/32) + i%4.  Which k
-// a step takes is free as long as both operands agree, which saves every
-// transposition here: a product whose k runs over the rows of an earlier
-// result takes that result's register i as its operand as it stands, with the
-// other operand read at row 8 (i/4) + 4 (l/32) + i%4.
+// Products run on the bf16 matrix cores, in pieces, for heads of up to 128 dims, and on
+// the fp32 instruction for wider ones and for few rows (attention_wide.h).  Lane l of a
+// wave holds of the operands of a 32x32 product row (or column) l % 32, at 1 or 8 k in its
+// half l / 32, and of the result column l % 32, register i row 8 (i/4) + 4 (l/32) + i%4.
+// Which k a step takes is free as long as both operands agree, which saves every
+// transposition of a result: a product whose k runs over the rows of an earlier result
+// takes that result's registers as its operand as they stand, with the other operand read
+// at those rows.
 #pragma once
 
 #include "gemm_tile.h"
@@ -25,8 +26,9 @@ namespace trs {
 typedef float at_f16 __attribute__((ext_vector_type(16)));
 typedef float at_f4 __attribute__((ext_vector_type(4)));
 
-constexpr int kTile = 32;      // keys or rows per tile in LDS
-constexpr int kRowsBlock = 128;  // rows (or keys) per block: 32 a wave
+constexpr int kTile = 32;        // keys or rows per tile in LDS
+constexpr int kRowsBlock = 128;  // rows (or keys) per block of the gradients: 32 a wave
+constexpr int kPiecesDim = 128;  // the widest heads that run in pieces
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnView {  // [batch, head, token, dim], unit stride along dim
@@ -85,63 +87,24 @@ __device__ __forceinline__ at_f4 row_chunk(const float *row, int c, int D) {
 // The row (of M or N) or k that register i of a result holds in this lane.
 __device__ __forceinline__ int result_row(int i, int half) { return 8 * (i >> 2) + 4 * half + (i & 3); }
 
-// A tile of kTile rows by 32 NT floats in LDS.  The pitch puts rows 4 banks
-// apart, so that 8 lanes reading 16 bytes each at one column cover 32 banks.
-template <int NT, int LANES = 256>
+// A tile of kTile rows by 32 NT floats in LDS, for blocks whose values the pieces below
+// do not hold.  The pitch puts rows 4 banks apart, so that 8 lanes reading 16 bytes each at
+// one column cover 32 banks.
+template <int NT, int LANES>
 struct Tile {
     static constexpr int kCols = 32 * NT, kPitch = kCols + 4, kFloats = kTile * kPitch;
-    static constexpr int kAll = kTile * kCols / 4, kChunks = (kAll + LANES - 1) / LANES;  // 16-byte chunks, and a lane's
-    // Columns a lane reads at once in a product over the tile's rows, and so the
-    // result tiles whose rows interleave: result tile u * W + w holds in its row
-    // rho the tile's column 32 W u + W rho + w.
-    static constexpr int W = NT % 4 == 0 ? 4 : NT % 2 == 0 ? 2 : 1;
-    typedef at_f4 Regs[kChunks];
 
-    __device__ __forceinline__ static int row_of(int q) { return ((int)threadIdx.x + q * LANES) / (kCols / 4); }
-    __device__ __forceinline__ static int col_of(int q) { return ((int)threadIdx.x + q * LANES) % (kCols / 4) * 4; }
-    __device__ __forceinline__ static bool has(int q) { return kAll % LANES == 0 || (int)threadIdx.x + q * LANES < kAll; }
     // row(r): the tile's row r in memory, or null for a row of zeros.
     template <class Row>
-    __device__ __forceinline__ static void load(Regs &v, int D, Row &&row) {
-#pragma unroll
-        for (int q = 0; q < kChunks; q++) {
-            const float *p = has(q) ? row(row_of(q)) : nullptr;
-            v[q] = p ? row_chunk(p, col_of(q), D) : at_f4{0.f, 0.f, 0.f, 0.f};
+    __device__ __forceinline__ static void stage(float *lds, int D, Row &&row) {
+#pragma unroll 1
+        for (int n = (int)threadIdx.x; n < kTile * kCols / 4; n += LANES) {
+            const int r = n / (kCols / 4), c = n % (kCols / 4) * 4;
+            const float *p = row(r);
+            *(at_f4 *)(lds + r * kPitch + c) = p ? row_chunk(p, c, D) : at_f4{0.f, 0.f, 0.f, 0.f};
         }
     }
-    // Whether a value of the lane's chunks is infinite or NaN.
-    __device__ __forceinline__ static bool store(const Regs &v, float *lds) {
-        float s = 0.f;
-#pragma unroll
-        for (int q = 0; q < kChunks; q++) {
-            if (has(q)) *(at_f4 *)(lds + row_of(q) * kPitch + col_of(q)) = v[q];
-            s += v[q][0] * 0.f + v[q][1] * 0.f + v[q][2] * 0.f + v[q][3] * 0.f;
-        }
-        return s != 0.f;
-    }
-    // A lane's operand of 32 rows held in registers: row `p` (null: zeros), at
-    // the k that load_frag reads.
-    __device__ __forceinline__ static void hold(at_f4 (&f)[NT * 4], const float *p, int D, int half, float scale) {
-#pragma unroll
-        for (int j = 0; j < NT * 4; j++) {
-            f[j] = p ? row_chunk(p, 8 * j + 4 * half, D) : at_f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int e = 0; e < 4; e++) f[j][e] *= scale;
-        }
-    }
-    // c += (the tile's rows) x (held rows), over the columns.
-    __device__ __forceinline__ static at_f16 times_held(const float *lds, const at_f4 (&f)[NT * 4], int lane) {
-        at_f16 c = (at_f16)(0.f);
-        const float *p = lds + (lane & 31) * kPitch + 4 * (lane >> 5);
-#pragma unroll
-        for (int j = 0; j < NT * 4; j++) {
-            const at_f4 x = *(const at_f4 *)(p + 8 * j);
-#pragma unroll
-            for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], f[j][e], c, 0, 0, 0);
-        }
-        return c;
-    }
-    // The same with the lane's row (null: zeros) read as it goes, for few registers.
+    // (the tile's rows) x (scale times the lane's row; null: zeros), over the columns.
     __device__ __forceinline__ static at_f16 times_row(const float *lds, const float *row, int D, float scale, int lane) {
         at_f16 c = (at_f16)(0.f);
         const float *p = lds + (lane & 31) * kPitch + 4 * (lane >> 5);
@@ -155,34 +118,11 @@ struct Tile {
         }
         return c;
     }
-    // acc[t] += (the tile's columns) x w over its rows: acc^T += w^T tile, for the
-    // NA result tiles from column c0 on (whole groups of W tiles).
-    template <int NA>
-    __device__ __forceinline__ static void add_product(at_f16 (&acc)[NA], int c0, const float *lds, const at_f16 &w, int lane) {
-        static_assert(NA % W == 0);
-        typedef float Vec __attribute__((ext_vector_type(W)));
-        const float *p = lds + 4 * (lane >> 5) * kPitch + c0 + W * (lane & 31);
-#pragma unroll
-        for (int i = 0; i < 16; i++)
-#pragma unroll
-            for (int u = 0; u < NA / W; u++) {
-                const float *at = p + (8 * (i >> 2) + (i & 3)) * kPitch + 32 * W * u;
-                if constexpr (W == 1) {
-                    acc[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(*at, w[i], acc[u], 0, 0, 0);
-                } else {
-                    const Vec x = *(const Vec *)at;
-#pragma unroll
-                    for (int e = 0; e < W; e++)
-                        acc[u * W + e] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], w[i], acc[u * W + e], 0, 0, 0);
-                }
-            }
-    }
-    // The same where the tile holds infinities or NaN: a pair whose row (of the
-    // tile) and column (of the lane) do not see each other adds nothing, where
-    // the matrix instruction would add 0 * NaN.
-    template <int NA, class Sees>
-    __device__ __forceinline__ static void add_product_seen(at_f16 (&acc)[NA], int c0, const float *lds, const at_f16 &w,
-                                                            int lane, Sees &&seen) {
+    // acc^T += w^T tile over its rows.  A pair of a row (of the tile) and a column (of the
+    // lane) that seen(row) leaves out adds nothing, where the matrix instruction would
+    // add 0 * NaN.
+    template <class Seen>
+    __device__ __forceinline__ static void add_product_seen(at_f16 (&acc)[NT], const float *lds, const at_f16 &w, int lane, Seen &&seen) {
 #pragma unroll 1
         for (int k = 0; k < kTile; k++) {
             const int i = (k >> 3) * 4 + (k & 3), from = (lane & 31) + 32 * ((k >> 2) & 1);
@@ -192,27 +132,19 @@ struct Tile {
             x = __shfl(x, from);
             if (!seen(k)) continue;
 #pragma unroll
-            for (int t = 0; t < NA; t++)
+            for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int r = 0; r < 16; r++)
-                    acc[t][r] += x * lds[k * kPitch + c0 + column(t, r, lane >> 5)];
+                for (int r = 0; r < 16; r++) acc[t][r] += x * lds[k * kPitch + 32 * t + result_row(r, lane >> 5)];
         }
     }
-    // The tile's column that register r of result tile t holds.
-    __device__ __forceinline__ static int column(int t, int r, int half) {
-        return 32 * W * (t / W) + W * result_row(r, half) + t % W;
-    }
-    // Writes f * acc^T from column c0 on: the lane's column of acc is the row at p.
-    template <int NA>
-    __device__ __forceinline__ static void write(const at_f16 (&acc)[NA], int c0, float *p, float f, int D, int half) {
+    // Writes f * acc^T: the lane's column of acc is the row at p.
+    __device__ __forceinline__ static void write(const at_f16 (&acc)[NT], float *p, float f, int D, int half) {
 #pragma unroll
-        for (int u = 0; u < NA / W; u++)
+        for (int t = 0; t < NT; t++)
 #pragma unroll
             for (int r = 0; r < 16; r++) {
-                const int c = c0 + column(u * W, r, half);
-#pragma unroll
-                for (int e = 0; e < W; e++)
-                    if (c + e < D) p[c + e] = acc[u * W + e][r] * f;
+                const int c = 32 * t + result_row(r, half);
+                if (c < D) p[c] = acc[t][r] * f;
             }
     }
 };
@@ -264,18 +196,20 @@ __device__ __forceinline__ void mfma_pieces(at_f16 &c, const Pieces &a, const Pi
 template <int WIDTH>
 struct Unit {
     float v[8];
-    __device__ __forceinline__ void load(const float *row, int u, int D, int lane) {
+    // `sure`: the unit's columns are all below D.
+    __device__ __forceinline__ void load(const float *row, int u, int D, int lane, bool sure = false) {
         const int c = 16 * u + 8 * (lane >> 5);
         if constexpr (WIDTH > 1) {
-            const bool in0 = WIDTH == 4 || c < D, in1 = WIDTH == 4 || c + 4 < D;
+            const bool in0 = WIDTH == 4 || sure || c < D, in1 = WIDTH == 4 || sure || c + 4 < D;
             const f4u x = *(const f4u *)(row + (in0 ? c : 0)), y = *(const f4u *)(row + (in1 ? c + 4 : 0));
 #pragma unroll
             for (int e = 0; e < 4; e++) v[e] = in0 ? x[e] : 0.f, v[4 + e] = in1 ? y[e] : 0.f;
         } else {
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float x = row[c + e < D ? c + e : 0];
-                v[e] = c + e < D ? x : 0.f;
+                const bool in = sure || c + e < D;
+                const float x = row[in ? c + e : 0];
+                v[e] = in ? x : 0.f;
             }
         }
     }
@@ -458,10 +392,12 @@ struct Notices {
 
 // Few rows a key head (attention_few.hip): row_tiles of 16 rows, `splits` parts.
 int launch_attention_few(const AttnArgs &a, hipStream_t s);
-// The gradients' kernel in pieces, for D up to 128: blocks of 128 keys over their windows'
+// The gradients in pieces, for D up to kPiecesDim: blocks of 128 keys over their windows'
 // rows, or over the rows beyond the window of the sinks (sink_tiles of 128 keys), and of 128
 // rows.
 void launch_attention_grad(const AttnArgs &a, uint32_t key_blocks, uint32_t row_blocks, hipStream_t s);
+// And of wider heads: waves of 16 keys, of 16 of the sinks' keys, and of 16 rows.
+void launch_attention_grad_wide(const AttnArgs &a, uint32_t key_units, uint32_t row_units, hipStream_t s);
 int attention_forward(AttnArgs a, hipStream_t s, int cu_count);
 int attention_backward(AttnArgs a, hipStream_t s, int cu_count);
 

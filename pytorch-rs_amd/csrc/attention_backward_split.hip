@@ -33,7 +33,7 @@ __device__ __forceinline__ float up_exp2(float x) {
 // The block's rows on the fp32 instruction, whatever the values.
 template <int NT, int NW>
 __device__ __forceinline__ void grad_rows_fp32(const AttnArgs &a, const RowBlock<NW> &r, float lse, float delta, float *lds,
-                                               Notices<NW> &notices, at_f16 (&acc)[NT]) {
+                                               at_f16 (&acc)[NT]) {
     using T = Tile<NT, 64 * NW>;
     const float *kb = a.k + r.b * a.ks.b + r.hk * a.ks.h, *vb = a.v + r.b * a.vs.b + r.hk * a.vs.h;
     const float *q = r.place >= 0 ? a.q + r.at(a, a.qs) : nullptr, *u = r.place >= 0 ? a.up + r.at(a, a.us) : nullptr;
@@ -42,11 +42,8 @@ __device__ __forceinline__ void grad_rows_fp32(const AttnArgs &a, const RowBlock
 #pragma unroll 1
     for (int t = 0; t < r.tiles; t++) {
         const int j0 = r.first_key(t);
-        typename T::Regs x;
-        T::load(x, a.D, [&](int k) { return r.read(j0 + k) ? kb + (int64_t)(j0 + k) * a.ks.s : nullptr; });
-        notices.word[0][r.wave] = __builtin_amdgcn_ballot_w64(T::store(x, lds)) != 0;
-        T::load(x, a.D, [&](int k) { return r.read(j0 + k) ? vb + (int64_t)(j0 + k) * a.vs.s : nullptr; });
-        T::store(x, lds + T::kFloats);
+        T::stage(lds, a.D, [&](int k) { return r.read(j0 + k) ? kb + (int64_t)(j0 + k) * a.ks.s : nullptr; });
+        T::stage(lds + T::kFloats, a.D, [&](int k) { return r.read(j0 + k) ? vb + (int64_t)(j0 + k) * a.vs.s : nullptr; });
         __syncthreads();
         if (r.any(a, j0)) {
             at_f16 s = T::times_row(lds, q, a.D, a.scale2, r.lane);
@@ -56,7 +53,7 @@ __device__ __forceinline__ void grad_rows_fp32(const AttnArgs &a, const RowBlock
                 s[e] = __builtin_amdgcn_exp2f(s[e] - lse) * (d[e] - delta);
                 if (!sees(a, r.place, j0 + result_row(e, r.half))) s[e] = 0.f;
             }
-            T::add_product_seen(acc, 0, lds, s, r.lane, [&](int k) { return sees(a, r.place, j0 + k); });
+            T::add_product_seen(acc, lds, s, r.lane, [&](int k) { return sees(a, r.place, j0 + k); });
         }
         __syncthreads();
     }
@@ -93,9 +90,9 @@ __device__ __forceinline__ void rows_block(const AttnArgs &a, uint32_t id, char 
 #pragma unroll
         for (int s = 0; s < 2 * NT; s++) {
             Unit<WIDTH> x;
-            x.load(a.q + r.at(a, a.qs), s, a.D, r.lane);
+            x.load(a.q + r.at(a, a.qs), s, a.D, r.lane, s < 2 * NT - 2);
             qp[s] = x.split(live ? a.scale2 * kUp : 0.f);
-            x.load(a.up + r.at(a, a.us), s, a.D, r.lane);
+            x.load(a.up + r.at(a, a.us), s, a.D, r.lane, s < 2 * NT - 2);
             up[s] = x.split(live ? kUp : 0.f);
         }
 #pragma unroll
@@ -147,8 +144,8 @@ __device__ __forceinline__ void rows_block(const AttnArgs &a, uint32_t id, char 
         notices.word[1][r.wave] = not_finite(acc, 0.f);
         __syncthreads();
         if (__builtin_expect(notices.any(1), 0)) {
-            grad_rows_fp32<NT, NW>(a, r, lse, delta, (float *)lds, notices, acc);
-            if (r.row < a.rows) T::write(acc, 0, a.dq + r.at(a, a.dqs), a.scale, a.D, r.half);
+            grad_rows_fp32<NT, NW>(a, r, lse, delta, (float *)lds, acc);
+            if (r.row < a.rows) T::write(acc, a.dq + r.at(a, a.dqs), a.scale, a.D, r.half);
             return;
         }
     }
@@ -214,7 +211,7 @@ struct RowFacts {
 
 template <int NT>
 __device__ __forceinline__ void grad_keys_fp32(const AttnArgs &a, const KeyBlock &k, float *lds, RowFacts &facts,
-                                               Notices<4> &notices, at_f16 (&dk)[NT], at_f16 (&dv)[NT]) {
+                                               at_f16 (&dk)[NT], at_f16 (&dv)[NT]) {
     using T = Tile<NT, 256>;
     const bool live = k.key < k.keys;
     const float *kp = live ? a.k + k.b * a.ks.b + k.hk * a.ks.h + (int64_t)k.key * a.ks.s : nullptr;
@@ -230,11 +227,8 @@ __device__ __forceinline__ void grad_keys_fp32(const AttnArgs &a, const KeyBlock
             const int i = (int)a.by_group.divide((uint32_t)row), g = row - i * a.group;
             return p + k.b * v.b + (int64_t)(k.hk * a.group + g) * v.h + (int64_t)i * v.s;
         };
-        typename T::Regs x;
-        T::load(x, a.D, [&](int r) { return row_at(a.q, a.qs, r); });
-        notices.word[0][k.wave] = __builtin_amdgcn_ballot_w64(T::store(x, lds)) != 0;
-        T::load(x, a.D, [&](int r) { return row_at(a.up, a.us, r); });
-        notices.word[1][k.wave] = __builtin_amdgcn_ballot_w64(T::store(x, lds + T::kFloats)) != 0;
+        T::stage(lds, a.D, [&](int r) { return row_at(a.q, a.qs, r); });
+        T::stage(lds + T::kFloats, a.D, [&](int r) { return row_at(a.up, a.us, r); });
         if (threadIdx.x < kTile) {
             const int row = r0 + (int)threadIdx.x;
             float lse = 0.f, delta = 0.f;
@@ -258,8 +252,8 @@ __device__ __forceinline__ void grad_keys_fp32(const AttnArgs &a, const KeyBlock
                 if (!k.pair(a, facts.place[0][r])) p[e] = d[e] = 0.f;
             }
             const auto seen = [&](int r) { return k.pair(a, facts.place[0][r]); };
-            T::add_product_seen(dv, 0, lds + T::kFloats, p, k.lane, seen);
-            T::add_product_seen(dk, 0, lds, d, k.lane, seen);
+            T::add_product_seen(dv, lds + T::kFloats, p, k.lane, seen);
+            T::add_product_seen(dk, lds, d, k.lane, seen);
         }
         __syncthreads();
     }
@@ -306,9 +300,9 @@ __device__ __forceinline__ void keys_block(const AttnArgs &a, uint32_t id, char 
 #pragma unroll
         for (int s = 0; s < 2 * NT; s++) {
             Unit<WIDTH> x;
-            x.load(a.k + k.b * a.ks.b + k.hk * a.ks.h + (int64_t)key * a.ks.s, s, a.D, k.lane);
+            x.load(a.k + k.b * a.ks.b + k.hk * a.ks.h + (int64_t)key * a.ks.s, s, a.D, k.lane, s < 2 * NT - 2);
             kp[s] = x.split(live ? a.scale2 * kUp : 0.f);
-            x.load(a.v + k.b * a.vs.b + k.hk * a.vs.h + (int64_t)key * a.vs.s, s, a.D, k.lane);
+            x.load(a.v + k.b * a.vs.b + k.hk * a.vs.h + (int64_t)key * a.vs.s, s, a.D, k.lane, s < 2 * NT - 2);
             vp[s] = x.split(live ? kUp : 0.f);
         }
 #pragma unroll
@@ -377,7 +371,7 @@ __device__ __forceinline__ void keys_block(const AttnArgs &a, uint32_t id, char 
         again = notices.any(0);
         if (__builtin_expect(again, 0)) {
             __syncthreads();
-            grad_keys_fp32<NT>(a, k, (float *)lds, facts, notices, dk, dv);
+            grad_keys_fp32<NT>(a, k, (float *)lds, facts, dk, dv);
         }
     }
     if (k.key >= (k.far ? a.sinks : a.Sk)) return;
@@ -393,8 +387,8 @@ __device__ __forceinline__ void keys_block(const AttnArgs &a, uint32_t id, char 
         pv = a.dv + k.b * a.dvs.b + k.hk * a.dvs.h + (int64_t)k.key * a.dvs.s;
     }
     if (again) {
-        T::write(dk, 0, pk, a.scale, a.D, k.half);
-        T::write(dv, 0, pv, 1.f, a.D, k.half);
+        T::write(dk, pk, a.scale, a.D, k.half);
+        T::write(dv, pv, 1.f, a.D, k.half);
     } else {
         write_row<WIDTH>(dk, pk, kDown2, a.scale, a.D, k.half);
         write_row<WIDTH>(dv, pv, kDown2, 1.f, a.D, k.half);

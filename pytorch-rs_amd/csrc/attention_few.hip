@@ -7,47 +7,20 @@
 // v_mfma_f32_16x16x4_f32 takes them from: no LDS, no barrier, nothing that waits
 // for another wave.  Lane l holds of an operand row (column) l % 16 at k = l / 16,
 // of a result column l % 16, register i row 4 (l/16) + i.
-//   S^T = K Q^T: k runs over the dims 16 j + 4 (l/16) + e, so that a lane's four
-//     steps are 16 bytes of its key.
-//   O^T += V^T P^T: k runs over the keys 4 (l/16) + i, where the lane has P as a
-//     result; a lane reads W consecutive dims of its key at once, which go to W
-//     result tiles: tile u W + w holds in its row rho dim 16 W u + W rho + w.
 // The waves of a block join their maxima and sums in LDS, blocks in a second
 // pass.
 #include <hip/hip_runtime.h>
 
-#include "attention.h"
+#include "attention_wide.h"
 
 namespace trs {
 
 namespace {
 
-typedef float at_f2 __attribute__((ext_vector_type(2)));
-
-// N floats of a row from column c on; columns from D on are 0.  MODE 0: D is the
-// padded width; 1: D is a multiple of 4; 2: any D.  No branch around a load:
-// what lies past the row's end is read at its start.
-template <int N, int MODE>
-__device__ __forceinline__ void take(float *v, const float *row, int c, int D) {
-    typedef float Vec __attribute__((ext_vector_type(N), aligned(4)));
-    if constexpr (MODE == 2) {
-#pragma unroll
-        for (int e = 0; e < N; e++) {
-            const float x = row[c + e < D ? c + e : 0];
-            v[e] = c + e < D ? x : 0.f;
-        }
-    } else {
-        const bool in = MODE == 0 || c < D;
-        const Vec x = *(const Vec *)(row + (in ? c : 0));
-#pragma unroll
-        for (int e = 0; e < N; e++) v[e] = in ? x[e] : 0.f;
-    }
-}
-
 // DP: the width, a multiple of 32.  NW waves a block.
 template <int DP, int NW, int MODE>
 __global__ void __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) attn_few(AttnArgs a) {
-    constexpr int KJ = DP / 16, W = DP % 64 == 0 ? 4 : 2, VU = DP / (16 * W), TO = DP / 16;
+    using T = Wide<DP, MODE>;
     __shared__ float out_o[NW][16][DP + 4];
     __shared__ float out_ml[NW][16][2];
     const int lane = (int)threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
@@ -77,42 +50,29 @@ __global__ void __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) attn_few(AttnArgs 
 
     const float *kb = a.k + b * a.ks.b + hk * a.ks.h, *vb = a.v + b * a.vs.b + hk * a.vs.h;
     const float *qrow = a.q + b * a.qs.b + (int64_t)(hk * a.group + g) * a.qs.h + (int64_t)i * a.qs.s;
-    float q[KJ][4], k[KJ][4], v[4][VU][W];
-    const auto load_k = [&](int t) {
-        const float *p = kb + (int64_t)read_key(first_key(t) + col) * a.ks.s;
-#pragma unroll
-        for (int j = 0; j < KJ; j++) take<4, MODE>(k[j], p, 16 * j + 4 * quarter, a.D);
-    };
+    typename T::Along q, k;
+    typename T::Across v;
+    const auto load_k = [&](int t) { T::load(k, kb + (int64_t)read_key(first_key(t) + col) * a.ks.s, a.D, quarter); };
     const auto load_v = [&](int t) {
-        const int j0 = first_key(t) + 4 * quarter;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const float *p = vb + (int64_t)read_key(j0 + e) * a.vs.s;
-#pragma unroll
-            for (int u = 0; u < VU; u++) take<W, MODE>(v[e][u], p, 16 * W * u + W * col, a.D);
-        }
+        T::load(v, [&](int n) { return vb + (int64_t)read_key(first_key(t) + 4 * quarter + n) * a.vs.s; }, a.D, col);
     };
-    at_f4 acc[TO];
+    at_f4 acc[T::TO];
 #pragma unroll
-    for (int t = 0; t < TO; t++) acc[t] = (at_f4)(0.f);
+    for (int t = 0; t < T::TO; t++) acc[t] = (at_f4)(0.f);
     float most = -__builtin_inff(), sum = 0.f;
     if (t0 < t1) {
         load_k(t0);
         load_v(t0);
+        T::load(q, qrow, a.D, quarter);
 #pragma unroll
-        for (int j = 0; j < KJ; j++) {
-            take<4, MODE>(q[j], qrow, 16 * j + 4 * quarter, a.D);
+        for (int j = 0; j < T::KJ; j++)
 #pragma unroll
             for (int e = 0; e < 4; e++) q[j][e] *= a.scale2;
-        }
     }
     for (int t = t0; t < t1; t++) {
         const int j0 = first_key(t), next = t + 1 < t1 ? t + 1 : t;  // the last tile's loads repeat it
         at_f4 s = (at_f4)(0.f);
-#pragma unroll
-        for (int j = 0; j < KJ; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[j][e], q[j][e], s, 0, 0, 0);
+        T::product(s, k, q);
         load_k(next);
 #pragma unroll
         for (int e = 0; e < 4; e++)
@@ -128,50 +88,19 @@ __global__ void __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) attn_few(AttnArgs 
         most = now;
         if (__builtin_amdgcn_ballot_w64(keep != 1.f)) {
 #pragma unroll
-            for (int c = 0; c < TO; c++) acc[c] *= keep;
+            for (int c = 0; c < T::TO; c++) acc[c] *= keep;
         }
-        float bad = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-#pragma unroll
-            for (int u = 0; u < VU; u++)
-#pragma unroll
-                for (int w = 0; w < W; w++) bad += v[e][u][w] * 0.f;
-        if (__builtin_expect(__builtin_amdgcn_ballot_w64(bad != 0.f) == 0, 1)) {
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-#pragma unroll
-                for (int u = 0; u < VU; u++)
-#pragma unroll
-                    for (int w = 0; w < W; w++)
-                        acc[u * W + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[e][u][w], s[e], acc[u * W + w], 0, 0, 0);
-        } else {
-            // Infinities or NaN: a pair that does not see each other adds nothing.
-#pragma unroll 1
-            for (int n = 0; n < 16; n++) {
-                float p = 0.f;
-#pragma unroll
-                for (int e = 0; e < 4; e++) p = (n & 3) == e ? s[e] : p;
-                p = __shfl(p, col + 16 * (n >> 2));
-                if (!sees(a, place, j0 + n)) continue;
-                const float *x = vb + (int64_t)(j0 + n) * a.vs.s;
-#pragma unroll
-                for (int c = 0; c < TO; c++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int d = 16 * W * (c / W) + W * (4 * quarter + e) + c % W;
-                        if (d < a.D) acc[c][e] += p * x[d];
-                    }
-            }
-        }
+        if (__builtin_expect(!T::bad(v), 1)) T::add(acc, v, s);
+        else
+            T::add_seen(acc, s, a.D, col, quarter, [&](int n) { return vb + (int64_t)(j0 + n) * a.vs.s; }, [&](int n) { return sees(a, place, j0 + n); });
         load_v(next);
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
 #pragma unroll
-    for (int c = 0; c < TO; c++)
+    for (int c = 0; c < T::TO; c++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) out_o[wave][col][16 * W * (c / W) + W * (4 * quarter + e) + c % W] = acc[c][e];
+        for (int e = 0; e < 4; e++) out_o[wave][col][T::column(c, e, quarter)] = acc[c][e];
     if (quarter == 0) out_ml[wave][col][0] = most, out_ml[wave][col][1] = sum;
     __syncthreads();
     // The waves' shares of row r, and the row's place in the output.

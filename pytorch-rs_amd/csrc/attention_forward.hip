@@ -7,7 +7,10 @@ namespace trs {
 
 namespace {
 
-constexpr int kFewRows = 32;   // rows a key head that attn_few takes
+// Rows a key head that attn_few takes; of more than 128 dims it takes any.  4000 keys, few / this
+// kernel, us: 1 head of 128, 64 rows 24 / 42, 512 39 / 48; 8 heads 32 rows 30 / 36, 64 42 / 38;
+// 64 heads 32 rows 69 / 140, 64 116 / 143, 96 176 / 149.
+constexpr int kFewRows = 64;
 constexpr int kPartTiles = 2;  // the least key tiles of a part, a wave
 
 // A row of the softmax so far: maximum and sum are of base-2 exponents, log2(e)
@@ -48,59 +51,28 @@ struct RowState {
 };
 
 // The rows of a block over its key tiles t0 to t1 on the fp32 matrix instruction,
-// whatever the values: tiles staged in LDS.  S^T = K Q^T puts a row of the softmax in
-// a lane (and its other half), and P^T is the operand of O^T += V^T P^T as it
-// stands.  FAST: queries held in registers and the next tile loaded ahead; else
-// neither, for few registers.
-template <int NT, int NW, bool FAST>
-__device__ __forceinline__ void rows_fp32(const AttnArgs &a, const RowBlock<NW> &r, int t0, int t1, float *lds,
-                                          Notices<NW> &notices, RowState<NT> &state) {
+// whatever the values: a tile at a time staged in LDS, few registers.  S^T = K Q^T puts a
+// row of the softmax in a lane (and its other half), and P^T is the operand of
+// O^T += V^T P^T as it stands.
+template <int NT, int NW>
+__device__ __forceinline__ void rows_fp32(const AttnArgs &a, const RowBlock<NW> &r, int t0, int t1, float *lds, RowState<NT> &state) {
     using T = Tile<NT, 64 * NW>;
-    const auto buffer = [&](int n, int which) { return lds + (2 * n + which) * T::kFloats; };
     const float *kb = a.k + r.b * a.ks.b + r.hk * a.ks.h, *vb = a.v + r.b * a.vs.b + r.hk * a.vs.h;
     const float *q = r.place >= 0 ? a.q + r.at(a, a.qs) : nullptr;
-    typename T::Regs kr, vr;
-    // A key that no row of the block sees is not read.
-    const auto load = [&](int t, typename T::Regs &x, const float *p, int64_t stride) {
-        const int j0 = r.first_key(t);
-        T::load(x, a.D, [&](int k) { return r.read(j0 + k) ? p + (int64_t)(j0 + k) * stride : nullptr; });
-    };
-    const auto store = [&](int n, bool bad) { notices.word[n][r.wave] = __builtin_amdgcn_ballot_w64(bad) != 0; };
     state.clear();
-    at_f4 qf[FAST ? NT * 4 : 1];
-    if constexpr (FAST) {
-        if (t0 < t1) load(t0, kr, kb, a.ks.s), load(t0, vr, vb, a.vs.s);
-        T::hold(qf, q, a.D, r.half, a.scale2);
-        if (t0 < t1) T::store(kr, buffer(0, 0)), store(0, T::store(vr, buffer(0, 1)));
-        __syncthreads();
-    }
 #pragma unroll 1
     for (int t = t0; t < t1; t++) {
-        const int n = FAST ? (t - t0) & 1 : 0, j0 = r.first_key(t);
-        if constexpr (FAST) {
-            if (t + 1 < t1) load(t + 1, kr, kb, a.ks.s), load(t + 1, vr, vb, a.vs.s);
-        } else {
-            load(t, kr, kb, a.ks.s);
-            T::store(kr, buffer(0, 0));
-            load(t, kr, vb, a.vs.s);
-            store(0, T::store(kr, buffer(0, 1)));
-            __syncthreads();
-        }
+        const int j0 = r.first_key(t);
+        // A key that no row of the block sees is not read.
+        T::stage(lds, a.D, [&](int k) { return r.read(j0 + k) ? kb + (int64_t)(j0 + k) * a.ks.s : nullptr; });
+        T::stage(lds + T::kFloats, a.D, [&](int k) { return r.read(j0 + k) ? vb + (int64_t)(j0 + k) * a.vs.s : nullptr; });
+        __syncthreads();
         if (r.any(a, j0)) {
-            at_f16 s;
-            if constexpr (FAST) s = T::times_held(buffer(n, 0), qf, r.lane);
-            else s = T::times_row(buffer(n, 0), q, a.D, a.scale2, r.lane);
-            if (!r.all(a, j0)) {
+            at_f16 s = T::times_row(lds, q, a.D, a.scale2, r.lane);
 #pragma unroll
-                for (int e = 0; e < 16; e++)
-                    if (!sees(a, r.place, j0 + result_row(e, r.half))) s[e] = -__builtin_inff();
-            }
+            for (int e = 0; e < 16; e++) s[e] = sees(a, r.place, j0 + result_row(e, r.half)) ? s[e] : -__builtin_inff();
             state.weigh(s, 1.f);
-            if (FAST && __builtin_expect(!notices.any(n), 1)) T::add_product(state.acc, 0, buffer(n, 1), s, r.lane);
-            else T::add_product_seen(state.acc, 0, buffer(n, 1), s, r.lane, [&](int k) { return sees(a, r.place, j0 + k); });
-        }
-        if constexpr (FAST) {
-            if (t + 1 < t1) T::store(kr, buffer(n ^ 1, 0)), store(n ^ 1, T::store(vr, buffer(n ^ 1, 1)));
+            T::add_product_seen(state.acc, lds + T::kFloats, s, r.lane, [&](int k) { return sees(a, r.place, j0 + k); });
         }
         __syncthreads();
     }
@@ -123,26 +95,15 @@ __device__ __forceinline__ void write_rows(const AttnArgs &a, const RowBlock<NW>
     if (a.lse && r.half == 0) a.lse[r.index(a)] = (most + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-template <int NT, int NW>
-__global__ void __launch_bounds__(64 * NW, 1) attn_rows_fp32(AttnArgs a) {
-    using T = Tile<NT, 64 * NW>;
-    __shared__ __attribute__((aligned(16))) float lds[4 * T::kFloats];
-    __shared__ Notices<NW> notices;
-    const int part = (int)(blockIdx.x % (uint32_t)a.splits);
-    const RowBlock<NW> r(a, blockIdx.x / (uint32_t)a.splits);
-    RowState<NT> state;
-    rows_fp32<NT, NW, true>(a, r, (int)((int64_t)r.tiles * part / a.splits), (int)((int64_t)r.tiles * (part + 1) / a.splits), lds, notices, state);
-    write_rows(a, r, part, state, 1.f, [&](float *p, float f) { T::write(state.acc, 0, p, f, a.D, r.half); });
-}
-
-// The same on the bf16 matrix cores, in pieces: the block splits a key tile once for
+// 32 NW rows of a key head on the bf16 matrix cores, in pieces: the block splits a key tile once for
 // its waves, into one of two LDS buffers while it computes from the other; the loads from
 // memory are a tile further ahead.
 template <int NT, int NW, int WIDTH>
 __global__ void __launch_bounds__(64 * NW, 2) attn_rows(AttnArgs a) {
     using T = Tile<NT, 64 * NW>;
     constexpr int UNITS = 4 * NT, OWN = (UNITS + NW - 1) / NW;  // of keys and values; of a wave (some twice)
-    constexpr int kBuffer = 3 * UNITS * 1024, kBytes = 2 * kBuffer > 16 * T::kFloats ? 2 * kBuffer : 16 * T::kFloats;
+    constexpr int kBuffer = 3 * UNITS * 1024, kBytes = 2 * kBuffer;
+    static_assert(kBytes >= 8 * T::kFloats, "the fp32 tiles fit the pieces' LDS");
     __shared__ __attribute__((aligned(1024))) char lds[kBytes];
     __shared__ Notices<NW> notices;
     const int part = (int)(blockIdx.x % (uint32_t)a.splits);
@@ -168,7 +129,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_rows(AttnArgs a) {
 #pragma unroll
         for (int s = 0; s < 2 * NT; s++) {
             Unit<WIDTH> x;
-            x.load(a.q + r.at(a, a.qs), s, a.D, r.lane);
+            x.load(a.q + r.at(a, a.qs), s, a.D, r.lane, s < 2 * NT - 2);
             q[s] = x.split(r.place >= 0 ? a.scale2 * kUp : 0.f);
         }
 #pragma unroll
@@ -219,8 +180,8 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_rows(AttnArgs a) {
         __syncthreads();
         if (__builtin_expect(notices.any(0), 0)) {
             __syncthreads();
-            rows_fp32<NT, NW, false>(a, r, t0, t1, (float *)lds, notices, state);
-            write_rows(a, r, part, state, 1.f, [&](float *p, float f) { T::write(state.acc, 0, p, f, a.D, r.half); });
+            rows_fp32<NT, NW>(a, r, t0, t1, (float *)lds, state);
+            write_rows(a, r, part, state, 1.f, [&](float *p, float f) { T::write(state.acc, p, f, a.D, r.half); });
             return;
         }
     }
@@ -281,9 +242,8 @@ void launch_rows(const AttnArgs &a, dim3 grid, hipStream_t s) {
 
 int attention_forward(AttnArgs a, hipStream_t s, int cu_count) {
     const int64_t heads = (int64_t)a.batch * a.kv_heads;
-    const bool few = a.rows <= kFewRows;
-    // 8 waves a block share a key tile's splitting, 4 where the width leaves a wave no half of the registers.
-    const int rows_block = few ? 16 : a.D <= 128 ? 256 : 128, tile = few ? 16 : kTile, waves = few ? 4 : 1;
+    const bool few = a.rows <= kFewRows || a.D > kPiecesDim;
+    const int rows_block = few ? 16 : 256, tile = few ? 16 : kTile, waves = few ? 4 : 1;
     a.row_tiles = (a.rows + rows_block - 1) / rows_block;
     // The keys in parts where the rows' blocks leave CUs without one.
     const int64_t blocks = heads * a.row_tiles, keys = std::min<int64_t>(a.Sk, (int64_t)a.window + a.sinks + rows_block / std::max(a.group, 1));
@@ -306,8 +266,7 @@ int attention_forward(AttnArgs a, hipStream_t s, int cu_count) {
         else if (a.D <= 32) launch_rows<1>(a, grid, s);
         else if (a.D <= 64) launch_rows<2>(a, grid, s);
         else if (a.D <= 96) launch_rows<3>(a, grid, s);
-        else if (a.D <= 128) launch_rows<4>(a, grid, s);
-        else hipLaunchKernelGGL((attn_rows_fp32<8, 4>), grid, dim3(256), 0, s, a);
+        else launch_rows<4>(a, grid, s);
         TRS_LAUNCH_CHECK("attention launch");
         if (a.splits > 1) {
             hipLaunchKernelGGL(attn_join, dim3((unsigned)join_blocks), dim3(256), 0, s, a);
