@@ -402,8 +402,7 @@ int trs_head_norm_rope_backward_f32(int n, const float *const *x, const trs_layo
  * sinks >= 0.  lse (or null) receives log(sum(exp(scale q k))) as
  * [batch, heads, Sq], -inf where nothing is seen.  Sums are fp32, products
  * fp32 or exact in pieces (trs_matmul_f32); the order of the sums is fixed.  Inputs may have any strides (one
- * with no unit stride along dim, or 2^24 elements or more from token to token, is
- * copied first, into the block cache); outputs
+ * with no unit stride along dim is copied first, into the block cache); outputs
  * need a unit stride along dim and share no memory with inputs.  Few rows over
  * many keys are split over the keys, into a workspace from the block cache. */
 int trs_window_attention_f32(const float *q, const trs_layout *lq, const float *k, const trs_layout *lk,

@@ -47,9 +47,10 @@ struct AttnArgs {
     int32_t window, sinks;
     float scale, scale2;  // scale2 = scale * log2(e)
     SmallDivisor by_group;
-    // Work split over the keys (forward): the parts, their unnormalised
+    // Work split over the keys (forward): a block of rows has up to `splits` parts, in
+    // attn_rows one for every part_tiles of its key tiles; the parts' unnormalised
     // outputs [part][batch, key head, row][part_width], and (maximum, sum).
-    int32_t splits, row_tiles, part_width;
+    int32_t splits, part_tiles, row_tiles, part_width;
     float *part_o, *part_ml;
     // Work split over the rows (backward).
     int32_t key_tiles, row_splits, sink_tiles, sink_splits;
@@ -266,9 +267,6 @@ __device__ __forceinline__ Pieces across(const char *lds, int u, int slot, int l
 // step's matrix instructions to run under (a wave issues in order, so it has to stand
 // among them).  `f` holds step 0's fragment; next(f) reads the one that follows the last
 // step's, with that step.
-#ifndef ATTN_V
-#define ATTN_V 8
-#endif
 template <int STEPS, class Read, class Multiply, class Work, class Next>
 __device__ __forceinline__ void steps(Pieces &f, Read &&read, Multiply &&multiply, Work &&work, Next &&next) {
 #pragma unroll
@@ -282,7 +280,7 @@ __device__ __forceinline__ void steps(Pieces &f, Read &&read, Multiply &&multipl
 #pragma unroll
         for (int i = 0; i < 6; i++) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction
-            __builtin_amdgcn_sched_group_barrier(0x002, ATTN_V, 0);  // vector instructions
+            __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);  // vector instructions (3 and 6 measured alike)
         }
         __builtin_amdgcn_sched_barrier(0);
     }
@@ -324,24 +322,43 @@ __device__ __forceinline__ bool not_finite(const at_f16 (&acc)[N], float more) {
     return __builtin_amdgcn_ballot_w64(s != 0.f) != 0;
 }
 
-// What a block of 32 rows a wave works on: its rows, their places, and the key
-// tiles that they see, the sinks' first and then the window's.
+// The tiles of 1 << SHIFT keys that rows r0 to r1 of a key head see, the sinks' first and
+// then the window's.
+template <int SHIFT>
+struct KeyTiles {
+    int key_lo, key_hi, sinks, first, nsink, tiles;
+
+    KeyTiles() = default;
+    __host__ __device__ __forceinline__ KeyTiles(const AttnArgs &a, const Sequence &seq, int r0, int r1) {
+        const int lo = seq.first + (int)a.by_group.divide((uint32_t)r0) - a.window + 1;
+        key_lo = lo > 0 ? lo : 0, key_hi = seq.first + (int)a.by_group.divide((uint32_t)(r1 - 1));
+        sinks = a.sinks < key_hi + 1 ? a.sinks : key_hi + 1;
+        first = key_lo >> SHIFT;
+        const int before = (sinks + (1 << SHIFT) - 1) >> SHIFT;
+        nsink = key_hi < 0 ? 0 : before < first ? before : first;
+        tiles = key_hi < 0 ? 0 : nsink + (key_hi >> SHIFT) - first + 1;
+    }
+    __host__ __device__ __forceinline__ int parts(const AttnArgs &a) const {
+        const int n = tiles > a.part_tiles ? (tiles + a.part_tiles - 1) / a.part_tiles : 1;
+        return n < a.splits ? n : a.splits;
+    }
+    __device__ __forceinline__ int first_key(int t) const { return (t < nsink ? t : first + t - nsink) << SHIFT; }
+    // Whether a row sees key j.
+    __device__ __forceinline__ bool read(int j) const { return j <= key_hi && (j >= key_lo || j < sinks); }
+};
+
+// What a block of 32 rows a wave works on: its rows, their places, and their key tiles.
 template <int NW>
-struct RowBlock {
+struct RowBlock : KeyTiles<5> {
     int lane, half, wave;
     int hk, b, row, i, g;  // the lane's row: query i of head hk * group + g
     int place;             // below 0: sees nothing
     int wave_lo, wave_hi;  // places of the wave's rows
     bool whole;            // the wave has 32 rows
-    int key_lo, key_hi, sinks, first, nsink, tiles;
 
-    // id: over tiles of 32 NW rows, key heads and batches.
-    __device__ __forceinline__ RowBlock(const AttnArgs &a, uint32_t id) {
+    __device__ __forceinline__ RowBlock(const AttnArgs &a, int kv_head, int tile, int batch) : hk(kv_head), b(batch) {
         lane = (int)threadIdx.x & 63, half = lane >> 5;
         wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-        const int tile = (int)(id % (uint32_t)a.row_tiles);
-        id /= (uint32_t)a.row_tiles;
-        hk = (int)(id % (uint32_t)a.kv_heads), b = (int)(id / (uint32_t)a.kv_heads);
         const Sequence seq = sequence_of(a, b);
         const auto place_of = [&](int r) { return seq.first + (int)a.by_group.divide((uint32_t)r); };
         const int r0 = tile * 32 * NW, r1 = min(r0 + 32 * NW, a.rows), last = a.rows - 1;
@@ -352,15 +369,8 @@ struct RowBlock {
         wave_lo = place_of(min(w0, last));
         wave_hi = w0 < w1 ? place_of(w1 - 1) : -1;
         whole = w1 - w0 == 32;
-        key_hi = place_of(r1 - 1), key_lo = max(0, place_of(r0) - a.window + 1);
-        sinks = min(a.sinks, key_hi + 1);
-        first = key_lo / kTile;
-        nsink = key_hi < 0 ? 0 : min((sinks + kTile - 1) / kTile, first);
-        tiles = key_hi < 0 ? 0 : nsink + key_hi / kTile - first + 1;
+        (KeyTiles<5> &)*this = KeyTiles<5>(a, seq, r0, r1);
     }
-    __device__ __forceinline__ int first_key(int t) const { return (t < nsink ? t : first + t - nsink) * kTile; }
-    // Whether a row of the block sees key j.
-    __device__ __forceinline__ bool read(int j) const { return j <= key_hi && (j >= key_lo || j < sinks); }
     // Whether a row of the wave sees a key of the tile at j0, and whether all see all.
     __device__ __forceinline__ bool any(const AttnArgs &a, int j0) const {
         return j0 <= wave_hi && (wave_lo - (j0 + kTile - 1) < a.window || j0 < a.sinks);
@@ -391,7 +401,7 @@ struct Notices {
 };
 
 // Few rows a key head (attention_few.hip): row_tiles of 16 rows, `splits` parts.
-int launch_attention_few(const AttnArgs &a, hipStream_t s);
+int launch_attention_few(const AttnArgs &a, dim3 grid, hipStream_t s);
 // The gradients in pieces, for D up to kPiecesDim: blocks of 128 keys over their windows'
 // rows, or over the rows beyond the window of the sinks (sink_tiles of 128 keys), and of 128
 // rows.

@@ -10,7 +10,7 @@ namespace trs {
 
 namespace {
 
-constexpr int64_t kMaxHeadDim = 256, kMaxTokens = (int64_t)1 << 30, kMaxTokenStride = (int64_t)1 << 24;
+constexpr int64_t kMaxHeadDim = 256, kMaxTokens = (int64_t)1 << 30;
 
 // The operands of a call, in the order of the entry points' arguments.
 struct AttnCall {
@@ -43,15 +43,15 @@ int check_output(const trs_layout *l, const char *what) {
     return TRS_OK;
 }
 
-// An input whose last dim has a unit stride and whose tokens lie near enough for
-// 32-bit offsets in a tile: itself, or a contiguous copy in the block cache.
+// An input whose last dim has a unit stride: itself, or a contiguous copy in the
+// block cache.
 struct Dense {
     const float *at = nullptr;
     AttnView view{};
     void *copy = nullptr;
     int take(const float *p, const trs_layout *l) {
         if (layout_numel(l) == 0) return TRS_OK;
-        if ((l->stride[3] == 1 || l->shape[3] == 1) && (l->stride[2] < kMaxTokenStride || l->shape[2] == 1)) {
+        if (l->stride[3] == 1 || l->shape[3] == 1) {
             at = p + l->offset;
             view = {l->stride[0], l->stride[1], l->stride[2]};
             return TRS_OK;

@@ -107,7 +107,7 @@ int attention_backward(AttnArgs a, hipStream_t s, int cu_count) {
     const int64_t row_blocks = heads * a.row_tiles;
     const int64_t key_blocks = heads * (a.sink_tiles * a.sink_splits + (int64_t)a.key_tiles * a.row_splits);
     const int64_t delta_blocks = ((int64_t)a.batch * a.heads * a.Sq + 15) / 16;
-    if ((row_blocks + key_blocks) >> 31 || delta_blocks >> 31)
+    if ((row_blocks + key_blocks) >> 24 || delta_blocks >> 24)  // a launch has fewer than 2^32 lanes
         return set_error(TRS_E_INVALID_ARGUMENT, "attention gradient over too many blocks");
     const int64_t deltas = ((int64_t)a.batch * a.heads * a.Sq + 63) / 64 * 64;
     const int64_t sink_floats = heads * a.sink_tiles * far * block * a.D;

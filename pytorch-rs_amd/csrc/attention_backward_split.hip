@@ -66,7 +66,8 @@ __device__ __forceinline__ void rows_block(const AttnArgs &a, uint32_t id, char 
     using T = Tile<NT, 64 * NW>;
     constexpr int UNITS = 4 * NT, OWN = NT;  // of keys and values; of a wave
     constexpr int kBuffer = 3 * UNITS * 1024;
-    const RowBlock<NW> r(a, id);
+    const uint32_t rest = id / (uint32_t)a.kv_heads;
+    const RowBlock<NW> r(a, (int)(id % (uint32_t)a.kv_heads), a.row_tiles - 1 - (int)(rest % (uint32_t)a.row_tiles), (int)(rest / (uint32_t)a.row_tiles));
     const float *kb = a.k + r.b * a.ks.b + r.hk * a.ks.h, *vb = a.v + r.b * a.vs.b + r.hk * a.vs.h;
     Unit<WIDTH> in[OWN];
     const auto load = [&](int t) {  // past the last tile: that one

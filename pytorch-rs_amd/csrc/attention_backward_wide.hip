@@ -27,19 +27,15 @@ __device__ __forceinline__ void rows_unit(const AttnArgs &a, int head, int tile)
     const int64_t h = (int64_t)hk * a.group + g, at = ((int64_t)b * a.heads + h) * a.Sq + i;
     const bool live = r0 + col < a.rows && seq.first + i >= 0;
     const int place = live ? seq.first + i : -1;
-    const int lo = seq.first + (int)a.by_group.divide((uint32_t)r0), hi = seq.first + (int)a.by_group.divide((uint32_t)(r1 - 1));
-    const int key_lo = max(0, lo - a.window + 1), key_hi = hi;
-    const int sinks = min(a.sinks, key_hi + 1), first = key_lo >> 4;
-    const int nsink = key_hi < 0 ? 0 : min((sinks + 15) >> 4, first);
-    const int tiles = key_hi < 0 ? 0 : nsink + (key_hi >> 4) - first + 1;
+    const KeyTiles<4> keys(a, seq, r0, r1);
+    const int tiles = keys.tiles;
     at_f4 acc[T::TO];
 #pragma unroll
     for (int t = 0; t < T::TO; t++) acc[t] = (at_f4)(0.f);
     if (tiles > 0) {
         const float *kb = a.k + b * a.ks.b + hk * a.ks.h, *vb = a.v + b * a.vs.b + hk * a.vs.h;
-        const auto first_key = [&](int t) { return (t < nsink ? t : first + t - nsink) << 4; };
         // Past the last key, and past the last tile: that one.
-        const auto key = [&](int t, int n) { return (int64_t)min(first_key(min(t, tiles - 1)) + n, key_hi); };
+        const auto key = [&](int t, int n) { return (int64_t)min(keys.first_key(min(t, tiles - 1)) + n, keys.key_hi); };
         typename T::Along q, u, k, v;
         typename T::Across k2;
         T::load(k, kb + key(0, col) * a.ks.s, a.D, quarter);
@@ -52,7 +48,7 @@ __device__ __forceinline__ void rows_unit(const AttnArgs &a, int head, int tile)
             for (int e = 0; e < 4; e++) q[j][e] = live ? q[j][e] * a.scale2 : 0.f, u[j][e] = live ? u[j][e] : 0.f;
 #pragma unroll 1
         for (int t = 0; t < tiles; t++) {
-            const int j0 = first_key(t);
+            const int j0 = keys.first_key(t);
             const auto row2 = [&](int n) { return kb + key(t, n) * a.ks.s; };
             at_f4 s = (at_f4)(0.f), d = (at_f4)(0.f);
             T::load(v, vb + key(t, col) * a.vs.s, a.D, quarter);

@@ -21,32 +21,27 @@ namespace {
 template <int DP, int NW, int MODE>
 __global__ void __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) attn_few(AttnArgs a) {
     using T = Wide<DP, MODE>;
-    __shared__ float out_o[NW][16][DP + 4];
+    __shared__ __attribute__((aligned(16))) float out_o[NW][16][DP + 4];
     __shared__ float out_ml[NW][16][2];
     const int lane = (int)threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     uint32_t id = blockIdx.x;
-    const int part = (int)(id % (uint32_t)a.splits);
-    id /= (uint32_t)a.splits;
+    const int hk = (int)(id % (uint32_t)a.kv_heads);
+    id /= (uint32_t)a.kv_heads;
     const int tile = (int)(id % (uint32_t)a.row_tiles);
     id /= (uint32_t)a.row_tiles;
-    const int hk = (int)(id % (uint32_t)a.kv_heads), b = (int)(id / (uint32_t)a.kv_heads);
+    const int b = (int)(id % (uint32_t)a.batch), part = (int)(id / (uint32_t)a.batch);
 
     const Sequence seq = sequence_of(a, b);
     const int r0 = tile * 16, r1 = min(r0 + 16, a.rows), row = min(r0 + col, a.rows - 1);
     const int i = (int)a.by_group.divide((uint32_t)row), g = row - i * a.group;
     const int place = r0 + col < a.rows ? seq.first + i : -1;
-    const int lo = seq.first + (int)a.by_group.divide((uint32_t)r0), hi = seq.first + (int)a.by_group.divide((uint32_t)(r1 - 1));
-    const int key_lo = max(0, lo - a.window + 1), key_hi = hi;
-    const int sinks = min(a.sinks, key_hi + 1);
-    const int first = key_lo >> 4;
-    const int nsink = key_hi < 0 ? 0 : min((sinks + 15) >> 4, first);
-    const int tiles = key_hi < 0 ? 0 : nsink + (key_hi >> 4) - first + 1;
-    const int waves = a.splits * NW, mine = part * NW + wave;
+    const KeyTiles<4> keys(a, seq, r0, r1);
+    const int tiles = keys.tiles, waves = a.splits * NW, mine = part * NW + wave;
     const int t0 = (int)((int64_t)tiles * mine / waves), t1 = (int)((int64_t)tiles * (mine + 1) / waves);
-    const auto first_key = [&](int t) { return (t < nsink ? t : first + t - nsink) << 4; };
+    const auto first_key = [&](int t) { return keys.first_key(t); };
     // A key that no row of the block sees is not read: the last one that is seen stands for it.
-    const auto read_key = [&](int j) { return j <= key_hi && (j >= key_lo || j < sinks) ? j : key_hi; };
+    const auto read_key = [&](int j) { return keys.read(j) ? j : keys.key_hi; };
 
     const float *kb = a.k + b * a.ks.b + hk * a.ks.h, *vb = a.v + b * a.vs.b + hk * a.vs.h;
     const float *qrow = a.q + b * a.qs.b + (int64_t)(hk * a.group + g) * a.qs.h + (int64_t)i * a.qs.s;
@@ -127,7 +122,7 @@ __global__ void __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) attn_few(AttnArgs 
             p = a.part_o + at * a.part_width + d;
             if (d == 0) a.part_ml[2 * at] = top, a.part_ml[2 * at + 1] = total;
         } else {
-            o *= total == 0.f ? 0.f : 1.f / total;
+            o *= seq.first + at_i < 0 ? 0.f : 1.f / total;
             p = a.out + b * a.os.b + h * a.os.h + (int64_t)at_i * a.os.s + d;
             if (a.lse && d == 0) a.lse[((int64_t)b * a.heads + h) * a.Sq + at_i] = (top + __builtin_amdgcn_logf(total)) * kLn2;
         }
@@ -146,10 +141,7 @@ void launch(const AttnArgs &a, dim3 grid, hipStream_t s) {
 
 }  // namespace
 
-int launch_attention_few(const AttnArgs &a, hipStream_t s) {
-    const int64_t blocks = (int64_t)a.batch * a.kv_heads * a.row_tiles * a.splits;
-    if (blocks >> 31) return set_error(TRS_E_INVALID_ARGUMENT, "attention over %lld blocks of rows", (long long)blocks);
-    const dim3 grid((unsigned)blocks);
+int launch_attention_few(const AttnArgs &a, dim3 grid, hipStream_t s) {
     if (a.D <= 32) launch<32, 4>(a, grid, s);
     else if (a.D <= 64) launch<64, 4>(a, grid, s);
     else if (a.D <= 96) launch<96, 4>(a, grid, s);

@@ -11,7 +11,8 @@ namespace {
 // kernel, us: 1 head of 128, 64 rows 24 / 42, 512 39 / 48; 8 heads 32 rows 30 / 36, 64 42 / 38;
 // 64 heads 32 rows 69 / 140, 64 116 / 143, 96 176 / 149.
 constexpr int kFewRows = 64;
-constexpr int kPartTiles = 2;  // the least key tiles of a part, a wave
+constexpr int kPartTiles = 2, kMostParts = 64;  // the least key tiles of a part, a wave; the most parts
+constexpr int kForwardRows = 256;               // rows of a block, 32 a wave
 
 // A row of the softmax so far: maximum and sum are of base-2 exponents, log2(e)
 // going into the queries with the scale.  A lane holds its row's sum over half of
@@ -78,21 +79,50 @@ __device__ __forceinline__ void rows_fp32(const AttnArgs &a, const RowBlock<NW> 
     }
 }
 
-// The rows' outputs, or the part's, through write(row, factor).  `unit`: of the maximum.
+// The rows' outputs, or the part's (of several), through write(row, factor).  `unit`: of
+// the maximum.
 template <int NT, int NW, class Write>
-__device__ __forceinline__ void write_rows(const AttnArgs &a, const RowBlock<NW> &r, int part, RowState<NT> &state, float unit,
+__device__ __forceinline__ void write_rows(const AttnArgs &a, const RowBlock<NW> &r, int part, int parts, RowState<NT> &state, float unit,
                                            Write &&write) {
     const float sum = state.sum + __shfl_xor(state.sum, 32), most = state.most * unit;
     if (r.row >= a.rows) return;
-    if (a.splits > 1) {
+    if (parts > 1) {
         const int64_t at = (((int64_t)part * a.batch + r.b) * a.kv_heads + r.hk) * a.rows + r.row;
         write(a.part_o + at * a.part_width, 1.f);
         if (r.half == 0) a.part_ml[2 * at] = most, a.part_ml[2 * at + 1] = sum;
         return;
     }
-    // A row that sees nothing gives 0 and a logarithm of -inf.
-    write(a.out + r.at(a, a.os), sum == 0.f ? 0.f : 1.f / sum);
+    // A row that sees nothing gives 0 and a logarithm of -inf; one whose scores are all -inf,
+    // NaN, as the formula does.
+    write(a.out + r.at(a, a.os), r.place < 0 ? 0.f : 1.f / sum);
     if (a.lse && r.half == 0) a.lse[r.index(a)] = (most + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+// The key tiles of tile t of kForwardRows rows in the longest sequence that may be.
+__host__ __device__ __forceinline__ KeyTiles<5> longest(const AttnArgs &a, int t) {
+    const int r0 = t * kForwardRows, r1 = r0 + kForwardRows;
+    return KeyTiles<5>(a, Sequence{a.Sk, a.Sk - a.Sq}, r0, r1 < a.rows ? r1 : a.rows);
+}
+
+// Of the parts of a key head's tiles of rows, in that order, number n: every lane counts a
+// tile's.
+__device__ __forceinline__ void find_part(const AttnArgs &a, int n, int lane, int &tile, int &part) {
+    tile = part = 0;
+    for (int t0 = 0; t0 < a.row_tiles; t0 += 64) {
+        int sum = t0 + lane < a.row_tiles ? longest(a, t0 + lane).parts(a) : 0;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int before = __shfl_up(sum, d);
+            sum += lane >= d ? before : 0;
+        }
+        const int all = __builtin_amdgcn_readlane(sum, 63);
+        if (n < all) {
+            const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > n));
+            tile = t0 + l, part = l ? n - __builtin_amdgcn_readlane(sum, l - 1) : n;
+            return;
+        }
+        n -= all;
+    }
 }
 
 // 32 NW rows of a key head on the bf16 matrix cores, in pieces: the block splits a key tile once for
@@ -106,9 +136,23 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_rows(AttnArgs a) {
     static_assert(kBytes >= 8 * T::kFloats, "the fp32 tiles fit the pieces' LDS");
     __shared__ __attribute__((aligned(1024))) char lds[kBytes];
     __shared__ Notices<NW> notices;
-    const int part = (int)(blockIdx.x % (uint32_t)a.splits);
-    const RowBlock<NW> r(a, blockIdx.x / (uint32_t)a.splits);
-    const int t0 = (int)((int64_t)r.tiles * part / a.splits), t1 = (int)((int64_t)r.tiles * (part + 1) / a.splits);
+    // Heads first: the chip's parts with an L2 each take them in turn, and so read the fewer
+    // keys twice (prompt of 4096 tokens, 32 heads of 128, 8 key heads, window 1024: 339 us with
+    // the tiles first, 333 so).  Then the rows' tiles, the last ones, which see the most keys,
+    // first; then batches.
+    const uint32_t heads = (uint32_t)a.kv_heads * (a.splits > 1 ? (uint32_t)a.batch : 1u);
+    const uint32_t head = blockIdx.x % heads, rest = blockIdx.x / heads;
+    int part = 0, tile, batch;
+    if (a.splits > 1) {
+        batch = (int)(head / (uint32_t)a.kv_heads);
+        find_part(a, (int)rest, (int)threadIdx.x & 63, tile, part);
+    } else {
+        tile = a.row_tiles - 1 - (int)(rest % (uint32_t)a.row_tiles), batch = (int)(rest / (uint32_t)a.row_tiles);
+    }
+    const RowBlock<NW> r(a, (int)(head % (uint32_t)a.kv_heads), tile, batch);
+    const int parts = r.parts(a);
+    if (part >= parts) return;
+    const int t0 = (int)((int64_t)r.tiles * part / parts), t1 = (int)((int64_t)r.tiles * (part + 1) / parts);
     const float *kb = a.k + r.b * a.ks.b + r.hk * a.ks.h, *vb = a.v + r.b * a.vs.b + r.hk * a.vs.h;
     Unit<WIDTH> in[OWN];
     const auto unit = [&](int q) { return min(r.wave + q * NW, UNITS - 1); };
@@ -140,16 +184,20 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_rows(AttnArgs a) {
             const int j0 = r.first_key(t);
             char *const buf = lds + ((t - t0) & 1) * kBuffer, *const other = lds + ((t - t0) & 1 ? 0 : kBuffer);
             __syncthreads();
-            at_f16 s = (at_f16)(0.f);
             Splitting x;
+            const auto stage = [&](int i) { in[i / 4].template store_pair<UNITS>(x, i % 4, other, unit(i / 4), r.lane); };
+            if (!r.any(a, j0)) {  // no row of the wave sees the tile
+#pragma unroll
+                for (int i = 0; i < 4 * OWN; i++) stage(i);
+                load(t + 2);
+                continue;
+            }
+            at_f16 s = (at_f16)(0.f);
             {
                 const auto read = [&](int n) { return along<UNITS>(buf, n, r.lane); };
                 Pieces f = read(0);
                 steps<2 * NT>(
-                    f, read, [&](int n, const Pieces &now) { mfma_pieces(s, now, q[n]); },
-                    [&](int n) {
-                        dealt(4 * OWN, n, 2 * NT, [&](int i) { in[i / 4].template store_pair<UNITS>(x, i % 4, other, unit(i / 4), r.lane); });
-                    },
+                    f, read, [&](int n, const Pieces &now) { mfma_pieces(s, now, q[n]); }, [&](int n) { dealt(4 * OWN, n, 2 * NT, stage); },
                     [](Pieces &) {});
             }
             load(t + 2);
@@ -181,15 +229,16 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_rows(AttnArgs a) {
         if (__builtin_expect(notices.any(0), 0)) {
             __syncthreads();
             rows_fp32<NT, NW>(a, r, t0, t1, (float *)lds, state);
-            write_rows(a, r, part, state, 1.f, [&](float *p, float f) { T::write(state.acc, p, f, a.D, r.half); });
+            write_rows(a, r, part, parts, state, 1.f, [&](float *p, float f) { T::write(state.acc, p, f, a.D, r.half); });
             return;
         }
     }
-    write_rows(a, r, part, state, kDown2, [&](float *p, float f) { write_row<WIDTH>(state.acc, p, kDown, f, a.D, r.half); });
+    write_rows(a, r, part, parts, state, kDown2, [&](float *p, float f) { write_row<WIDTH>(state.acc, p, kDown, f, a.D, r.half); });
 }
 
 // The parts of a row, joined: four columns a lane.  Every part is read before the
 // first is added, up to eight: one memory latency, not one a part.
+template <bool FEW>
 __global__ void __launch_bounds__(256) attn_join(AttnArgs a) {
     const int64_t rows = (int64_t)a.batch * a.kv_heads * a.rows;
     const uint32_t quads = (uint32_t)a.part_width / 4;
@@ -200,14 +249,20 @@ __global__ void __launch_bounds__(256) attn_join(AttnArgs a) {
     const int row = (int)(r - head * a.rows), b = (int)(head / a.kv_heads), hk = (int)(head - (int64_t)b * a.kv_heads);
     const int i = (int)a.by_group.divide((uint32_t)row);
     const int64_t h = (int64_t)hk * a.group + row - i * a.group;
+    int parts = a.splits;
+    if constexpr (!FEW) {
+        const int r0 = row / kForwardRows * kForwardRows;
+        parts = KeyTiles<5>(a, sequence_of(a, b), r0, min(r0 + kForwardRows, a.rows)).parts(a);
+        if (parts == 1) return;  // its block wrote it
+    }
     float most = -__builtin_inff(), sum = 0.f;
     at_f4 o = (at_f4)(0.f);
-    for (int p0 = 0; p0 < a.splits; p0 += 8) {
+    for (int p0 = 0; p0 < parts; p0 += 8) {
         float m[8], l[8];
         at_f4 x[8];
 #pragma unroll
         for (int p = 0; p < 8; p++) {
-            const int64_t at = min(p0 + p, a.splits - 1) * rows + r;
+            const int64_t at = min(p0 + p, parts - 1) * rows + r;
             m[p] = a.part_ml[2 * at], l[p] = a.part_ml[2 * at + 1];
             x[p] = *(const at_f4 *)(a.part_o + at * a.part_width + d);
         }
@@ -218,12 +273,12 @@ __global__ void __launch_bounds__(256) attn_join(AttnArgs a) {
         sum *= keep, o *= keep, most = now;
 #pragma unroll
         for (int p = 0; p < 8; p++) {
-            if (p0 + p >= a.splits) break;
+            if (p0 + p >= parts) break;
             const float f = __builtin_amdgcn_exp2f(m[p] - base);
             sum += l[p] * f, o += x[p] * f;
         }
     }
-    o *= sum == 0.f ? 0.f : 1.f / sum;
+    o *= sequence_of(a, b).first + i < 0 ? 0.f : 1.f / sum;
     float *out = a.out + b * a.os.b + h * a.os.h + (int64_t)i * a.os.s + d;
 #pragma unroll
     for (int q = 0; q < 4; q++)
@@ -233,9 +288,39 @@ __global__ void __launch_bounds__(256) attn_join(AttnArgs a) {
 
 template <int NT>
 void launch_rows(const AttnArgs &a, dim3 grid, hipStream_t s) {
-    if (a.D == 32 * NT) hipLaunchKernelGGL((attn_rows<NT, 8, 4>), grid, dim3(512), 0, s, a);
-    else if (a.D % 4 == 0) hipLaunchKernelGGL((attn_rows<NT, 8, 2>), grid, dim3(512), 0, s, a);
-    else hipLaunchKernelGGL((attn_rows<NT, 8, 1>), grid, dim3(512), 0, s, a);
+    constexpr int NW = kForwardRows / 32;
+    const dim3 block(64 * NW);
+    if (a.D == 32 * NT) hipLaunchKernelGGL((attn_rows<NT, NW, 4>), grid, block, 0, s, a);
+    else if (a.D % 4 == 0) hipLaunchKernelGGL((attn_rows<NT, NW, 2>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((attn_rows<NT, NW, 1>), grid, block, 0, s, a);
+}
+
+// Parts of about as many key tiles in all blocks of rows, which see from few keys to all: the
+// shortest of which there are at most `want`, so that the chip holds all of them at once.
+// Returns how many a key head has.  Lengths are not known here: every sequence counts as the
+// longest, and in shorter ones a block's last parts have nothing to do.  (As many parts in
+// every block, us / so, causal: 32 heads of 128 over 8, 768 tokens 69 / 50, 1024 88 / 71; 8 heads of
+// 128, 2048 tokens 86 / 68; 32 heads, 300 tokens 30 / 34; 3 x 1000 tokens, 6 heads of 80, window
+// 200 35 / 31.)
+int64_t choose_parts(AttnArgs &a, int64_t heads, int64_t want) {
+    a.splits = 1, a.part_tiles = INT32_MAX;
+    want /= heads;
+    if (a.row_tiles >= want) return a.row_tiles;
+    int most = 0;
+    for (int t = 0; t < a.row_tiles; t++) most = std::max(most, longest(a, t).tiles);
+    const auto parts = [&](int length) {
+        a.part_tiles = length, a.splits = std::max(1, (most + length - 1) / length);
+        int64_t n = 0;
+        for (int t = 0; t < a.row_tiles; t++) n += longest(a, t).parts(a);
+        return n;
+    };
+    int lo = std::max(kPartTiles, (most + kMostParts - 1) / kMostParts), hi = std::max(most, lo);  // parts as long as `hi` are few enough
+    while (lo < hi) {
+        const int mid = lo + (hi - lo) / 2;
+        if (parts(mid) <= want) hi = mid;
+        else lo = mid + 1;
+    }
+    return parts(lo);
 }
 
 }  // namespace
@@ -243,33 +328,40 @@ void launch_rows(const AttnArgs &a, dim3 grid, hipStream_t s) {
 int attention_forward(AttnArgs a, hipStream_t s, int cu_count) {
     const int64_t heads = (int64_t)a.batch * a.kv_heads;
     const bool few = a.rows <= kFewRows || a.D > kPiecesDim;
-    const int rows_block = few ? 16 : 256, tile = few ? 16 : kTile, waves = few ? 4 : 1;
-    a.row_tiles = (a.rows + rows_block - 1) / rows_block;
     // The keys in parts where the rows' blocks leave CUs without one.
-    const int64_t blocks = heads * a.row_tiles, keys = std::min<int64_t>(a.Sk, (int64_t)a.window + a.sinks + rows_block / std::max(a.group, 1));
-    const int64_t most = std::max<int64_t>(1, keys / tile / waves / kPartTiles), want = (few ? 4 : 1) * (int64_t)cu_count;
-    a.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({most, want / blocks, 64}));
-    if ((blocks * a.splits) >> 31) return set_error(TRS_E_INVALID_ARGUMENT, "attention over %lld blocks of rows", (long long)blocks);
+    int64_t blocks;
+    if (few) {
+        a.row_tiles = (a.rows + 15) / 16;
+        const int64_t rows = heads * a.row_tiles, keys = std::min<int64_t>(a.Sk, (int64_t)a.window + a.sinks + 16 / std::max(a.group, 1));
+        a.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({keys / 16 / 4 / kPartTiles, 4 * (int64_t)cu_count / rows, kMostParts}));
+        blocks = rows * a.splits;
+    } else {
+        a.row_tiles = (a.rows + kForwardRows - 1) / kForwardRows;
+        blocks = heads * choose_parts(a, heads, cu_count);
+    }
+    if (blocks * (few ? 256 : 2 * kForwardRows) >> 32)  // a launch has fewer lanes
+        return set_error(TRS_E_INVALID_ARGUMENT, "attention over %lld blocks of rows", (long long)blocks);
     a.part_width = (a.D + 3) / 4 * 4;
     const int64_t parts = a.splits * heads * a.rows, join_blocks = (heads * a.rows * (a.part_width / 4) + 255) / 256;
     void *ws = nullptr;
-    if (a.splits > 1 && join_blocks >> 31) a.splits = 1;
     if (a.splits > 1) {
         const int rc = trs_alloc((size_t)(parts * (a.part_width + 2)) * sizeof(float), &ws);
-        if (rc == TRS_E_ALLOCATION_FAILED) a.splits = 1;  // the parts are for speed alone
+        if (rc == TRS_E_ALLOCATION_FAILED) a.splits = 1, blocks = heads * a.row_tiles;  // the parts are for speed alone
         else if (rc) return rc;
         a.part_o = (float *)ws, a.part_ml = a.part_o + parts * a.part_width;
     }
     const auto launch = [&]() -> int {
-        const dim3 grid((unsigned)(blocks * a.splits));
-        if (few) TRS_CHECK(launch_attention_few(a, s));
+        const dim3 grid((unsigned)blocks);
+        if (few) TRS_CHECK(launch_attention_few(a, grid, s));
         else if (a.D <= 32) launch_rows<1>(a, grid, s);
         else if (a.D <= 64) launch_rows<2>(a, grid, s);
         else if (a.D <= 96) launch_rows<3>(a, grid, s);
         else launch_rows<4>(a, grid, s);
         TRS_LAUNCH_CHECK("attention launch");
         if (a.splits > 1) {
-            hipLaunchKernelGGL(attn_join, dim3((unsigned)join_blocks), dim3(256), 0, s, a);
+            const dim3 joins((unsigned)join_blocks);
+            if (few) hipLaunchKernelGGL(attn_join<true>, joins, dim3(256), 0, s, a);
+            else hipLaunchKernelGGL(attn_join<false>, joins, dim3(256), 0, s, a);
             TRS_LAUNCH_CHECK("attention join launch");
         }
         return TRS_OK;

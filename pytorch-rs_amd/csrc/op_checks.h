@@ -67,7 +67,7 @@ struct SmallDivisor {
         s = 31 + l;
         m = (uint32_t)(((1ull << s) + d - 1) / d);
     }
-    __device__ __forceinline__ uint32_t divide(uint32_t r) const { return (uint32_t)((uint64_t)r * m >> s); }
+    __host__ __device__ __forceinline__ uint32_t divide(uint32_t r) const { return (uint32_t)((uint64_t)r * m >> s); }
 };
 
 }  // namespace trs
