@@ -85,8 +85,8 @@ __device__ __forceinline__ float group_sum(float v) {
     return v;
 }
 
-// Eight entries of a row: four of its first half and the four that lie dim/2
-// on, so that both partners of every pair (rot == dim) are in the lane.
+// Eight entries of a row: four of the first half of what is turned and the four that lie
+// rot/2 on, so that both partners of every pair are in the lane; or eight that pass.
 struct Eight {
     f4u a, b;
 };
@@ -96,7 +96,7 @@ template <int SIGN>
 __device__ __forceinline__ void turn(Eight &v, const NormArgs &a, int64_t position, int at) {
     const float *c = a.cos + position * a.table_stride, *s = a.sin + position * a.table_stride;
     if (a.interleaved) {
-        const int64_t half = a.dim / 2;
+        const int64_t half = a.rot / 2;
 #pragma unroll
         for (int p = 0; p < 2; p++) {
             f4u &x = p ? v.b : v.a;
@@ -131,16 +131,17 @@ __device__ __forceinline__ void store8(float *p, int64_t half, const Eight &v) {
 
 __device__ __forceinline__ int which(const NormArgs &a) { return a.count > 1 && (int)blockIdx.x >= a.t[1].first ? 1 : 0; }
 
-// Rows of whole eights (dim a multiple of 8, all of it rotated, unit strides):
-// LPR lanes a row, 256 / LPR rows a block, one block for each such group (2 x 4096 tokens, 40
-// heads of 128: 57.5 us, 5.9 TB/s; 63 with loads and stores through the caches, 64 and 68 with
-// two and four rows a lane on their way at once).
+// Rows of whole eights (dim and rot multiples of 8, unit strides): LPR lanes a row,
+// 256 / LPR rows a block, one block for each such group.  2 x 4096 tokens, 40 heads of 128:
+// 57.5 us, 5.9 TB/s; 63 with loads and stores through the caches, 64 and 68 with two and four rows
+// a lane on their way at once.  The gradients 91 us, 5.5 TB/s.
 template <int LPR, bool GRAD>
 __global__ void __launch_bounds__(256) norm_rows(NormArgs a) {
     const NormTensor &t = a.t[which(a)];
-    const int64_t half = a.dim / 2;
-    const int sub = (int)threadIdx.x % LPR, at = sub * 4;
-    const bool in = at < half;
+    const int sub = (int)threadIdx.x % LPR;
+    const bool in = sub * 8 < a.dim, turns = sub * 8 < a.rot;
+    const int at = turns ? sub * 4 : sub * 8;
+    const int64_t half = turns ? a.rot / 2 : 4;  // from the lane's first four to its others
     Eight w = {(f4u)(1.f), (f4u)(1.f)}, dw = {(f4u)(0.f), (f4u)(0.f)};
     if (in && t.w) w = load8(t.w + at, half);
     constexpr int RPB = 256 / LPR;
@@ -158,7 +159,7 @@ __global__ void __launch_bounds__(256) norm_rows(NormArgs a) {
         // A position that the tables do not hold gives NaN, and no read past them.
         const bool known = row.position >= 0 && row.position < a.table_rows;
         if constexpr (GRAD) {
-            if (on && known) turn<-1>(g, a, row.position, at);
+            if (on && known && turns) turn<-1>(g, a, row.position, at);
         }
         float sum = 0.f, dot = 0.f;
 #pragma unroll
@@ -183,7 +184,7 @@ __global__ void __launch_bounds__(256) norm_rows(NormArgs a) {
             }
         }
         if constexpr (!GRAD) {
-            if (known) turn<1>(y, a, row.position, at);
+            if (known && turns) turn<1>(y, a, row.position, at);
         }
         if (!known) y = {(f4u)(__builtin_nanf("")), (f4u)(__builtin_nanf(""))};
         store8(t.y + at_row(t.ys, row) + at, half, y);
@@ -194,10 +195,11 @@ __global__ void __launch_bounds__(256) norm_rows(NormArgs a) {
         __shared__ float part[RPB][LPR * 8];
         const int g = (int)threadIdx.x / LPR;
 #pragma unroll
-        for (int e = 0; e < 4; e++) part[g][at + e] = dw.a[e], part[g][LPR * 4 + at + e] = dw.b[e];
+        for (int e = 0; e < 4; e++) part[g][sub * 8 + e] = dw.a[e], part[g][sub * 8 + 4 + e] = dw.b[e];
         __syncthreads();
         for (int d = (int)threadIdx.x; d < a.dim; d += 256) {
-            const int col = d < half ? d : LPR * 4 + d - (int)half;
+            const int second = (int)a.rot / 2;
+            const int col = d >= a.rot ? d : d < second ? d / 4 * 8 + d % 4 : (d - second) / 4 * 8 + 4 + d % 4;
             float s = part[0][col];
             for (int i = 1; i < RPB; i++) s += part[i][col];
             t.parts[block * a.dim + d] = s;
@@ -206,7 +208,8 @@ __global__ void __launch_bounds__(256) norm_rows(NormArgs a) {
 }
 
 // Any dim up to kMaxDim, any part of it rotated, any strides: a wave a row, the
-// entries dealt to its lanes, partners read again from the cache.
+// entries dealt to its lanes, partners read again from the cache (2 x 4096 tokens, 40
+// heads of 80, 36 of them turned: 151 us; 40 of them, in eights, 46).
 template <bool GRAD>
 __global__ void __launch_bounds__(256) norm_any(NormArgs a) {
     const NormTensor &t = a.t[which(a)];
@@ -409,7 +412,7 @@ int run_norm(const NormCall &c) {
     a.inv_dim = 1.0f / (float)a.dim;
     DeviceState *dev = device_state();
     if (!dev) return TRS_E_NO_DEVICE;
-    whole = a.rot == a.dim && a.dim % 8 == 0 && a.dim <= 512;
+    whole = a.rot % 8 == 0 && a.dim % 8 == 0 && a.dim <= 512;
     for (int i = 0; i < c.n; i++) {
         NormTensor &t = a.t[i];
         const trs_layout *lx = &c.lx[i], *lo = &c.lo[i], *lu = GRAD ? &c.lup[i] : lx;

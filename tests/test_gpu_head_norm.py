@@ -87,6 +87,25 @@ def test_gradients_match_64_bits(shape):
         assert_within(dw, want[1], bound[1], "dw")
 
 
+# Eights that pass beside eights that are turned.
+PARTIAL = [(1, 3, 1, 9, 80, 40, False), (2, 2, 1, 33, 96, 16, True), (1, 2, 2, 5, 128, 8, False), (1, 5, 1, 70, 64, 0, False),
+           (1, 1, 1, 130, 24, 8, False), (1, 2, 1, 3, 512, 256, False), (2, 3, 1, 17, 256, 248, True)]
+
+
+@pytest.mark.parametrize("shape", PARTIAL, ids=str)
+def test_part_of_a_head_turned(shape):
+    B, hq, hk, S, D, rot, inter = shape
+    (xq, uq, wq), (xk, uk, wk) = make(11, B, hq, S, D), make(12, B, hk, S, D)
+    got, cos, sin, at = run([(xq, None), (xk, None)], [wq, wk], rot, inter, start=2)
+    for y, x, w in zip(got, (xq, xk), (wq, wk)):
+        assert_within(y, norm_rope_reference(x, w, EPS, cos, sin, at, inter), bounds(x, w))
+    got, cos, sin, at = run([(xq, uq), (xk, uk)], [wq, wk], rot, inter, grad=True)
+    for (dx, dw), x, u, w in zip(got, (xq, xk), (uq, uk), (wq, wk)):
+        want, bound = norm_rope_reference(x, w, EPS, cos, sin, at, inter, u), bounds(x, w, u)
+        assert_within(dx, want[0], bound[0], "dx")
+        assert_within(dw, want[1], bound[1], "dw")
+
+
 @pytest.mark.parametrize("place", [{"order": (0, 1, 2, 3), "offset": 1}, {"order": TOKENS, "pad": 3}, {"order": (0, 1, 2, 3), "step": 2},
                                    {"order": (3, 2, 1, 0)}], ids=str)
 def test_strides_and_orders_without_a_weight(place):
