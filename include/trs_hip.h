@@ -381,7 +381,7 @@ int trs_head_norm_rope_f32(int n, const float *const *x, const trs_layout *lx, c
 /* Its gradients: dx (n tensors, layouts ldx) and dweight (n pointers to dim
  * floats, any of them or the array null: not wanted).  The rows' shares of
  * dweight are added in a fixed order, in a workspace from the block cache of at
- * most 4 * dim floats per CU and tensor. */
+ * most 2 * dim floats per CU and tensor. */
 int trs_head_norm_rope_backward_f32(int n, const float *const *x, const trs_layout *lx, const float *const *weight,
                                     float eps, const float *cos, const float *sin, const trs_layout *ltab,
                                     int interleaved, const int32_t *positions, int64_t start, const float *const *up,
@@ -400,11 +400,13 @@ int trs_head_norm_rope_backward_f32(int n, const float *const *x, const trs_layo
  * sequence's last are not read, and what stands in one that a query does not see,
  * NaN included, does not reach that query.  window >= 1 (INT64_MAX: no window);
  * sinks >= 0.  lse (or null) receives log(sum(exp(scale q k))) as
- * [batch, heads, Sq], -inf where nothing is seen.  Sums are fp32, products
- * fp32 or exact in pieces (trs_matmul_f32); the order of the sums is fixed.  Inputs may have any strides (one
- * with no unit stride along dim is copied first, into the block cache); outputs
- * need a unit stride along dim and share no memory with inputs.  Few rows over
- * many keys are split over the keys, into a workspace from the block cache. */
+ * [batch, heads, Sq], -inf where nothing is seen.  A query all of
+ * whose scores are -inf gives NaN.  Sums are fp32, products on the fp32 matrix
+ * cores or, in pieces as in trs_matmul_f32, the bf16 ones; the order of the sums
+ * is fixed.  Inputs may have any strides (one with no unit stride along dim is
+ * copied first, into the block cache); outputs need a unit stride along dim and
+ * share no memory with inputs.  Few rows over many keys are split over the keys,
+ * into a workspace from the block cache; where it has none they are not. */
 int trs_window_attention_f32(const float *q, const trs_layout *lq, const float *k, const trs_layout *lk,
                              const float *v, const trs_layout *lv, const int32_t *lengths, int64_t window,
                              int64_t sinks, float scale, float *out, const trs_layout *lo, float *lse);

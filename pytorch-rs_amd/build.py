@@ -44,8 +44,8 @@ HIP_SOURCES = ["pw_binary.hip", "pw_binary_muldiv.hip", "pw_scalar.hip", "pw_una
                "dropout.hip", "head_norm.hip", "attention.hip", "attention_forward.hip", "attention_few.hip", "attention_backward.hip",
                "attention_backward_split.hip", "attention_backward_wide.hip"]
 # Flags of one source.  The attention gradients hold over 256 registers a lane: with the matrix
-# results in the vector registers, and not the accumulation ones, nothing spills (47 registers did
-# at a head dim of 128, 1.72 ms where the kernel now takes 1.29).
+# results in the vector registers, and not the accumulation ones, nothing spills at a head dim of
+# 128 (a training step of 4096 tokens, 32 heads, window 2048: 2.86 ms without, 2.50 with).
 SOURCE_FLAGS = {f"attention_backward_{kind}.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for kind in ("split", "wide")}
 ENGINE_SOURCES = ["engine.cpp", "py_module.cpp"]
 

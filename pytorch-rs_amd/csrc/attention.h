@@ -182,13 +182,18 @@ __device__ __forceinline__ void mfma_pieces(at_f16 &c, const Pieces &a, const Pi
     for (int i = 0; i < 6; i++) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[PA[i]], b.p[PB[i]], c, 0, 0, 0);
 }
 
+// A lane's 16 bytes of a unit (the next comment): row lane % 32 at columns 8 (lane/32) on.
+__device__ __forceinline__ int unit_place(int lane) { return (lane ^ lane >> 5 << 2) * 16; }
+
 // A tile of kTile rows by 32 NT columns of one tensor or of two, as pieces in LDS.  A
 // unit is 16 columns, 1 KiB of each piece, loaded, split and stored by one wave: (row,
-// column) at 512 (column/8) + 16 row + 2 (column%8), which is the order of a fragment
-// whose k runs along the columns (lane l: row l % 32 at columns 8 (l/32) on), free
-// of bank conflicts.  A fragment whose k runs across the rows is read from the same
-// bytes by the transposing load: 16 lanes ask for 4 rows by 16 columns, four columns of
-// a row each, and each gets its own column's four rows.
+// column) at 512 (column/8) + 16 (row ^ 4 (column/8)) + 2 (column%8), which is the order of a
+// fragment whose k runs along the columns (lane l: row l % 32 at columns 8 (l/32) on).  A
+// fragment whose k runs across the rows is read from the same bytes by the transposing
+// load: 16 lanes ask for 4 rows by 16 columns, four columns of a row each, and each gets
+// its own column's four rows; the exchange of rows puts their two halves on different
+// banks (prompt of 4096 tokens, 32 heads of 128: a third of the conflicts, 327 -> 326 us; rows
+// exchanged by the unit too leave none, but cost two registers, 331).
 //
 // Columns from D on are 0.  No branch stands around a load, which would wait for all of
 // them: what must not be read is read elsewhere in the row and then 0.  WIDTH 4: D is the
@@ -227,7 +232,7 @@ struct Unit {
         if (i == 3) {
             const Pieces y = x.done();
 #pragma unroll
-            for (int p = 0; p < 3; p++) *(gt_bf8 *)(lds + (p * UNITS + u) * 1024 + lane * 16) = y.p[p];
+            for (int p = 0; p < 3; p++) *(gt_bf8 *)(lds + (p * UNITS + u) * 1024 + unit_place(lane)) = y.p[p];
         }
     }
     template <int UNITS>
@@ -242,7 +247,7 @@ template <int UNITS>
 __device__ __forceinline__ Pieces along(const char *lds, int u, int lane) {
     Pieces x;
 #pragma unroll
-    for (int p = 0; p < 3; p++) x.p[p] = *(const gt_bf8 *)(lds + (p * UNITS + u) * 1024 + lane * 16);
+    for (int p = 0; p < 3; p++) x.p[p] = *(const gt_bf8 *)(lds + (p * UNITS + u) * 1024 + unit_place(lane));
     return x;
 }
 // Units u and u + 1 as 32 columns: k runs across rows 16 slot to 16 slot + 15, in the
@@ -252,7 +257,8 @@ __device__ __forceinline__ Pieces across(const char *lds, int u, int slot, int l
     typedef short S4 __attribute__((ext_vector_type(4)));
     typedef short S8 __attribute__((ext_vector_type(8)));
     typedef S4 __attribute__((address_space(3))) *Lds;
-    const char *at = lds + (lane >> 4 & 1) * 1024 + (lane >> 1 & 1) * 512 + (4 * (lane >> 5) + (lane >> 2 & 3)) * 16 + (lane & 1) * 8;
+    const int second = lane >> 1 & 1;
+    const char *at = lds + (lane >> 4 & 1) * 1024 + second * 512 + (4 * (lane >> 5 ^ second) + (lane >> 2 & 3)) * 16 + (lane & 1) * 8;
     Pieces x;
 #pragma unroll
     for (int p = 0; p < 3; p++) {

@@ -127,7 +127,10 @@ __device__ __forceinline__ void find_part(const AttnArgs &a, int n, int lane, in
 
 // 32 NW rows of a key head on the bf16 matrix cores, in pieces: the block splits a key tile once for
 // its waves, into one of two LDS buffers while it computes from the other; the loads from
-// memory are a tile further ahead.
+// memory are a tile further ahead.  Bound by the card's power and, behind it, by issue: prompt
+// of 4096 tokens, 32 heads of 128 over 8, window 1024, 326-338 us by card, 1.16 PFLOP/s of bf16
+// products, the matrix cores busy for 62% of the time (of a large product 1.24 and 63%).
+// Blocks of four waves, which split every tile for half the rows, take 427.
 template <int NT, int NW, int WIDTH>
 __global__ void __launch_bounds__(64 * NW, 2) attn_rows(AttnArgs a) {
     using T = Tile<NT, 64 * NW>;
@@ -237,7 +240,8 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_rows(AttnArgs a) {
 }
 
 // The parts of a row, joined: four columns a lane.  Every part is read before the
-// first is added, up to eight: one memory latency, not one a part.
+// first is added, up to eight: one memory latency, not one a part.  3 to 6 us, of which most is
+// the launch behind another.
 template <bool FEW>
 __global__ void __launch_bounds__(256) attn_join(AttnArgs a) {
     const int64_t rows = (int64_t)a.batch * a.kv_heads * a.rows;
