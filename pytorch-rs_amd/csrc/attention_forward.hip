@@ -104,6 +104,13 @@ __host__ __device__ __forceinline__ KeyTiles<5> longest(const AttnArgs &a, int t
     return KeyTiles<5>(a, Sequence{a.Sk, a.Sk - a.Sq}, r0, r1 < a.rows ? r1 : a.rows);
 }
 
+// The parts of tile t of a sequence's rows, which see the tiles `keys`.  Where a shorter
+// sequence's window begins elsewhere in a tile it may touch one tile more than the longest's:
+// it still has no more parts than the longest has, for which blocks are launched.
+__device__ __forceinline__ int parts_of(const AttnArgs &a, const KeyTiles<5> &keys, int t) {
+    return min(keys.parts(a), longest(a, t).parts(a));
+}
+
 // Of the parts of a key head's tiles of rows, in that order, number n: every lane counts a
 // tile's.
 __device__ __forceinline__ void find_part(const AttnArgs &a, int n, int lane, int &tile, int &part) {
@@ -153,7 +160,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_rows(AttnArgs a) {
         tile = a.row_tiles - 1 - (int)(rest % (uint32_t)a.row_tiles), batch = (int)(rest / (uint32_t)a.row_tiles);
     }
     const RowBlock<NW> r(a, (int)(head % (uint32_t)a.kv_heads), tile, batch);
-    const int parts = r.parts(a);
+    const int parts = parts_of(a, r, tile);
     if (part >= parts) return;
     const int t0 = (int)((int64_t)r.tiles * part / parts), t1 = (int)((int64_t)r.tiles * (part + 1) / parts);
     const float *kb = a.k + r.b * a.ks.b + r.hk * a.ks.h, *vb = a.v + r.b * a.vs.b + r.hk * a.vs.h;
@@ -255,8 +262,8 @@ __global__ void __launch_bounds__(256) attn_join(AttnArgs a) {
     const int64_t h = (int64_t)hk * a.group + row - i * a.group;
     int parts = a.splits;
     if constexpr (!FEW) {
-        const int r0 = row / kForwardRows * kForwardRows;
-        parts = KeyTiles<5>(a, sequence_of(a, b), r0, min(r0 + kForwardRows, a.rows)).parts(a);
+        const int t = row / kForwardRows, r0 = t * kForwardRows;
+        parts = parts_of(a, KeyTiles<5>(a, sequence_of(a, b), r0, min(r0 + kForwardRows, a.rows)), t);
         if (parts == 1) return;  // its block wrote it
     }
     float most = -__builtin_inff(), sum = 0.f;

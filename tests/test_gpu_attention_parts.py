@@ -163,3 +163,26 @@ def test_refusals_of_the_gradients():
     refused(E, "unit stride", q, k, v, 4, 0, 1.0, out, lse, up, g[0], turned, g[2])
     assert abi.lib.trs_window_attention_backward_f32(
         *q.arg, *k.arg, *v.arg, None, 4, 0, 1.0, *out.arg, lse.ptr, up.dev.ptr, None, *g[0].arg, *g[1].arg, *g[2].arg) == E
+
+
+#        H hk  tokens D  window sinks lengths   parts
+SHIFTED = [
+    (3, 1, 174, 16, 40, 0, [174, 134], 3),
+    (3, 1, 174, 64, 66, 3, [161, 174], 3),
+    (10, 2, 174, 40, 53, 3, [174, 134], 3),
+    (6, 2, 211, 128, 40, 3, [211, 171], 3),
+]
+
+
+@pytest.mark.parametrize("shape", SHIFTED, ids=str)
+def test_a_shorter_window_over_one_tile_more(shape):
+    """A shorter sequence's window begins elsewhere in a tile of keys than the longest's and
+    touches one tile more; all of its parts are computed.  What the workspace holds before
+    is NaN."""
+    H, hk, n, D, window, sinks, lengths, parts = shape
+    q, k, v, _ = inputs(7, 2, H, hk, n, n, D)
+    want = attention_reference(q, k, v, window, sinks, np.float32(0.2), lengths)
+    DeviceArray.from_numpy(np.full(parts * 2 * H * n * (D + 2), np.nan, np.float32)).free()
+    out, lse = run(q, k, v, window, sinks, 0.2, lengths)
+    assert_within(out, *want["out"], "out")
+    assert_within(lse, *want["lse"], "lse")
