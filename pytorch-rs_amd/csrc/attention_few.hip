@@ -2,7 +2,7 @@
 // tokens over a cache.
 //
 // Bound by reading the keys and values once: 16 sequences of 1600 to 8192 keys, 8 key heads
-// of 128, window 4096 (470 MB) 90 us, 5.2 TB/s; a sum over 1 GiB reads 5.9.  A wave takes 16 rows (the query
+// of 128, window 4096 (470 MB) 90-93 us, 5.1-5.2 TB/s; a sum over 1 GiB reads 5.9.  A wave takes 16 rows (the query
 // heads that share the key head, and the few tokens) and streams its share of
 // the keys 16 at a time, straight from memory into the registers that
 // v_mfma_f32_16x16x4_f32 takes them from: no LDS, no barrier, nothing that waits
