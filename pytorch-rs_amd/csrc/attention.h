@@ -51,6 +51,7 @@ struct AttnArgs {
     // attn_rows one for every part_tiles of its key tiles; the parts' unnormalised
     // outputs [part][batch, key head, row][part_width], and (maximum, sum).
     int32_t splits, part_tiles, row_tiles, part_width;
+    int32_t few_waves;  // waves of a block of attn_few
     float *part_o, *part_ml;
     // Work split over the rows (backward).
     int32_t key_tiles, row_splits, sink_tiles, sink_splits;

@@ -6,10 +6,9 @@
 // computes from the other, the loads from memory a tile further ahead: one barrier a
 // tile.  Bound by the card's power and by issue: 4096 tokens, 32 heads of 128 over 8, window
 // 2048 1.86 to 2.1 ms by card, up to 1.24 PFLOP/s of bf16 products, the matrix cores busy for 61% of
-// the time.  The
-// block has a CU to itself (512 registers a lane) above dims of 64, and a
-// wave a SIMD nothing to run beside but its own instructions: so splitting and
-// exponentials stand among the matrix instructions (steps()).
+// the time.  The block has a CU to itself (512 registers a lane) above dims of 64, and a wave
+// a SIMD nothing to run beside but its own instructions: so splitting and exponentials stand
+// among the matrix instructions (steps()).
 //
 // Queries, keys, values and upstream rows are taken times 2^40, and P as 2^40 P, so
 // that no piece of a value or weight is lost.  A block whose sums are not finite does

@@ -8,7 +8,7 @@
 // v_mfma_f32_16x16x4_f32 takes them from: no LDS, no barrier, nothing that waits
 // for another wave.  Lane l holds of an operand row (column) l % 16 at k = l / 16,
 // of a result column l % 16, register i row 4 (l/16) + i.
-// The waves of a block join their maxima and sums in LDS, blocks in a second
+// The waves of a block join their maxima and sums in LDS, blocks, if several have a row, in a second
 // pass.
 #include <hip/hip_runtime.h>
 
@@ -18,9 +18,9 @@ namespace trs {
 
 namespace {
 
-// DP: the width, a multiple of 32.  NW waves a block.
+// DP: the width, a multiple of 32.  NW waves a block (16 or 8, the CU to itself: dims that are multiples of four).
 template <int DP, int NW, int MODE>
-__global__ void __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) attn_few(AttnArgs a) {
+__global__ void __launch_bounds__(64 * NW, NW > 8 ? 4 : DP <= 128 ? 2 : 1) attn_few(AttnArgs a) {
     using T = Wide<DP, MODE>;
     __shared__ __attribute__((aligned(16))) float out_o[NW][16][DP + 4];
     __shared__ float out_ml[NW][16][2];
@@ -137,13 +137,17 @@ template <int DP, int NW>
 void launch(const AttnArgs &a, dim3 grid, hipStream_t s) {
     if (a.D == DP) hipLaunchKernelGGL((attn_few<DP, NW, 0>), grid, dim3(64 * NW), 0, s, a);
     else if (a.D % 4 == 0) hipLaunchKernelGGL((attn_few<DP, NW, 1>), grid, dim3(64 * NW), 0, s, a);
-    else hipLaunchKernelGGL((attn_few<DP, NW, 2>), grid, dim3(64 * NW), 0, s, a);
+    else if constexpr (NW == 4) hipLaunchKernelGGL((attn_few<DP, NW, 2>), grid, dim3(64 * NW), 0, s, a);
 }
 
 }  // namespace
 
 int launch_attention_few(const AttnArgs &a, dim3 grid, hipStream_t s) {
-    if (a.D <= 32) launch<32, 4>(a, grid, s);
+    if (a.few_waves == 16 && a.D <= 32) launch<32, 16>(a, grid, s);
+    else if (a.few_waves == 16) launch<64, 16>(a, grid, s);
+    else if (a.few_waves == 8 && a.D <= 96) launch<96, 8>(a, grid, s);
+    else if (a.few_waves == 8) launch<128, 8>(a, grid, s);
+    else if (a.D <= 32) launch<32, 4>(a, grid, s);
     else if (a.D <= 64) launch<64, 4>(a, grid, s);
     else if (a.D <= 96) launch<96, 4>(a, grid, s);
     else if (a.D <= 128) launch<128, 4>(a, grid, s);

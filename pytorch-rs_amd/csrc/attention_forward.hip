@@ -345,12 +345,22 @@ int attention_forward(AttnArgs a, hipStream_t s, int cu_count) {
         a.row_tiles = (a.rows + 15) / 16;
         const int64_t rows = heads * a.row_tiles, keys = std::min<int64_t>(a.Sk, (int64_t)a.window + a.sinks + 16 / std::max(a.group, 1));
         a.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({keys / 16 / 4 / kPartTiles, 4 * (int64_t)cu_count / rows, kMostParts}));
+        // Where blocks of 16 waves (8 above 64 dims, for their registers) do what the parts would, the
+        // second launch is saved.  One of them fills a CU: so where one round of them takes all CUs and the
+        // sequences are alike, or where the keys are few.  us in parts / so: 8 heads of 64, 260 keys
+        // 12.2 / 9.3, 383 11.9 / 11.0, 520 10.8 / 11.9; 8 of 128, 300 keys 12.4 / 13.4; 256 of 64, 1000 keys
+        // 26.7 / 23.0; 256 of 128, 300 20.5 / 16.3, 4000 182 / 178; 128 of 128, 2000 55 / 60; 384 of
+        // 128, 1000 72 / 77.
+        const bool full = 8 * rows >= 7 * (int64_t)cu_count && a.D <= kPiecesDim && !a.lengths;
+        const bool whole = a.splits > 1 && rows <= cu_count && a.D % 4 == 0 && (full || (a.splits == 2 && a.D <= 64));
+        a.few_waves = !whole ? 4 : a.D <= 64 ? 16 : 8;
+        if (whole) a.splits = 1;
         blocks = rows * a.splits;
     } else {
         a.row_tiles = (a.rows + kForwardRows - 1) / kForwardRows;
         blocks = heads * choose_parts(a, heads, cu_count);
     }
-    if (blocks * (few ? 256 : 2 * kForwardRows) >> 32)  // a launch has fewer lanes
+    if (blocks * (few ? 1024 : 2 * kForwardRows) >> 32)  // a launch has fewer lanes
         return set_error(TRS_E_INVALID_ARGUMENT, "attention over %lld blocks of rows", (long long)blocks);
     a.part_width = (a.D + 3) / 4 * 4;
     const int64_t parts = a.splits * heads * a.rows, join_blocks = (heads * a.rows * (a.part_width / 4) + 255) / 256;

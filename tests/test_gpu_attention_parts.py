@@ -186,3 +186,32 @@ def test_a_shorter_window_over_one_tile_more(shape):
     out, lse = run(q, k, v, window, sinks, 0.2, lengths)
     assert_within(out, *want["out"], "out")
     assert_within(lse, *want["lse"], "lse")
+
+
+#        B  H hk  sq  sk   D  window sinks lengths
+WHOLE = [
+    (1, 8, 8, 1, 300, 64, EVERY, 0, None),     # few keys: blocks of 16 waves, no parts
+    (1, 8, 2, 3, 383, 32, 200, 5, None),
+    (3, 4, 2, 2, 290, 48, EVERY, 0, [290, 1, 0]),
+    (1, 2, 1, 5, 257, 20, EVERY, 0, None),
+    (1, 2, 2, 1, 260, 50, EVERY, 0, None),     # a width in parts all the same
+    (2, 128, 128, 1, 500, 64, EVERY, 0, None),  # a head for every CU: blocks of 16 waves, and of 8
+    (2, 128, 128, 1, 500, 80, 130, 7, None),
+    (4, 64, 64, 2, 270, 128, EVERY, 0, None),
+    (4, 128, 64, 1, 270, 100, EVERY, 0, [270, 33, 1, 0]),
+]
+
+
+@pytest.mark.parametrize("shape", WHOLE, ids=str)
+def test_few_rows_in_blocks_of_many_waves(shape):
+    *sizes, window, sinks, lengths = shape
+    q, k, v, _ = inputs(8, *sizes)
+    v[0, 0, sizes[4] - 1] = np.inf  # the last key: not seen by any but the last query
+    seen_last = slice(sizes[3] - 1, sizes[3])
+    want = attention_reference(q, k, np.where(np.isfinite(v), v, 0), window, sinks, np.float32(0.2), lengths)
+    out, lse = run(q, k, v, window, sinks, 0.2, lengths)
+    group = sizes[1] // sizes[2]
+    assert np.isinf(out[0, :group, seen_last]).all()
+    out[0, :group, seen_last] = want["out"][0][0, :group, seen_last]
+    assert_within(out, *want["out"], "out")
+    assert_within(lse, *want["lse"], "lse")
