@@ -360,7 +360,7 @@ int attention_forward(AttnArgs a, hipStream_t s, int cu_count) {
         a.row_tiles = (a.rows + kForwardRows - 1) / kForwardRows;
         blocks = heads * choose_parts(a, heads, cu_count);
     }
-    if (blocks * (few ? 1024 : 2 * kForwardRows) >> 32)  // a launch has fewer lanes
+    if (blocks * (few ? 64 * a.few_waves : 2 * kForwardRows) >> 32)  // a launch has fewer lanes
         return set_error(TRS_E_INVALID_ARGUMENT, "attention over %lld blocks of rows", (long long)blocks);
     a.part_width = (a.D + 3) / 4 * 4;
     const int64_t parts = a.splits * heads * a.rows, join_blocks = (heads * a.rows * (a.part_width / 4) + 255) / 256;
