@@ -158,7 +158,8 @@ struct Tile {
 // subnormals included, stands above bf16's least value and nothing is lost.
 // An infinity, a NaN or a value (or sum) beyond what is left of the range, 2^87 and
 // 2^47, shows as a result that is not finite; the block then does its rows again on
-// the fp32 instruction.
+// the fp32 instruction.  A score of -inf alone would show in no result, it weighs nothing:
+// scores are looked at before any is hidden (Lowest).
 constexpr float kUp = 0x1p40f, kDown = 0x1p-40f, kUp2 = 0x1p80f, kDown2 = 0x1p-80f;
 
 struct Pieces {
@@ -317,6 +318,21 @@ __device__ __forceinline__ void write_row(const at_f16 (&acc)[NT], float *p, flo
             }
         }
 }
+
+// Whether any score so far was -inf.  As unsigned numbers its bits are above those of every
+// score that is not NaN: a maximum of three takes two scores at a time, and no comparison.
+struct Lowest {
+    uint32_t bits = 0;
+    __device__ __forceinline__ void add(const at_f16 &s) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const uint32_t x = __builtin_bit_cast(uint32_t, s[e]);
+            bits = bits > x ? bits : x;
+        }
+    }
+    // Whether one is, in any lane of the wave.
+    __device__ __forceinline__ bool infinite() const { return __builtin_amdgcn_ballot_w64(bits >= 0xff800000u) != 0; }
+};
 
 // Whether a value is an infinity or NaN in any lane of the wave.
 template <int N>

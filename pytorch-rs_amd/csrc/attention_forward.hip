@@ -178,6 +178,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_rows(AttnArgs a) {
     RowState<NT> state;
     state.clear();
     if (t0 < t1) {
+        Lowest lowest;
         load(t0);
         Pieces q[2 * NT];
 #pragma unroll
@@ -211,6 +212,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_rows(AttnArgs a) {
                     [](Pieces &) {});
             }
             load(t + 2);
+            lowest.add(s);
             if (!r.all(a, j0)) {
 #pragma unroll
                 for (int e = 0; e < 16; e++) s[e] = sees(a, r.place, j0 + result_row(e, r.half)) ? s[e] : -__builtin_inff();
@@ -234,7 +236,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_rows(AttnArgs a) {
             }
         }
         __syncthreads();
-        notices.word[0][r.wave] = not_finite(state.acc, state.sum);
+        notices.word[0][r.wave] = not_finite(state.acc, state.sum) || lowest.infinite();
         __syncthreads();
         if (__builtin_expect(notices.any(0), 0)) {
             __syncthreads();

@@ -1,0 +1,99 @@
+"""Attention whose scores are large: sums beyond the range of the bf16 pieces, which hold
+a score up to 2^47, against 64 bits.  The scale of most tests is ln 2, whose product
+with log2(e) is 1 in fp32: scores of whole numbers are exact there, and so is what is
+compared, but for the weights' and the sums' own rounding."""
+import numpy as np
+import pytest
+
+from attention_util import EVERY, LEAST, U, Placed, assert_within, attention, ints, seen
+from trs_backend.abi import DeviceArray, check
+
+pytestmark = pytest.mark.gpu
+LN2 = np.float32(np.log(2))
+
+
+def exact(q, k, v, window, sinks, scale, lengths=None):
+    """{name: (value, bound)} of out and lse in 64 bits, for scores that fp32 holds exactly
+    or all off alike: weights are off by the exponential and the sums, (n + 16) u."""
+    B, H, sq, _ = q.shape
+    G, sk = H // k.shape[1], k.shape[2]
+    res = {"out": (np.zeros(q.shape), np.zeros(q.shape)), "lse": (np.full(q.shape[:3], -np.inf), np.zeros(q.shape[:3]))}
+    for b in range(B):
+        n = sk if lengths is None else lengths[b]
+        mask = seen(sq, n, window, sinks)
+        live = mask.any(1)
+        for h in range(H):
+            Q, K, V = (t.astype(np.float64) for t in (q[b, h][live], k[b, h // G, :n], v[b, h // G, :n]))
+            s = np.where(mask[live], Q @ K.T * float(scale), -np.inf)
+            top = s.max(1, keepdims=True)
+            e = np.exp(s - top)
+            P = e / e.sum(1, keepdims=True)
+            lse = (top + np.log(e.sum(1, keepdims=True)))[:, 0]
+            for name, value, bound in (("out", P @ V, 2 * (n + 16) * U * (P @ abs(V)) + n * LEAST),
+                                       ("lse", lse, (n + 16) * U + 16 * U * abs(lse))):
+                res[name][0][b, h, live], res[name][1][b, h, live] = value, bound
+    return res
+
+
+def values(seed, *shape):
+    return np.random.default_rng(seed).standard_normal(shape).astype(np.float32)
+
+
+def forward(q, k, v, window, sinks, scale, lengths=None):
+    out, rows = Placed(shape=q.shape), int(np.prod(q.shape[:3]))
+    lse = DeviceArray(4 * rows)
+    check(attention(*(Placed(t) for t in (q, k, v)), window, sinks, scale, out, lse, None if lengths is None else ints(lengths)))
+    got = {"out": out.numpy(), "lse": lse.to_numpy(count=rows).reshape(q.shape[:3])}
+    assert out.untouched()
+    return got
+
+
+def compare(got, want):
+    for name, value in got.items():
+        assert_within(value, *want[name], what=name)
+
+
+#        B  H hk  sq   sk  window sinks lengths
+SHAPES = [
+    (1, 2, 1, 100, 100, EVERY, 0, None),
+    (1, 1, 1, 300, 300, 40, 3, None),
+    (1, 1, 1, 1200, 1200, EVERY, 0, None),     # keys in parts
+    (2, 4, 2, 90, 400, 200, 5, [400, 61]),     # the first queries of the second sequence see nothing
+    (1, 2, 1, 3, 200, EVERY, 0, None),         # few rows
+]
+DIMS = (8, 32, 48, 64, 96, 128, 200)
+
+
+@pytest.mark.parametrize("D", DIMS)
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_finite_scores_far_below_zero(shape, D):
+    """Every score of -2^50 (they weigh alike), and scores of which the largest, far below
+    the others, weighs all."""
+    B, H, hk, sq, sk, *mask = shape
+    q, v = np.full((B, H, sq, D), 2.0 ** 24, np.float32), values(D, B, hk, sk, D)
+    k = np.zeros((B, hk, sk, D), np.float32)
+    k[..., 0] = -2.0 ** 26
+    compare(forward(q, k, v, *mask[:2], LN2, mask[2]), exact(q, k, v, *mask[:2], LN2, mask[2]))
+    k[..., 0] -= 2.0 ** 10 * np.arange(sk)
+    compare(forward(q, k, v, *mask[:2], LN2, mask[2]), exact(q, k, v, *mask[:2], LN2, mask[2]))
+
+
+def test_one_key_whatever_its_score():
+    """A first query sees itself alone: its output is its value's, 64 products of -1e14 each."""
+    q, k, v = np.full((1, 1, 70, 64), 1e7, np.float32), np.full((1, 1, 70, 64), -1e7, np.float32), values(0, 1, 1, 70, 64)
+    got = forward(q, k, v, EVERY, 0, 0.125)
+    assert np.array_equal(got["out"][0, 0, 0], v[0, 0, 0])
+    want = exact(q, k, v, EVERY, 0, 0.125)  # all scores are the same sum
+    compare({"out": got["out"]}, want)
+
+
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_sums_that_leave_the_range_on_their_way(shape, D):
+    """Half of a score's products are -2^45, the others 2^45: it is what is left, a small
+    whole number, though the first half's sum is beyond the pieces' range."""
+    B, H, hk, sq, sk, *mask = shape
+    q, k, v = np.full((B, H, sq, D), 2.0 ** 22, np.float32), np.zeros((B, hk, sk, D), np.float32), values(D, B, hk, sk, D)
+    k[:, :, ::2, : D // 2], k[:, :, ::2, D // 2:] = -2.0 ** 23, 2.0 ** 23
+    # Both halves' sums are multiples of 2^45, so nothing is rounded.
+    compare(forward(q, k, v, *mask[:2], LN2, mask[2]), exact(q, k, v, *mask[:2], LN2, mask[2]))
