@@ -88,6 +88,7 @@ __device__ __forceinline__ void rows_block(const AttnArgs &a, uint32_t id, char 
 #pragma unroll
     for (int t = 0; t < NT; t++) acc[t] = (at_f16)(0.f);
     if (r.tiles > 0) {
+        Lowest lowest;
         load(0);
         Pieces qp[2 * NT], up[2 * NT];
 #pragma unroll
@@ -121,6 +122,7 @@ __device__ __forceinline__ void rows_block(const AttnArgs &a, uint32_t id, char 
                     [](Pieces &) {});
             }
             load(t + 2);
+            lowest.add(s);
             if (!r.all(a, j0)) {
 #pragma unroll
                 for (int e = 0; e < 16; e++) s[e] = sees(a, r.place, j0 + result_row(e, r.half)) ? s[e] : -__builtin_inff();
@@ -144,7 +146,7 @@ __device__ __forceinline__ void rows_block(const AttnArgs &a, uint32_t id, char 
                 [](Pieces &) {});
         }
         __syncthreads();
-        notices.word[1][r.wave] = not_finite(acc, 0.f);
+        notices.word[1][r.wave] = not_finite(acc, 0.f) || lowest.infinite();
         __syncthreads();
         if (__builtin_expect(notices.any(1), 0)) {
             grad_rows_fp32<NT, NW>(a, r, lse, delta, (float *)lds, acc);
@@ -296,6 +298,7 @@ __device__ __forceinline__ void keys_block(const AttnArgs &a, uint32_t id, char 
     for (int t = 0; t < NT; t++) dk[t] = dv[t] = (at_f16)(0.f);
     bool again = false;
     if (k.t0 < k.t1) {
+        Lowest lowest;
         load(k.t0);
         const bool live = k.key < k.keys;
         const int key = live ? k.key : 0;
@@ -332,6 +335,7 @@ __device__ __forceinline__ void keys_block(const AttnArgs &a, uint32_t id, char 
 #pragma unroll
             for (int e = 0; e < 16; e++) lse16[e] = facts.lse[n2][result_row(e, k.half)];
             store_facts(n2 ^ 1);
+            lowest.add(p);
             if (!k.all(a, t)) {
 #pragma unroll
                 for (int e = 0; e < 16; e++) p[e] = k.pair(a, facts.place[n2][result_row(e, k.half)]) ? p[e] : -__builtin_inff();
@@ -369,7 +373,7 @@ __device__ __forceinline__ void keys_block(const AttnArgs &a, uint32_t id, char 
             }
         }
         __syncthreads();
-        notices.word[0][k.wave] = not_finite(dk, 0.f) || not_finite(dv, 0.f);
+        notices.word[0][k.wave] = not_finite(dk, 0.f) || not_finite(dv, 0.f) || lowest.infinite();
         __syncthreads();
         again = notices.any(0);
         if (__builtin_expect(again, 0)) {

@@ -5,7 +5,7 @@ compared, but for the weights' and the sums' own rounding."""
 import numpy as np
 import pytest
 
-from attention_util import EVERY, LEAST, U, Placed, assert_within, attention, ints, seen
+from attention_util import EVERY, LEAST, U, Placed, assert_within, attention, attention_grad, ints, seen
 from trs_backend.abi import DeviceArray, check
 
 pytestmark = pytest.mark.gpu
@@ -35,6 +35,38 @@ def exact(q, k, v, window, sinks, scale, lengths=None):
     return res
 
 
+def exact_gradients(q, k, v, window, sinks, scale, up, lengths=None):
+    """{name: (value, bound)} of dq, dk and dv for such scores.  A weight is read back from the
+    row's logarithm, which is off by up to 2^-15 of itself however large it is; the rest are
+    sums of magnitudes."""
+    B, H, sq, D = q.shape
+    G, sk = H // k.shape[1], k.shape[2]
+    R = sq * G
+    res = {n: (np.zeros(t.shape), np.zeros(t.shape)) for n, t in (("dq", q), ("dk", k), ("dv", v))}
+    for b in range(B):
+        n = sk if lengths is None else lengths[b]
+        mask = seen(sq, n, window, sinks)
+        live = mask.any(1)
+        for h in range(H):
+            kv = h // G
+            Q, K, V, W = (t.astype(np.float64) for t in (q[b, h][live], k[b, kv, :n], v[b, kv, :n], up[b, h][live]))
+            s = np.where(mask[live], Q @ K.T * float(scale), -np.inf)
+            P = np.exp(s - s.max(1, keepdims=True))
+            P /= P.sum(1, keepdims=True)
+            o = P @ V
+            dS = P * (W @ V.T - (W * o).sum(1, keepdims=True)) * float(scale)
+            A = P * (abs(W) @ abs(V).T + (abs(W) * (P @ abs(V))).sum(1, keepdims=True)) * abs(float(scale))
+            rel = (2 * n + 32) * U + 2.0 ** -15
+            eS = A * (2 * rel + (2 * D + 32) * U) + LEAST * (1 + A / np.where(P > 0, P, 1))
+            res["dq"][0][b, h, live] = dS @ K
+            res["dq"][1][b, h, live] = eS @ abs(K) + (n + 16) * U * (A @ abs(K))
+            res["dk"][0][b, kv, :n] += dS.T @ Q
+            res["dk"][1][b, kv, :n] += eS.T @ abs(Q) + (R + 64) * U * (A.T @ abs(Q)) + R * LEAST
+            res["dv"][0][b, kv, :n] += P.T @ W
+            res["dv"][1][b, kv, :n] += rel * (P.T @ abs(W)) + (R + 64) * U * (P.T @ abs(W)) + LEAST * (R + abs(W).sum(0))
+    return res
+
+
 def values(seed, *shape):
     return np.random.default_rng(seed).standard_normal(shape).astype(np.float32)
 
@@ -45,6 +77,17 @@ def forward(q, k, v, window, sinks, scale, lengths=None):
     check(attention(*(Placed(t) for t in (q, k, v)), window, sinks, scale, out, lse, None if lengths is None else ints(lengths)))
     got = {"out": out.numpy(), "lse": lse.to_numpy(count=rows).reshape(q.shape[:3])}
     assert out.untouched()
+    return got
+
+
+def gradients(q, k, v, window, sinks, scale, up, lengths=None):
+    P, out, lse = [Placed(t) for t in (q, k, v)], Placed(shape=q.shape), DeviceArray(4 * int(np.prod(q.shape[:3])))
+    lens = None if lengths is None else ints(lengths)
+    check(attention(*P, window, sinks, scale, out, lse, lens))
+    grads = [Placed(shape=t.shape) for t in (q, k, v)]
+    check(attention_grad(*P, window, sinks, scale, out, lse, Placed(up), *grads, lens))
+    got = dict(zip(("dq", "dk", "dv"), (g.numpy() for g in grads)))
+    assert all(g.untouched() for g in grads)
     return got
 
 
@@ -97,3 +140,5 @@ def test_sums_that_leave_the_range_on_their_way(shape, D):
     k[:, :, ::2, : D // 2], k[:, :, ::2, D // 2:] = -2.0 ** 23, 2.0 ** 23
     # Both halves' sums are multiples of 2^45, so nothing is rounded.
     compare(forward(q, k, v, *mask[:2], LN2, mask[2]), exact(q, k, v, *mask[:2], LN2, mask[2]))
+    up = values(D + 1, *q.shape)
+    compare(gradients(q, k, v, *mask[:2], LN2, up, mask[2]), exact_gradients(q, k, v, *mask[:2], LN2, up, mask[2]))
