@@ -412,8 +412,11 @@ int trs_window_attention_f32(const float *q, const trs_layout *lq, const float *
                              int64_t sinks, float scale, float *out, const trs_layout *lo, float *lse);
 /* Its gradients, from the forward call's arguments, out and lse, and the
  * upstream gradient of out; those of a shared key head are summed over its query
- * heads, and keys that no query sees get 0.  No atomic adds: the result is the
- * same bits each time.  Takes a workspace from the block cache. */
+ * heads, and keys that no query sees get 0.  The softmax is taken from lse; of a
+ * row whose lse is beyond 256 either way one float would hold it in too few bits,
+ * and maximum and sum are worked out again (up to twice the time, where all rows
+ * are such).  No atomic adds: the result is the same bits each time.  Takes a
+ * workspace from the block cache. */
 int trs_window_attention_backward_f32(const float *q, const trs_layout *lq, const float *k, const trs_layout *lk,
                                       const float *v, const trs_layout *lv, const int32_t *lengths, int64_t window,
                                       int64_t sinks, float scale, const float *out, const trs_layout *lo,

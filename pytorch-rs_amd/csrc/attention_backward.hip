@@ -1,7 +1,7 @@
 // attention_backward.hip -- the gradients of attention.h's attention: their host part,
 // and what comes before and after the products.
 //
-// With P = exp(scale Q K^T - lse) over the pairs that see each other and
+// With P = exp(scale Q K^T - lse) (of a row: RowFacts) over the pairs that see each other and
 // delta = rowsum(dO o):
 //   dS = P (dO V^T - delta),  dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO.
 // P and dO V^T are worked out twice, over rows for dQ and over keys for dK and dV (seven
@@ -23,24 +23,141 @@ namespace {
 // (2 x 2048 tokens, whose parts are longer, alike).
 constexpr int kPartTiles = 2;
 
-// delta of every row: 16 lanes a row.
-__global__ void __launch_bounds__(256) attn_delta(AttnArgs a, float *delta) {
-    const int64_t rows = (int64_t)a.batch * a.heads * a.Sq;
-    const int sub = (int)threadIdx.x & 15;
-    const int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-    float s = 0.f;
-    if (r < rows) {
-        const int64_t bh = r / a.Sq, i = r - bh * a.Sq, b = bh / a.heads, h = bh - b * a.heads;
-        const float *o = a.out + b * a.os.b + h * a.os.h + i * a.os.s, *u = a.up + b * a.us.b + h * a.us.h + i * a.us.s;
-        for (int d = sub * 4; d < a.D; d += 64) {
-            const at_f4 x = row_chunk(o, d, a.D), y = row_chunk(u, d, a.D);
+// Maximum and sum of the lane's row, over the keys that it sees: R rows a wave, lane l has row
+// l % R and a tile's keys key(register, l / R) of the scores that tile(key's row) gives, in `unit`s.
+// Straight from memory, few rows need it.
+template <int R, class Key, class Tile>
+__device__ __forceinline__ void statistics(const AttnArgs &a, const Sequence &seq, int b, int hk, int r0, int r1, int place, float unit,
+                                           Key &&key, Tile &&tile, float &base, float &share) {
+    constexpr int E = R * R / 64;
+    const int lane = (int)threadIdx.x & 63;
+    const KeyTiles<R == 32 ? 5 : 4> keys(a, seq, r0, r1);
+    const float *kb = a.k + b * a.ks.b + hk * a.ks.h;
+    float most = -__builtin_inff(), sum = 0.f;
+#pragma unroll 1
+    for (int t = 0; t < keys.tiles; t++) {
+        const int j0 = keys.first_key(t);
+        auto s = tile(kb + (int64_t)min(j0 + lane % R, keys.key_hi) * a.ks.s);
+        float m = -__builtin_inff();
 #pragma unroll
-            for (int e = 0; e < 4; e++) s += x[e] * y[e];
+        for (int e = 0; e < E; e++) {
+            s[e] = sees(a, place, j0 + key(e, lane / R)) ? s[e] : -__builtin_inff();
+            m = __builtin_fmaxf(m, s[e]);
         }
+#pragma unroll
+        for (int d = R; d < 64; d *= 2) m = __builtin_fmaxf(m, __shfl_xor(m, d));
+        const float now = __builtin_fmaxf(most, m), from = now == -__builtin_inff() ? 0.f : now;
+        sum *= __builtin_amdgcn_exp2f((most - from) * unit);
+#pragma unroll
+        for (int e = 0; e < E; e++) sum += __builtin_amdgcn_exp2f((s[e] - from) * unit);
+        most = now;
     }
 #pragma unroll
-    for (int d = 1; d < 16; d *= 2) s += __shfl_xor(s, d);
-    if (r < rows && sub == 0) delta[r] = s;
+    for (int d = R; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+    base = most * unit, share = 1.f / sum;
+}
+
+// The facts of 16 rows of a key head a wave (333 tokens, 4 heads of 32 3.7 us, with 32 rows 4.6; 4096
+// tokens, 32 heads of 128 22.4 and 24.5).
+template <bool WIDE>
+__global__ void __launch_bounds__(64) attn_facts(AttnArgs a) {
+    constexpr int R = 16, COLS = WIDE ? 16 : 32;  // of a product
+    const int lane = (int)threadIdx.x, sub = lane & 15;
+    const uint32_t tiles = (uint32_t)(a.rows + R - 1) / R, rest = blockIdx.x / (uint32_t)a.kv_heads;
+    const int hk = (int)(blockIdx.x % (uint32_t)a.kv_heads), tile = (int)(rest % tiles), b = (int)(rest / tiles);
+    const int r0 = tile * R, r1 = min(r0 + R, a.rows);
+    // Query, head and [batch, head, token] of a row of the wave.
+    const auto find = [&](int n, int &i, int &h) {
+        const int row = min(r0 + n, r1 - 1);
+        i = (int)a.by_group.divide((uint32_t)row), h = hk * a.group + row - i * a.group;
+        return ((int64_t)b * a.heads + h) * a.Sq + i;
+    };
+    int i, h;
+    const int64_t at = find(lane % COLS, i, h);
+    const Sequence seq = sequence_of(a, b);
+    const int place = seq.first + i;
+    const float lse = a.lse[at];
+    // delta: 16 lanes a row, the rows' loads together.
+    float delta[R / 4] = {};
+    const float *out[R / 4], *up[R / 4];
+#pragma unroll
+    for (int n = 0; n < R / 4; n++) {
+        int i, h;
+        find(4 * n + lane / 16, i, h);
+        out[n] = a.out + b * a.os.b + h * a.os.h + i * a.os.s, up[n] = a.up + b * a.us.b + h * a.us.h + i * a.us.s;
+    }
+    const auto add = [&](auto &&chunk) {
+        for (int d = sub * 4; d < a.D; d += 64)
+#pragma unroll
+            for (int n = 0; n < R / 4; n++) {
+                const at_f4 x = chunk(out[n], d), y = chunk(up[n], d);
+#pragma unroll
+                for (int e = 0; e < 4; e++) delta[n] += x[e] * y[e];
+            }
+    };
+    if (a.D % 4 == 0) add([](const float *p, int d) { return __builtin_bit_cast(at_f4, *(const f4u *)(p + d)); });
+    else add([&](const float *p, int d) { return row_chunk(p, d, a.D); });
+    float base = lse * kLog2e, base32 = base;
+    float share = __builtin_amdgcn_exp2f(-(__builtin_fmaf(lse, kLog2e, -base) + lse * kLog2eLow)), share32 = share;
+    const bool again = place >= 0 && !(__builtin_fabsf(lse) <= kMostLse);
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(again) != 0, 0)) {
+        const float *q = a.q + b * a.qs.b + h * a.qs.h + i * a.qs.s;
+        const auto row = [&](int c) { return row_chunk(q, c, a.D) * a.scale2; };
+        const int mine = r0 + lane % COLS < r1 ? place : -1;
+        float x, y;
+        if constexpr (WIDE) {
+            statistics<16>(
+                a, seq, b, hk, r0, r1, mine, 1.f, [](int e, int quarter) { return 4 * quarter + e; },
+                [&](const float *k) {
+                    at_f4 c = (at_f4)(0.f);
+#pragma unroll 1
+                    for (int j = 0; j < a.D; j += 16) {
+                        const at_f4 u = row_chunk(k, j + 4 * (lane >> 4), a.D), w = row(j + 4 * (lane >> 4));
+#pragma unroll
+                        for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(u[e], w[e], c, 0, 0, 0);
+                    }
+                    return c;
+                },
+                x, y);
+        } else {
+            const auto key = [](int e, int half) { return result_row(e, half); };
+            statistics<32>(
+                a, seq, b, hk, r0, r1, mine, kDown2, key,
+                [&](const float *k) {
+                    at_f16 c = (at_f16)(0.f);
+#pragma unroll 1
+                    for (int u = 0; 16 * u < a.D; u++) {
+                        Unit<1> n, m;
+#pragma unroll
+                        for (int e = 0; e < 8; e += 4) {
+                            const int d = 16 * u + 8 * (lane >> 5) + e;
+                            const at_f4 x = row_chunk(k, d, a.D), y = row_chunk(q, d, a.D);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) n.v[e + i] = x[i], m.v[e + i] = y[i];
+                        }
+                        mfma_pieces<true>(c, n.split(kUp), m.split(a.scale2 * kUp));
+                    }
+                    return c;
+                },
+                x, y);
+            if (again) base = x, share = y;
+            statistics<32>(
+                a, seq, b, hk, r0, r1, mine, 1.f, key,
+                [&](const float *k) { return product_fp32(a.D, lane >> 5, [&](int c) { return row_chunk(k, c, a.D); }, row); }, x, y);
+        }
+        if (again) base32 = x, share32 = y;
+    }
+    if (lane < r1 - r0) {
+        a.facts.pieces.base[at] = base, a.facts.pieces.share[at] = share * kUp;
+        a.facts.fp32.base[at] = base32, a.facts.fp32.share[at] = share32;
+    }
+#pragma unroll
+    for (int n = 0; n < R / 4; n++) {
+#pragma unroll
+        for (int d = 1; d < 16; d *= 2) delta[n] += __shfl_xor(delta[n], d);
+        const int row = 4 * n + lane / 16;
+        if (sub == 0 && row < r1 - r0) a.facts.delta[find(row, i, h)] = delta[n];
+    }
 }
 
 // dk and dv of the first `count` keys: the parts over the rows, or what the one part
@@ -106,21 +223,23 @@ int attention_backward(AttnArgs a, hipStream_t s, int cu_count) {
     const int far = a.sink_tiles ? a.sink_splits : 0;
     const int64_t row_blocks = heads * a.row_tiles;
     const int64_t key_blocks = heads * (a.sink_tiles * a.sink_splits + (int64_t)a.key_tiles * a.row_splits);
-    const int64_t delta_blocks = ((int64_t)a.batch * a.heads * a.Sq + 15) / 16;
-    if ((row_blocks + key_blocks) >> 24 || delta_blocks >> 24)  // a launch has fewer than 2^32 lanes
+    const int64_t fact_units = heads * ((a.rows + 15) / 16);
+    if ((row_blocks + key_blocks) >> 24 || fact_units >> 25)  // a launch has fewer than 2^32 lanes
         return set_error(TRS_E_INVALID_ARGUMENT, "attention gradient over too many blocks");
-    const int64_t deltas = ((int64_t)a.batch * a.heads * a.Sq + 63) / 64 * 64;
+    const int64_t facts = ((int64_t)a.batch * a.heads * a.Sq + 63) / 64 * 64;
     const int64_t sink_floats = heads * a.sink_tiles * far * block * a.D;
     const int64_t part_floats = a.row_splits > 1 ? heads * a.row_splits * a.Sk * a.D : 0;
     void *ws = nullptr;
-    TRS_CHECK(trs_alloc((size_t)(deltas + 2 * sink_floats + 2 * part_floats) * sizeof(float), &ws));
-    float *delta = (float *)ws;
-    a.delta = delta;
-    a.sink_k = delta + deltas, a.sink_v = a.sink_k + sink_floats;
+    TRS_CHECK(trs_alloc((size_t)(5 * facts + 2 * sink_floats + 2 * part_floats) * sizeof(float), &ws));
+    float *const f = (float *)ws;
+    a.facts = RowFacts{f, {f + facts, f + 2 * facts}, {f + 3 * facts, f + 4 * facts}};
+    a.sink_k = f + 5 * facts, a.sink_v = a.sink_k + sink_floats;
     a.part_k = a.sink_v + sink_floats, a.part_v = a.part_k + part_floats;
     const auto launch = [&]() -> int {
         // No rows: the keys' gradients are 0.  No keys: the rows' are.
-        if (delta_blocks) hipLaunchKernelGGL(attn_delta, dim3((unsigned)delta_blocks), dim3(256), 0, s, a, delta);
+        const dim3 fact_blocks((unsigned)fact_units);
+        if (fact_units && wide) hipLaunchKernelGGL(attn_facts<true>, fact_blocks, dim3(64), 0, s, a);
+        else if (fact_units) hipLaunchKernelGGL(attn_facts<false>, fact_blocks, dim3(64), 0, s, a);
         TRS_LAUNCH_CHECK("attention gradient launch");
         if (key_blocks + row_blocks) {
             if (wide) launch_attention_grad_wide(a, (uint32_t)key_blocks, (uint32_t)row_blocks, s);

@@ -34,11 +34,12 @@ __device__ __forceinline__ float up_exp2(float x) {
 
 // The block's rows on the fp32 instruction, whatever the values.
 template <int NT, int NW>
-__device__ __forceinline__ void grad_rows_fp32(const AttnArgs &a, const RowBlock<NW> &r, float lse, float delta, float *lds,
+__device__ __forceinline__ void grad_rows_fp32(const AttnArgs &a, const RowBlock<NW> &r, float delta, float *lds,
                                                at_f16 (&acc)[NT]) {
     using T = Tile<NT, 64 * NW>;
     const float *kb = a.k + r.b * a.ks.b + r.hk * a.ks.h, *vb = a.v + r.b * a.vs.b + r.hk * a.vs.h;
     const float *q = r.place >= 0 ? a.q + r.at(a, a.qs) : nullptr, *u = r.place >= 0 ? a.up + r.at(a, a.us) : nullptr;
+    const float base = r.place >= 0 ? a.facts.fp32.base[r.index(a)] : 0.f, share = r.place >= 0 ? a.facts.fp32.share[r.index(a)] : 0.f;
 #pragma unroll
     for (int t = 0; t < NT; t++) acc[t] = (at_f16)(0.f);
 #pragma unroll 1
@@ -52,7 +53,7 @@ __device__ __forceinline__ void grad_rows_fp32(const AttnArgs &a, const RowBlock
             const at_f16 d = T::times_row(lds + T::kFloats, u, a.D, 1.f, r.lane);
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-                s[e] = __builtin_amdgcn_exp2f(s[e] - lse) * (d[e] - delta);
+                s[e] = __builtin_exp2f(s[e] - base) * share * (d[e] - delta);
                 if (!sees(a, r.place, j0 + result_row(e, r.half))) s[e] = 0.f;
             }
             T::add_product_seen(acc, lds, s, r.lane, [&](int k) { return sees(a, r.place, j0 + k); });
@@ -83,7 +84,7 @@ __device__ __forceinline__ void rows_block(const AttnArgs &a, uint32_t id, char 
     };
     const bool live = r.place >= 0;
     const int64_t at = r.index(a);
-    const float lse = live ? a.lse[at] * kLog2e : 0.f, delta = live ? a.delta[at] : 0.f;
+    const float base = live ? a.facts.pieces.base[at] : 0.f, share = live ? a.facts.pieces.share[at] : 0.f, delta = live ? a.facts.delta[at] : 0.f;
     at_f16 acc[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) acc[t] = (at_f16)(0.f);
@@ -97,7 +98,7 @@ __device__ __forceinline__ void rows_block(const AttnArgs &a, uint32_t id, char 
             x.load(a.q + r.at(a, a.qs), s, a.D, r.lane, s < 2 * NT - 2);
             qp[s] = x.split(live ? a.scale2 * kUp : 0.f);
             x.load(a.up + r.at(a, a.us), s, a.D, r.lane, s < 2 * NT - 2);
-            up[s] = x.split(live ? kUp : 0.f);
+            up[s] = x.split(share);
         }
 #pragma unroll
         for (int n = 0; n < OWN; n++) in[n].template store<UNITS>(lds, r.wave + n * NW, r.lane);
@@ -107,15 +108,19 @@ __device__ __forceinline__ void rows_block(const AttnArgs &a, uint32_t id, char 
             const int j0 = r.first_key(t);
             char *const buf = lds + (t & 1) * kBuffer, *const other = lds + (t & 1 ? 0 : kBuffer);
             __syncthreads();
-            // dO V^T - delta, times 2^80: the sum starts from -delta.  (The scores' does not start
-            // from -lse: it is the larger part, and every product would be rounded to it.)
-            at_f16 s = (at_f16)(0.f), d = (at_f16)(-delta * kUp2);
+            // share (dO V^T - delta), times 2^80: the sum starts from delta's part.  (The scores' does
+            // not start from -base: it is the larger part, and every product would be rounded to it.)
+            at_f16 s = (at_f16)(0.f), d = (at_f16)(-delta * (share * kUp));
             Splitting x;
             {
                 const auto read = [&](int n) { return along<UNITS>(buf, (n & 1) * 2 * NT + n / 2, r.lane); };
                 Pieces f = read(0);
                 steps<4 * NT>(
-                    f, read, [&](int n, const Pieces &now) { mfma_pieces(n & 1 ? d : s, now, n & 1 ? up[n / 2] : qp[n / 2]); },
+                    f, read,
+                    [&](int n, const Pieces &now) {
+                        if (n & 1) mfma_pieces(d, now, up[n / 2]);
+                        else mfma_pieces<true>(s, now, qp[n / 2]);  // the scores of keys_block, bit for bit
+                    },
                     [&](int n) {
                         dealt(4 * OWN, n, 4 * NT, [&](int i) { in[i / 4].template store_pair<UNITS>(x, i % 4, other, r.wave + i / 4 * NW, r.lane); });
                     },
@@ -127,8 +132,9 @@ __device__ __forceinline__ void rows_block(const AttnArgs &a, uint32_t id, char 
 #pragma unroll
                 for (int e = 0; e < 16; e++) s[e] = sees(a, r.place, j0 + result_row(e, r.half)) ? s[e] : -__builtin_inff();
             }
-            const auto weigh = [&](int e) {  // 2^40 dS
-                return __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], kDown2, -lse)) * (d[e] * kDown);
+            const auto weigh = [&](int e) {  // 2^40 dS; the weight's root is not subnormal where the weight is
+                const float root = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], kDown2 / 2, -base / 2));
+                return root * (root * (d[e] * kDown));
             };
             const auto read = [&](int n) { return across<UNITS>(buf, 2 * (n % NT), n / NT, r.lane); };
             Pieces f = read(0);
@@ -149,7 +155,7 @@ __device__ __forceinline__ void rows_block(const AttnArgs &a, uint32_t id, char 
         notices.word[1][r.wave] = not_finite(acc, 0.f) || lowest.infinite();
         __syncthreads();
         if (__builtin_expect(notices.any(1), 0)) {
-            grad_rows_fp32<NT, NW>(a, r, lse, delta, (float *)lds, acc);
+            grad_rows_fp32<NT, NW>(a, r, delta, (float *)lds, acc);
             if (r.row < a.rows) T::write(acc, a.dq + r.at(a, a.dqs), a.scale, a.D, r.half);
             return;
         }
@@ -208,14 +214,15 @@ struct KeyBlock {
 };
 
 // A tile's rows, as the waves of a block share them; two tiles in turn.
-struct RowFacts {
-    float lse[2][kTile];    // in base 2
-    float delta[2][kTile];  // -2^80 delta, what the sum of dO V^T starts from
+struct TileFacts {
+    float base[2][kTile];
+    float delta[2][kTile];  // -2^80 share delta, what the sum of share dO V^T starts from
     int place[2][kTile];    // -1: past the last row
+    float share[kTile];     // for the fp32 form, whose delta is delta
 };
 
 template <int NT>
-__device__ __forceinline__ void grad_keys_fp32(const AttnArgs &a, const KeyBlock &k, float *lds, RowFacts &facts,
+__device__ __forceinline__ void grad_keys_fp32(const AttnArgs &a, const KeyBlock &k, float *lds, TileFacts &facts,
                                                at_f16 (&dk)[NT], at_f16 (&dv)[NT]) {
     using T = Tile<NT, 256>;
     const bool live = k.key < k.keys;
@@ -236,23 +243,23 @@ __device__ __forceinline__ void grad_keys_fp32(const AttnArgs &a, const KeyBlock
         T::stage(lds + T::kFloats, a.D, [&](int r) { return row_at(a.up, a.us, r); });
         if (threadIdx.x < kTile) {
             const int row = r0 + (int)threadIdx.x;
-            float lse = 0.f, delta = 0.f;
+            float base = 0.f, delta = 0.f, share = 0.f;
             int place = -1;
             if (row < k.rhi) {
                 const int i = (int)a.by_group.divide((uint32_t)row), g = row - i * a.group;
                 const int64_t at = ((int64_t)k.b * a.heads + k.hk * a.group + g) * a.Sq + i;
-                lse = a.lse[at] * kLog2e, delta = a.delta[at], place = k.first + i;
+                base = a.facts.fp32.base[at], share = a.facts.fp32.share[at], delta = a.facts.delta[at], place = k.first + i;
             }
-            facts.lse[0][threadIdx.x] = lse, facts.delta[0][threadIdx.x] = delta, facts.place[0][threadIdx.x] = place;
+            facts.base[0][threadIdx.x] = base, facts.delta[0][threadIdx.x] = delta, facts.place[0][threadIdx.x] = place, facts.share[threadIdx.x] = share;
         }
         __syncthreads();
         {
-            at_f16 p = T::times_row(lds, kp, a.D, a.scale2, k.lane);
+            at_f16 p = T::times_row(lds, kp, a.D, 1.f, k.lane, a.scale2);
             at_f16 d = T::times_row(lds + T::kFloats, vp, a.D, 1.f, k.lane);
 #pragma unroll
             for (int e = 0; e < 16; e++) {
                 const int r = result_row(e, k.half);
-                p[e] = __builtin_exp2f(p[e] - facts.lse[0][r]);
+                p[e] = __builtin_exp2f(p[e] - facts.base[0][r]) * facts.share[r];
                 d[e] = p[e] * (d[e] - facts.delta[0][r]);
                 if (!k.pair(a, facts.place[0][r])) p[e] = d[e] = 0.f;
             }
@@ -266,7 +273,7 @@ __device__ __forceinline__ void grad_keys_fp32(const AttnArgs &a, const KeyBlock
 
 // A block of 128 keys over the row tiles that make pairs with them.
 template <int NT, int WIDTH>
-__device__ __forceinline__ void keys_block(const AttnArgs &a, uint32_t id, char *lds, RowFacts &facts, Notices<4> &notices) {
+__device__ __forceinline__ void keys_block(const AttnArgs &a, uint32_t id, char *lds, TileFacts &facts, Notices<4> &notices) {
     using T = Tile<NT, 256>;
     constexpr int UNITS = 4 * NT, kBuffer = 3 * UNITS * 1024;  // of queries and upstream rows
     const KeyBlock k(a, id);
@@ -275,7 +282,7 @@ __device__ __forceinline__ void keys_block(const AttnArgs &a, uint32_t id, char 
     // A lane's row of a tile, and what the waves share of it.  Past the part's last tile
     // that one is loaded, past the last row that one.
     Unit<WIDTH> in[NT];
-    float lse = 0.f, delta = 0.f;
+    float base = 0.f, delta = 0.f, share = 0.f;
     int place = -1;
     const auto load = [&](int t) {
         const int at = k.rlo + min(t, k.t1 - 1) * kTile + (k.lane & 31), row = min(at, k.rhi - 1);
@@ -287,11 +294,14 @@ __device__ __forceinline__ void keys_block(const AttnArgs &a, uint32_t id, char 
             in[n].load(unit < 2 * NT ? q : u, unit < 2 * NT ? unit : unit - 2 * NT, a.D, k.lane);
         }
         const int64_t fact = ((int64_t)k.b * a.heads + k.hk * a.group + g) * a.Sq + i;
-        lse = a.lse[fact], delta = a.delta[fact];
+        base = a.facts.pieces.base[fact], share = a.facts.pieces.share[fact], delta = a.facts.delta[fact];
         place = at < k.rhi ? k.first + i : -1;
     };
+    // Queries are scaled, as rows_block has them, and upstream rows taken times their share.
+    const float up_q = kUp * a.scale2;
+    const auto up_to = [&](int n) { return 4 * n + 4 <= 2 * NT || (4 * n < 2 * NT && k.wave + 4 * n < 2 * NT) ? up_q : share; };
     const auto store_facts = [&](int n) {
-        if (threadIdx.x < kTile) facts.lse[n][threadIdx.x] = lse * kLog2e, facts.delta[n][threadIdx.x] = delta * -kUp2, facts.place[n][threadIdx.x] = place;
+        if (threadIdx.x < kTile) facts.base[n][threadIdx.x] = base, facts.delta[n][threadIdx.x] = delta * (share * -kUp), facts.place[n][threadIdx.x] = place;
     };
     at_f16 dk[NT], dv[NT];
 #pragma unroll
@@ -307,12 +317,12 @@ __device__ __forceinline__ void keys_block(const AttnArgs &a, uint32_t id, char 
         for (int s = 0; s < 2 * NT; s++) {
             Unit<WIDTH> x;
             x.load(a.k + k.b * a.ks.b + k.hk * a.ks.h + (int64_t)key * a.ks.s, s, a.D, k.lane, s < 2 * NT - 2);
-            kp[s] = x.split(live ? a.scale2 * kUp : 0.f);
+            kp[s] = x.split(live ? kUp : 0.f);
             x.load(a.v + k.b * a.vs.b + k.hk * a.vs.h + (int64_t)key * a.vs.s, s, a.D, k.lane, s < 2 * NT - 2);
             vp[s] = x.split(live ? kUp : 0.f);
         }
 #pragma unroll
-        for (int n = 0; n < NT; n++) in[n].template store<UNITS>(lds, k.wave + 4 * n, k.lane);
+        for (int n = 0; n < NT; n++) in[n].template store<UNITS>(lds, k.wave + 4 * n, k.lane, up_to(n));
         store_facts(0);
         load(k.t0 + 1);
 #pragma unroll 1
@@ -329,11 +339,11 @@ __device__ __forceinline__ void keys_block(const AttnArgs &a, uint32_t id, char 
                 Pieces f = read(0);
                 steps<4 * NT>(
                     f, read, [&](int n, const Pieces &now) { mfma_pieces(n & 1 ? d : p, now, n & 1 ? vp[n / 2] : kp[n / 2]); },
-                    [&](int n) { in[n / 4].template store_pair<UNITS>(x, n % 4, other, k.wave + n / 4 * 4, k.lane); }, [](Pieces &) {});
+                    [&](int n) { in[n / 4].template store_pair<UNITS>(x, n % 4, other, k.wave + n / 4 * 4, k.lane, up_to(n / 4)); }, [](Pieces &) {});
             }
-            at_f16 lse16;
+            at_f16 base16;
 #pragma unroll
-            for (int e = 0; e < 16; e++) lse16[e] = facts.lse[n2][result_row(e, k.half)];
+            for (int e = 0; e < 16; e++) base16[e] = facts.base[n2][result_row(e, k.half)];
             store_facts(n2 ^ 1);
             lowest.add(p);
             if (!k.all(a, t)) {
@@ -341,7 +351,7 @@ __device__ __forceinline__ void keys_block(const AttnArgs &a, uint32_t id, char 
                 for (int e = 0; e < 16; e++) p[e] = k.pair(a, facts.place[n2][result_row(e, k.half)]) ? p[e] : -__builtin_inff();
             }
             // 2^40 P and 2^40 dS come pair by pair, each eight of them ahead of the products that take them.
-            const auto pair_p = [&](int e) { return p[e] = up_exp2(__builtin_fmaf(p[e], kDown2, -lse16[e])); };
+            const auto pair_p = [&](int e) { return p[e] = up_exp2(__builtin_fmaf(p[e], kDown2, -base16[e])); };
             const auto pair_d = [&](int e) { return p[e] * (d[e] * kDown2); };
             // dV's first 16 rows, its others, dK's first, its others.
             const auto read = [&](int n) { return across<UNITS>(buf, (n < 2 * NT ? 2 * NT : 0) + 2 * (n % NT), n / NT % 2, k.lane); };
@@ -397,7 +407,7 @@ __device__ __forceinline__ void keys_block(const AttnArgs &a, uint32_t id, char 
         T::write(dk, pk, a.scale, a.D, k.half);
         T::write(dv, pv, 1.f, a.D, k.half);
     } else {
-        write_row<WIDTH>(dk, pk, kDown2, a.scale, a.D, k.half);
+        write_row<WIDTH>(dk, pk, kDown2, kLn2, a.D, k.half);  // scale / scale2
         write_row<WIDTH>(dv, pv, kDown2, 1.f, a.D, k.half);
     }
 }
@@ -410,7 +420,7 @@ __global__ void __launch_bounds__(256, NT <= 2 ? 2 : 1) attn_grad(AttnArgs a, ui
     constexpr int kBytes = 2 * 3 * 4 * NT * 1024;
     static_assert(kBytes >= 8 * T::kFloats, "the fp32 tiles fit the pieces' LDS");
     __shared__ __attribute__((aligned(1024))) char lds[kBytes];
-    __shared__ RowFacts facts;
+    __shared__ TileFacts facts;
     __shared__ Notices<4> notices;
     if (blockIdx.x < key_blocks) keys_block<NT, WIDTH>(a, blockIdx.x, lds, facts, notices);
     else rows_block<NT, WIDTH>(a, blockIdx.x - key_blocks, lds, notices);

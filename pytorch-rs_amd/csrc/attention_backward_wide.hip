@@ -41,11 +41,12 @@ __device__ __forceinline__ void rows_unit(const AttnArgs &a, int head, int tile)
         T::load(k, kb + key(0, col) * a.ks.s, a.D, quarter);
         T::load(q, a.q + b * a.qs.b + h * a.qs.h + (int64_t)i * a.qs.s, a.D, quarter);
         T::load(u, a.up + b * a.us.b + h * a.us.h + (int64_t)i * a.us.s, a.D, quarter);
-        const float lse = live ? a.lse[at] * kLog2e : 0.f, delta = live ? a.delta[at] : 0.f;
+        const float base = live ? a.facts.fp32.base[at] : 0.f, share = live ? a.facts.fp32.share[at] : 0.f;
+        const float delta = live ? a.facts.delta[at] * share : 0.f;
 #pragma unroll
         for (int j = 0; j < T::KJ; j++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) q[j][e] = live ? q[j][e] * a.scale2 : 0.f, u[j][e] = live ? u[j][e] : 0.f;
+            for (int e = 0; e < 4; e++) q[j][e] = live ? q[j][e] * a.scale2 : 0.f, u[j][e] = live ? u[j][e] * share : 0.f;
 #pragma unroll 1
         for (int t = 0; t < tiles; t++) {
             const int j0 = keys.first_key(t);
@@ -58,7 +59,7 @@ __device__ __forceinline__ void rows_unit(const AttnArgs &a, int head, int tile)
             T::load(k, kb + key(t + 1, col) * a.ks.s, a.D, quarter);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                s[e] = __builtin_amdgcn_exp2f(s[e] - lse) * (d[e] - delta);
+                s[e] = __builtin_exp2f(s[e] - base) * (d[e] - delta);
                 s[e] = sees(a, place, j0 + 4 * quarter + e) ? s[e] : 0.f;
             }
             if (__builtin_expect(!T::bad(k2), 1)) T::add(acc, k2, s);
@@ -91,7 +92,7 @@ __device__ __forceinline__ void keys_unit(const AttnArgs &a, int head, int tile,
     for (int t = 0; t < T::TO; t++) dk[t] = dv[t] = (at_f4)(0.f);
     if (t0 < t1) {
         const float *qb = a.q + b * a.qs.b + (int64_t)hk * a.group * a.qs.h, *ub = a.up + b * a.us.b + (int64_t)hk * a.group * a.us.h;
-        const float *lse = a.lse + ((int64_t)b * a.heads + hk * a.group) * a.Sq, *delta = a.delta + ((int64_t)b * a.heads + hk * a.group) * a.Sq;
+        const int64_t facts = ((int64_t)b * a.heads + hk * a.group) * a.Sq;
         // Past the last row, and past the last tile: that one.
         const auto row_of = [&](int t, int n, int &i, int &g) {
             const int row = min(rlo + min(t, t1 - 1) * 16 + n, rhi - 1);
@@ -112,16 +113,17 @@ __device__ __forceinline__ void keys_unit(const AttnArgs &a, int head, int tile,
 #pragma unroll
         for (int j = 0; j < T::KJ; j++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) k[j][e] = live ? k[j][e] * a.scale2 : 0.f, v[j][e] = live ? v[j][e] : 0.f;
+            for (int e = 0; e < 4; e++) k[j][e] = live ? k[j][e] : 0.f, v[j][e] = live ? v[j][e] : 0.f;
 #pragma unroll 1
         for (int t = t0; t < t1; t++) {
-            float l4[4], d4[4];
+            float base[4], share[4], delta[4];
             int place[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 int i, g;
                 row_of(t, 4 * quarter + e, i, g);
-                l4[e] = lse[(int64_t)g * a.Sq + i], d4[e] = delta[(int64_t)g * a.Sq + i];
+                const int64_t at = facts + (int64_t)g * a.Sq + i;
+                base[e] = a.facts.fp32.base[at], share[e] = a.facts.fp32.share[at], delta[e] = a.facts.delta[at] * share[e];
                 place[e] = rlo + t * 16 + 4 * quarter + e < rhi ? seq.first + i : -1;
             }
             const auto pair = [&](int place) { return (key < keys) & (key <= place) & ((place - key < a.window) != far); };
@@ -135,15 +137,15 @@ __device__ __forceinline__ void keys_unit(const AttnArgs &a, int head, int tile,
             typename T::Along u;
             at_f4 p = (at_f4)(0.f), d = (at_f4)(0.f);
             T::load(u, row_at(ub, a.us, t, col), a.D, quarter);
-            T::product(p, q, k);
+            T::product(p, q, k, a.scale2);  // as rows_unit takes it: queries are scaled
             T::load(x, [&](int n) { return u2(4 * quarter + n); }, a.D, col);
             T::product(d, u, v);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 // Subnormals too: a key may have no larger weight.
-                const float w = __builtin_exp2f(p[e] - l4[e] * kLog2e);
-                p[e] = pair(place[e]) ? w : 0.f;
-                d[e] = pair(place[e]) ? w * (d[e] - d4[e]) : 0.f;
+                const float w = __builtin_exp2f(p[e] - base[e]);
+                p[e] = pair(place[e]) ? w * share[e] : 0.f;
+                d[e] = pair(place[e]) ? w * (d[e] * share[e] - delta[e]) : 0.f;
             }
             typename T::Across y;
             T::load(y, [&](int n) { return q2(4 * quarter + n); }, a.D, col);

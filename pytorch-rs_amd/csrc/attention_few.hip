@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(64 * NW, NW > 8 ? 4 : DP <= 128 ? 2 : 1) attn_
         } else {
             o *= seq.first + at_i < 0 ? 0.f : 1.f / total;
             p = a.out + b * a.os.b + h * a.os.h + (int64_t)at_i * a.os.s + d;
-            if (a.lse && d == 0) a.lse[((int64_t)b * a.heads + h) * a.Sq + at_i] = (top + __builtin_amdgcn_logf(total)) * kLn2;
+            if (a.lse && d == 0) a.lse[((int64_t)b * a.heads + h) * a.Sq + at_i] = log_sum(top, total);
         }
 #pragma unroll
         for (int e = 0; e < 4; e++)

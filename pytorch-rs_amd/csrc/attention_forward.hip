@@ -95,7 +95,7 @@ __device__ __forceinline__ void write_rows(const AttnArgs &a, const RowBlock<NW>
     // A row that sees nothing gives 0 and a logarithm of -inf; one whose scores are all -inf,
     // NaN, as the formula does.
     write(a.out + r.at(a, a.os), r.place < 0 ? 0.f : 1.f / sum);
-    if (a.lse && r.half == 0) a.lse[r.index(a)] = (most + __builtin_amdgcn_logf(sum)) * kLn2;
+    if (a.lse && r.half == 0) a.lse[r.index(a)] = log_sum(most, sum);
 }
 
 // The key tiles of tile t of kForwardRows rows in the longest sequence that may be.
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(256) attn_join(AttnArgs a) {
 #pragma unroll
     for (int q = 0; q < 4; q++)
         if (d + q < a.D) out[q] = o[q];
-    if (a.lse && d == 0) a.lse[((int64_t)b * a.heads + h) * a.Sq + i] = (most + __builtin_amdgcn_logf(sum)) * kLn2;
+    if (a.lse && d == 0) a.lse[((int64_t)b * a.heads + h) * a.Sq + i] = log_sum(most, sum);
 }
 
 template <int NT>

@@ -59,12 +59,12 @@ struct Wide {
             for (int u = 0; u < VU; u++) take<W, MODE>(v[i][u], p, 16 * W * u + W * col, D, 16 * W * (u + 1) <= kLeast);
         }
     }
-    // c += x y^T over the columns.
-    __device__ __forceinline__ static void product(at_f4 &c, const Along &x, const Along &y) {
+    // c += (scale x) y^T over the columns.
+    __device__ __forceinline__ static void product(at_f4 &c, const Along &x, const Along &y, float scale = 1.f) {
 #pragma unroll
         for (int j = 0; j < KJ; j++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j][e], y[j][e], c, 0, 0, 0);
+            for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j][e] * scale, y[j][e], c, 0, 0, 0);
     }
     // acc^T += w^T x over the rows.
     __device__ __forceinline__ static void add(at_f4 (&acc)[TO], const Across &x, const at_f4 &w) {

@@ -142,3 +142,58 @@ def test_sums_that_leave_the_range_on_their_way(shape, D):
     compare(forward(q, k, v, *mask[:2], LN2, mask[2]), exact(q, k, v, *mask[:2], LN2, mask[2]))
     up = values(D + 1, *q.shape)
     compare(gradients(q, k, v, *mask[:2], LN2, up, mask[2]), exact_gradients(q, k, v, *mask[:2], LN2, up, mask[2]))
+
+
+@pytest.mark.parametrize("D", DIMS)
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_gradients_of_scores_far_below_zero(shape, D):
+    """Scores of -2^50 that weigh alike, and ones of which the largest weighs all: a row's
+    logarithm is no more exact than 2^27 there."""
+    B, H, hk, sq, sk, *mask = shape
+    q, v, up = np.full((B, H, sq, D), 2.0 ** 24, np.float32), values(D, B, hk, sk, D), values(D + 1, B, H, sq, D)
+    k = np.zeros((B, hk, sk, D), np.float32)
+    k[..., 0] = -2.0 ** 26
+    compare(gradients(q, k, v, *mask[:2], LN2, up, mask[2]), exact_gradients(q, k, v, *mask[:2], LN2, up, mask[2]))
+    k[..., 0] -= 2.0 ** 10 * np.arange(sk)
+    compare(gradients(q, k, v, *mask[:2], LN2, up, mask[2]), exact_gradients(q, k, v, *mask[:2], LN2, up, mask[2]))
+
+
+#          B  H hk  sq   sk   window sinks lengths
+OFFSETS = [
+    (1, 2, 1, 100, 100, EVERY, 0, None),
+    (2, 4, 2, 90, 200, 60, 5, [200, 61]),
+    (1, 1, 1, 420, 420, 50, 40, None),      # sinks' rows far past them
+    (1, 3, 1, 5, 130, EVERY, 0, None),
+]
+
+
+@pytest.mark.parametrize("offset", [0, 300, 1e5, -1e5, 2.0 ** 20, 2.0 ** 25, -2.0 ** 30, 2.0 ** 40], ids=str)
+@pytest.mark.parametrize("D", [32, 64, 128, 160, 256])
+@pytest.mark.parametrize("shape", OFFSETS, ids=str)
+def test_gradients_under_a_common_offset(shape, D, offset):
+    """Scores of whole numbers with an offset that all of a row share, in two rows of three: it
+    changes no weight.  Every score and sum is exact; differences are of at least a unit in
+    the last place of the offset."""
+    B, H, hk, sq, sk, *mask = shape
+    step = max(1.0, abs(offset) * 2.0 ** -23)
+    q, k = np.zeros((B, H, sq, D), np.float32), values(1, B, hk, sk, D)
+    q[..., 0] = np.where(np.arange(sq) % 3, 2.0 ** 5, 0)
+    q[..., 1] = np.exp2(np.floor(np.log2(step))) * (1 + np.arange(sq) % 2)
+    k[..., 0], k[..., 1] = offset / 2.0 ** 5, -(np.arange(sk) * 7 % 4)
+    v, up = values(2, *k.shape), values(3, *q.shape)
+    compare(gradients(q, k, v, *mask[:2], LN2, up, mask[2]), exact_gradients(q, k, v, *mask[:2], LN2, up, mask[2]))
+
+
+@pytest.mark.parametrize("D", [32, 64, 128, 200])
+@pytest.mark.parametrize("std", [20.0, 200.0, 1e6])
+def test_the_weights_of_a_row_sum_to_one_in_the_gradients(D, std):
+    """Scores of any size, rounded as they may be: the gradients of the values add up to the
+    upstream rows, here those whose logarithm is large."""
+    q, k = (np.float32(std) * values(s, 1, 4, 150, D) for s in (5, 6))
+    k, v, up = k[:, :2], values(7, 1, 2, 150, D), values(8, *q.shape)
+    up[abs(forward(q, k, v, 70, 3, 0.2)["lse"]) <= 256] = 0
+    assert up.any()
+    dv = gradients(q, k, v, 70, 3, 0.2, up)["dv"].astype(np.float64)
+    rows = up.reshape(1, 2, 300, D).astype(np.float64)
+    # Weights of 150 keys and their sum, and sums over 300 rows.
+    assert_within(dv.sum(2), rows.sum(2), (2 * 150 + 300 + 64) * U * abs(rows).sum(2), "dv")
