@@ -121,6 +121,7 @@ __global__ void __launch_bounds__(64) attn_facts(AttnArgs a) {
                 x, y);
         } else {
             const auto key = [](int e, int half) { return result_row(e, half); };
+            Lowest lowest;
             statistics<32>(
                 a, seq, b, hk, r0, r1, mine, kDown2, key,
                 [&](const float *k) {
@@ -137,10 +138,12 @@ __global__ void __launch_bounds__(64) attn_facts(AttnArgs a) {
                         }
                         mfma_pieces<true>(c, n.split(kUp), m.split(a.scale2 * kUp));
                     }
+                    lowest.add(c);
                     return c;
                 },
                 x, y);
-            if (again) base = x, share = y;
+            // A score beyond the pieces' range may be in one block of keys: NaN sends all to the fp32 form.
+            if (again) base = lowest.infinite() ? __builtin_nanf("") : x, share = y;
             statistics<32>(
                 a, seq, b, hk, r0, r1, mine, 1.f, key,
                 [&](const float *k) { return product_fp32(a.D, lane >> 5, [&](int c) { return row_chunk(k, c, a.D); }, row); }, x, y);

@@ -197,3 +197,18 @@ def test_the_weights_of_a_row_sum_to_one_in_the_gradients(D, std):
     rows = up.reshape(1, 2, 300, D).astype(np.float64)
     # Weights of 150 keys and their sum, and sums over 300 rows.
     assert_within(dv.sum(2), rows.sum(2), (2 * 150 + 300 + 64) * U * abs(rows).sum(2), "dv")
+
+
+@pytest.mark.parametrize("D", [64, 80, 128])
+def test_a_sum_that_leaves_the_range_counts_in_every_block_of_keys(D):
+    """Scores of 2^12 whose sums, of some keys of the first block alone, pass -2^49 on their way:
+    these keys weigh as much as the others, whose gradients other blocks work out."""
+    n = 300
+    q, k = np.full((1, 2, n, D), 2.0 ** 22, np.float32), np.zeros((1, 1, n, D), np.float32)
+    q[..., 32:] = 0
+    q[..., 40], k[..., 40] = 2.0 ** 5, 2.0 ** 7
+    k[:, :, :40:2, :16], k[:, :, :40:2, 16:32] = -2.0 ** 23, 2.0 ** 23
+    v, up = values(D, *k.shape), values(D + 1, *q.shape)
+    for sinks, window in ((0, EVERY), (30, 64)):
+        compare(forward(q, k, v, window, sinks, LN2), exact(q, k, v, window, sinks, LN2))
+        compare(gradients(q, k, v, window, sinks, LN2, up), exact_gradients(q, k, v, window, sinks, LN2, up))
