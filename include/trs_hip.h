@@ -99,6 +99,10 @@ int trs_alloc(size_t bytes, void **ptr);
  * operands with no unit stride cannot be had runs the one-lane-per-output
  * kernel; a split K whose workspace cannot be had runs unsplit. */
 int trs_debug_fail_allocs_after(int64_t n);
+/* Test hook of the same kind, for fallbacks to a smaller workspace: every
+ * trs_alloc of more than `bytes` bytes fails with TRS_E_ALLOCATION_FAILED;
+ * 0 removes the limit. */
+int trs_debug_fail_allocs_above(size_t bytes);
 /* Test hook (no counterpart in the reference; for the tests of the
  * pointwise kernels' grid-stride loops, which only launches of more than
  * 2^22 blocks reach otherwise): every pointwise launch planned after it uses
@@ -416,7 +420,9 @@ int trs_window_attention_f32(const float *q, const trs_layout *lq, const float *
  * row whose lse is beyond 256 either way one float would hold it in too few bits,
  * and maximum and sum are worked out again (up to twice the time, where all rows
  * are such).  No atomic adds: the result is the same bits each time.  Takes a
- * workspace from the block cache. */
+ * workspace from the block cache: 20 bytes a query and head, and where there is
+ * memory the key gradients in up to 16 parts and those of the sinks in up to 64
+ * (one of the sinks' at least, if the window is shorter than the keys). */
 int trs_window_attention_backward_f32(const float *q, const trs_layout *lq, const float *k, const trs_layout *lk,
                                       const float *v, const trs_layout *lv, const int32_t *lengths, int64_t window,
                                       int64_t sinks, float scale, const float *out, const trs_layout *lo,

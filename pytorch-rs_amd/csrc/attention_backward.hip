@@ -164,9 +164,9 @@ __global__ void __launch_bounds__(64) attn_facts(AttnArgs a) {
 }
 
 // dk and dv of the first `count` keys: the parts over the rows, or what the one part
-// wrote, and the sinks' `far` parts of tiles of `tile` keys, in a fixed order.  Eight parts
-// are read at a time: one memory latency for all of them.
-__global__ void __launch_bounds__(256) attn_reduce(AttnArgs a, int count, int tile, int far) {
+// wrote, and the sinks' `far` parts, in a fixed order.  Eight parts are read at a time: one
+// memory latency for all of them.
+__global__ void __launch_bounds__(256) attn_reduce(AttnArgs a, int count, int far) {
     const int64_t heads = (int64_t)a.batch * a.kv_heads, n = heads * count * a.D;
     const auto add = [](float &x, float &y, const float *px, const float *py, int64_t step, int parts) {
         for (int p = 0; p < parts; p += 8) {
@@ -195,8 +195,8 @@ __global__ void __launch_bounds__(256) attn_reduce(AttnArgs a, int count, int ti
             x = *dk, y = *dv;
         }
         if (far && key < a.sinks) {
-            const int64_t at = (((head * a.sink_tiles + key / tile) * far) * tile + key % tile) * a.D + d;
-            add(x, y, a.sink_k + at, a.sink_v + at, (int64_t)tile * a.D, far);
+            const int64_t at = (head * far * a.sinks + key) * a.D + d;
+            add(x, y, a.sink_k + at, a.sink_v + at, (int64_t)a.sinks * a.D, far);
         }
         *dk = x, *dv = y;
     }
@@ -223,21 +223,28 @@ int attention_backward(AttnArgs a, hipStream_t s, int cu_count) {
     a.sink_splits = 1;
     if (a.sink_tiles)
         a.sink_splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(64, std::max<int64_t>(1, a.rows / tile) * a.row_splits / near_tiles));
-    const int far = a.sink_tiles ? a.sink_splits : 0;
     const int64_t row_blocks = heads * a.row_tiles;
-    const int64_t key_blocks = heads * (a.sink_tiles * a.sink_splits + (int64_t)a.key_tiles * a.row_splits);
+    const int64_t most_blocks = row_blocks + heads * (a.sink_tiles * a.sink_splits + (int64_t)a.key_tiles * a.row_splits);
     const int64_t fact_units = heads * ((a.rows + 15) / 16);
-    if ((row_blocks + key_blocks) >> 24 || fact_units >> 25)  // a launch has fewer than 2^32 lanes
+    if (most_blocks >> 24 || fact_units >> 25)  // a launch has fewer than 2^32 lanes
         return set_error(TRS_E_INVALID_ARGUMENT, "attention gradient over too many blocks");
     const int64_t facts = ((int64_t)a.batch * a.heads * a.Sq + 63) / 64 * 64;
-    const int64_t sink_floats = heads * a.sink_tiles * far * block * a.D;
-    const int64_t part_floats = a.row_splits > 1 ? heads * a.row_splits * a.Sk * a.D : 0;
+    const auto sink_floats = [&] { return a.sink_tiles ? heads * a.sink_splits * a.sinks * a.D : 0; };
+    const auto part_floats = [&] { return a.row_splits > 1 ? heads * a.row_splits * a.Sk * a.D : 0; };
     void *ws = nullptr;
-    TRS_CHECK(trs_alloc((size_t)(5 * facts + 2 * sink_floats + 2 * part_floats) * sizeof(float), &ws));
+    const auto take = [&] { return trs_alloc((size_t)(5 * facts + 2 * sink_floats() + 2 * part_floats()) * sizeof(float), &ws); };
+    int got = take();
+    if (got == TRS_E_ALLOCATION_FAILED && (a.row_splits > 1 || a.sink_splits > 1)) {  // the parts are for speed alone
+        a.row_splits = a.sink_splits = 1;
+        got = take();
+    }
+    TRS_CHECK(got);
+    const int far = a.sink_tiles ? a.sink_splits : 0;
+    const int64_t key_blocks = heads * (a.sink_tiles * a.sink_splits + (int64_t)a.key_tiles * a.row_splits);
     float *const f = (float *)ws;
     a.facts = RowFacts{f, {f + facts, f + 2 * facts}, {f + 3 * facts, f + 4 * facts}};
-    a.sink_k = f + 5 * facts, a.sink_v = a.sink_k + sink_floats;
-    a.part_k = a.sink_v + sink_floats, a.part_v = a.part_k + part_floats;
+    a.sink_k = f + 5 * facts, a.sink_v = a.sink_k + sink_floats();
+    a.part_k = a.sink_v + sink_floats(), a.part_v = a.part_k + part_floats();
     const auto launch = [&]() -> int {
         // No rows: the keys' gradients are 0.  No keys: the rows' are.
         const dim3 fact_blocks((unsigned)fact_units);
@@ -252,7 +259,7 @@ int attention_backward(AttnArgs a, hipStream_t s, int cu_count) {
         const int count = a.row_splits > 1 ? a.Sk : a.sink_tiles ? std::min(a.sinks, a.Sk) : 0;
         if (count) {
             const int64_t n = heads * count * a.D;
-            hipLaunchKernelGGL(attn_reduce, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 1 << 20)), dim3(256), 0, s, a, count, block, far);
+            hipLaunchKernelGGL(attn_reduce, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 1 << 20)), dim3(256), 0, s, a, count, far);
             TRS_LAUNCH_CHECK("attention gradient launch");
         }
         return TRS_OK;

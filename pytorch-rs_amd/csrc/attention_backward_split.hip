@@ -394,7 +394,7 @@ __device__ __forceinline__ void keys_block(const AttnArgs &a, uint32_t id, char 
     if (k.key >= (k.far ? a.sinks : a.Sk)) return;
     float *pk, *pv;
     if (k.far) {
-        const int64_t at = (((int64_t)k.head * a.sink_tiles + k.tile) * a.sink_splits + k.part) * kRowsBlock + k.key % kRowsBlock;
+        const int64_t at = ((int64_t)k.head * a.sink_splits + k.part) * a.sinks + k.key;
         pk = a.sink_k + at * a.D, pv = a.sink_v + at * a.D;
     } else if (a.row_splits > 1) {
         const int64_t at = ((int64_t)k.part * a.batch * a.kv_heads + k.head) * a.Sk + k.key;

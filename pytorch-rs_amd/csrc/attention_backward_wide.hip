@@ -159,7 +159,7 @@ __device__ __forceinline__ void keys_unit(const AttnArgs &a, int head, int tile,
     if (key >= (far ? a.sinks : a.Sk)) return;
     float *pk, *pv;
     if (far) {
-        const int64_t at = (((int64_t)head * a.sink_tiles + tile) * a.sink_splits + part) * 16 + col;
+        const int64_t at = ((int64_t)head * a.sink_splits + part) * a.sinks + key;
         pk = a.sink_k + at * a.D, pv = a.sink_v + at * a.D;
     } else if (a.row_splits > 1) {
         const int64_t at = ((int64_t)part * a.batch * a.kv_heads + head) * a.Sk + key;

@@ -210,6 +210,7 @@ using namespace trs;
 namespace trs {
 // Allocations trs_alloc grants before it refuses every one (-1: no limit).
 std::atomic<int64_t> g_allocs_before_failure{-1};
+std::atomic<size_t> g_most_alloc_bytes{SIZE_MAX};
 std::atomic<int64_t> g_pw_grid_cap{0};
 }  // namespace trs
 
@@ -264,6 +265,11 @@ int trs_debug_fail_allocs_after(int64_t n) {
     return TRS_OK;
 }
 
+int trs_debug_fail_allocs_above(size_t bytes) {
+    trs::g_most_alloc_bytes.store(bytes ? bytes : SIZE_MAX);
+    return TRS_OK;
+}
+
 int trs_debug_pointwise_grid_cap(int64_t blocks) {
     if (blocks < 0) return set_error(TRS_E_INVALID_ARGUMENT, "negative grid cap");
     trs::g_pw_grid_cap.store(blocks);
@@ -283,6 +289,8 @@ int trs_alloc(size_t bytes, void **ptr) {
                 return set_error(TRS_E_ALLOCATION_FAILED, "allocation refused (trs_debug_fail_allocs_after)");
             if (trs::g_allocs_before_failure.compare_exchange_weak(left, left - 1)) break;
         }
+        if (bytes > trs::g_most_alloc_bytes.load())
+            return set_error(TRS_E_ALLOCATION_FAILED, "allocation of %zu bytes refused (trs_debug_fail_allocs_above)", bytes);
         const size_t rounded = round_block(bytes);
         {
             std::lock_guard<std::mutex> lock(dev->cache_mu);
