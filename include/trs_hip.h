@@ -378,7 +378,8 @@ int trs_dropout_f32(const float *x, const trs_layout *lx, double p, uint64_t see
  * (TRS_E_INVALID_ARGUMENT), and a row whose own position does not is NaN.
  * weight: n pointers to dim floats each, any of them (or the array) null for
  * ones.  dim is at most 1024.  Inputs may have any strides; outputs share no
- * memory with inputs. */
+ * element with inputs, nor with each other (slices of one buffer along a dim that
+ * all have, the heads of a fused projection, do not). */
 int trs_head_norm_rope_f32(int n, const float *const *x, const trs_layout *lx, const float *const *weight, float eps,
                            const float *cos, const float *sin, const trs_layout *ltab, int interleaved,
                            const int32_t *positions, int64_t start, float *const *out, const trs_layout *lo);
@@ -409,7 +410,7 @@ int trs_head_norm_rope_backward_f32(int n, const float *const *x, const trs_layo
  * cores or, in pieces as in trs_matmul_f32, the bf16 ones; the order of the sums
  * is fixed.  Inputs may have any strides (one with no unit stride along dim is
  * copied first, into the block cache); outputs need a unit stride along dim and
- * share no memory with inputs.  Few rows over many keys are split over the keys,
+ * share no element with inputs (as with the norm's).  Few rows over many keys are split over the keys,
  * into a workspace from the block cache; where it has none they are not. */
 int trs_window_attention_f32(const float *q, const trs_layout *lq, const float *k, const trs_layout *lk,
                              const float *v, const trs_layout *lv, const int32_t *lengths, int64_t window,
