@@ -248,6 +248,13 @@ def _indices(values, like):
     return index_buffer(values, like.device)
 
 
+def _integer(op, name, value) -> int:
+    """A whole number of any type; nothing is cut to one."""
+    if not isinstance(value, (int, float, _np.integer, _np.floating)) or value != value // 1 or math.isinf(value):
+        raise TypeError(f"{op}(): argument '{name}' must be int, not {value!r}")
+    return int(value)
+
+
 def _tensor_arguments(op, **tensors):
     for name, t in tensors.items():
         if not isinstance(t, _C.Tensor):
@@ -276,7 +283,8 @@ def head_norm_rope(query, key, query_weight, key_weight, cos, sin, *, eps: float
             _tensor_arguments("head_norm_rope", **{name: w})
             if len(w.shape) != 1:
                 raise RuntimeError(f"head_norm_rope weight has {len(w.shape)} dims, expected 1")
-    out = _C.head_norm_rope(xs, ws, cos, sin, float(eps), bool(interleaved), int(start), _indices(positions, query))
+    start = _integer("head_norm_rope", "start", start)
+    out = _C.head_norm_rope(xs, ws, cos, sin, float(eps), bool(interleaved), start, _indices(positions, query))
     return out[0] if key is None else tuple(out)
 
 
@@ -291,12 +299,14 @@ def window_attention(query, key, value, *, window=None, sinks: int = 0, scale=No
     an ``index_buffer``) are the keys that each sequence of a cache has.  A query
     that sees nothing gives 0.  Gradients reach queries, keys and values."""
     _tensor_arguments("window_attention", query=query, key=key, value=value)
-    if window is not None and int(window) < 1:
+    window = None if window is None else _integer("window_attention", "window", window)
+    sinks = _integer("window_attention", "sinks", sinks)
+    if window is not None and window < 1:
         raise ValueError(f"window_attention window has to be at least 1, but got {window}")
-    if int(sinks) < 0:
+    if sinks < 0:
         raise ValueError(f"window_attention sinks have to be at least 0, but got {sinks}")
     if scale is None:
         scale = 1.0 / math.sqrt(query.shape[-1]) if len(query.shape) and query.shape[-1] else 1.0
     every = (1 << 63) - 1
-    return _C.window_attention(query, key, value, every if window is None else min(int(window), every), min(int(sinks), every),
+    return _C.window_attention(query, key, value, every if window is None else min(window, every), min(sinks, every),
                                float(scale), _indices(key_lengths, query))
