@@ -115,7 +115,7 @@ int run(const AttnCall &c) {
         };
         TRS_CHECK(check_memory(ops));
     }
-    if (D == 0 || B == 0 || (grad ? H * Sq == 0 && HK * Sk == 0 : H * Sq == 0)) return TRS_OK;
+    if (B == 0 || (grad ? H * Sq == 0 && HK * Sk == 0 : H * Sq == 0)) return TRS_OK;
     DeviceState *dev = device_state();
     if (!dev) return TRS_E_NO_DEVICE;
     AttnArgs a{};
