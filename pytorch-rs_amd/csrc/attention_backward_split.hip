@@ -32,7 +32,8 @@ __device__ __forceinline__ float up_exp2(float x) {
 
 // ---- dQ -----------------------------------------------------------------------
 
-// The block's rows on the fp32 instruction, whatever the values.
+// The block's rows on the fp32 instruction, whatever the values.  dS is scaled, not its sums, which
+// would leave the range ahead of the gradients.
 template <int NT, int NW>
 __device__ __forceinline__ void grad_rows_fp32(const AttnArgs &a, const RowBlock<NW> &r, float delta, float *lds,
                                                at_f16 (&acc)[NT]) {
@@ -53,7 +54,7 @@ __device__ __forceinline__ void grad_rows_fp32(const AttnArgs &a, const RowBlock
             const at_f16 d = T::times_row(lds + T::kFloats, u, a.D, 1.f, r.lane);
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-                s[e] = __builtin_exp2f(s[e] - base) * share * (d[e] - delta);
+                s[e] = __builtin_exp2f(s[e] - base) * share * (d[e] - delta) * a.scale;
                 if (!sees(a, r.place, j0 + result_row(e, r.half))) s[e] = 0.f;
             }
             T::add_product_seen(acc, lds, s, r.lane, [&](int k) { return sees(a, r.place, j0 + k); });
@@ -156,7 +157,7 @@ __device__ __forceinline__ void rows_block(const AttnArgs &a, uint32_t id, char 
         __syncthreads();
         if (__builtin_expect(notices.any(1), 0)) {
             grad_rows_fp32<NT, NW>(a, r, delta, (float *)lds, acc);
-            if (r.row < a.rows) T::write(acc, a.dq + r.at(a, a.dqs), a.scale, a.D, r.half);
+            if (r.row < a.rows) T::write(acc, a.dq + r.at(a, a.dqs), 1.f, a.D, r.half);
             return;
         }
     }
@@ -260,7 +261,7 @@ __device__ __forceinline__ void grad_keys_fp32(const AttnArgs &a, const KeyBlock
             for (int e = 0; e < 16; e++) {
                 const int r = result_row(e, k.half);
                 p[e] = __builtin_exp2f(p[e] - facts.base[0][r]) * facts.share[r];
-                d[e] = p[e] * (d[e] - facts.delta[0][r]);
+                d[e] = p[e] * (d[e] - facts.delta[0][r]) * a.scale;
                 if (!k.pair(a, facts.place[0][r])) p[e] = d[e] = 0.f;
             }
             const auto seen = [&](int r) { return k.pair(a, facts.place[0][r]); };
@@ -404,7 +405,7 @@ __device__ __forceinline__ void keys_block(const AttnArgs &a, uint32_t id, char 
         pv = a.dv + k.b * a.dvs.b + k.hk * a.dvs.h + (int64_t)k.key * a.dvs.s;
     }
     if (again) {
-        T::write(dk, pk, a.scale, a.D, k.half);
+        T::write(dk, pk, 1.f, a.D, k.half);
         T::write(dv, pv, 1.f, a.D, k.half);
     } else {
         write_row<WIDTH>(dk, pk, kDown2, kLn2, a.D, k.half);  // scale / scale2

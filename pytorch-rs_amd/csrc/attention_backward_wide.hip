@@ -59,14 +59,14 @@ __device__ __forceinline__ void rows_unit(const AttnArgs &a, int head, int tile)
             T::load(k, kb + key(t + 1, col) * a.ks.s, a.D, quarter);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                s[e] = __builtin_exp2f(s[e] - base) * (d[e] - delta);
+                s[e] = __builtin_exp2f(s[e] - base) * (d[e] - delta) * a.scale;  // its sums might leave the range
                 s[e] = sees(a, place, j0 + 4 * quarter + e) ? s[e] : 0.f;
             }
             if (__builtin_expect(!T::bad(k2), 1)) T::add(acc, k2, s);
             else T::add_seen(acc, s, a.D, col, quarter, row2, [&](int n) { return sees(a, place, j0 + n); });
         }
     }
-    if (r0 + col < a.rows) T::write(acc, a.dq + b * a.dqs.b + h * a.dqs.h + (int64_t)i * a.dqs.s, a.scale, a.D, quarter);
+    if (r0 + col < a.rows) T::write(acc, a.dq + b * a.dqs.b + h * a.dqs.h + (int64_t)i * a.dqs.s, 1.f, a.D, quarter);
 }
 
 // dK and dV of 16 keys, over the rows whose window holds them, or (far) over the rows
@@ -145,7 +145,7 @@ __device__ __forceinline__ void keys_unit(const AttnArgs &a, int head, int tile,
                 // Subnormals too: a key may have no larger weight.
                 const float w = __builtin_exp2f(p[e] - base[e]);
                 p[e] = pair(place[e]) ? w * share[e] : 0.f;
-                d[e] = pair(place[e]) ? w * (d[e] * share[e] - delta[e]) : 0.f;
+                d[e] = pair(place[e]) ? w * (d[e] * share[e] - delta[e]) * a.scale : 0.f;
             }
             typename T::Across y;
             T::load(y, [&](int n) { return q2(4 * quarter + n); }, a.D, col);
@@ -168,7 +168,7 @@ __device__ __forceinline__ void keys_unit(const AttnArgs &a, int head, int tile,
         pk = a.dk + b * a.dks.b + hk * a.dks.h + (int64_t)key * a.dks.s;
         pv = a.dv + b * a.dvs.b + hk * a.dvs.h + (int64_t)key * a.dvs.s;
     }
-    T::write(dk, pk, a.scale, a.D, quarter);
+    T::write(dk, pk, 1.f, a.D, quarter);
     T::write(dv, pv, 1.f, a.D, quarter);
 }
 

@@ -212,3 +212,21 @@ def test_a_sum_that_leaves_the_range_counts_in_every_block_of_keys(D):
     for sinks, window in ((0, EVERY), (30, 64)):
         compare(forward(q, k, v, window, sinks, LN2), exact(q, k, v, window, sinks, LN2))
         compare(gradients(q, k, v, window, sinks, LN2, up), exact_gradients(q, k, v, window, sinks, LN2, up))
+
+
+@pytest.mark.parametrize("D", [16, 64, 128, 160])
+def test_gradients_just_within_the_range(D):
+    """dS K and dS^T Q that would leave fp32's range unscaled: by a scale of 2^-10 the gradients do not."""
+    scale = np.float32(2.0 ** -10)
+    q, k, v, up = (values(s, 1, 2, 80, D) for s in range(4))
+    k, v = k[:, :1], np.float32(1e16) * v[:, :1]
+    for side in (0, 1):
+        big = [np.float32(1e12 if side == 0 else 1e-12) * k, np.float32(1e-12 if side == 0 else 1e12) * q]
+        want = exact_gradients(big[1], big[0], v, 40, 2, scale, up)
+        name = ("dq", "dk")[side]
+        f = np.float32(2.0 ** 124 / abs(want[name][0]).max())  # sums of magnitudes stay within the range
+        want = exact_gradients(big[1], big[0], v, 40, 2, scale, f * up)
+        assert abs(want[name][0] / scale).max() > 3.5e38
+        got = gradients(big[1], big[0], v, 40, 2, scale, f * up)
+        # Scores are within 1/100 of 0; their rounding is far below the bound's weights'.
+        assert_within(got[name], *want[name], what=name)
