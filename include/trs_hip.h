@@ -32,7 +32,10 @@
  *   - A non-empty view whose element count, last element offset or last byte
  *     offset leaves 64 bits is rejected with TRS_E_INDEX_OVERFLOW.
  *   - All work is queued in order on one HIP stream per device (trs_stream);
- *     only trs_memcpy_d2h and trs_synchronize block the host.
+ *     only trs_memcpy_d2h and trs_synchronize block the host.  The stream is a
+ *     non-blocking one: work on other streams, the default stream too, is not
+ *     ordered with it, so a caller whose operands another stream writes, reads
+ *     or frees waits for it before the call, or for this one after.
  *   - Callable from any thread; the allocator and the fusion cache are
  *     internally locked.
  */
@@ -406,7 +409,9 @@ int trs_head_norm_rope_backward_f32(int n, const float *const *x, const trs_layo
  * NaN included, does not reach that query.  window >= 1 (INT64_MAX: no window);
  * sinks >= 0.  lse (or null) receives log(sum(exp(scale q k))) as
  * [batch, heads, Sq], -inf where nothing is seen.  A query all of
- * whose scores are -inf gives NaN.  Sums are fp32, products on the fp32 matrix
+ * whose scores are -inf gives NaN; finite scores of any size do not.  (Values are
+ * summed ahead of the division by the weights' sum: ones within the number of
+ * keys of fp32's largest may give infinities.)  Sums are fp32, products on the fp32 matrix
  * cores or, in pieces as in trs_matmul_f32, the bf16 ones; the order of the sums
  * is fixed.  Inputs may have any strides (one with no unit stride along dim is
  * copied first, into the block cache); outputs need a unit stride along dim and

@@ -5,8 +5,9 @@
 // rows for the gradients.  It is split into one of two buffers while the block
 // computes from the other, the loads from memory a tile further ahead: one barrier a
 // tile.  Bound by the card's power and by issue: 4096 tokens, 32 heads of 128 over 8, window
-// 2048 1.86 to 2.1 ms by card, up to 1.24 PFLOP/s of bf16 products, the matrix cores busy for 61% of
-// the time.  The block has a CU to itself (512 registers a lane) above dims of 64, and a wave
+// 2048 1.9 to 2.1 ms by card, up to 1.2 PFLOP/s of bf16 products, the matrix cores busy for 53% of
+// the cycles and the other vector instructions' issue 28%; 2 x 2048 tokens, 16 heads of 64 200 us, 47%
+// and 34%.  The block has a CU to itself (512 registers a lane) above dims of 64, and a wave
 // a SIMD nothing to run beside but its own instructions: so splitting and exponentials stand
 // among the matrix instructions (steps()).
 //

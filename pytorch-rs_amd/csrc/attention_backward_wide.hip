@@ -3,7 +3,7 @@
 //
 // A tile's pieces and the operands held for it would not fit a CU's LDS and a lane's 512
 // registers there, nor would fp32 tiles staged in LDS without spilling (a training step of 2048
-// tokens, 16 heads of 256, window 512: 4066 us so, 1381 now).  So every wave works alone, on 16 keys or 16 rows, with its operands
+// tokens, 16 heads of 256, window 512: 4066 us so, 1340 now).  So every wave works alone, on 16 keys or 16 rows, with its operands
 // straight from memory (attention_wide.h): the next operand is asked for while the one
 // before is multiplied, and the four waves of a block take neighbours, whose rows
 // they find in the L1.  Bound by the fp32 matrix instruction's rate and the L2's.

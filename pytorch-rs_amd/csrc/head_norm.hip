@@ -209,7 +209,8 @@ __global__ void __launch_bounds__(256) norm_rows(NormArgs a) {
 
 // Any dim up to kMaxDim, any part of it rotated, any strides: a wave a row, the
 // entries dealt to its lanes, partners read again from the cache (2 x 4096 tokens, 40
-// heads of 80, 36 of them turned: 151 us; 40 of them, in eights, 46).
+// heads of 80, 36 of them turned: 151 to 176 us by card; 40 of them, in eights, 46.  The
+// gradients 340 and 76).
 template <bool GRAD>
 __global__ void __launch_bounds__(256) norm_any(NormArgs a) {
     const NormTensor &t = a.t[which(a)];
