@@ -230,3 +230,14 @@ def test_gradients_just_within_the_range(D):
         got = gradients(big[1], big[0], v, 40, 2, scale, f * up)
         # Scores are within 1/100 of 0; their rounding is far below the bound's weights'.
         assert_within(got[name], *want[name], what=name)
+
+
+@pytest.mark.parametrize("D", [8, 32, 64, 80, 128, 200])
+def test_weights_of_scores_beyond_the_range_sum_to_one_in_the_gradients(D):
+    """The same of scores of about 1e17 either way, some rows' small: blocks on the fp32 instruction."""
+    q, k = (np.float32(1e9) * values(s, 1, 4, 150, D) for s in (5, 6))
+    q[:, :, ::7] *= np.float32(1e-19)
+    k, v, up = k[:, :2], values(7, 1, 2, 150, D), values(8, *q.shape)
+    dv = gradients(q, k, v, 70, 3, 0.2, up)["dv"].astype(np.float64)
+    rows = up.reshape(1, 2, 300, D).astype(np.float64)
+    assert_within(dv.sum(2), rows.sum(2), (2 * 150 + 300 + 64) * U * abs(rows).sum(2), "dv")
