@@ -436,6 +436,85 @@ int trs_window_attention_backward_f32(const float *q, const trs_layout *lq, cons
                                       const trs_layout *ldq, float *dk, const trs_layout *ldk, float *dv,
                                       const trs_layout *ldv);
 
+/* ---- a paged cache and what reads and writes it (new; no counterpart in the reference) */
+
+/* The rotation of queries and keys, n = 1 or 2 tensors [batch, head, token, dim] in
+ * one launch (they share batch, tokens and dim), by positions of 1 to 4 axes (time,
+ * height, width): pair j of the first `rot` entries, (j, j + rot/2) or, interleaved,
+ * (2j, 2j+1), turns by the angle whose cosine and sine stand in entry j of the tables'
+ * row positions[axis][batch][token], axis = pair_axis[j]:
+ *     (u, w) -> (u cos - w sin, w cos + u sin)
+ * The tables are [rows, rot/2] with the layout ltab and a unit stride along a row;
+ * rot <= dim, and entries from rot on pass.  pair_axis: rot/2 bytes of host memory,
+ * each below `axes`, or null for axis 0 throughout.  positions: int32 on the device,
+ * contiguous, or null for start + token on every axis; start + t has to lie in the
+ * tables (TRS_E_INVALID_ARGUMENT), and a pair whose own position does not is NaN.
+ * `inverse` turns by the negative angles, which is the gradient of the rotation.
+ * dim is at most 1024.  Inputs may have any strides; an output may be its own input's
+ * view (in place) and shares no element with anything else. */
+int trs_rope_axes_f32(int n, const float *const *x, const trs_layout *lx, const float *cos, const float *sin,
+                      const trs_layout *ltab, int interleaved, int axes, const uint8_t *pair_axis,
+                      const int32_t *positions, int64_t start, int inverse, float *const *out, const trs_layout *lo);
+
+/* Types of a cache's entries. */
+#define TRS_PAGES_F32 0
+#define TRS_PAGES_BF16 1
+
+/* A cache of keys and values in pages.  k and v are pools [page, key head, token of
+ * the page, dim], of float32 or bfloat16, with any strides but a unit one along dim
+ * (one buffer may hold both).  table [batch, table_width] and lengths [batch] are int32
+ * on the device, contiguous: token t of sequence b stands in page
+ * table[b][t / tokens a page] at t % tokens a page, and lengths[b], taken into
+ * [0, table_width * tokens a page], is the number of tokens that the sequence has, the
+ * ones that a call brings among them.  Entries of the table for tokens that a call
+ * neither writes nor sees are not looked at. */
+typedef struct trs_paged_cache {
+    void *k, *v;
+    trs_layout lk, lv;
+    int32_t type;
+    int32_t reserved;
+    const int32_t *table;
+    int64_t table_width;
+    const int32_t *lengths;
+} trs_paged_cache;
+
+/* Writes the keys and values of T new tokens a sequence, [batch, key head, T, dim], to
+ * their pages, the keys turned on the way as trs_rope_axes_f32 turns them; with q
+ * [batch, head, T, dim], its turned queries go to q_out in the same launch (q null: none).
+ * Token t of sequence b stands at place lengths[b] - T + t; one before place 0 is
+ * padding, of which nothing is written.  positions as above, or null for the place
+ * itself on every axis (a padding query turns as at place 0); a pair whose position the
+ * tables do not hold is NaN.  cos, sin and ltab null: nothing is turned.  Values go to
+ * bfloat16 pages rounded to the nearest, ties to even.  A token whose entry of the table
+ * is no page of the pool is not written.  Where two tokens of a call have the same place
+ * in the pool, it holds entries of either.  Everything else in the pools stays as it is.
+ * dim is at most 1024.  Pools and q_out share no memory with inputs; q_out may be q's
+ * own view. */
+int trs_paged_append_f32(const trs_paged_cache *cache, const float *k, const trs_layout *lk, const float *v,
+                         const trs_layout *lv, const float *q, const trs_layout *lq, float *q_out,
+                         const trs_layout *lqo, const float *cos, const float *sin, const trs_layout *ltab,
+                         int interleaved, int axes, const uint8_t *pair_axis, const int32_t *positions);
+
+/* trs_window_attention_f32 over a paged cache: q [batch, heads, Sq, dim], dim at most
+ * 256, head h reads key head h / (heads / key heads).  Of a sequence of n tokens query i
+ * stands at place p = n - Sq + i and sees key j where
+ *     j <= p  and  (p - j < window  or  j < sinks).
+ * A query that sees nothing (p < 0) gives 0 whatever it holds.  Keys j < shared of every
+ * sequence are read through the table's first row, and their products are taken for
+ * the rows of all sequences together: the prefix that a batch has in common is read
+ * once and not once a sequence (shared = 0: none; one above the table's tokens counts as
+ * all of them).  A query that sees a key whose entry of the table is no page of the pool
+ * gives NaN.  What stands in keys that a query does not see, NaN included, does not reach
+ * it.  window >= 1 (INT64_MAX: no window); sinks >= 0.  lse (or null) receives
+ * log(sum(exp(scale q k))) as [batch, heads, Sq], -inf where nothing is seen.  Sums are
+ * fp32 and their order is fixed; products as in trs_window_attention_f32, with a
+ * bfloat16 key or value as it stands.  q may have any strides (one with no unit stride
+ * along dim is copied first, into the block cache); out needs a unit stride along dim and
+ * shares no memory with anything else.  There is no gradient: trs_window_attention_f32
+ * has one. */
+int trs_paged_attention_f32(const float *q, const trs_layout *lq, const trs_paged_cache *cache, int64_t shared,
+                            int64_t window, int64_t sinks, float scale, float *out, const trs_layout *lo, float *lse);
+
 /* ---- pointwise fusion compiler (new; no counterpart in the reference) */
 
 /* Compile a pointwise IR program to a gfx950 kernel with hipRTC (-O3,

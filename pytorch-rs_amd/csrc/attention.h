@@ -460,6 +460,30 @@ struct Notices {
     }
 };
 
+// An input whose last dim has a unit stride: itself, or a contiguous copy in the
+// block cache.
+struct Dense {
+    const float *at = nullptr;
+    AttnView view{};
+    void *copy = nullptr;
+    int take(const float *p, const trs_layout *l) {
+        if (layout_numel(l) == 0) return TRS_OK;
+        if (l->stride[3] == 1 || l->shape[3] == 1) {
+            at = p + l->offset;
+            view = {l->stride[0], l->stride[1], l->stride[2]};
+            return TRS_OK;
+        }
+        const trs_layout c = contiguous_like(l);
+        TRS_CHECK(trs_alloc((size_t)layout_numel(l) * sizeof(float), &copy));
+        at = (const float *)copy;
+        view = {c.stride[0], c.stride[1], c.stride[2]};
+        return trs_unary_f32(TRS_COPY, p, l, (float *)copy, &c);
+    }
+    ~Dense() {
+        if (copy) (void)trs_free(copy);
+    }
+};
+
 // Few rows a key head (attention_few.hip): row_tiles of 16 rows, `splits` parts.
 int launch_attention_few(const AttnArgs &a, dim3 grid, hipStream_t s);
 // The gradients in pieces, for D up to kPiecesDim: blocks of 128 keys over their windows'

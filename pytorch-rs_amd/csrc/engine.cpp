@@ -433,6 +433,7 @@ const char *node_name(Node n) {
     case Node::Fused: return "FusedBackward0";
     case Node::Dropout: return "DropoutBackward0";
     case Node::HeadNormRope: return "HeadNormRopeBackward0";
+    case Node::RopeAxes: return "RopeAxesBackward0";
     case Node::WindowAttention: return "WindowAttentionBackward0";
     }
     return "UnknownBackward";
@@ -1289,6 +1290,127 @@ Tensor window_attention(const Tensor &q, const Tensor &k, const Tensor &v, Atten
     return out;
 }
 
+// The rotation's tables and positions for tensors like x; `what` names the call.
+static void check_rotation(const char *what, const Tensor &x, const Tensor &cos, const Tensor &sin, const RotationSpec &spec) {
+    require_same_device(x, cos);
+    require_same_device(x, sin);
+    if (cos.shape.size() != 2 || cos.shape != sin.shape)
+        throw TensorError(std::string(what) + " tables have shapes " + dims_str(cos.shape) + " and " + dims_str(sin.shape) +
+                          ", expected two of (positions, pairs)");
+    if (cos.requires_grad() || sin.requires_grad()) throw TensorError(std::string(what) + " records no gradient of its tables");
+    if (!spec.pair_axes.empty() && (int64_t)spec.pair_axes.size() != cos.shape[1])
+        throw TensorError(std::string(what) + " has axes for " + std::to_string(spec.pair_axes.size()) + " pairs, and tables of " +
+                          std::to_string(cos.shape[1]));
+    const IndexPtr &pos = spec.positions;
+    const Dims one{x.shape[0], x.shape[2]}, several{spec.axes, x.shape[0], x.shape[2]};
+    if (pos && (!(pos->device == x.device()) || !(pos->shape == several || (spec.axes == 1 && pos->shape == one))))
+        throw TensorError(std::string(what) + " positions have shape " + dims_str(pos->shape) +
+                          ", expected (axes, batch, tokens) on the tensors' device");
+}
+static void check_heads(const char *what, const Tensor &x) {
+    x.require_cuda(what);
+    if (x.shape.size() != 4)
+        throw TensorError(std::string(what) + " takes tensors of 4 dims (batch, head, token, dim), got " + dims_str(x.shape));
+}
+static const uint8_t *pair_axes(const RotationSpec &spec) { return spec.pair_axes.empty() ? nullptr : spec.pair_axes.data(); }
+
+std::vector<Tensor> rope_axes(const std::vector<Tensor> &xs, const Tensor &cos, const Tensor &sin, RotationSpec spec) {
+    if (xs.empty() || xs.size() > 2) throw TensorError("rope_axes takes one or two tensors");
+    std::vector<const float *> px;
+    std::vector<float *> po;
+    std::vector<trs_layout> lx, lo;
+    std::vector<Tensor> outs;
+    for (const Tensor &x : xs) {
+        check_heads("rope_axes", x);
+        require_same_device(xs[0], x);
+        outs.push_back(empty_rows_like(x));
+        px.push_back(x.storage->dptr);
+        po.push_back(outs.back().storage->dptr);
+        lx.push_back(x.abi_layout());
+        lo.push_back(outs.back().abi_layout());
+    }
+    check_rotation("rope_axes", xs[0], cos, sin, spec);
+    const Tensor c = cos.contiguous(), s = sin.contiguous();
+    const trs_layout lt = abi_layout_of(c.shape, layout::contiguous_strides(c.shape), 0);
+    check(trs_rope_axes_f32((int)xs.size(), px.data(), lx.data(), c.storage->dptr + c.offset, s.storage->dptr + s.offset, &lt,
+                            spec.interleaved, spec.axes, pair_axes(spec), spec.positions ? spec.positions->dptr : nullptr, spec.start, 0,
+                            po.data(), lo.data()));
+    for (size_t i = 0; i < xs.size(); i++) {
+        if (!records(xs[i])) continue;
+        auto fn = std::make_unique<GradFn>();
+        fn->kind = GradKind::RopeAxes;
+        fn->node = Node::RopeAxes;
+        fn->rotation = spec;
+        fn->rotation.tables = {save(c, true), save(s, true)};
+        fn->inputs.push_back(save(xs[i], false));
+        attach(outs[i], std::move(fn));
+    }
+    return outs;
+}
+
+// The cache's description for a batch.
+static trs_paged_cache cache_of(const char *what, const PagedCache &c, const IndexBuffer &table, const IndexBuffer &lengths, const Tensor &x) {
+    if (!(c.device == x.device()) || !(table.device == x.device()) || !(lengths.device == x.device()))
+        throw TensorError(std::string(what) + " takes a cache, a table and lengths on the tensors' device");
+    if (table.shape.size() != 2 || table.shape[0] != x.shape[0])
+        throw TensorError(std::string(what) + " table has shape " + dims_str(table.shape) + ", expected (batch, pages)");
+    if (lengths.shape != Dims{x.shape[0]})
+        throw TensorError(std::string(what) + " lengths have shape " + dims_str(lengths.shape) + ", expected (batch)");
+    const Dims shape{c.pages, c.heads, c.page, c.dim};
+    trs_paged_cache d{};
+    d.k = c.k, d.v = c.v;
+    d.lk = d.lv = abi_layout_of(shape, layout::contiguous_strides(shape), 0);
+    d.type = c.type;
+    d.table = table.dptr, d.table_width = table.shape[1];
+    d.lengths = lengths.dptr;
+    return d;
+}
+static void refuse_gradient(const char *what, std::initializer_list<const Tensor *> ts) {
+    for (const Tensor *t : ts)
+        if (t->storage && records(*t)) throw TensorError(std::string(what) + " records no gradient: call it under no_grad or with detached tensors");
+}
+
+Tensor paged_append(const PagedCache &cache, const IndexBuffer &table, const IndexBuffer &lengths, const Tensor &k, const Tensor &v,
+                    const Tensor &q, const Tensor &cos, const Tensor &sin, const RotationSpec &spec) {
+    for (const Tensor *t : {&k, &v, &q}) {
+        if (!t->storage) continue;
+        check_heads("paged_append", *t);
+        require_same_device(k, *t);
+    }
+    refuse_gradient("paged_append", {&k, &v, &q});
+    const trs_paged_cache d = cache_of("paged_append", cache, table, lengths, k);
+    Tensor c, s, out;
+    trs_layout lt{};
+    const bool turns = cos.storage != nullptr;
+    if (turns) {
+        check_rotation("paged_append", k, cos, sin, spec);
+        c = cos.contiguous(), s = sin.contiguous();
+        lt = abi_layout_of(c.shape, layout::contiguous_strides(c.shape), 0);
+    }
+    const trs_layout lk = k.abi_layout(), lv = v.abi_layout();
+    trs_layout lq{}, lo{};
+    if (q.storage) {
+        out = empty_rows_like(q);
+        lq = q.abi_layout(), lo = out.abi_layout();
+    }
+    check(trs_paged_append_f32(&d, k.storage->dptr, &lk, v.storage->dptr, &lv, q.storage ? q.storage->dptr : nullptr, q.storage ? &lq : nullptr,
+                               q.storage ? out.storage->dptr : nullptr, q.storage ? &lo : nullptr, turns ? c.storage->dptr + c.offset : nullptr,
+                               turns ? s.storage->dptr + s.offset : nullptr, turns ? &lt : nullptr, spec.interleaved, spec.axes, pair_axes(spec),
+                               spec.positions ? spec.positions->dptr : nullptr));
+    return out;
+}
+
+Tensor paged_attention(const Tensor &q, const PagedCache &cache, const IndexBuffer &table, const IndexBuffer &lengths, int64_t shared,
+                       int64_t window, int64_t sinks, float scale) {
+    check_heads("paged_attention", q);
+    refuse_gradient("paged_attention", {&q});
+    const trs_paged_cache d = cache_of("paged_attention", cache, table, lengths, q);
+    Tensor out = empty_rows_like(q);
+    const trs_layout lq = q.abi_layout(), lo = out.abi_layout();
+    check(trs_paged_attention_f32(q.storage->dptr, &lq, &d, shared, window, sinks, scale, out.storage->dptr, &lo, nullptr));
+    return out;
+}
+
 float Tensor::item() const {
     if (numel != 1)
         throw TensorError("a Tensor with " + std::to_string(numel) + " elements cannot be converted to Scalar");
@@ -1359,6 +1481,9 @@ void validate(const GradFn &fn) {
     case GradKind::HeadNormRope:
         if (!fn.inputs[0].values) throw TensorError(kGraphFreed);
         break;
+    case GradKind::RopeAxes:
+        if (fn.rotation.tables.empty()) throw TensorError(kGraphFreed);
+        break;
     case GradKind::WindowAttention:
         if (!fn.attention.lse) throw TensorError(kGraphFreed);
         break;
@@ -1389,6 +1514,10 @@ void consume(GradFn &fn) {
     case GradKind::MaskApply: fn.mask.reset(); break;
     case GradKind::HeadNormRope:
         for (auto &in : fn.inputs) in.values.reset();
+        fn.rotation.tables.clear();
+        fn.rotation.positions.reset();
+        break;
+    case GradKind::RopeAxes:
         fn.rotation.tables.clear();
         fn.rotation.positions.reset();
         break;
@@ -1517,6 +1646,19 @@ void apply_grad_fn(const GradFn &fn, Grad up, Device dev, std::map<GradKey, Grad
         Grad g = new_grad(dev, in.shape);
         check(trs_dropout_f32(up.st->dptr, &lup, fn.dropout.p, fn.dropout.seed, fn.dropout.offset, g.st->dptr, &lup));
         add_gradient(grads, in.autograd, in.output_nr, std::move(g));
+        return;
+    }
+    case GradKind::RopeAxes: {  // the rotation by the negative angles
+        const SavedTensor &in = fn.inputs[0];
+        if (!in.autograd) return;
+        const RotationSpec &r = fn.rotation;
+        Grad dx = new_grad(dev, in.shape);
+        const trs_layout lt = abi_layout_of(r.tables[0].shape, layout::contiguous_strides(r.tables[0].shape), 0);
+        const float *pu = up.st->dptr;
+        float *pdx = dx.st->dptr;
+        check(trs_rope_axes_f32(1, &pu, &lup, r.tables[0].values->dptr + r.tables[0].offset, r.tables[1].values->dptr + r.tables[1].offset, &lt,
+                                r.interleaved, r.axes, pair_axes(r), r.positions ? r.positions->dptr : nullptr, r.start, 1, &pdx, &lup));
+        add_gradient(grads, in.autograd, in.output_nr, std::move(dx));
         return;
     }
     case GradKind::HeadNormRope: {
@@ -1817,6 +1959,30 @@ std::shared_ptr<IndexBuffer> IndexBuffer::from_host(const int32_t *data, const D
         check(trs_memcpy_h2d(b->dptr, data, bytes));
     }
     return b;
+}
+
+// ---- paged caches ------------------------------------------------------------------------
+
+PagedCache::~PagedCache() {
+    if (k || v) select_device_quietly(device);
+    if (k) (void)trs_free(k);
+    if (v) (void)trs_free(v);
+}
+
+CachePtr PagedCache::create(int64_t pages, int64_t heads, int64_t page, int64_t dim, int type, Device device) {
+    if (!device.is_cuda()) throw TensorError("paged caches live on the device");
+    if (pages < 1 || heads < 1 || page < 1 || dim < 1) throw TensorError("a paged cache has at least one page, key head, token a page and dim");
+    int64_t bytes = type == TRS_PAGES_BF16 ? 2 : 4;
+    for (int64_t n : {pages, heads, page, dim})
+        if (__builtin_mul_overflow(bytes, n, &bytes)) throw TensorError("a paged cache's size overflows 64 bits");
+    select_device(device);
+    auto c = std::make_shared<PagedCache>();
+    c->device = device, c->pages = pages, c->heads = heads, c->page = page, c->dim = dim, c->type = type;
+    for (void **p : {&c->k, &c->v}) {
+        if (trs_alloc((size_t)bytes, p) != TRS_OK) throw TensorError("failed to allocate " + std::to_string(bytes) + " bytes of pages");
+        check(trs_memset_zero(*p, (size_t)bytes));
+    }
+    return c;
 }
 
 // ---- fusion ------------------------------------------------------------------------------

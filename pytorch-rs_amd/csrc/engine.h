@@ -85,7 +85,7 @@ using MetaPtr = std::shared_ptr<AutogradMeta>;
 enum class Node {
     Add, Alias, Clone, Multiply, Negate, Permute, Relu, ReflectedSubtract, Subtract, Sum, MatrixTranspose,
     Transpose, View, Select, Exp, Mm, Bmm, AddTensor, SubTensor, Squeeze, SqueezeDimension, SqueezeDimensions,
-    Unsqueeze, Fused, Dropout, HeadNormRope, WindowAttention
+    Unsqueeze, Fused, Dropout, HeadNormRope, WindowAttention, RopeAxes
 };
 const char *node_name(Node n);
 
@@ -100,7 +100,7 @@ struct SavedTensor {
 
 enum class GradKind {
     Multiply, MultiplyScalar, Negate, Relu, Sum, Identity, Permute, Index, AddTensor, SubTensor, Matmul, Exp,
-    MaskApply, Transfer, Fused, Dropout, HeadNormRope, WindowAttention
+    MaskApply, Transfer, Fused, Dropout, HeadNormRope, WindowAttention, RopeAxes
 };
 
 // The backward of a fused node: one compiled pointwise program whose
@@ -135,6 +135,18 @@ struct IndexBuffer {
 };
 using IndexPtr = std::shared_ptr<IndexBuffer>;
 
+// Pools of keys and values in HBM, in pages (trs_paged_cache): [page, key head,
+// token of the page, dim] each, zero at first.
+struct PagedCache {
+    Device device;
+    int64_t pages = 0, heads = 0, page = 0, dim = 0;
+    int type = TRS_PAGES_F32;
+    void *k = nullptr, *v = nullptr;
+    ~PagedCache();
+    static std::shared_ptr<PagedCache> create(int64_t pages, int64_t heads, int64_t page, int64_t dim, int type, Device device);
+};
+using CachePtr = std::shared_ptr<PagedCache>;
+
 // What the attention block's nodes keep beside their inputs.
 struct DropoutSpec {
     double p = 0.0;
@@ -146,6 +158,8 @@ struct RotationSpec {
     int64_t start = 0;
     IndexPtr positions;
     std::vector<SavedTensor> tables;  // cosines, sines
+    int axes = 1;                     // of the rotation by several
+    std::vector<uint8_t> pair_axes;   // empty: axis 0 throughout
 };
 struct AttentionSpec {
     int64_t window = 0, sinks = 0;
@@ -272,6 +286,18 @@ std::vector<Tensor> head_norm_rope(const std::vector<Tensor> &xs, const std::vec
 // Causal attention with a sliding window and first tokens that stay visible
 // (trs_window_attention_f32).
 Tensor window_attention(const Tensor &q, const Tensor &k, const Tensor &v, AttentionSpec spec);
+
+// The rotation of one or two tensors [batch, head, token, dim] by positions of
+// several axes (trs_rope_axes_f32).
+std::vector<Tensor> rope_axes(const std::vector<Tensor> &xs, const Tensor &cos, const Tensor &sin, RotationSpec spec);
+// Keys and values of new tokens into the cache (trs_paged_append_f32); returns the
+// turned query where there is one.  A tensor without storage stands for none: of the
+// query, or of both tables.
+Tensor paged_append(const PagedCache &cache, const IndexBuffer &table, const IndexBuffer &lengths, const Tensor &k, const Tensor &v,
+                    const Tensor &q, const Tensor &cos, const Tensor &sin, const RotationSpec &spec);
+// Attention over the cache (trs_paged_attention_f32).
+Tensor paged_attention(const Tensor &q, const PagedCache &cache, const IndexBuffer &table, const IndexBuffer &lengths, int64_t shared,
+                       int64_t window, int64_t sinks, float scale);
 
 // Thread-local no-grad depth (src/grad_mode.rs:5-38).
 void enter_no_grad();

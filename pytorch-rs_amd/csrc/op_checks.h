@@ -27,34 +27,34 @@ inline int check_written_once(const trs_layout *l, const char *what) {
     return TRS_OK;
 }
 
-// Whether two views of 4-byte elements, whose first are at a and b, may share a byte.  Where both
+// Whether two views of elements of `size` bytes, whose first are at a and b, may share a byte.  Where both
 // have their largest stride in common, what lies within a step of one is compared with what lies
 // within the steps of the other that are beside it, as far as the strides agree (slices of one
 // buffer); from there on views count as whole ranges.
-inline bool may_share(uintptr_t a, const trs_layout *la, uintptr_t b, const trs_layout *lb) {
+inline bool may_share(uintptr_t a, const trs_layout *la, uintptr_t b, const trs_layout *lb, int64_t size = 4) {
     struct Dims {
-        int64_t size[TRS_MAX_RANK], stride[TRS_MAX_RANK], reach[TRS_MAX_RANK + 1];  // largest first; reach: of the dims from here on
+        int64_t count[TRS_MAX_RANK], stride[TRS_MAX_RANK], reach[TRS_MAX_RANK + 1];  // largest first; reach: of the dims from here on
         int n = 0;
         explicit Dims(const trs_layout *l) {
             for (int d = 0; d < l->rank; d++) {
                 if (l->shape[d] <= 1 || l->stride[d] == 0) continue;
                 int i = n++;
-                for (; i > 0 && stride[i - 1] < l->stride[d]; i--) size[i] = size[i - 1], stride[i] = stride[i - 1];
-                size[i] = l->shape[d], stride[i] = l->stride[d];
+                for (; i > 0 && stride[i - 1] < l->stride[d]; i--) count[i] = count[i - 1], stride[i] = stride[i - 1];
+                count[i] = l->shape[d], stride[i] = l->stride[d];
             }
             reach[n] = 0;
-            for (int i = n; i-- > 0;) reach[i] = reach[i + 1] + (size[i] - 1) * stride[i];
+            for (int i = n; i-- > 0;) reach[i] = reach[i + 1] + (count[i] - 1) * stride[i];
         }
     };
     const Dims x(la), y(lb);
     // b's dims from j on against a's from i on, b's first element `apart` bytes behind a's.
     const auto meet = [&](auto &&self, int i, int j, int64_t apart) -> bool {
-        if (apart >= (x.reach[i] + 1) * 4 || -apart >= (y.reach[j] + 1) * 4) return false;
+        if (apart >= (x.reach[i] + 1) * size || -apart >= (y.reach[j] + 1) * size) return false;
         if (i == x.n || j == y.n || x.stride[i] != y.stride[j]) return true;
         // Step s of a's dim and t of b's, for every k = s - t at which what lies within them may meet.
-        const int64_t pitch = x.stride[i] * 4;
-        const int64_t first = std::max((apart - (x.reach[i + 1] + 1) * 4) / pitch - 1, 1 - y.size[j]);
-        const int64_t last = std::min((apart + (y.reach[j + 1] + 1) * 4) / pitch + 1, x.size[i] - 1);
+        const int64_t pitch = x.stride[i] * size;
+        const int64_t first = std::max((apart - (x.reach[i + 1] + 1) * size) / pitch - 1, 1 - y.count[j]);
+        const int64_t last = std::min((apart + (y.reach[j + 1] + 1) * size) / pitch + 1, x.count[i] - 1);
         if (last - first > 8) return true;  // neither holds its steps apart
         for (int64_t k = first; k <= last; k++)
             if (self(self, i + 1, j + 1, apart - k * pitch)) return true;

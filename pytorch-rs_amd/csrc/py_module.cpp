@@ -218,6 +218,14 @@ PYBIND11_MODULE(_trs_native, m) {
         return IndexBuffer::from_host(arr.data(), shape, Device::parse(device));
     });
 
+    py::class_<PagedCache, std::shared_ptr<PagedCache>>(m, "PagedCache")
+        .def(py::init([](int64_t pages, int64_t heads, int64_t page, int64_t dim, bool bf16, const std::string &device) {
+            return PagedCache::create(pages, heads, page, dim, bf16 ? TRS_PAGES_BF16 : TRS_PAGES_F32, Device::parse(device));
+        }))
+        .def_property_readonly("shape", [](const PagedCache &c) { return to_tuple(Dims{c.pages, c.heads, c.page, c.dim}); })
+        .def_property_readonly("dtype", [](const PagedCache &c) { return c.type == TRS_PAGES_BF16 ? "bfloat16" : "float32"; })
+        .def_property_readonly("device", [](const PagedCache &c) { return c.device.str(); });
+
     m.def("empty_pinned", &empty_pinned, py::arg("shape"), py::arg("dtype") = "float32");
     m.def("copy_into", &copy_into, py::arg("tensor"), py::arg("out"));
     m.def("bytes_from_numpy",
@@ -332,6 +340,24 @@ PYBIND11_MODULE(_trs_native, m) {
               spec.eps = eps, spec.interleaved = interleaved, spec.start = start, spec.positions = std::move(positions);
               return head_norm_rope(xs, w, cos, sin, std::move(spec));
           });
+    m.def("rope_axes", [](const std::vector<Tensor> &xs, const Tensor &cos, const Tensor &sin, bool interleaved, int axes,
+                          std::vector<uint8_t> pair_axes, int64_t start, IndexPtr positions) {
+        RotationSpec spec;
+        spec.interleaved = interleaved, spec.start = start, spec.positions = std::move(positions);
+        spec.axes = axes, spec.pair_axes = std::move(pair_axes);
+        return rope_axes(xs, cos, sin, std::move(spec));
+    });
+    m.def("paged_append", [](const PagedCache &cache, const IndexBuffer &table, const IndexBuffer &lengths, const Tensor &k, const Tensor &v,
+                             const py::object &q, const py::object &cos, const py::object &sin, bool interleaved, int axes,
+                             std::vector<uint8_t> pair_axes, IndexPtr positions) -> py::object {
+        const auto tensor = [](const py::object &o) { return o.is_none() ? Tensor{} : o.cast<Tensor>(); };
+        RotationSpec spec;
+        spec.interleaved = interleaved, spec.positions = std::move(positions);
+        spec.axes = axes, spec.pair_axes = std::move(pair_axes);
+        Tensor out = paged_append(cache, table, lengths, k, v, tensor(q), tensor(cos), tensor(sin), spec);
+        return q.is_none() ? py::object(py::none()) : py::cast(out);
+    });
+    m.def("paged_attention", &paged_attention);
     m.def("window_attention", [](const Tensor &q, const Tensor &k, const Tensor &v, int64_t window, int64_t sinks, float scale,
                                  IndexPtr lengths) {
         return window_attention(q, k, v, AttentionSpec{window, sinks, scale, std::move(lengths), nullptr});

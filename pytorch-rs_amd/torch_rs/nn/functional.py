@@ -310,3 +310,101 @@ def window_attention(query, key, value, *, window=None, sinks: int = 0, scale=No
     every = (1 << 63) - 1
     return _C.window_attention(query, key, value, every if window is None else min(window, every), min(sinks, every),
                                float(scale), _indices(key_lengths, query))
+
+
+def _pair_axes(op, positions, pair_axes, axes=None):
+    """The number of axes, and the axis of every pair as bytes (none: axis 0)."""
+    if positions is not None:
+        axes = positions.shape[0] if len(positions.shape) == 3 else 1
+    if pair_axes is None:
+        return axes or 1, []
+    pair_axes = [_integer(op, "pair_axes", a) for a in pair_axes]
+    axes = axes or max(pair_axes, default=0) + 1
+    if not 1 <= axes <= 4:
+        raise ValueError(f"{op} positions have 1 to 4 axes, but got {axes}")
+    for a in pair_axes:
+        if not 0 <= a < axes:
+            raise ValueError(f"{op} pair_axes have to be between 0 and {axes - 1}, but got {a}")
+    return axes, pair_axes
+
+
+def rope_axes(query, key, cos, sin, *, positions=None, pair_axes=None, start: int = 0, interleaved: bool = False):
+    """The rotation of queries and keys [batch, head, token, dim] by positions of
+    several axes (time, height, width), in one launch; returns both.
+
+    ``cos`` and ``sin`` are tables [positions, pairs]: the pairs (j, j + pairs) or,
+    ``interleaved``, (2j, 2j + 1) of the first 2 * pairs entries turn by entry j of row
+    ``positions[pair_axes[j]][batch][token]``.  ``positions`` are [axes, batch, token]
+    integers, or an ``index_buffer`` of that shape ([batch, token] for one axis), or None
+    for ``start + token`` on every axis; ``pair_axes`` gives each pair's axis (None: 0).
+    ``key`` may be None, and the query alone is returned then.  Gradients reach queries and
+    keys."""
+    _tensor_arguments("rope_axes", query=query, cos=cos, sin=sin)
+    xs = [query]
+    if key is not None:
+        _tensor_arguments("rope_axes", key=key)
+        xs.append(key)
+    start = _integer("rope_axes", "start", start)
+    positions = _indices(positions, query)
+    axes, pair_axes = _pair_axes("rope_axes", positions, pair_axes)
+    out = _C.rope_axes(xs, cos, sin, bool(interleaved), axes, pair_axes, start, positions)
+    return out[0] if key is None else tuple(out)
+
+
+def paged_cache(pages: int, kv_heads: int, page: int, dim: int, dtype: str = "float32", device="cuda"):
+    """Pools of keys and values in ``pages`` pages of ``page`` tokens, zero at first; "float32" or "bfloat16"."""
+    from .. import _device_str
+    if dtype not in ("float32", "bfloat16"):
+        raise TypeError(f"paged_cache(): dtype must be 'float32' or 'bfloat16', not {dtype!r}")
+    sizes = [_integer("paged_cache", name, value) for name, value in (("pages", pages), ("kv_heads", kv_heads), ("page", page), ("dim", dim))]
+    return _C.PagedCache(*sizes, dtype == "bfloat16", _device_str(device, "paged_cache"))
+
+
+def _cache_arguments(op, cache, table, lengths, like):
+    if not isinstance(cache, _C.PagedCache):
+        raise TypeError(f"{op}(): argument 'cache' must be PagedCache, not {_type_name(cache)}")
+    return _indices(table, like), _indices(lengths, like)
+
+
+def paged_append(cache, table, lengths, key, value, cos=None, sin=None, *, query=None, positions=None, pair_axes=None, interleaved: bool = False):
+    """Writes new tokens' keys and values [batch, key head, token, dim] to the pages that
+    ``table`` ([batch, pages] integers, or an ``index_buffer``) gives, the keys turned on the
+    way as ``rope_axes`` turns them (``cos`` None: as they are); returns the turned
+    ``query`` [batch, head, token, dim], if there is one.
+
+    ``lengths`` ([batch]) are the tokens that each sequence has with the new ones: token t
+    stands at place ``lengths - tokens + t``, which is also its position on every axis
+    where ``positions`` is None.  Tokens before place 0 are padding and are not written.
+    Records no gradient."""
+    _tensor_arguments("paged_append", key=key, value=value)
+    if (cos is None) != (sin is None):
+        raise ValueError("paged_append takes both tables, cos and sin, or neither")
+    for name, t in (("cos", cos), ("sin", sin), ("query", query)):
+        if t is not None:
+            _tensor_arguments("paged_append", **{name: t})
+    table, lengths = _cache_arguments("paged_append", cache, table, lengths, key)
+    positions = _indices(positions, key)
+    axes, pair_axes = _pair_axes("paged_append", positions, pair_axes)
+    return _C.paged_append(cache, table, lengths, key, value, query, cos, sin, bool(interleaved), axes, pair_axes, positions)
+
+
+def paged_attention(query, cache, table, lengths, *, window=None, sinks: int = 0, scale=None, shared: int = 0):
+    """``window_attention`` of ``query`` [batch, heads, tokens, dim] over a paged cache.
+
+    The last query of a sequence stands at its last token, ``lengths`` of ``table``'s
+    (see ``paged_append``).  The first ``shared`` tokens of every sequence are read
+    through the table's first row, once for the whole batch: a prefix that all have in
+    common.  Records no gradient."""
+    _tensor_arguments("paged_attention", query=query)
+    table, lengths = _cache_arguments("paged_attention", cache, table, lengths, query)
+    window = None if window is None else _integer("paged_attention", "window", window)
+    sinks, shared = _integer("paged_attention", "sinks", sinks), _integer("paged_attention", "shared", shared)
+    if window is not None and window < 1:
+        raise ValueError(f"paged_attention window has to be at least 1, but got {window}")
+    if sinks < 0 or shared < 0:
+        raise ValueError(f"paged_attention sinks and shared have to be at least 0, but got {sinks} and {shared}")
+    if scale is None:
+        scale = 1.0 / math.sqrt(query.shape[-1]) if len(query.shape) and query.shape[-1] else 1.0
+    every = (1 << 63) - 1
+    return _C.paged_attention(query, cache, table, lengths, min(shared, every), every if window is None else min(window, every),
+                              min(sinks, every), float(scale))

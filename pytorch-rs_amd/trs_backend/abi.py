@@ -44,6 +44,24 @@ class Layout(ctypes.Structure):
         return tuple(self.stride[i] for i in range(self.rank))
 
 
+PAGES_F32, PAGES_BF16 = 0, 1
+
+
+class PagedCache(ctypes.Structure):
+    """trs_paged_cache: pools of keys and values, the page table and the sequences' lengths."""
+    _fields_ = [
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("lk", Layout),
+        ("lv", Layout),
+        ("type", c_int32),
+        ("reserved", c_int32),
+        ("table", c_void_p),
+        ("table_width", c_int64),
+        ("lengths", c_void_p),
+    ]
+
+
 class TrsError(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(f"{ERROR_NAMES.get(code, code)}: {message}")
@@ -145,6 +163,12 @@ _SIGNATURES = {
     "trs_window_attention_backward_f32": ([c_void_p, _LP, c_void_p, _LP, c_void_p, _LP, c_void_p, c_int64, c_int64, c_float,
                                            c_void_p, _LP, c_void_p, c_void_p, _LP, c_void_p, _LP, c_void_p, _LP,
                                            c_void_p, _LP], c_int),
+    "trs_rope_axes_f32": ([c_int, _PP, _LP, c_void_p, c_void_p, _LP, c_int, c_int, c_void_p, c_void_p, c_int64, c_int, _PP, _LP],
+                          c_int),
+    "trs_paged_append_f32": ([POINTER(PagedCache), c_void_p, _LP, c_void_p, _LP, c_void_p, _LP, c_void_p, _LP, c_void_p, c_void_p,
+                              _LP, c_int, c_int, c_void_p, c_void_p], c_int),
+    "trs_paged_attention_f32": ([c_void_p, _LP, POINTER(PagedCache), c_int64, c_int64, c_int64, c_float, c_void_p, _LP, c_void_p],
+                                c_int),
     "trs_pointwise_plan": ([c_int, POINTER(c_void_p), POINTER(_LP), POINTER(c_int), c_void_p, _LP, c_int, c_int,
                             POINTER(PwPlanInfo)], c_int),
     "trs_pointwise_plan_access": ([c_int, POINTER(c_void_p), POINTER(_LP), POINTER(c_int), c_void_p, _LP, c_int, c_int,
