@@ -4,60 +4,135 @@
 
 #include <cmath>
 
-#include "attention.h"
-#include "paged.h"
+#include "paged_attention.h"
 
 namespace trs {
 
 namespace {
 
 constexpr int64_t kMaxHeadDim = 256;
+constexpr int kFewTile = 16;  // rows of a tile of paged_few
 
-struct PagedArgs {
-    Pages pages;
-    const float *q;
-    float *out, *lse;
-    AttnView qs, os;
-    int32_t batch, heads, kv_heads, group, Sq, D;
-    int32_t window, sinks, shared;
-    float scale2;
-};
+// The parts of a row, joined: four columns a lane.  Every part is read before the first is
+// added, up to eight.
+__global__ void __launch_bounds__(256) paged_join(PagedArgs a) {
+    const int64_t rows = (int64_t)a.batch * a.kv_heads * a.seq_rows;
+    const uint32_t quads = (uint32_t)a.part_width / 4;
+    const int64_t lane = (int64_t)blockIdx.x * 256 + threadIdx.x, at = lane / quads;
+    if (at >= rows) return;
+    const int d = (int)(lane - at * quads) * 4;
+    const int64_t head = at / a.seq_rows;
+    const int r = (int)(at - head * a.seq_rows), b = (int)(head / a.kv_heads), hk = (int)(head - (int64_t)b * a.kv_heads);
+    float most = -__builtin_inff(), sum = 0.f;
+    at_f4 o = (at_f4)(0.f);
+    for (int n = 0; n < a.stages; n++) {
+        const PagedStage &s = a.stage[n];
+        const int one = s.together ? b * a.seq_rows + r : r, tile = one / s.tile_rows;
+        const int entry = s.together ? tile : b * s.row_tiles + tile;
+        const int2 blocks = s.found[(int64_t)hk * s.entries + entry];
+        if (a.stages == 1 && blocks.x == blocks.y) return;  // its block wrote it
+        const int parts = blocks.y - blocks.x + 1;
+        for (int p0 = 0; p0 < parts; p0 += 8) {
+            float m[8], l[8];
+            at_f4 x[8];
+#pragma unroll
+            for (int p = 0; p < 8; p++) {
+                const int w = min(blocks.x + p0 + p, blocks.y);
+                const int64_t part = ((int64_t)hk * s.slots + slot_of_part(a, s, w, entry, w == blocks.x)) * s.tile_rows + one - tile * s.tile_rows;
+                m[p] = s.part_ml[2 * part], l[p] = s.part_ml[2 * part + 1];
+                x[p] = *(const at_f4 *)(s.part_o + part * a.part_width + d);
+            }
+            float now = most;
+#pragma unroll
+            for (int p = 0; p < 8; p++) now = __builtin_fmaxf(now, m[p]);
+            const float base = now == -__builtin_inff() ? 0.f : now, keep = __builtin_amdgcn_exp2f(most - base);
+            sum *= keep, o *= keep, most = now;
+#pragma unroll
+            for (int p = 0; p < 8; p++) {
+                if (p0 + p >= parts) break;
+                const float f = __builtin_amdgcn_exp2f(m[p] - base);
+                sum += l[p] * f, o += x[p] * f;
+            }
+        }
+    }
+    const int i = (int)a.by_group.divide((uint32_t)r);
+    const int64_t h = (int64_t)hk * a.group + r - i * a.group;
+    o *= a.pages.keys_of(b) - a.Sq + i < 0 ? 0.f : 1.f / sum;
+    float *out = a.out + b * a.os.b + h * a.os.h + (int64_t)i * a.os.s + d;
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+        if (d + q < a.D) out[q] = o[q];
+    if (a.lse && d == 0) a.lse[((int64_t)b * a.heads + h) * a.Sq + i] = log_sum(most, sum);
+}
 
-// A wave a query: a key at a time, its entries dealt to the lanes.
-template <class E>
-__global__ void __launch_bounds__(64) paged_each(PagedArgs a) {
-    const int lane = (int)threadIdx.x;
-    const int64_t id = blockIdx.x;
-    const int i = (int)(id % a.Sq), h = (int)(id / a.Sq % a.heads), b = (int)(id / a.Sq / a.heads), hk = h / a.group;
-    const int place = a.pages.keys_of(b) - a.Sq + i;
-    const float *qp = a.q + b * a.qs.b + h * a.qs.h + i * a.qs.s;
-    float q[4], acc[4] = {0.f, 0.f, 0.f, 0.f}, most = -__builtin_inff(), sum = 0.f;
-    for (int e = 0; e < 4; e++) q[e] = lane + 64 * e < a.D ? qp[lane + 64 * e] * a.scale2 : 0.f;
-    const auto key = [&](int j) {
-        const int at = a.pages.page_of(j < a.shared ? 0 : b, j), slot = a.pages.slot_of(j);
-        const bool held = a.pages.holds(at);
-        const int64_t page = held ? at : 0;
-        const E *k = (const E *)a.pages.k + page * a.pages.ks.p + hk * a.pages.ks.h + slot * a.pages.ks.s;
-        const E *v = (const E *)a.pages.v + page * a.pages.vs.p + hk * a.pages.vs.h + slot * a.pages.vs.s;
-        float s = 0.f;
-        for (int e = 0; e < 4; e++)
-            if (lane + 64 * e < a.D) s += q[e] * (float)k[lane + 64 * e];
-        for (int d = 1; d < 64; d *= 2) s += __shfl_xor(s, d);
-        if (!held) s = __builtin_nanf("");
-        const float now = __builtin_fmaxf(most, s), base = now == -__builtin_inff() ? 0.f : now;
-        const float keep = __builtin_amdgcn_exp2f(most - base), p = __builtin_amdgcn_exp2f(s - base);
-        sum = sum * keep + p;
-        most = now;
-        for (int e = 0; e < 4; e++)
-            if (lane + 64 * e < a.D) acc[e] = acc[e] * keep + p * (float)v[lane + 64 * e];
+// A stage of keys [from, to): its tiles of rows, and the blocks that share them.
+PagedStage plan_stage(const PagedArgs &a, bool together, int from, int to, int cu_count, int shift) {
+    PagedStage s{};
+    s.together = together, s.from = from, s.to = to;
+    s.tile_rows = kFewTile;
+    const int64_t rows = together ? (int64_t)a.batch * a.seq_rows : a.seq_rows;
+    s.row_tiles = (int32_t)((rows + s.tile_rows - 1) / s.tile_rows);
+    s.entries = (int32_t)(together ? s.row_tiles : (int64_t)s.row_tiles * a.batch);
+    s.least = shift == 4 ? 8 : 4;
+    s.blocks = std::max(1, 2 * cu_count / a.kv_heads);
+    return s;
+}
+
+// Whether the stages have memory for parts; the parts are for speed alone.
+int take_parts(PagedArgs &a, void **ws) {
+    size_t floats = 0, found = 0;
+    for (int i = 0; i < a.stages; i++) {
+        PagedStage &s = a.stage[i];
+        s.slots = a.stages > 1 ? (int64_t)s.blocks + s.entries : 2 * (int64_t)s.blocks;
+        floats += (size_t)(a.kv_heads * s.slots * s.tile_rows) * (size_t)(a.part_width + 2);
+        found += (size_t)a.kv_heads * (size_t)s.entries;
+    }
+    TRS_CHECK(trs_alloc(floats * sizeof(float) + found * sizeof(int2), ws));
+    float *p = (float *)*ws;
+    for (int i = 0; i < a.stages; i++) {
+        PagedStage &s = a.stage[i];
+        const size_t parts = (size_t)(a.kv_heads * s.slots * s.tile_rows);
+        s.part_o = p, s.part_ml = p + parts * (size_t)a.part_width;
+        p += parts * (size_t)(a.part_width + 2);
+    }
+    for (int i = 0; i < a.stages; i++) {
+        PagedStage &s = a.stage[i];
+        s.found = (int2 *)p;
+        p += 2 * (size_t)a.kv_heads * (size_t)s.entries;
+    }
+    return TRS_OK;
+}
+
+int paged_forward(PagedArgs &a, bool bf16, DeviceState *dev) {
+    const int shift = bf16 ? 5 : 4;
+    a.part_width = (a.D + 3) / 4 * 4;
+    a.stages = 0;
+    if (a.shared > 0 && a.batch > 1 && (int64_t)a.batch * a.seq_rows < (int64_t)1 << 31) {
+        a.all_rows = a.batch * a.seq_rows, a.by_seq_rows = SmallDivisor((uint32_t)a.seq_rows);
+        a.stage[a.stages++] = plan_stage(a, true, 0, a.shared, dev->cu_count, shift);
+    }
+    const int from = a.stages ? a.shared : 0;
+    if (from < a.pages.capacity || a.stages == 0) a.stage[a.stages++] = plan_stage(a, false, from, a.pages.capacity, dev->cu_count, shift);
+    void *ws = nullptr;
+    const int rc0 = take_parts(a, &ws);
+    if (rc0 == TRS_E_ALLOCATION_FAILED) {
+        a.stages = 1;
+        a.stage[0] = plan_stage(a, false, 0, a.pages.capacity, dev->cu_count, shift);
+        a.stage[0].blocks = 0;
+    } else if (rc0) {
+        return rc0;
+    }
+    const auto launch = [&]() -> int {
+        TRS_CHECK(launch_paged_few(a, 0, a.stages, bf16, dev->stream));
+        if (!ws) return TRS_OK;
+        const int64_t lanes = (int64_t)a.batch * a.kv_heads * a.seq_rows * (a.part_width / 4);
+        if ((lanes + 255) / 256 >> 24) return set_error(TRS_E_INVALID_ARGUMENT, "attention over %lld rows", (long long)a.batch * a.seq_rows);
+        hipLaunchKernelGGL(paged_join, dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, dev->stream, a);
+        TRS_LAUNCH_CHECK("paged attention join launch");
+        return TRS_OK;
     };
-    const int first = max(place - a.window + 1, 0);
-    for (int j = 0; j < min(a.sinks, first); j++) key(j);
-    for (int j = first; j <= place; j++) key(j);
-    float *op = a.out + b * a.os.b + h * a.os.h + i * a.os.s;
-    for (int e = 0; e < 4; e++)
-        if (lane + 64 * e < a.D) op[lane + 64 * e] = place < 0 ? 0.f : acc[e] / sum;
-    if (a.lse && lane == 0) a.lse[((int64_t)b * a.heads + h) * a.Sq + i] = log_sum(most, sum);
+    const int rc = launch(), frc = ws ? trs_free(ws) : TRS_OK;
+    return rc ? rc : frc;
 }
 
 int run_paged(const float *q, const trs_layout *lq, const trs_paged_cache *cache, int64_t shared, int64_t window, int64_t sinks, float scale,
@@ -105,13 +180,11 @@ int run_paged(const float *q, const trs_layout *lq, const trs_paged_cache *cache
     a.lse = lse;
     a.batch = (int32_t)B, a.heads = (int32_t)H, a.kv_heads = (int32_t)HK, a.group = (int32_t)(H / HK), a.Sq = (int32_t)Sq, a.D = (int32_t)D;
     const int64_t most = std::max(a.pages.capacity, 1);
-    a.window = (int32_t)std::min(window, most), a.sinks = (int32_t)std::min(sinks, most), a.shared = (int32_t)std::min(shared, most);
+    a.window = (int32_t)std::min(window, most), a.sinks = (int32_t)std::min(sinks, most), a.shared = (int32_t)std::min<int64_t>(shared, a.pages.capacity);
     a.scale2 = scale * kLog2e;
-    if (rows >> 26) return set_error(TRS_E_INDEX_OVERFLOW, "attention over %lld rows", (long long)rows);
-    if (cache->type == TRS_PAGES_BF16) hipLaunchKernelGGL(paged_each<__bf16>, dim3((unsigned)rows), dim3(64), 0, dev->stream, a);
-    else hipLaunchKernelGGL(paged_each<float>, dim3((unsigned)rows), dim3(64), 0, dev->stream, a);
-    TRS_LAUNCH_CHECK("paged attention launch");
-    return TRS_OK;
+    a.seq_rows = a.group * a.Sq;
+    a.by_group = SmallDivisor((uint32_t)a.group);
+    return paged_forward(a, cache->type == TRS_PAGES_BF16, dev);
 }
 
 }  // namespace
