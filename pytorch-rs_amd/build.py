@@ -42,7 +42,8 @@ HIP_FLAGS = [
 HIP_SOURCES = ["pw_binary.hip", "pw_binary_muldiv.hip", "pw_scalar.hip", "pw_unary.hip", "pw_mask.hip",
                "pointwise.hip", "runtime.hip", "transfer.hip", "gemm.hip", "gemm_skinny.hip", "fusion.hip",
                "dropout.hip", "head_norm.hip", "attention.hip", "attention_forward.hip", "attention_few.hip", "attention_backward.hip",
-               "attention_backward_split.hip", "attention_backward_wide.hip", "rope.hip", "paged_attention.hip", "paged_few.hip"]
+               "attention_backward_split.hip", "attention_backward_wide.hip", "rope.hip", "paged_attention.hip", "paged_few.hip",
+               "paged_rows.hip"]
 # Flags of one source.  The attention gradients hold over 256 registers a lane: with the matrix
 # results in the vector registers, and not the accumulation ones, nothing spills at a head dim of
 # 128 (a training step of 4096 tokens, 32 heads, window 2048: 2.86 ms without, 2.50 with).

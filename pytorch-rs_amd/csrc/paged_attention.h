@@ -187,6 +187,14 @@ __device__ __forceinline__ int64_t slot_of_part(const PagedArgs &a, const PagedS
     return a.stages > 1 ? (int64_t)w + entry : 2 * (int64_t)w + starts;
 }
 
+// Whether rows of the pages are read in vectors: ones of 16 bytes need that alignment in bfloat16 pages; float32's need none.
+inline bool paged_vectors(const PagedArgs &a, bool bf16) {
+    const auto aligned = [](const void *p, const PoolView &v) { return (uintptr_t)p % 16 == 0 && v.p % 8 == 0 && v.h % 8 == 0 && v.s % 8 == 0; };
+    return bf16 ? a.D % 8 == 0 && aligned(a.pages.k, a.pages.ks) && aligned(a.pages.v, a.pages.vs) : a.D % 4 == 0;
+}
+
+// Many rows (paged_rows.hip): one stage, tiles of 128 or 256 rows, heads of up to kPiecesDim.
+int launch_paged_rows(const PagedArgs &a, int stage, bool bf16, hipStream_t s);
 // Few rows a sequence, or of all (paged_few.hip): stages [from, from + count).
 int launch_paged_few(const PagedArgs &a, int from, int count, bool bf16, hipStream_t s);
 

@@ -12,6 +12,7 @@ namespace {
 
 constexpr int64_t kMaxHeadDim = 256;
 constexpr int kFewTile = 16;  // rows of a tile of paged_few
+constexpr int kFewRows = 32;
 
 // The parts of a row, joined: four columns a lane.  Every part is read before the first is
 // added, up to eight.
@@ -66,15 +67,20 @@ __global__ void __launch_bounds__(256) paged_join(PagedArgs a) {
 }
 
 // A stage of keys [from, to): its tiles of rows, and the blocks that share them.
-PagedStage plan_stage(const PagedArgs &a, bool together, int from, int to, int cu_count, int shift) {
+PagedStage plan_stage(const PagedArgs &a, bool together, int from, int to, int cu_count, bool bf16) {
     PagedStage s{};
     s.together = together, s.from = from, s.to = to;
-    s.tile_rows = kFewTile;
     const int64_t rows = together ? (int64_t)a.batch * a.seq_rows : a.seq_rows;
+    s.tile_rows = rows <= kFewRows || a.D > kPiecesDim ? kFewTile : rows <= 128 && bf16 ? 128 : 256;
     s.row_tiles = (int32_t)((rows + s.tile_rows - 1) / s.tile_rows);
     s.entries = (int32_t)(together ? s.row_tiles : (int64_t)s.row_tiles * a.batch);
-    s.least = shift == 4 ? 8 : 4;
-    s.blocks = std::max(1, 2 * cu_count / a.kv_heads);
+    if (s.tile_rows == kFewTile) {
+        s.least = bf16 ? 4 : 8;
+        s.blocks = std::max(1, 2 * cu_count / a.kv_heads);
+    } else {
+        s.least = 2;
+        s.blocks = std::max(1, cu_count * (256 / s.tile_rows) / a.kv_heads);
+    }
     return s;
 }
 
@@ -104,26 +110,30 @@ int take_parts(PagedArgs &a, void **ws) {
 }
 
 int paged_forward(PagedArgs &a, bool bf16, DeviceState *dev) {
-    const int shift = bf16 ? 5 : 4;
     a.part_width = (a.D + 3) / 4 * 4;
     a.stages = 0;
     if (a.shared > 0 && a.batch > 1 && (int64_t)a.batch * a.seq_rows < (int64_t)1 << 31) {
         a.all_rows = a.batch * a.seq_rows, a.by_seq_rows = SmallDivisor((uint32_t)a.seq_rows);
-        a.stage[a.stages++] = plan_stage(a, true, 0, a.shared, dev->cu_count, shift);
+        a.stage[a.stages++] = plan_stage(a, true, 0, a.shared, dev->cu_count, bf16);
     }
     const int from = a.stages ? a.shared : 0;
-    if (from < a.pages.capacity || a.stages == 0) a.stage[a.stages++] = plan_stage(a, false, from, a.pages.capacity, dev->cu_count, shift);
+    if (from < a.pages.capacity || a.stages == 0) a.stage[a.stages++] = plan_stage(a, false, from, a.pages.capacity, dev->cu_count, bf16);
     void *ws = nullptr;
     const int rc0 = take_parts(a, &ws);
     if (rc0 == TRS_E_ALLOCATION_FAILED) {
         a.stages = 1;
-        a.stage[0] = plan_stage(a, false, 0, a.pages.capacity, dev->cu_count, shift);
+        a.stage[0] = plan_stage(a, false, 0, a.pages.capacity, dev->cu_count, bf16);
         a.stage[0].blocks = 0;
     } else if (rc0) {
         return rc0;
     }
     const auto launch = [&]() -> int {
-        TRS_CHECK(launch_paged_few(a, 0, a.stages, bf16, dev->stream));
+        const auto few = [&](int i) { return a.stage[i].tile_rows == kFewTile; };
+        if (a.stages == 2 && few(0) && few(1)) {
+            TRS_CHECK(launch_paged_few(a, 0, 2, bf16, dev->stream));
+        } else {
+            for (int i = 0; i < a.stages; i++) TRS_CHECK(few(i) ? launch_paged_few(a, i, 1, bf16, dev->stream) : launch_paged_rows(a, i, bf16, dev->stream));
+        }
         if (!ws) return TRS_OK;
         const int64_t lanes = (int64_t)a.batch * a.kv_heads * a.seq_rows * (a.part_width / 4);
         if ((lanes + 255) / 256 >> 24) return set_error(TRS_E_INVALID_ARGUMENT, "attention over %lld rows", (long long)a.batch * a.seq_rows);
@@ -156,7 +166,8 @@ int run_paged(const float *q, const trs_layout *lq, const trs_paged_cache *cache
     if (sinks < 0) return set_error(TRS_E_INVALID_ARGUMENT, "attention sinks have to be at least 0, got %lld", (long long)sinks);
     if (shared < 0) return set_error(TRS_E_INVALID_ARGUMENT, "shared keys have to be at least 0, got %lld", (long long)shared);
     if (!std::isfinite(scale)) return set_error(TRS_E_INVALID_ARGUMENT, "attention scale has to be finite");
-    if (Sq > kMaxPagedTokens || B > INT32_MAX || H > INT32_MAX || (HK > 0 && (H / HK) * Sq > kMaxPagedTokens))
+    if (Sq > kMaxPagedTokens || B > INT32_MAX || H > INT32_MAX || (HK > 0 && (H / HK) * Sq > kMaxPagedTokens) ||
+        (HK > 0 && B * (((H / HK) * Sq + kFewTile - 1) / kFewTile) > INT32_MAX))
         return set_error(TRS_E_INDEX_OVERFLOW, "attention over more than 2^30 tokens, or rows that share a key head");
     TRS_CHECK(check_written_once(lo, "output"));
     if (D > 1 && lo->stride[3] != 1) return set_error(TRS_E_INVALID_ARGUMENT, "output needs a unit stride along its last dim");

@@ -413,11 +413,7 @@ int launch_paged_few(const PagedArgs &args, int from, int count, bool bf16, hipS
         return set_error(TRS_E_INVALID_ARGUMENT, "attention over %lld blocks of rows", (long long)(blocks[0] + blocks[1]));
     a.few_blocks = (int32_t)blocks[0];
     const dim3 grid((unsigned)(blocks[0] + blocks[1]));
-    // Vectors of 16 bytes need that alignment of every row of bfloat16 pages (8 where rows are narrow); float32's need none.
-    const auto aligned = [](const void *p, const PoolView &v) {
-        return (uintptr_t)p % 16 == 0 && v.p % 8 == 0 && v.h % 8 == 0 && v.s % 8 == 0;
-    };
-    const bool vectors = bf16 ? a.D % 8 == 0 && aligned(a.pages.k, a.pages.ks) && aligned(a.pages.v, a.pages.vs) : a.D % 4 == 0;
+    const bool vectors = paged_vectors(a, bf16);
     if (bf16) {
         if (a.D <= 64) launch_width<Bf16Pages, 64>(a, from, vectors, grid, s);
         else if (a.D <= 128) launch_width<Bf16Pages, 128>(a, from, vectors, grid, s);
