@@ -9,7 +9,7 @@
 
 namespace trs {
 
-constexpr int64_t kMaxPagedTokens = (int64_t)1 << 30;  // of a sequence
+constexpr int64_t kMaxPagedTokens = (int64_t)1 << 29;  // of a sequence
 
 struct PoolView {  // [page, key head, token of the page], unit stride along dim
     int64_t p, h, s;
@@ -51,7 +51,7 @@ inline int check_cache(const trs_paged_cache *c, int64_t batch, Pages *out) {
     if (c->table_width < 0) return set_error(TRS_E_INVALID_ARGUMENT, "page table has a width of %lld", (long long)c->table_width);
     if (page < 1) return set_error(TRS_E_INVALID_ARGUMENT, "pages hold no token");
     if (pages > INT32_MAX || page > kMaxPagedTokens || c->table_width > kMaxPagedTokens / page)
-        return set_error(TRS_E_INDEX_OVERFLOW, "a paged cache of more than 2^31 pages, or of more than 2^30 tokens a sequence");
+        return set_error(TRS_E_INDEX_OVERFLOW, "a paged cache of more than 2^31 pages, or of more than 2^29 tokens a sequence");
     if (pages == 0 && c->table_width > 0) return set_error(TRS_E_INVALID_ARGUMENT, "paged cache has no pages");
     if (batch > 0 && !c->lengths) return set_error(TRS_E_INVALID_ARGUMENT, "lengths are null");
     if (batch > 0 && c->table_width > 0 && !c->table) return set_error(TRS_E_INVALID_ARGUMENT, "page table is null");

@@ -8,10 +8,10 @@
 // each, or, for the prefix that a batch shares, of all its sequences one behind another.
 //
 // Lengths are on the device, so the work is divided there.  A stage's tiles of rows (its
-// entries) have as many key tiles as their rows see; all of them in a list, the W blocks
-// of a key head take equal shares of it: block w the tiles from T w / W on, of an entry's
-// end, some whole entries and the next one's start.  What a block has of an entry that
-// others have too is a part, joined by a second launch.
+// entries) have as many key tiles as their rows see; all of them in a list, the workers of a key
+// head (waves of paged_few, blocks of paged_rows) take equal shares of it: an entry's end, some
+// whole entries and the next one's start.  What a worker has of an entry that others have too is
+// a part, joined by a second launch.
 #pragma once
 
 #include "attention.h"
@@ -25,11 +25,12 @@ struct PagedStage {
     int32_t row_tiles;  // of a sequence, or of all
     int32_t entries;
     int32_t tile_rows;
-    int32_t blocks;      // W; 0: a block for every entry
-    int32_t least;       // the least key tiles of a block that has others beside it
+    int32_t workers;     // of a key head; 0: one for every entry
+    int32_t least;       // the least key tiles of a worker that has others beside it
+    SmallDivisor by_row_tiles;
     int64_t slots;       // of parts, a key head
     float *part_o, *part_ml;  // [key head][slot][row of the tile]: part_width floats, and (maximum, sum)
-    int2 *found;              // [key head][entry]: the first and the last block that have tiles of it
+    int2 *found;              // [key head][entry]: the first and the last worker that have tiles of it
 };
 
 struct PagedArgs {
@@ -44,7 +45,8 @@ struct PagedArgs {
     int32_t seq_rows;  // Sq * group
     int32_t all_rows;  // batch * seq_rows; only where rows are together
     SmallDivisor by_group, by_seq_rows;
-    int32_t stages, few_blocks;  // few_blocks: of the first of two stages that one launch has
+    int32_t stages;
+    int32_t few_workers, few_all;  // of paged_few's launch: of the first of its stages, and of all
     PagedStage stage[2];
 };
 
@@ -68,6 +70,10 @@ struct PagedKeys {
     __device__ __forceinline__ int first_key(int t) const { return (t < sink_tiles ? sink_first + t : first + t - sink_tiles) << SHIFT; }
 };
 
+// What is the same in all lanes, where the compiler cannot tell: to scalar registers.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) { return (int64_t)(uint32_t)uniform((int)x) | (int64_t)uniform((int)(x >> 32)) << 32; }
+
 // The least and the most keys of a sequence of the batch (every lane of the wave calls it).
 __device__ __forceinline__ int2 keys_of_all(const PagedArgs &a, int lane) {
     int lo = a.pages.capacity, hi = 0;
@@ -77,78 +83,84 @@ __device__ __forceinline__ int2 keys_of_all(const PagedArgs &a, int lane) {
     }
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) lo = min(lo, __shfl_xor(lo, d)), hi = max(hi, __shfl_xor(hi, d));
-    return make_int2(lo, hi);
+    return make_int2(uniform(lo), uniform(hi));
 }
 
-// A stage's list of tiles, and a block's share of it.
+// A stage's list of tiles, and worker w's share of it: tiles `pos` to `end`.  (Below 2^31 tiles,
+// which the host sees to.)  Every lane of the wave calls it.
 template <int SHIFT>
 struct PagedShare {
     const PagedArgs &a;
     const PagedStage &s;
-    int2 all;        // together: the batch's least and most keys
-    int blocks;      // that have a share
-    int64_t total, pos, end;  // tiles: of the list, of the share
-    int entry;       // the entry of tile `pos`
-    int64_t before;  // tiles ahead of that entry
+    int2 all;                // together: the batch's least and most keys
+    uint32_t base, extra;    // the tiles of a worker; the first `extra` have one more
+    uint32_t pos, end;
+    int entry;               // the entry of tile `pos`
+    uint32_t before;         // tiles ahead of that entry
 
-    // Entry e: at least one tile, so that every row is written by some block.
-    __device__ __forceinline__ PagedKeys<SHIFT> keys(int e) const {
-        if (s.together) return PagedKeys<SHIFT>(a, s, all.x - a.Sq, all.y - 1);
-        const int b = e / s.row_tiles, t = e - b * s.row_tiles, n = a.pages.keys_of(b);
-        const int r0 = t * s.tile_rows, r1 = min(r0 + s.tile_rows, a.seq_rows) - 1;
+    __device__ __forceinline__ int sequence_of(int e) const { return (int)s.by_row_tiles.divide((uint32_t)e); }
+    // What entry e of a sequence of n tokens sees.
+    __device__ __forceinline__ PagedKeys<SHIFT> keys(int e, int n) const {
+        const int r0 = (e - sequence_of(e) * s.row_tiles) * s.tile_rows, r1 = min(r0 + s.tile_rows, a.seq_rows) - 1;
         return PagedKeys<SHIFT>(a, s, n - a.Sq + (int)a.by_group.divide((uint32_t)r0), n - a.Sq + (int)a.by_group.divide((uint32_t)r1));
     }
+    __device__ __forceinline__ PagedKeys<SHIFT> keys(int e) const {
+        return s.together ? PagedKeys<SHIFT>(a, s, all.x - a.Sq, all.y - 1) : keys(e, a.pages.keys_of(sequence_of(e)));
+    }
+    // At least one tile, so that every row is written by some worker.
     __device__ __forceinline__ int tiles_of(int e) const { return max(keys(e).tiles, 1); }
-
+    __device__ __forceinline__ uint32_t start_of(uint32_t w) const { return w * base + min(w, extra); }
+    // The worker that has tile x of the list.
+    __device__ __forceinline__ int worker_of(uint32_t x) const {
+        const uint32_t longer = extra * (base + 1);
+        return (int)(x < longer ? x / (base + 1) : extra + (x - longer) / base);
+    }
+    __device__ __forceinline__ void divide(uint32_t total, uint32_t w) {
+        const uint32_t workers = min((uint32_t)s.workers, (total + s.least - 1) / s.least);
+        base = total / workers, extra = total - base * workers;
+        pos = w < workers ? start_of(w) : 0, end = w < workers ? start_of(w + 1) : 0;
+    }
     __device__ __forceinline__ PagedShare(const PagedArgs &args, const PagedStage &stage, int w, int lane) : a(args), s(stage) {
         all = s.together ? keys_of_all(a, lane) : make_int2(0, 0);
-        if (s.blocks == 0) {  // an entry each
-            blocks = s.entries, entry = w, before = pos = 0, end = total = w < s.entries ? tiles_of(w) : 0;
-            return;
-        }
-        if (s.together) {
-            total = (int64_t)s.entries * tiles_of(0);
-        } else {
-            int64_t sum = 0;
-            for (int e = lane; e < s.entries; e += 64) sum += tiles_of(e);
-#pragma unroll
-            for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
-            total = sum;
-        }
-        blocks = (int)min((int64_t)s.blocks, (total + s.least - 1) / s.least);
-        pos = w < blocks ? total * w / blocks : 0, end = w < blocks ? total * (w + 1) / blocks : 0;
         entry = 0, before = 0;
-        if (pos >= end) return;
-        if (s.together) {
-            const int each = tiles_of(0);
-            entry = (int)(pos / each), before = (int64_t)entry * each;
-            return;
-        }
-        // The last entry that begins at or ahead of `pos`.
-        for (int e0 = 0; e0 < s.entries; e0 += 64) {
-            const int mine = e0 + lane < s.entries ? tiles_of(e0 + lane) : 0;
-            int64_t sum = mine;
+        if (s.workers == 0) {  // an entry each
+            entry = w, base = extra = pos = 0, end = w < s.entries ? uniform(tiles_of(w)) : 0;
+        } else if (s.together) {
+            const uint32_t each = tiles_of(0);
+            divide(s.entries * each, w);
+            if (pos < end) entry = (int)(pos / each), before = entry * each;
+        } else {
+            // The tiles up to each entry, 64 of them at a time, and the last one that begins at or ahead of `pos`.
+            const auto up_to = [&](int e0) {
+                uint32_t sum = e0 + lane < s.entries ? tiles_of(e0 + lane) : 0;
 #pragma unroll
-            for (int d = 1; d < 64; d *= 2) {
-                const int64_t more = __shfl_up(sum, d);
-                sum += lane >= d ? more : 0;
-            }
-            const int64_t group = __shfl(sum, 63);
-            if (pos < before + group) {
-                const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before + sum > pos));
-                before += __shfl(sum - mine, l);
-                entry = e0 + l;
-                break;
-            }
-            before += group;
+                for (int d = 1; d < 64; d *= 2) {
+                    const uint32_t more = __shfl_up(sum, d);
+                    sum += lane >= d ? more : 0;
+                }
+                return sum;
+            };
+            const auto last = [](uint32_t sum) { return (uint32_t)__builtin_amdgcn_readlane(sum, 63); };
+            const uint32_t first = up_to(0);
+            uint32_t total = last(first), sum = first;
+            for (int e0 = 64; e0 < s.entries; e0 += 64) total += last(up_to(e0));
+            divide(total, w);
+            if (pos >= end) return;
+            int e0 = 0;
+            while (pos >= before + last(sum)) before += last(sum), e0 += 64, sum = up_to(e0);
+            const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before + sum > pos));
+            if (l) before += (uint32_t)__builtin_amdgcn_readlane(sum, l - 1);
+            entry = e0 + l;
         }
-        entry = __builtin_amdgcn_readfirstlane(entry);
     }
-    __device__ __forceinline__ bool more() const { return pos < end; }
+    // To the next entry, behind one of so many tiles.
     __device__ __forceinline__ void next(int tiles) { pos = before = before + tiles, entry++; }
-    // The block that has tile x of the list.
-    __device__ __forceinline__ int block_of(int64_t x) const { return (int)(((x + 1) * blocks - 1) / total); }
 };
+
+// Whether a row at `place` sees key j of the stage.
+__device__ __forceinline__ bool paged_sees(const PagedArgs &a, const PagedStage &s, int place, int j) {
+    return (j <= min(place, s.to - 1)) & (j >= s.from) & ((place - j < a.window) | (j < a.sinks));
+}
 
 // A lane's row of an entry.
 struct PagedRow {
@@ -164,7 +176,7 @@ struct PagedRow {
             r = in - b * a.seq_rows;
             rows = all < a.all_rows;
         } else {
-            b = entry / s.row_tiles;
+            b = (int)s.by_row_tiles.divide((uint32_t)entry);
             const int one = (entry - b * s.row_tiles) * s.tile_rows + at;
             r = min(one, a.seq_rows - 1);
             rows = one < a.seq_rows;
@@ -177,9 +189,6 @@ struct PagedRow {
     bool is;  // there is such a row
     __device__ __forceinline__ int64_t at(const AttnView &v) const { return b * v.b + h * v.h + i * v.s; }
     __device__ __forceinline__ int64_t index(const PagedArgs &a) const { return ((int64_t)b * a.heads + h) * a.Sq + i; }
-    __device__ __forceinline__ bool sees(const PagedArgs &a, const PagedStage &s, int j) const {
-        return (j <= min(place, s.to - 1)) & (j >= s.from) & ((place - j < a.window) | (j < a.sinks));
-    }
 };
 
 // A part's place, and where an entry's parts are.

@@ -14,56 +14,64 @@ constexpr int64_t kMaxHeadDim = 256;
 constexpr int kFewTile = 16;  // rows of a tile of paged_few
 constexpr int kFewRows = 32;
 
-// The parts of a row, joined: four columns a lane.  Every part is read before the first is
-// added, up to eight.
-__global__ void __launch_bounds__(256) paged_join(PagedArgs a) {
+// The parts of a row, joined by a wave: a lane has four columns of every 64 / quads-th part, `quads`
+// lanes a part (a power of two), four of its parts on their way at once.
+__global__ void __launch_bounds__(256) paged_join(PagedArgs a, int quads) {
     const int64_t rows = (int64_t)a.batch * a.kv_heads * a.seq_rows;
-    const uint32_t quads = (uint32_t)a.part_width / 4;
-    const int64_t lane = (int64_t)blockIdx.x * 256 + threadIdx.x, at = lane / quads;
-    if (at >= rows) return;
-    const int d = (int)(lane - at * quads) * 4;
-    const int64_t head = at / a.seq_rows;
-    const int r = (int)(at - head * a.seq_rows), b = (int)(head / a.kv_heads), hk = (int)(head - (int64_t)b * a.kv_heads);
-    float most = -__builtin_inff(), sum = 0.f;
-    at_f4 o = (at_f4)(0.f);
-    for (int n = 0; n < a.stages; n++) {
-        const PagedStage &s = a.stage[n];
-        const int one = s.together ? b * a.seq_rows + r : r, tile = one / s.tile_rows;
-        const int entry = s.together ? tile : b * s.row_tiles + tile;
-        const int2 blocks = s.found[(int64_t)hk * s.entries + entry];
-        if (a.stages == 1 && blocks.x == blocks.y) return;  // its block wrote it
-        const int parts = blocks.y - blocks.x + 1;
-        for (int p0 = 0; p0 < parts; p0 += 8) {
-            float m[8], l[8];
-            at_f4 x[8];
+    const int lane = (int)threadIdx.x & 63, quad = lane & (quads - 1), groups = 64 / quads, group = lane / quads;
+    for (int64_t at = blockIdx.x * 4ll + (threadIdx.x >> 6); at < rows; at += gridDim.x * 4ll) {
+        const int64_t head = at / a.seq_rows;
+        const int r = (int)(at - head * a.seq_rows), b = (int)(head / a.kv_heads), hk = (int)(head - (int64_t)b * a.kv_heads);
+        const int d = min(quad * 4, a.part_width - 4);
+        float most = -__builtin_inff(), sum = 0.f;
+        at_f4 o = (at_f4)(0.f);
+        // Another maximum, sum and output of the row.
+        const auto add = [&](float m, float l, const at_f4 &x) {
+            const float now = __builtin_fmaxf(most, m), base = now == -__builtin_inff() ? 0.f : now;
+            const float keep = __builtin_amdgcn_exp2f(most - base), f = __builtin_amdgcn_exp2f(m - base);
+            sum = sum * keep + l * f, o = o * keep + x * f, most = now;
+        };
+        bool whole = false;
+        for (int n = 0; n < a.stages; n++) {
+            const PagedStage &s = a.stage[n];
+            const int one = s.together ? b * a.seq_rows + r : r, tile = one / s.tile_rows;
+            const int entry = s.together ? tile : b * s.row_tiles + tile;
+            const int2 workers = s.found[(int64_t)hk * s.entries + entry];
+            whole = a.stages == 1 && workers.x == workers.y;  // its worker wrote it
+            if (whole) break;
+            for (int w0 = workers.x + group; w0 <= workers.y; w0 += 4 * groups) {
+                float m[4], l[4];
+                at_f4 x[4];
 #pragma unroll
-            for (int p = 0; p < 8; p++) {
-                const int w = min(blocks.x + p0 + p, blocks.y);
-                const int64_t part = ((int64_t)hk * s.slots + slot_of_part(a, s, w, entry, w == blocks.x)) * s.tile_rows + one - tile * s.tile_rows;
-                m[p] = s.part_ml[2 * part], l[p] = s.part_ml[2 * part + 1];
-                x[p] = *(const at_f4 *)(s.part_o + part * a.part_width + d);
-            }
-            float now = most;
+                for (int p = 0; p < 4; p++) {
+                    const int w = min(w0 + p * groups, workers.y);
+                    const int64_t part = ((int64_t)hk * s.slots + slot_of_part(a, s, w, entry, w == workers.x)) * s.tile_rows + one - tile * s.tile_rows;
+                    m[p] = s.part_ml[2 * part], l[p] = s.part_ml[2 * part + 1];
+                    x[p] = *(const at_f4 *)(s.part_o + part * a.part_width + d);
+                }
 #pragma unroll
-            for (int p = 0; p < 8; p++) now = __builtin_fmaxf(now, m[p]);
-            const float base = now == -__builtin_inff() ? 0.f : now, keep = __builtin_amdgcn_exp2f(most - base);
-            sum *= keep, o *= keep, most = now;
-#pragma unroll
-            for (int p = 0; p < 8; p++) {
-                if (p0 + p >= parts) break;
-                const float f = __builtin_amdgcn_exp2f(m[p] - base);
-                sum += l[p] * f, o += x[p] * f;
+                for (int p = 0; p < 4; p++)
+                    if (w0 + p * groups <= workers.y) add(m[p], l[p], x[p]);
             }
         }
-    }
-    const int i = (int)a.by_group.divide((uint32_t)r);
-    const int64_t h = (int64_t)hk * a.group + r - i * a.group;
-    o *= a.pages.keys_of(b) - a.Sq + i < 0 ? 0.f : 1.f / sum;
-    float *out = a.out + b * a.os.b + h * a.os.h + (int64_t)i * a.os.s + d;
+        if (whole) continue;
+        for (int step = quads; step < 64; step *= 2) {
+            const float m = __shfl_xor(most, step), l = __shfl_xor(sum, step);
+            at_f4 x;
 #pragma unroll
-    for (int q = 0; q < 4; q++)
-        if (d + q < a.D) out[q] = o[q];
-    if (a.lse && d == 0) a.lse[((int64_t)b * a.heads + h) * a.Sq + i] = log_sum(most, sum);
+            for (int e = 0; e < 4; e++) x[e] = __shfl_xor(o[e], step);
+            add(m, l, x);
+        }
+        if (group != 0) continue;
+        const int i = (int)a.by_group.divide((uint32_t)r);
+        const int64_t h = (int64_t)hk * a.group + r - i * a.group;
+        o *= a.pages.keys_of(b) - a.Sq + i < 0 ? 0.f : 1.f / sum;
+        float *out = a.out + b * a.os.b + h * a.os.h + (int64_t)i * a.os.s + quad * 4;
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+            if (quad * 4 + q < a.D) out[q] = o[q];
+        if (a.lse && quad == 0) a.lse[((int64_t)b * a.heads + h) * a.Sq + i] = log_sum(most, sum);
+    }
 }
 
 // A stage of keys [from, to): its tiles of rows, and the blocks that share them.
@@ -75,12 +83,15 @@ PagedStage plan_stage(const PagedArgs &a, bool together, int from, int to, int c
     s.row_tiles = (int32_t)((rows + s.tile_rows - 1) / s.tile_rows);
     s.entries = (int32_t)(together ? s.row_tiles : (int64_t)s.row_tiles * a.batch);
     if (s.tile_rows == kFewTile) {
-        s.least = bf16 ? 4 : 8;
-        s.blocks = std::max(1, 2 * cu_count / a.kv_heads);
+        s.least = 2;
+        s.workers = std::max(1, 8 * cu_count / a.kv_heads);
     } else {
         s.least = 2;
-        s.blocks = std::max(1, cu_count * (256 / s.tile_rows) / a.kv_heads);
+        s.workers = std::max(1, cu_count * (256 / s.tile_rows) / a.kv_heads);
     }
+    s.by_row_tiles = SmallDivisor((uint32_t)s.row_tiles);
+    const int64_t most = (to >> (bf16 || s.tile_rows != kFewTile ? 5 : 4)) + 2;  // key tiles of an entry
+    if (most * s.entries >> 31) s.workers = 0;
     return s;
 }
 
@@ -89,7 +100,7 @@ int take_parts(PagedArgs &a, void **ws) {
     size_t floats = 0, found = 0;
     for (int i = 0; i < a.stages; i++) {
         PagedStage &s = a.stage[i];
-        s.slots = a.stages > 1 ? (int64_t)s.blocks + s.entries : 2 * (int64_t)s.blocks;
+        s.slots = a.stages > 1 ? (int64_t)s.workers + s.entries : 2 * (int64_t)s.workers;
         floats += (size_t)(a.kv_heads * s.slots * s.tile_rows) * (size_t)(a.part_width + 2);
         found += (size_t)a.kv_heads * (size_t)s.entries;
     }
@@ -118,12 +129,13 @@ int paged_forward(PagedArgs &a, bool bf16, DeviceState *dev) {
     }
     const int from = a.stages ? a.shared : 0;
     if (from < a.pages.capacity || a.stages == 0) a.stage[a.stages++] = plan_stage(a, false, from, a.pages.capacity, dev->cu_count, bf16);
+    if (a.pages.capacity == 0) a.stages = 0;  // nobody sees anything
     void *ws = nullptr;
-    const int rc0 = take_parts(a, &ws);
+    const int rc0 = a.stages ? take_parts(a, &ws) : TRS_OK;
     if (rc0 == TRS_E_ALLOCATION_FAILED) {
-        a.stages = 1;
+        a.stages = 1, a.stage[1] = PagedStage{};
         a.stage[0] = plan_stage(a, false, 0, a.pages.capacity, dev->cu_count, bf16);
-        a.stage[0].blocks = 0;
+        a.stage[0].workers = 0;
     } else if (rc0) {
         return rc0;
     }
@@ -134,10 +146,11 @@ int paged_forward(PagedArgs &a, bool bf16, DeviceState *dev) {
         } else {
             for (int i = 0; i < a.stages; i++) TRS_CHECK(few(i) ? launch_paged_few(a, i, 1, bf16, dev->stream) : launch_paged_rows(a, i, bf16, dev->stream));
         }
-        if (!ws) return TRS_OK;
-        const int64_t lanes = (int64_t)a.batch * a.kv_heads * a.seq_rows * (a.part_width / 4);
-        if ((lanes + 255) / 256 >> 24) return set_error(TRS_E_INVALID_ARGUMENT, "attention over %lld rows", (long long)a.batch * a.seq_rows);
-        hipLaunchKernelGGL(paged_join, dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, dev->stream, a);
+        if (!ws && a.stages) return TRS_OK;
+        int quads = 1;
+        while (quads * 4 < a.part_width) quads *= 2;
+        const int64_t rows = (int64_t)a.batch * a.kv_heads * a.seq_rows;
+        hipLaunchKernelGGL(paged_join, dim3((unsigned)std::min<int64_t>((rows + 3) / 4, 1 << 22)), dim3(256), 0, dev->stream, a, quads);
         TRS_LAUNCH_CHECK("paged attention join launch");
         return TRS_OK;
     };
@@ -168,7 +181,7 @@ int run_paged(const float *q, const trs_layout *lq, const trs_paged_cache *cache
     if (!std::isfinite(scale)) return set_error(TRS_E_INVALID_ARGUMENT, "attention scale has to be finite");
     if (Sq > kMaxPagedTokens || B > INT32_MAX || H > INT32_MAX || (HK > 0 && (H / HK) * Sq > kMaxPagedTokens) ||
         (HK > 0 && B * (((H / HK) * Sq + kFewTile - 1) / kFewTile) > INT32_MAX))
-        return set_error(TRS_E_INDEX_OVERFLOW, "attention over more than 2^30 tokens, or rows that share a key head");
+        return set_error(TRS_E_INDEX_OVERFLOW, "attention over more than 2^29 tokens, or rows that share a key head");
     TRS_CHECK(check_written_once(lo, "output"));
     if (D > 1 && lo->stride[3] != 1) return set_error(TRS_E_INVALID_ARGUMENT, "output needs a unit stride along its last dim");
     const int64_t rows = B * H * Sq;

@@ -2,9 +2,8 @@
 //
 // Bound by reading the keys and values once.  A wave takes 16 rows and streams its share
 // of the keys straight from the pages into the registers that the matrix instructions take
-// them from: no LDS, no barrier, nothing that waits for another wave.  The waves of a block
-// join their maxima and sums in LDS; what several blocks have of an entry is joined by a second
-// launch.
+// them from: no LDS, no barrier, nothing that waits for another wave.  What several waves have
+// of an entry is joined by a second launch.
 //
 // float32 pages: tiles of 16 keys on v_mfma_f32_16x16x4_f32, as attention_wide.h has them.
 // bfloat16 pages: tiles of 32 keys on v_mfma_f32_16x16x32_bf16.  A key is an operand as it
@@ -61,6 +60,7 @@ struct FloatPages {
     }
     __device__ __forceinline__ void add(at_f4 (&acc)[kTiles], const at_f4 (&p)[1]) const { T::add(acc, v, p[0]); }
     __device__ __forceinline__ static int column(int t, int i, int quarter) { return T::column(t, i, quarter); }
+    __device__ __forceinline__ static void write(const at_f4 (&acc)[kTiles], float *p, int D, int quarter) { T::write(acc, p, 1.f, D, quarter); }
 };
 
 template <int DP, int MODE>
@@ -158,231 +158,277 @@ struct Bf16Pages {
             }
     }
     __device__ __forceinline__ static int column(int t, int i, int quarter) { return 16 * W * (t / W) + W * (4 * quarter + i) + t % W; }
+    // acc^T: the lane's column of acc is the row at p.
+    __device__ __forceinline__ static void write(const at_f4 (&acc)[kTiles], float *p, int D, int quarter) {
+#pragma unroll
+        for (int u = 0; u < VU; u++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 0; e < W; e += 4) {
+                    const int d = column(u * W + e, i, quarter);
+                    const f4u x = {acc[u * W + e][i], acc[u * W + e + 1][i], acc[u * W + e + 2][i], acc[u * W + e + 3][i]};
+                    if (MODE == 0 || (MODE == 1 && d < D)) {
+                        *(f4u *)(p + d) = x;
+                    } else if (MODE == 2) {
+#pragma unroll
+                        for (int n = 0; n < 4; n++)
+                            if (d + n < D) p[d + n] = x[n];
+                    }
+                }
+    }
 };
 
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
 
-// Of a tile's keys: where they stand.
-template <class E, int HALVES, bool ONE>
-struct Places {
-    const E *k[HALVES], *v[HALVES];  // ONE: of the half's first key
-    int last[HALVES];                // ONE: its last key that is read
-    bool held[HALVES];
+// A wave's way along its share of the list: a tile of an entry.
+template <int SHIFT>
+struct Step {
+    PagedKeys<SHIFT> keys;
+    int entry, owner;  // owner: the sequence whose pages are read
+    int tiles;         // of the entry
+    int from, t, to;   // the entry's tiles that are the wave's, and the one that this is
+    uint32_t before;   // tiles ahead of the entry
+
+    __device__ __forceinline__ Step(const PagedShare<SHIFT> &share)
+        : keys(share.keys(share.entry)), entry(share.entry), owner(share.s.together ? 0 : share.sequence_of(share.entry)) {
+        tiles = max(keys.tiles, 1), before = share.before;
+        from = t = (int)(share.pos - share.before), to = min(tiles, (int)(share.end - share.before));
+    }
 };
 
 // ONE: pages hold a multiple of 16 tokens, and no 16 keys are the first sequence's in part, so that a
 // half's keys stand in one page, and its entry of the table is read by the scalar unit.
 template <class T, bool ONE>
-__device__ __forceinline__ void few_rows(const PagedArgs &a, const PagedStage &s, int hk, int w, float (&out_o)[kWaves][kTileRows][T::kTiles * 16 + 4],
-                                         float (&out_ml)[kWaves][kTileRows][2]) {
+struct Places {
+    using E = typename T::E;
+    const E *k[T::kHalves], *v[T::kHalves];  // ONE: of the half's first key
+    int last[T::kHalves];                    // ONE: its last key that is read
+    uint32_t absent;                         // ONE: halves whose page the pool does not have
+
+    int owner, j0, end;  // else: the sequence, the tile's first key and the last one that is read
+
+    // The page and the token of it that a key stands in; past the last key that is read, that one's.  (An
+    // entry that sees nothing has a tile none of whose keys is seen: any key that there is will do.)
+    __device__ __forceinline__ static bool find(const PagedArgs &a, int first_row_to, int owner, int j, int last, int64_t &page, int &slot) {
+        const int at = max(min(j, last), 0), id = a.pages.page_of(at < first_row_to ? 0 : owner, at);
+        const bool held = a.pages.holds(id);
+        page = held ? id : 0, slot = a.pages.slot_of(at);
+        return held;
+    }
+    __device__ __forceinline__ Places(const PagedArgs &a, int first_row_to, const E *kb, const E *vb, const Step<T::kShift> &x) {
+        j0 = x.keys.first_key(x.t), owner = x.owner, end = x.keys.last;
+        if constexpr (ONE) {
+            absent = 0;
+#pragma unroll
+            for (int h = 0; h < T::kHalves; h++) {
+                const int at = max(min(j0 + 16 * h, end & ~15), 0);
+                int64_t page;
+                int slot;
+                if (!find(a, first_row_to, owner, at, end, page, slot)) absent |= 1u << h;
+                k[h] = kb + page * a.pages.ks.p + slot * a.pages.ks.s;
+                v[h] = vb + page * a.pages.vs.p + slot * a.pages.vs.s;
+                last[h] = max(min(end - at, 15), 0);
+            }
+        }
+    }
+    __device__ __forceinline__ const E *k_row(const PagedArgs &a, int first_row_to, const E *kb, int h, int n) const {
+        if constexpr (ONE) return k[h] + (int64_t)min(n, last[h]) * a.pages.ks.s;
+        int64_t page;
+        int slot;
+        find(a, first_row_to, owner, j0 + 16 * h + n, end, page, slot);
+        return kb + page * a.pages.ks.p + slot * a.pages.ks.s;
+    }
+    __device__ __forceinline__ const E *v_row(const PagedArgs &a, int first_row_to, const E *vb, int h, int n) const {
+        if constexpr (ONE) return v[h] + (int64_t)min(n, last[h]) * a.pages.vs.s;
+        int64_t page;
+        int slot;
+        find(a, first_row_to, owner, j0 + 16 * h + n, end, page, slot);
+        return vb + page * a.pages.vs.p + slot * a.pages.vs.s;
+    }
+    // Whether the pool has the page of key n of half h.
+    __device__ __forceinline__ bool held(const PagedArgs &a, int first_row_to, int h, int n) const {
+        if constexpr (ONE) return !(absent >> h & 1);
+        int64_t page;
+        int slot;
+        return find(a, first_row_to, owner, j0 + 16 * h + n, end, page, slot);
+    }
+};
+
+// A wave's share of a key head's tiles, one behind another whatever entries they belong to: the
+// next tile's loads are on their way while one is worked on, and the page after that looked up.
+template <class T, bool ONE>
+__device__ __forceinline__ void few_rows(const PagedArgs &a, const PagedStage &s, int hk, int w) {
     using E = typename T::E;
     constexpr int H = T::kHalves;
     const int lane = (int)threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    PagedShare<T::kShift> share(a, s, w, lane);
+    if (share.pos >= share.end) return;
     const E *const kb = (const E *)a.pages.k + hk * a.pages.ks.h, *const vb = (const E *)a.pages.v + hk * a.pages.vs.h;
-    for (PagedShare<T::kShift> share(a, s, w, lane); share.more();) {
-        const int entry = share.entry;
-        const PagedKeys<T::kShift> keys = share.keys(entry);
-        const int tiles = max(keys.tiles, 1);
-        const int ta = (int)(share.pos - share.before), tb = (int)min((int64_t)tiles, share.end - share.before);
-        const int64_t before = share.before;
-        const PagedRow row(a, s, entry, hk, col);
-        const int owner = s.together ? 0 : entry / s.row_tiles;  // the sequence whose keys these are
-        const int n = keys.tiles ? tb - ta : 0;
-        const int t0 = ta + n * wave / kWaves, t1 = ta + n * (wave + 1) / kWaves;
+    const int first_row_to = s.from < a.shared ? a.shared : 0;  // keys below it are the first sequence's
+    Step<T::kShift> now(share), ahead = now;
+    const uint32_t count = share.end - share.pos;
+    // `ahead` to the tile behind it; past the wave's last tile it stays.
+    const auto advance = [&]() {
+        if (ahead.t + 1 < ahead.to) {
+            ahead.t++;
+        } else if (share.before + ahead.tiles < share.end) {
+            share.next(ahead.tiles);
+            ahead = Step<T::kShift>(share);
+        }
+    };
+    using P = Places<T, ONE>;
+    T ops;
+    P here(a, first_row_to, kb, vb, now);
+    const auto load_k = [&](const P &p) { ops.load_k([&](int h, int n) { return p.k_row(a, first_row_to, kb, h, n); }, a.D, col, quarter); };
+    const auto load_v = [&](const P &p) { ops.load_v([&](int h, int n) { return p.v_row(a, first_row_to, vb, h, n); }, a.D, col, quarter); };
+    load_k(here);
+    load_v(here);
+    int place = 0;
+    const auto load_q = [&]() {
+        const PagedRow row(a, s, now.entry, hk, col);
+        place = row.place;
+        ops.load_q(a.q + row.at(a.qs), a.D, quarter, a.scale2);
+    };
+    load_q();
+    advance();
+    P next(a, first_row_to, kb, vb, ahead);
 
-        const int first_row_to = s.from < a.shared ? a.shared : 0;  // keys below it are the first sequence's
-        const auto page_at = [&](int j) { return a.pages.page_of(j < first_row_to ? 0 : owner, j); };
-        // A key that is not read: the last one that is seen stands for it.
-        const auto places = [&](int t, Places<E, H, ONE> &p) {
-            const int j0 = keys.first_key(min(t, t1 - 1));
+    at_f4 acc[T::kTiles];
+    float most, sum;
+    uint32_t lowest;
+    const auto clear = [&]() {
 #pragma unroll
-            for (int h = 0; h < H; h++) {
-                if constexpr (ONE) {
-                    const int at = min(j0 + 16 * h, keys.last & ~15), id = page_at(at), slot = a.pages.slot_of(at);
-                    p.held[h] = a.pages.holds(id);
-                    const int64_t page = p.held[h] ? id : 0;
-                    p.k[h] = kb + page * a.pages.ks.p + slot * a.pages.ks.s;
-                    p.v[h] = vb + page * a.pages.vs.p + slot * a.pages.vs.s;
-                    p.last[h] = min(keys.last - at, 15);
-                }
-            }
-        };
-        const auto any_place = [&](int j, bool &held, int64_t &page, int &slot) {
-            const int at = min(j, keys.last), id = page_at(at);
-            held = a.pages.holds(id);
-            page = held ? id : 0, slot = a.pages.slot_of(at);
-        };
-        const auto k_row = [&](int t, const Places<E, H, ONE> &p, int h, int x) -> const E * {
-            if constexpr (ONE) return p.k[h] + (int64_t)min(x, p.last[h]) * a.pages.ks.s;
-            bool held;
-            int64_t page;
-            int slot;
-            any_place(keys.first_key(min(t, t1 - 1)) + 16 * h + x, held, page, slot);
-            return kb + page * a.pages.ks.p + slot * a.pages.ks.s;
-        };
-        const auto v_row = [&](int t, const Places<E, H, ONE> &p, int h, int x) -> const E * {
-            if constexpr (ONE) return p.v[h] + (int64_t)min(x, p.last[h]) * a.pages.vs.s;
-            bool held;
-            int64_t page;
-            int slot;
-            any_place(keys.first_key(min(t, t1 - 1)) + 16 * h + x, held, page, slot);
-            return vb + page * a.pages.vs.p + slot * a.pages.vs.s;
-        };
-
-        at_f4 acc[T::kTiles];
+        for (int c = 0; c < T::kTiles; c++) acc[c] = (at_f4)(0.f);
+        most = -__builtin_inff(), sum = 0.f, lowest = 0;
+    };
+    // A key at a time, for what a query sees, or does not, of infinities and NaN.
+    const auto each_key = [&]() {
+        const PagedRow row(a, s, now.entry, hk, col);
+        const float *q = a.q + row.at(a.qs);
+#pragma unroll 1
+        for (int t = now.from; t < now.to; t++)
+#pragma unroll 1
+            for (int x = 0; x < 16 * H; x++) {
+                const int j = now.keys.first_key(t) + x;
+                int64_t page;
+                int slot;
+                const bool held = P::find(a, first_row_to, now.owner, j, now.keys.last, page, slot);
+                const E *kp = kb + page * a.pages.ks.p + slot * a.pages.ks.s, *vp = vb + page * a.pages.vs.p + slot * a.pages.vs.s;
+                float y = 0.f;
+                for (int c = quarter; c < a.D; c += 4) y += q[c] * a.scale2 * to_float(kp[c]);
+                y += __shfl_xor(y, 16);
+                y += __shfl_xor(y, 32);
+                if (!paged_sees(a, s, place, j)) continue;
+                if (!held) y = __builtin_nanf("");
+                const float top = __builtin_fmaxf(most, y), base = top == -__builtin_inff() ? 0.f : top;
+                const float keep = __builtin_amdgcn_exp2f(most - base), p = __builtin_amdgcn_exp2f(y - base);
+                sum = sum * keep + (quarter == 0 ? p : 0.f);
+                most = top;
 #pragma unroll
-        for (int t = 0; t < T::kTiles; t++) acc[t] = (at_f4)(0.f);
-        float most = -__builtin_inff(), sum = 0.f;
-        if (t0 < t1) {
-            T ops;
-            Places<E, H, ONE> now, next;
-            places(t0, now);
-            ops.load_k([&](int h, int x) { return k_row(t0, now, h, x); }, a.D, col, quarter);
-            ops.load_v([&](int h, int x) { return v_row(t0, now, h, x); }, a.D, col, quarter);
-            ops.load_q(a.q + row.at(a.qs), a.D, quarter, a.scale2);
-            places(t0 + 1, next);
-            uint32_t lowest = 0;
-            for (int t = t0; t < t1; t++) {
-                const int j0 = keys.first_key(t);
-                at_f4 x[H];
-                ops.scores(x);
-                ops.load_k([&](int h, int y) { return k_row(t + 1, next, h, y); }, a.D, col, quarter);
-                float m = -__builtin_inff();
-#pragma unroll
-                for (int h = 0; h < H; h++)
+                for (int c = 0; c < T::kTiles; c++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const int j = j0 + 16 * h + 4 * quarter + e;
-                        const uint32_t bits = __float_as_uint(x[h][e]);
-                        lowest = lowest > bits ? lowest : bits;
-                        bool held = true;
-                        if constexpr (ONE) held = now.held[h];
-                        else held = a.pages.holds(page_at(min(j, keys.last)));
-                        const float y = held ? x[h][e] * T::kDownScale : __builtin_nanf("");
-                        x[h][e] = row.sees(a, s, j) ? y : -__builtin_inff();
-                        m = __builtin_fmaxf(m, x[h][e]);
-                    }
-                m = __builtin_fmaxf(m, __shfl_xor(m, 16));
-                m = __builtin_fmaxf(m, __shfl_xor(m, 32));
-                const float top = __builtin_fmaxf(most, m), base = top == -__builtin_inff() ? 0.f : top;
-                const float keep = __builtin_amdgcn_exp2f(most - base);
-                float add = 0.f;
-#pragma unroll
-                for (int h = 0; h < H; h++) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) x[h][e] = __builtin_amdgcn_exp2f(x[h][e] - base);
-                    add += (x[h][0] + x[h][1]) + (x[h][2] + x[h][3]);
-                }
-                sum = sum * keep + add;
-                most = top;
-                if (__builtin_amdgcn_ballot_w64(keep != 1.f)) {
-#pragma unroll
-                    for (int c = 0; c < T::kTiles; c++) acc[c] *= keep;
-                }
-                ops.add(acc, x);
-                ops.load_v([&](int h, int y) { return v_row(t + 1, next, h, y); }, a.D, col, quarter);
-                now = next;
-                places(t + 2, next);
-            }
-            // A sum that is not finite, or a score of -inf, which shows in no result: what a query
-            // sees may hold that, or what it does not see; a key at a time then.
-            float odd = sum * 0.f;
-#pragma unroll
-            for (int c = 0; c < T::kTiles; c++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) odd += acc[c][e] * 0.f;
-            if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd != 0.f || lowest >= 0xff800000u) != 0, 0)) {
-#pragma unroll
-                for (int c = 0; c < T::kTiles; c++) acc[c] = (at_f4)(0.f);
-                most = -__builtin_inff(), sum = 0.f;
-                const float *q = a.q + row.at(a.qs);
-#pragma unroll 1
-                for (int t = t0; t < t1; t++)
-#pragma unroll 1
-                    for (int x = 0; x < 16 * H; x++) {
-                        const int j = keys.first_key(t) + x;
-                        bool held;
-                        int64_t page;
-                        int slot;
-                        any_place(j, held, page, slot);
-                        const E *kp = kb + page * a.pages.ks.p + slot * a.pages.ks.s, *vp = vb + page * a.pages.vs.p + slot * a.pages.vs.s;
-                        float y = 0.f;
-                        for (int c = quarter; c < a.D; c += 4) y += q[c] * a.scale2 * to_float(kp[c]);
-                        y += __shfl_xor(y, 16);
-                        y += __shfl_xor(y, 32);
-                        if (!row.sees(a, s, j)) continue;
-                        if (!held) y = __builtin_nanf("");
-                        const float top = __builtin_fmaxf(most, y), base = top == -__builtin_inff() ? 0.f : top;
-                        const float keep = __builtin_amdgcn_exp2f(most - base), p = __builtin_amdgcn_exp2f(y - base);
-                        sum = sum * keep + (quarter == 0 ? p : 0.f);
-                        most = top;
-#pragma unroll
-                        for (int c = 0; c < T::kTiles; c++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const int d = T::column(c, e, quarter);
-                                acc[c][e] = acc[c][e] * keep + (d < a.D ? p * to_float(vp[d]) : 0.f);
-                            }
+                        const int d = T::column(c, e, quarter);
+                        acc[c][e] = acc[c][e] * keep + (d < a.D ? p * to_float(vp[d]) : 0.f);
                     }
             }
-        }
-        sum += __shfl_xor(sum, 16);
-        sum += __shfl_xor(sum, 32);
-        __syncthreads();  // the last entry's have been read
+    };
+    // The entry's rows, or the wave's part of them.
+    const auto write = [&]() {
+        // A sum that is not finite, or a score of -inf, which shows in no result.
+        float odd = sum * 0.f;
 #pragma unroll
         for (int c = 0; c < T::kTiles; c++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) out_o[wave][col][T::column(c, e, quarter)] = acc[c][e];
-        if (quarter == 0) out_ml[wave][col][0] = most, out_ml[wave][col][1] = sum;
-        __syncthreads();
-        const bool whole = ta == 0 && tb == tiles && a.stages == 1;
-        const int64_t slot = slot_of_part(a, s, w, entry, ta == 0), part0 = ((int64_t)hk * s.slots + slot) * kTileRows;
-        constexpr int kQuads = T::kTiles * 4;
-        for (int x = (int)threadIdx.x; x < kTileRows * kQuads; x += 64 * kWaves) {
-            const int r = x / kQuads, d = x % kQuads * 4;
-            const PagedRow o(a, s, entry, hk, r);
-            if (!o.is || d >= a.D) continue;
-            float top = -__builtin_inff(), total = 0.f;
-#pragma unroll
-            for (int v = 0; v < kWaves; v++) top = __builtin_fmaxf(top, out_ml[v][r][0]);
-            const float base = top == -__builtin_inff() ? 0.f : top;
-            at_f4 y = (at_f4)(0.f);
-#pragma unroll
-            for (int v = 0; v < kWaves; v++) {
-                const float f = __builtin_amdgcn_exp2f(out_ml[v][r][0] - base);
-                total += out_ml[v][r][1] * f;
-                y += *(const at_f4 *)&out_o[v][r][d] * f;
-            }
+            for (int e = 0; e < 4; e++) odd += acc[c][e] * 0.f;
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd != 0.f || lowest >= 0xff800000u) != 0, 0)) {
+            clear();
+            each_key();
+        }
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        const PagedRow row(a, s, now.entry, hk, col);
+        const bool whole = now.from == 0 && now.to == now.tiles && a.stages == 1;
+        if (row.is) {
             float *p;
             if (whole) {
-                y *= o.place < 0 ? 0.f : 1.f / total;
-                p = a.out + o.at(a.os) + d;
-                if (a.lse && d == 0) a.lse[o.index(a)] = log_sum(top, total);
-            } else {
-                p = s.part_o + (part0 + r) * a.part_width + d;
-                if (d == 0) s.part_ml[2 * (part0 + r)] = top, s.part_ml[2 * (part0 + r) + 1] = total;
-            }
+                const float f = row.place < 0 ? 0.f : 1.f / sum;
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (d + e < a.D) p[e] = y[e];
+                for (int c = 0; c < T::kTiles; c++) acc[c] *= f;
+                p = a.out + row.at(a.os);
+                if (a.lse && quarter == 0) a.lse[row.index(a)] = log_sum(most, sum);
+            } else {
+                const int64_t part = ((int64_t)hk * s.slots + slot_of_part(a, s, w, now.entry, now.from == 0)) * kTileRows + col;
+                p = s.part_o + part * a.part_width;
+                if (quarter == 0) s.part_ml[2 * part] = most, s.part_ml[2 * part + 1] = sum;
+            }
+            T::write(acc, p, a.D, quarter);
         }
-        if (ta == 0 && s.found && threadIdx.x == 0)
-            s.found[(int64_t)hk * s.entries + entry] = make_int2(share.block_of(before), share.block_of(before + tiles - 1));
-        share.next(tiles);
+        if (now.from == 0 && s.found && lane == 0)
+            s.found[(int64_t)hk * s.entries + now.entry] = make_int2(w, share.worker_of(now.before + now.tiles - 1));
+    };
+
+    clear();
+    for (uint32_t left = count; left > 0; left--) {
+        const int j0 = now.keys.first_key(now.t);
+        at_f4 x[H];
+        ops.scores(x);
+        load_k(next);
+        float m = -__builtin_inff();
+#pragma unroll
+        for (int h = 0; h < H; h++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int n = 4 * quarter + e;
+                const uint32_t bits = __float_as_uint(x[h][e]);
+                lowest = lowest > bits ? lowest : bits;
+                const float y = here.held(a, first_row_to, h, n) ? x[h][e] * T::kDownScale : __builtin_nanf("");
+                x[h][e] = paged_sees(a, s, place, j0 + 16 * h + n) ? y : -__builtin_inff();
+                m = __builtin_fmaxf(m, x[h][e]);
+            }
+        m = __builtin_fmaxf(m, __shfl_xor(m, 16));
+        m = __builtin_fmaxf(m, __shfl_xor(m, 32));
+        const float top = __builtin_fmaxf(most, m), base = top == -__builtin_inff() ? 0.f : top;
+        const float keep = __builtin_amdgcn_exp2f(most - base);
+        float add = 0.f;
+#pragma unroll
+        for (int h = 0; h < H; h++) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[h][e] = __builtin_amdgcn_exp2f(x[h][e] - base);
+            add += (x[h][0] + x[h][1]) + (x[h][2] + x[h][3]);
+        }
+        sum = sum * keep + add;
+        most = top;
+        if (__builtin_amdgcn_ballot_w64(keep != 1.f)) {
+#pragma unroll
+            for (int c = 0; c < T::kTiles; c++) acc[c] *= keep;
+        }
+        ops.add(acc, x);
+        load_v(next);
+        if (now.t + 1 == now.to) {
+            write();
+            now = ahead;
+            if (left > 1) load_q();
+            clear();
+        } else {
+            now.t++;
+        }
+        here = next;
+        advance();
+        next = P(a, first_row_to, kb, vb, ahead);
     }
 }
 
 template <class T, bool ONE>
 __global__ void __launch_bounds__(64 * kWaves, T::kTiles <= 8 ? 2 : 1) paged_few(PagedArgs a, int from) {
-    __shared__ __attribute__((aligned(16))) float out_o[kWaves][kTileRows][T::kTiles * 16 + 4];
-    __shared__ float out_ml[kWaves][kTileRows][2];
-    int id = (int)blockIdx.x;
-    const bool second = id >= a.few_blocks;
+    int id = (int)blockIdx.x * kWaves + uniform((int)threadIdx.x >> 6);
+    if (id >= a.few_all) return;  // the last block's waves without work
+    const bool second = id >= a.few_workers;
     const PagedStage &s = a.stage[from + second];
-    if (second) id -= a.few_blocks;
-    few_rows<T, ONE>(a, s, id % a.kv_heads, id / a.kv_heads, out_o, out_ml);
+    if (second) id -= a.few_workers;
+    few_rows<T, ONE>(a, s, id % a.kv_heads, id / a.kv_heads);
 }
 
 template <class T>
@@ -404,15 +450,15 @@ void launch_width(const PagedArgs &a, int from, bool vectors, dim3 grid, hipStre
 
 int launch_paged_few(const PagedArgs &args, int from, int count, bool bf16, hipStream_t s) {
     PagedArgs a = args;
-    int64_t blocks[2] = {0, 0};
+    int64_t waves[2] = {0, 0};
     for (int i = 0; i < count; i++) {
         const PagedStage &st = a.stage[from + i];
-        blocks[i] = (int64_t)a.kv_heads * (st.blocks ? st.blocks : st.entries);
+        waves[i] = (int64_t)a.kv_heads * (st.workers ? st.workers : st.entries);
     }
-    if ((blocks[0] + blocks[1]) * 64 * kWaves >> 32)
-        return set_error(TRS_E_INVALID_ARGUMENT, "attention over %lld blocks of rows", (long long)(blocks[0] + blocks[1]));
-    a.few_blocks = (int32_t)blocks[0];
-    const dim3 grid((unsigned)(blocks[0] + blocks[1]));
+    const int64_t all = waves[0] + waves[1];
+    if ((all + kWaves) * 64 >> 32) return set_error(TRS_E_INVALID_ARGUMENT, "attention over %lld tiles of rows", (long long)all);
+    a.few_workers = (int32_t)waves[0], a.few_all = (int32_t)all;
+    const dim3 grid((unsigned)((all + kWaves - 1) / kWaves));
     const bool vectors = paged_vectors(a, bf16);
     if (bf16) {
         if (a.D <= 64) launch_width<Bf16Pages, 64>(a, from, vectors, grid, s);

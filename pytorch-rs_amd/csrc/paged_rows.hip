@@ -116,19 +116,28 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_rows(PagedArgs a, int stage)
     const int hk = (int)(blockIdx.x % (uint32_t)a.kv_heads), w = (int)(blockIdx.x / (uint32_t)a.kv_heads);
     const E *const kb = (const E *)a.pages.k + hk * a.pages.ks.h, *const vb = (const E *)a.pages.v + hk * a.pages.vs.h;
     const auto unit = [&](int q) { return min(wave + q * NW, UNITS - 1); };
-    for (PagedShare<5> share(a, s, w, lane); share.more();) {
-        const int entry = share.entry;
+    for (PagedShare<5> share(a, s, w, lane); share.pos < share.end;) {
+        const int entry = uniform(share.entry);
         const PagedKeys<5> keys = share.keys(entry);
         const int tiles = max(keys.tiles, 1);
-        const int t0 = (int)(share.pos - share.before), end = (int)min((int64_t)tiles, share.end - share.before);
+        const int t0 = (int)(share.pos - share.before), end = min(tiles, (int)(share.end - share.before));
         const int t1 = keys.tiles ? end : t0;
-        const PagedRow r(a, s, entry, hk, wave * 32 + (lane & 31));
-        int lo = r.is ? r.place : INT32_MAX, hi = r.place;
+        // The lane's row, worked out where it is used: its parts are not held in registers over the tiles.
+        const auto row = [&]() {
+            int e = entry;
+            asm volatile("" : "+s"(e));
+            return PagedRow(a, s, e, hk, wave * 32 + (lane & 31));
+        };
+        const auto [place, is] = [&]() {
+            const PagedRow r = row();
+            return int2{r.place, r.is};
+        }();
+        int lo = is ? place : INT32_MAX, hi = place;
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) lo = min(lo, __shfl_xor(lo, d)), hi = max(hi, __shfl_xor(hi, d));
         const int wave_lo = __builtin_amdgcn_readfirstlane(lo), wave_hi = __builtin_amdgcn_readfirstlane(hi);
-        const bool whole = __builtin_amdgcn_ballot_w64(!r.is) == 0;
-        const int owner = s.together ? 0 : entry / s.row_tiles, first_row_to = s.from < a.shared ? a.shared : 0;
+        const bool whole = __builtin_amdgcn_ballot_w64(!is) == 0;
+        const int owner = s.together ? 0 : share.sequence_of(entry), first_row_to = s.from < a.shared ? a.shared : 0;
         at_f16 acc[NT];
 #pragma unroll
         for (int t = 0; t < NT; t++) acc[t] = (at_f16)(0.f);
@@ -154,11 +163,12 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_rows(PagedArgs a, int stage)
             load(t0, page_at(key_at(t0)));
             int id = page_at(key_at(t0 + 1));
             Pieces q[2 * NT];
+            const float *const q0 = a.q + row().at(a.qs);
 #pragma unroll
             for (int n = 0; n < 2 * NT; n++) {
                 Unit<WIDTH> x;
-                x.load(a.q + r.at(a.qs), n, a.D, lane);
-                if (r.place < 0) {  // nothing of a query that sees nothing
+                x.load(q0, n, a.D, lane);
+                if (place < 0) {  // nothing of a query that sees nothing
 #pragma unroll
                     for (int e = 0; e < 8; e++) x.v[e] = 0.f;
                 }
@@ -195,7 +205,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_rows(PagedArgs a, int stage)
                         for (int e = 0; e < 16; e++) {
                             const int k = result_row(e, half);
                             if (absent >> k & 1) x[e] = __builtin_nanf("");
-                            x[e] = r.sees(a, s, j0 + k) ? x[e] : -__builtin_inff();
+                            x[e] = paged_sees(a, s, place, j0 + k) ? x[e] : -__builtin_inff();
                         }
                     }
                     float m = x[0];
@@ -233,7 +243,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_rows(PagedArgs a, int stage)
 #pragma unroll
                 for (int t = 0; t < NT; t++) acc[t] = (at_f16)(0.f);
                 most = -__builtin_inff(), sum = 0.f, unit_out = 1.f;
-                const float *qp = a.q + r.at(a.qs);
+                const float *qp = a.q + row().at(a.qs);
 #pragma unroll 1
                 for (int t = t0; t < t1; t++)
 #pragma unroll 1
@@ -246,7 +256,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_rows(PagedArgs a, int stage)
                         float y = 0.f;
                         for (int c = half; c < a.D; c += 2) y += qp[c] * a.scale2 * as_float(kp[c]);
                         y += __shfl_xor(y, 32);
-                        if (!r.sees(a, s, j)) continue;
+                        if (!paged_sees(a, s, place, j)) continue;
                         if (!held) y = __builtin_nanf("");
                         const float top = __builtin_fmaxf(most, y), base = top == -__builtin_inff() ? 0.f : top;
                         const float keep = __builtin_amdgcn_exp2f(most - base), p = __builtin_amdgcn_exp2f(y - base);
@@ -263,7 +273,8 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_rows(PagedArgs a, int stage)
             }
         }
         sum += __shfl_xor(sum, 32);
-        if (r.is) {
+        if (is) {
+            const PagedRow r = row();
             if (t0 == 0 && end == tiles && a.stages == 1) {
                 write_row<WIDTH>(acc, a.out + r.at(a.os), unit_out, r.place < 0 ? 0.f : 1.f / sum, a.D, half);
                 if (a.lse && half == 0) a.lse[r.index(a)] = log_sum(most, sum);
@@ -274,7 +285,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_rows(PagedArgs a, int stage)
             }
         }
         if (t0 == 0 && s.found && threadIdx.x == 0)
-            s.found[(int64_t)hk * s.entries + entry] = make_int2(share.block_of(share.before), share.block_of(share.before + tiles - 1));
+            s.found[(int64_t)hk * s.entries + entry] = make_int2(share.worker_of(share.before), share.worker_of(share.before + tiles - 1));
         share.next(tiles);
     }
 }
@@ -305,7 +316,7 @@ void launch_type(const PagedArgs &a, int stage, bool vectors, dim3 grid, hipStre
 
 int launch_paged_rows(const PagedArgs &a, int stage, bool bf16, hipStream_t s) {
     const PagedStage &st = a.stage[stage];
-    const int64_t blocks = (int64_t)a.kv_heads * (st.blocks ? st.blocks : st.entries);
+    const int64_t blocks = (int64_t)a.kv_heads * (st.workers ? st.workers : st.entries);
     if (blocks * 2 * st.tile_rows >> 32) return set_error(TRS_E_INVALID_ARGUMENT, "attention over %lld blocks of rows", (long long)blocks);
     const dim3 grid((unsigned)blocks);
     if (bf16) launch_type<uint16_t>(a, stage, paged_vectors(a, bf16), grid, s);

@@ -18,6 +18,7 @@ namespace trs {
 namespace {
 
 constexpr int kMaxDim = 1024, kMostAxes = 4, kMaxPairs = kMaxDim / 2;
+constexpr int64_t kManyEights = 1 << 19;
 
 // A tensor to be turned, or moved as it is: [batch, head, token, dim].
 struct RopeJob {
@@ -25,14 +26,14 @@ struct RopeJob {
     void *y;  // the output, or a pool
     int64_t xs[4], ys[4];
     SmallDivisor by_chunk, by_inner;
-    int32_t heads, head_groups, units, batch_blocks;  // units of a sequence, and the blocks that they take
+    int32_t heads, units, batch_blocks;  // units of a sequence, and the blocks that they take
     int64_t first;                                    // first block
-    int32_t turns, paged;
+    int32_t turns, paged, heads_inner;  // rows walked with the heads innermost, else the tokens
 };
 
 struct RopeArgs {
     RopeJob job[3];
-    int32_t jobs, tokens, batch, dim, rot, interleaved, axes, heads_inner;
+    int32_t jobs, tokens, batch, dim, rot, interleaved, axes;
     float sign;
     int64_t blocks;
     const float *cos, *sin;
@@ -79,6 +80,46 @@ __device__ __forceinline__ Angle angle_of(const RopeArgs &a, int64_t row, int pa
     return known ? Angle{c, s} : Angle{__builtin_nanf(""), __builtin_nanf("")};
 }
 
+// (u, w) by an angle.
+__device__ __forceinline__ void turn(float &u, float &w, float co, float si) {
+    const float x = u * co - w * si;
+    w = w * co + u * si;
+    u = x;
+}
+
+// The angles of a lane's four pairs: p to p + 3, or, of neighbours, p and p + 1 and the two that lie
+// rot/4 behind them.
+struct Angles {
+    float co[4], si[4];
+};
+__device__ __forceinline__ Angles angles_of(const RopeArgs &a, int b, int t, const Token &k, int p) {
+    typedef float f2u __attribute__((ext_vector_type(2), aligned(4)));
+    Angles g;
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+        const int pair = i == 0 ? p : a.interleaved ? p + a.rot / 4 : p + 2, axis = axis_of(a, pair);
+        const int64_t row = row_of(a, axis, b, t, k);
+        if (axis == axis_of(a, pair + 1) && a.table_rows) {
+            const bool known = row >= 0 && row < a.table_rows;
+            const int64_t at = (known ? row : 0) * a.table_stride + pair;
+            const f2u c = *(const f2u *)(a.cos + at), s = *(const f2u *)(a.sin + at);
+            const float nan = __builtin_nanf("");
+#pragma unroll
+            for (int e = 0; e < 2; e++) g.co[i + e] = known ? c[e] : nan, g.si[i + e] = known ? s[e] * a.sign : nan;
+        } else {
+            const Angle x = angle_of(a, row, pair), y = angle_of(a, row_of(a, axis_of(a, pair + 1), b, t, k), pair + 1);
+            g.co[i] = x.co, g.si[i] = x.si, g.co[i + 1] = y.co, g.si[i + 1] = y.si;
+        }
+    }
+    return g;
+}
+
+typedef uint32_t u2u __attribute__((ext_vector_type(2), aligned(2)));
+__device__ __forceinline__ uint32_t to_bf16(float x, float y) {
+    typedef float F2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 B2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((F2{x, y}), B2));
+}
 __device__ __forceinline__ uint16_t to_bf16(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
 
 // Entries of any number, strides and rotation: a lane has a pair, or an entry that passes.
@@ -91,7 +132,7 @@ __device__ __forceinline__ void rope_pair(const RopeArgs &a, int64_t at_block) {
     if (u >= j.units) return;
     const int r = (int)j.by_chunk.divide((uint32_t)u), c = u - r * (int)j.by_chunk.d;
     const int outer = (int)j.by_inner.divide((uint32_t)r), inner = r - outer * (int)j.by_inner.d;
-    const int h = a.heads_inner ? inner : outer, t = a.heads_inner ? outer : inner;
+    const int h = j.heads_inner ? inner : outer, t = j.heads_inner ? outer : inner;
     const int rot = j.turns ? a.rot : 0, half = rot / 2;
     const bool pair = c < half;
     const int e0 = pair ? (a.interleaved ? 2 * c : c) : half + c, e1 = pair ? (a.interleaved ? e0 + 1 : e0 + half) : e0;
@@ -100,9 +141,7 @@ __device__ __forceinline__ void rope_pair(const RopeArgs &a, int64_t at_block) {
     float u0 = x[e0 * j.xs[3]], u1 = x[e1 * j.xs[3]];
     if (pair) {
         const Angle g = angle_of(a, row_of(a, axis_of(a, c), b, t, k), c);
-        const float v0 = u0 * g.co - u1 * g.si;
-        u1 = u1 * g.co + u0 * g.si;
-        u0 = v0;
+        turn(u0, u1, g.co, g.si);
     }
     if (!j.paged) {
         float *y = (float *)j.y + b * j.ys[0] + h * j.ys[1] + t * j.ys[2];
@@ -123,6 +162,68 @@ __device__ __forceinline__ void rope_pair(const RopeArgs &a, int64_t at_block) {
 }
 __global__ void __launch_bounds__(256) rope_pairs(RopeArgs a) {
     for (int64_t at = blockIdx.x; at < a.blocks; at += gridDim.x) rope_pair(a, at);
+}
+
+// Rows of whole eights (dim and rot multiples of 8, unit strides): a lane has four entries of the
+// first half of what is turned and the four that lie rot/2 on, so that both partners of every pair
+// are in it, or the like of what passes (eight in a row, read as two fours 32 bytes apart from lane
+// to lane, are slower); of HEADS heads of a token, whose angles are the same.
+template <int HEADS>
+__device__ __forceinline__ void rope_eight(const RopeArgs &a, int64_t at_block) {
+    int which = 0;
+    while (which + 1 < a.jobs && at_block >= a.job[which + 1].first) which++;
+    const RopeJob &j = a.job[which];
+    const int64_t block = at_block - j.first;
+    const int b = (int)(block / j.batch_blocks), u = (int)(block - (int64_t)b * j.batch_blocks) * 256 + (int)threadIdx.x;
+    if (u >= j.units) return;
+    const int r = (int)j.by_chunk.divide((uint32_t)u), c = u - r * (int)j.by_chunk.d;
+    const int outer = (int)j.by_inner.divide((uint32_t)r), inner = r - outer * (int)j.by_inner.d;
+    const int h0 = (j.heads_inner ? inner : outer) * HEADS, t = j.heads_inner ? outer : inner;
+    const int rot = j.turns ? a.rot : 0;
+    const bool turns = c * 8 < rot;
+    const int at = turns ? c * 4 : rot + (c - rot / 8) * 4, half = (turns ? rot : a.dim - rot) / 2;
+    const float *x = j.x + b * j.xs[0] + h0 * j.xs[1] + t * j.xs[2] + at;
+    float v[HEADS][8];
+#pragma unroll
+    for (int n = 0; n < HEADS; n++) {
+        const float *p = x + (h0 + n < j.heads ? n : 0) * j.xs[1];
+        const f4u y = __builtin_nontemporal_load((const f4u *)p), z = __builtin_nontemporal_load((const f4u *)(p + half));
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[n][e] = y[e], v[n][4 + e] = z[e];
+    }
+    const Token k = token_of(a, b, t);
+    if (turns) {
+        const Angles g = angles_of(a, b, t, k, a.interleaved ? at / 2 : at);
+#pragma unroll
+        for (int n = 0; n < HEADS; n++) {
+            if (a.interleaved) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) turn(v[n][2 * e], v[n][2 * e + 1], g.co[e], g.si[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) turn(v[n][e], v[n][4 + e], g.co[e], g.si[e]);
+            }
+        }
+    }
+    if (j.paged && k.id < 0) return;
+    const int64_t to = (j.paged ? k.id * j.ys[0] + k.slot * j.ys[2] : b * j.ys[0] + t * j.ys[2]) + h0 * j.ys[1] + at;
+#pragma unroll
+    for (int n = 0; n < HEADS; n++) {
+        if (h0 + n >= j.heads) break;
+        const int64_t y = to + n * j.ys[1];
+        if (j.paged && a.bf16) {
+            uint16_t *p = (uint16_t *)j.y + y;
+            *(u2u *)p = u2u{to_bf16(v[n][0], v[n][1]), to_bf16(v[n][2], v[n][3])};
+            *(u2u *)(p + half) = u2u{to_bf16(v[n][4], v[n][5]), to_bf16(v[n][6], v[n][7])};
+        } else {
+            __builtin_nontemporal_store((f4u{v[n][0], v[n][1], v[n][2], v[n][3]}), (f4u *)((float *)j.y + y));
+            __builtin_nontemporal_store((f4u{v[n][4], v[n][5], v[n][6], v[n][7]}), (f4u *)((float *)j.y + y + half));
+        }
+    }
+}
+template <int HEADS>
+__global__ void __launch_bounds__(256) rope_eights(RopeArgs a) {
+    for (int64_t at = blockIdx.x; at < a.blocks; at += gridDim.x) rope_eight<HEADS>(a, at);
 }
 
 // The rotation's arguments, as both entry points have them.
@@ -189,19 +290,24 @@ void to_pages(RopeJob &j, void *pool, const PoolView &v) {
 // Launches the jobs that have elements.
 int launch(RopeArgs &a) {
     int32_t n = 0;
-    int64_t blocks = 0;
-    a.heads_inner = 1;
-    for (int i = 0; i < a.jobs; i++)
-        if (a.job[i].xs[1] > a.job[i].xs[2] && a.job[i].heads > 1 && a.tokens > 1) a.heads_inner = 0;
+    int64_t blocks = 0, eights = 0;
+    bool whole = a.rot % 8 == 0 && a.dim % 8 == 0;
+    for (int i = 0; i < a.jobs; i++) {
+        const RopeJob &j = a.job[i];
+        whole = whole && j.xs[3] == 1 && j.ys[3] == 1;
+        eights += (int64_t)a.batch * j.heads * a.tokens * (a.dim / 8);
+    }
+    const int heads = whole && eights >= kManyEights ? 4 : 1;
     for (int i = 0; i < a.jobs; i++) {
         RopeJob j = a.job[i];
-        const int64_t chunks = j.turns ? a.dim - a.rot / 2 : a.dim;
-        const int64_t units = chunks * j.heads * a.tokens;
+        const int64_t chunks = whole ? a.dim / 8 : j.turns ? a.dim - a.rot / 2 : a.dim, groups = (j.heads + heads - 1) / heads;
+        const int64_t units = chunks * groups * a.tokens;
         if (units == 0 || a.batch == 0) continue;
         if (units >> 31) return set_error(TRS_E_INDEX_OVERFLOW, "rotation of more than 2^31 entries a sequence");
         j.units = (int32_t)units;
+        j.heads_inner = j.xs[1] <= j.xs[2];
         j.by_chunk = SmallDivisor((uint32_t)chunks);
-        j.by_inner = SmallDivisor((uint32_t)(a.heads_inner ? j.heads : a.tokens));
+        j.by_inner = SmallDivisor((uint32_t)(j.heads_inner ? groups : a.tokens));
         j.batch_blocks = (int32_t)((units + 255) / 256);
         j.first = blocks;
         blocks += (int64_t)j.batch_blocks * a.batch;
@@ -211,7 +317,10 @@ int launch(RopeArgs &a) {
     if (n == 0) return TRS_OK;
     DeviceState *dev = device_state();
     if (!dev) return TRS_E_NO_DEVICE;
-    hipLaunchKernelGGL(rope_pairs, dim3((unsigned)std::min<int64_t>(blocks, 1 << 22)), dim3(256), 0, dev->stream, a);
+    const dim3 grid((unsigned)std::min<int64_t>(blocks, 1 << 22));
+    if (!whole) hipLaunchKernelGGL(rope_pairs, grid, dim3(256), 0, dev->stream, a);
+    else if (heads > 1) hipLaunchKernelGGL(rope_eights<4>, grid, dim3(256), 0, dev->stream, a);
+    else hipLaunchKernelGGL(rope_eights<1>, grid, dim3(256), 0, dev->stream, a);
     TRS_LAUNCH_CHECK("rotation launch");
     return TRS_OK;
 }
@@ -237,7 +346,7 @@ int run_rope(int n, const float *const *x, const trs_layout *lx, const Rotation 
     }
     const int64_t batch = lx[0].shape[0], tokens = lx[0].shape[2];
     if (batch > INT32_MAX || tokens > kMaxPagedTokens || lx[0].shape[1] > INT32_MAX || lx[n - 1].shape[1] > INT32_MAX)
-        return set_error(TRS_E_INDEX_OVERFLOW, "rotation of more than 2^30 tokens, or of 2^31 sequences or heads");
+        return set_error(TRS_E_INDEX_OVERFLOW, "rotation of more than 2^29 tokens, or of 2^31 sequences or heads");
     a.batch = (int32_t)batch, a.tokens = (int32_t)tokens, a.dim = (int32_t)lx[0].shape[3];
     TRS_CHECK(take_rotation(r, a.dim, a));
     if (!r.positions && batch > 0 && tokens > 0 && (start < 0 || start > a.table_rows - tokens))
@@ -274,7 +383,7 @@ int run_append(const trs_paged_cache *cache, const float *k, const trs_layout *l
         return set_error(TRS_E_INVALID_ARGUMENT, "a query or its output without the query's layout");
     }
     if (batch > INT32_MAX || tokens > kMaxPagedTokens || lk->shape[1] > INT32_MAX || (query && lq->shape[1] > INT32_MAX))
-        return set_error(TRS_E_INDEX_OVERFLOW, "appending more than 2^30 tokens, or to 2^31 sequences or heads");
+        return set_error(TRS_E_INDEX_OVERFLOW, "appending more than 2^29 tokens, or to 2^31 sequences or heads");
     TRS_CHECK(check_cache(cache, batch, &a.pages));
     a.batch = (int32_t)batch, a.tokens = (int32_t)tokens, a.dim = (int32_t)lk->shape[3];
     a.appends = 1, a.bf16 = cache->type == TRS_PAGES_BF16, a.sign = 1.f;
