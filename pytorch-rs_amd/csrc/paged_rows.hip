@@ -88,6 +88,12 @@ struct Fragment {
         }
         return f;
     }
+    // What was written so far: the reads, then the products.
+    __device__ __forceinline__ static void in_order() {
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * PIECES, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, PIECES == 3 ? 6 : 3, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    }
     __device__ __forceinline__ void multiply(at_f16 &c, const Pieces &b) const {
         if constexpr (PIECES == 3) {
             const Pieces x{{p[0], p[1], p[2]}};
@@ -195,9 +201,17 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_rows(PagedArgs a, int stage)
                 missing0 = missing1, missing1 = missing;
                 // Whether a row of the wave sees a key of the tile.
                 if (j0 <= wave_hi && (wave_lo - (j0 + 31) < a.window || j0 < a.sinks)) {
+                    // Fragments are read a step ahead of their products.
+                    const auto value = [&](int n) { return F::template across<UNITS>(buf, 2 * NT + 2 * (n % NT), n / NT, lane); };
                     at_f16 x = (at_f16)(0.f);
+                    F f = F::template along<UNITS>(buf, 0, lane);
 #pragma unroll
-                    for (int n = 0; n < 2 * NT; n++) F::template along<UNITS>(buf, n, lane).multiply(x, q[n]);
+                    for (int n = 0; n < 2 * NT; n++) {
+                        const F now = f;
+                        f = n + 1 < 2 * NT ? F::template along<UNITS>(buf, n + 1, lane) : value(0);
+                        now.multiply(x, q[n]);
+                        F::in_order();
+                    }
                     lowest.add(x);
                     const bool all = whole && j0 >= s.from && j0 + 31 < s.to && j0 + 31 <= wave_lo && (wave_hi - j0 < a.window || j0 + 32 <= a.sinks);
                     if (!all || absent) {
@@ -212,12 +226,13 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_rows(PagedArgs a, int stage)
 #pragma unroll
                     for (int e = 1; e < 16; e++) m = __builtin_fmaxf(m, x[e]);
                     m = __builtin_fmaxf(m, __shfl_xor(m, 32));
-                    const float top = __builtin_fmaxf(most, m), base = top == -__builtin_inff() ? 0.f : top;
-                    const float keep = __builtin_amdgcn_exp2f((most - base) * kUnit);
+                    // (The unit is a power of two: the sum is rounded once.)
+                    const float top = __builtin_fmaxf(most, m), base = (top == -__builtin_inff() ? 0.f : top) * kUnit;
+                    const float keep = __builtin_amdgcn_exp2f(__builtin_fmaf(most, kUnit, -base));
                     float add[2] = {0.f, 0.f};
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
-                        x[e] = __builtin_amdgcn_exp2f((x[e] - base) * kUnit);
+                        x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], kUnit, -base));
                         add[e & 1] += x[e];
                     }
                     sum = sum * keep + (add[0] + add[1]);
@@ -233,7 +248,12 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_rows(PagedArgs a, int stage)
                         for (int i = 0; i < 4; i++) p.pair(i, x[8 * n + 2 * i], x[8 * n + 2 * i + 1]);
                         const Pieces y = p.done();
 #pragma unroll
-                        for (int c = 0; c < NT; c++) F::template across<UNITS>(buf, 2 * NT + 2 * c, n, lane).multiply(acc[c], y);
+                        for (int c = 0; c < NT; c++) {
+                            const F now = f;
+                            if (n * NT + c + 1 < 2 * NT) f = value(n * NT + c + 1);
+                            now.multiply(acc[c], y);
+                            F::in_order();
+                        }
                     }
                 }
             }
