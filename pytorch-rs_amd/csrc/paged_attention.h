@@ -124,7 +124,7 @@ struct PagedShare {
         all = s.together ? keys_of_all(a, lane) : make_int2(0, 0);
         entry = 0, before = 0;
         if (s.workers == 0) {  // an entry each
-            entry = w, base = extra = pos = 0, end = w < s.entries ? uniform(tiles_of(w)) : 0;
+            entry = w, base = extra = pos = 0, end = w < s.entries ? uniform(tiles_of(entry)) : 0;
         } else if (s.together) {
             const uint32_t each = tiles_of(0);
             divide(s.entries * each, w);

@@ -14,12 +14,13 @@ constexpr int64_t kMaxHeadDim = 256;
 constexpr int kFewTile = 16;  // rows of a tile of paged_few
 constexpr int kFewRows = 32;
 
-// The parts of a row, joined by a wave: a lane has four columns of every 64 / quads-th part, `quads`
-// lanes a part (a power of two), four of its parts on their way at once.
-__global__ void __launch_bounds__(256) paged_join(PagedArgs a, int quads) {
+// The parts of rows, joined: a lane has four columns of a row's every `groups`-th part, `quads` lanes a part
+// (a power of two), four of its parts on their way at once; a wave 64 / (quads groups) rows.
+__global__ void __launch_bounds__(256) paged_join(PagedArgs a, int quads, int groups) {
     const int64_t rows = (int64_t)a.batch * a.kv_heads * a.seq_rows;
-    const int lane = (int)threadIdx.x & 63, quad = lane & (quads - 1), groups = 64 / quads, group = lane / quads;
-    for (int64_t at = blockIdx.x * 4ll + (threadIdx.x >> 6); at < rows; at += gridDim.x * 4ll) {
+    const int lane = (int)threadIdx.x & 63, quad = lane & (quads - 1), group = lane / quads & (groups - 1), per = 64 / (quads * groups);
+    const int64_t first = (blockIdx.x * 4ll + (threadIdx.x >> 6)) * per + lane / (quads * groups), step = gridDim.x * 4ll * per;
+    for (int64_t at = first; at < rows; at += step) {
         const int64_t head = at / a.seq_rows;
         const int r = (int)(at - head * a.seq_rows), b = (int)(head / a.kv_heads), hk = (int)(head - (int64_t)b * a.kv_heads);
         const int d = min(quad * 4, a.part_width - 4);
@@ -55,11 +56,11 @@ __global__ void __launch_bounds__(256) paged_join(PagedArgs a, int quads) {
             }
         }
         if (whole) continue;
-        for (int step = quads; step < 64; step *= 2) {
-            const float m = __shfl_xor(most, step), l = __shfl_xor(sum, step);
+        for (int apart = quads; apart < quads * groups; apart *= 2) {
+            const float m = __shfl_xor(most, apart), l = __shfl_xor(sum, apart);
             at_f4 x;
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[e] = __shfl_xor(o[e], step);
+            for (int e = 0; e < 4; e++) x[e] = __shfl_xor(o[e], apart);
             add(m, l, x);
         }
         if (group != 0) continue;
@@ -130,15 +131,20 @@ int paged_forward(PagedArgs &a, bool bf16, DeviceState *dev) {
     const int from = a.stages ? a.shared : 0;
     if (from < a.pages.capacity || a.stages == 0) a.stage[a.stages++] = plan_stage(a, false, from, a.pages.capacity, dev->cu_count, bf16);
     if (a.pages.capacity == 0) a.stages = 0;  // nobody sees anything
-    void *ws = nullptr;
-    const int rc0 = a.stages ? take_parts(a, &ws) : TRS_OK;
-    if (rc0 == TRS_E_ALLOCATION_FAILED) {
+    // One stage with a worker for every entry: no parts, and nothing to join.
+    const auto entry_each = [&]() {
         a.stages = 1, a.stage[1] = PagedStage{};
         a.stage[0] = plan_stage(a, false, 0, a.pages.capacity, dev->cu_count, bf16);
         a.stage[0].workers = 0;
-    } else if (rc0) {
-        return rc0;
+    };
+    if (a.stages == 2 && (a.stage[0].workers == 0 || a.stage[1].workers == 0)) entry_each();
+    void *ws = nullptr;
+    if (a.stages && a.stage[0].workers) {
+        const int rc = take_parts(a, &ws);
+        if (rc == TRS_E_ALLOCATION_FAILED) entry_each();  // the parts are for speed alone
+        else if (rc) return rc;
     }
+    const bool joins = a.stages == 0 || a.stage[0].workers;
     const auto launch = [&]() -> int {
         const auto few = [&](int i) { return a.stage[i].tile_rows == kFewTile; };
         if (a.stages == 2 && few(0) && few(1)) {
@@ -146,11 +152,13 @@ int paged_forward(PagedArgs &a, bool bf16, DeviceState *dev) {
         } else {
             for (int i = 0; i < a.stages; i++) TRS_CHECK(few(i) ? launch_paged_few(a, i, 1, bf16, dev->stream) : launch_paged_rows(a, i, bf16, dev->stream));
         }
-        if (!ws && a.stages) return TRS_OK;
+        if (!joins) return TRS_OK;
         int quads = 1;
         while (quads * 4 < a.part_width) quads *= 2;
-        const int64_t rows = (int64_t)a.batch * a.kv_heads * a.seq_rows;
-        hipLaunchKernelGGL(paged_join, dim3((unsigned)std::min<int64_t>((rows + 3) / 4, 1 << 22)), dim3(256), 0, dev->stream, a, quads);
+        // Waves have parts of few rows each, blocks two or three of many.
+        const int groups = a.stages && few(a.stages - 1) ? 64 / quads : 1;
+        const int64_t lanes = (int64_t)a.batch * a.kv_heads * a.seq_rows * quads * groups;
+        hipLaunchKernelGGL(paged_join, dim3((unsigned)std::min<int64_t>((lanes + 255) / 256, 1 << 22)), dim3(256), 0, dev->stream, a, quads, groups);
         TRS_LAUNCH_CHECK("paged attention join launch");
         return TRS_OK;
     };

@@ -18,6 +18,9 @@ namespace trs {
 namespace {
 
 constexpr int kMaxDim = 1024, kMostAxes = 4, kMaxPairs = kMaxDim / 2;
+// Eights from which a lane has several heads of a token: 2 x 4096 tokens, 40 heads of 128, three axes, us with
+// one, two and four heads a lane: 74, 63, 61; gradients of 4 x 2047 tokens, 20 heads of 64: 41, 43, 39; two prompts
+// of 4096 tokens appended to float32 pages, 8 key heads of 128 and 32 of queries: 86, 73, 77.
 constexpr int64_t kManyEights = 1 << 19;
 
 // A tensor to be turned, or moved as it is: [batch, head, token, dim].
@@ -297,7 +300,7 @@ int launch(RopeArgs &a) {
         whole = whole && j.xs[3] == 1 && j.ys[3] == 1;
         eights += (int64_t)a.batch * j.heads * a.tokens * (a.dim / 8);
     }
-    const int heads = whole && eights >= kManyEights ? 4 : 1;
+    const int heads = !whole || eights < kManyEights ? 1 : a.appends ? 2 : 4;
     for (int i = 0; i < a.jobs; i++) {
         RopeJob j = a.job[i];
         const int64_t chunks = whole ? a.dim / 8 : j.turns ? a.dim - a.rot / 2 : a.dim, groups = (j.heads + heads - 1) / heads;
@@ -319,7 +322,8 @@ int launch(RopeArgs &a) {
     if (!dev) return TRS_E_NO_DEVICE;
     const dim3 grid((unsigned)std::min<int64_t>(blocks, 1 << 22));
     if (!whole) hipLaunchKernelGGL(rope_pairs, grid, dim3(256), 0, dev->stream, a);
-    else if (heads > 1) hipLaunchKernelGGL(rope_eights<4>, grid, dim3(256), 0, dev->stream, a);
+    else if (heads == 4) hipLaunchKernelGGL(rope_eights<4>, grid, dim3(256), 0, dev->stream, a);
+    else if (heads == 2) hipLaunchKernelGGL(rope_eights<2>, grid, dim3(256), 0, dev->stream, a);
     else hipLaunchKernelGGL(rope_eights<1>, grid, dim3(256), 0, dev->stream, a);
     TRS_LAUNCH_CHECK("rotation launch");
     return TRS_OK;

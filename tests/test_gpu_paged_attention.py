@@ -76,6 +76,8 @@ SHAPES = [
     (1, 3, 3, 90, 10, 100, [250], EVERY, 2),
     (40, 2, 1, 1, 64, 16, [7 * i % 300 for i in range(40)], EVERY, 0),
     (70, 4, 2, 1, 32, 16, [5 + i for i in range(70)], 20, 2),
+    (1, 64, 16, 1024, 16, 16, [1024], EVERY, 0),     # tiles of rows for every CU
+    (2, 64, 8, 1000, 24, 32, [700, 1100], 600, 3),
 ]
 
 
