@@ -12,7 +12,17 @@ namespace {
 
 constexpr int64_t kMaxHeadDim = 256;
 constexpr int kFewTile = 16;  // rows of a tile of paged_few
-constexpr int kFewRows = 32;
+// paged_few takes up to so many rows, and any number with fewer pairs of a row and a key in all, us in it / in
+// paged_rows: one token or a few over 4096 keys, 8 key heads of 128, bfloat16, 64 rows of 1, 4 and 16 sequences
+// 32 / 40, 46 / 50, 128 / 126, 128 rows 36 / 44, 66 / 56, 231 / 140; float32, 64 rows 36 / 44, 70 / 91, 218 / 292, 96 rows 45 / 46,
+// 98 / 93, 378 / 296; rows of a batch over shared keys, bfloat16, 128 rows over 8192 keys 52 / 57 and 32768 126 / 99, 256 over 1024
+// 38 / 43, 4096 54 / 52 and 8192 74 / 62, 512 over 1024 49 / 53 and 4096 81 / 68.
+constexpr int kFewRows = 64;
+constexpr int64_t kFewPairs = 1 << 23;
+// Shared keys are worked on together where that saves so much reading, us apart / together, 8 key heads of 128: bfloat16,
+// 2 sequences over 1024 keys (4 MiB) 17.2 / 17.9 and 4096 (16 MiB) 25.7 / 22.9, 4 over 1024 (12 MiB) 17.8 / 17.9, 8 over 256 (7 MiB)
+// 16.3 / 17.3 and 1024 (28 MiB) 21.3 / 18.5; float32, 4 over 1024 (24 MiB) 24.0 / 20.5, 8 over 256 (14 MiB) 19.1 / 19.0.
+constexpr int64_t kTogetherBytes = 16 << 20;
 
 // The parts of rows, joined: a lane has four columns of a row's every `groups`-th part, `quads` lanes a part
 // (a power of two), four of its parts on their way at once; a wave 64 / (quads groups) rows.
@@ -80,7 +90,9 @@ PagedStage plan_stage(const PagedArgs &a, bool together, int from, int to, int c
     PagedStage s{};
     s.together = together, s.from = from, s.to = to;
     const int64_t rows = together ? (int64_t)a.batch * a.seq_rows : a.seq_rows;
-    s.tile_rows = rows <= kFewRows || a.D > kPiecesDim ? kFewTile : rows <= 128 && bf16 ? 128 : 256;
+    const int64_t keys = std::min<int64_t>(to - from, (int64_t)a.window + a.sinks + a.Sq);
+    const bool few = rows <= kFewRows || a.D > kPiecesDim || rows * (together ? 1 : a.batch) * a.kv_heads * keys < kFewPairs;
+    s.tile_rows = few ? kFewTile : rows <= 128 && bf16 ? 128 : 256;
     s.row_tiles = (int32_t)((rows + s.tile_rows - 1) / s.tile_rows);
     s.entries = (int32_t)(together ? s.row_tiles : (int64_t)s.row_tiles * a.batch);
     if (s.tile_rows == kFewTile) {
@@ -124,7 +136,8 @@ int take_parts(PagedArgs &a, void **ws) {
 int paged_forward(PagedArgs &a, bool bf16, DeviceState *dev) {
     a.part_width = (a.D + 3) / 4 * 4;
     a.stages = 0;
-    if (a.shared > 0 && a.batch > 1 && (int64_t)a.batch * a.seq_rows < (int64_t)1 << 31) {
+    const int64_t saved = (int64_t)(a.batch - 1) * a.shared * a.kv_heads * a.D * (bf16 ? 4 : 8);
+    if (saved >= kTogetherBytes && (int64_t)a.batch * a.seq_rows < (int64_t)1 << 31) {
         a.all_rows = a.batch * a.seq_rows, a.by_seq_rows = SmallDivisor((uint32_t)a.seq_rows);
         a.stage[a.stages++] = plan_stage(a, true, 0, a.shared, dev->cu_count, bf16);
     }

@@ -44,11 +44,14 @@ class Cache:
         self.kind, self.page, self.lengths, self.shared = kind, page, list(lengths), shared
         width = max([-(-n // page) for n in lengths] + [0]) if width is None else width
         whole = shared // page
-        count = sum(max(-(-min(n, width * page) // page), 0) for n in lengths) + extra
+        # The first row has the shared tokens' pages however few of them are its own sequence's.
+        has = [min(max(n, shared if b == 0 and any(m > 0 for m in lengths) else 0, 0), width * page) for b, n in enumerate(lengths)]
+        has = [min(n, keys.shape[2]) if keys is not None and n > lengths[b] else n for b, n in enumerate(has)]
+        count = sum(-(-n // page) for n in has) + extra
         free = iter(rng.permutation(count))
         self.table = np.full((batch, width), -1, np.int32)
-        for b, n in enumerate(lengths):
-            for i in range(min(max(-(-n // page), 0), width)):
+        for b, n in enumerate(has):
+            for i in range(-(-n // page)):
                 if b > 0 and i < whole:
                     self.table[b, i] = elsewhere
                 else:
@@ -68,8 +71,8 @@ class Cache:
             if x is None:
                 continue
             view = self.view(which)
-            for b, n in enumerate(lengths):
-                for t in range(min(n, width * page)):
+            for b, n in enumerate(has):
+                for t in range(n):
                     if written is not None and t not in written:
                         continue
                     at = self.table[0 if t < shared else b, t // page]

@@ -76,13 +76,27 @@ SHAPES = [
     (1, 3, 3, 90, 10, 100, [250], EVERY, 2),
     (40, 2, 1, 1, 64, 16, [7 * i % 300 for i in range(40)], EVERY, 0),
     (70, 4, 2, 1, 32, 16, [5 + i for i in range(70)], 20, 2),
+]
+
+# Pairs of a row and a key enough for tiles of 128 and 256 rows.
+MANY = [
     (1, 64, 16, 1024, 16, 16, [1024], EVERY, 0),     # tiles of rows for every CU
     (2, 64, 8, 1000, 24, 32, [700, 1100], 600, 3),
+    (1, 16, 4, 700, 64, 16, [1000], EVERY, 0),
+    (2, 8, 2, 600, 128, 64, [1500, 900], EVERY, 0),
+    (1, 8, 2, 1000, 33, 16, [1200], EVERY, 0),       # a dim that no vector divides
+    (3, 6, 6, 700, 80, 16, [900, 700, 750], EVERY, 0),
+    (1, 16, 4, 900, 96, 48, [1500], 600, 40),
+    (1, 12, 4, 1000, 16, 10, [1000], EVERY, 2),      # pages that end inside a tile
+    (1, 8, 2, 1300, 24, 12, [2000], 300, 70),
+    (40, 8, 2, 30, 128, 16, [1000 - 20 * i for i in range(40)], EVERY, 0),  # 120 rows a sequence
+    (4, 16, 2, 300, 64, 16, [0, 1000, 299, 5], EVERY, 0),
+    (1, 5, 1, 1200, 128, 16, [1500], 1, 0),          # each query sees itself alone
 ]
 
 
 @KINDS
-@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("shape", SHAPES + MANY, ids=str)
 def test_attention_matches_64_bits(shape, kind):
     B, H, HK, sq, D, page, lengths, window, sinks = shape
     q, k, v = inputs(sq * 7 + D, B, H, HK, sq, max(lengths), D, kind)
@@ -109,9 +123,25 @@ SHARED = [
     (80, 8, 2, 1, 64, 16, [40 + i % 9 for i in range(80)], 32, EVERY, 0),
 ]
 
+# Shared keys enough to be worked on for the whole batch at once, by few rows or by many.
+TOGETHER = [
+    (33, 8, 2, 1, 64, 16, [1100 + i for i in range(33)], 1024, EVERY, 0),
+    (33, 8, 2, 1, 64, 16, [(1100 + i) * (i % 5 > 0) for i in range(33)], 1030, EVERY, 0),  # in a page's middle; sequences without tokens
+    (3, 16, 8, 2, 128, 16, [2300, 2100, 2049], 2048, 700, 9),
+    (17, 4, 4, 1, 80, 8, [1600 - 90 * i for i in range(17)], 1500, EVERY, 0),              # ones that end among the shared keys
+    (33, 4, 2, 1, 33, 10, [2000 + 5 * i for i in range(33)], 2000, EVERY, 0),
+    (9, 2, 2, 1, 256, 16, [2200 + i for i in range(9)], 2176, 1000, 0),
+    (33, 8, 2, 8, 64, 16, [4200 + 3 * i for i in range(33)], 4096, EVERY, 0),
+    (33, 8, 2, 8, 128, 16, [4200 + 3 * i for i in range(33)], 4096, 3000, 5),
+    (20, 8, 4, 40, 48, 16, [1600 - 20 * i for i in range(20)], 1330, EVERY, 0),
+    (20, 8, 4, 100, 32, 16, [1900 + i for i in range(20)], 1330, EVERY, 0),                # many rows of both kinds
+    (24, 16, 2, 12, 96, 24, [2100] * 24, 2100, EVERY, 0),                                  # nothing of their own
+    (34, 8, 2, 8, 20, 16, [4300 - 100 * i for i in range(34)], 4100, 2000, 40),
+]
+
 
 @KINDS
-@pytest.mark.parametrize("shape", SHARED, ids=str)
+@pytest.mark.parametrize("shape", SHARED + TOGETHER, ids=str)
 def test_keys_that_a_batch_shares(shape, kind):
     B, H, HK, sq, D, page, lengths, shared, window, sinks = shape
     q, k, v = inputs(sq + D + shared, B, H, HK, sq, max(lengths), D, kind)
@@ -126,6 +156,9 @@ def test_pools_and_queries_of_any_order(form, kind, order):
     for sq, D, page in ((1, 64, 16), (2, 48, 10), (150, 64, 16), (100, 20, 12)):
         q, k, v = inputs(sq, 2, 4, 2, sq, 200, D, kind)
         run(q, k, v, [200, 151], page, kind, 90, 3, form=form, order=order)
+    for D, page in ((64, 16), (20, 12)):  # many rows
+        q, k, v = inputs(D, 2, 16, 2, 400, 700, D, kind)
+        run(q, k, v, [700, 651], page, kind, 500, 3, form=form, order=order)
 
 
 @pytest.mark.parametrize("sq", [1, 100])
@@ -137,14 +170,20 @@ def test_a_query_without_a_unit_stride(sq):
     assert_within(out.numpy(), *attention_reference(q, k, v, EVERY, 0, 0.2, [120])["out"])
 
 
+# Heads, tokens and keys of few rows and of many.
+SIZES = pytest.mark.parametrize("H,sq,most", [(4, 1, 290), (4, 3, 290), (4, 130, 290), (16, 520, 1100)])
+
+
 @KINDS
 @pytest.mark.parametrize("D", [64, 80, 20])
-@pytest.mark.parametrize("sq", [1, 3, 130])
+@SIZES
 @pytest.mark.parametrize("shared", [0, 48])
-def test_hidden_values_that_are_not_finite_do_not_reach_a_query(kind, D, sq, shared):
+def test_hidden_values_that_are_not_finite_do_not_reach_a_query(kind, D, H, sq, most, shared):
     """NaN and infinities before the window and behind a sequence; queries of padding hold NaN."""
-    B, lengths, window, sinks = 2, [290, sq + 90], 60, 5
-    q, k, v = inputs(8, B, 4, 2, sq, 290, D, kind)
+    B, lengths, window, sinks = 2, [most, sq + 90], 60, 5
+    if H > 4:
+        window = 600
+    q, k, v = inputs(8, B, H, 2, sq, most, D, kind)
     share(k, v, shared)
     want = attention_reference(q, k, v, window, sinks, D ** -0.5, lengths)
     for b, n in enumerate(lengths):
@@ -158,10 +197,10 @@ def test_hidden_values_that_are_not_finite_do_not_reach_a_query(kind, D, sq, sha
 
 
 @KINDS
-@pytest.mark.parametrize("sq", [1, 130])
-def test_padded_queries_that_hold_nan_give_zero(kind, sq):
-    q, k, v = inputs(9, 3, 4, 2, sq, 200, 64, kind)
-    lengths = [200, 0, max(sq // 2, 0)]
+@SIZES
+def test_padded_queries_that_hold_nan_give_zero(kind, H, sq, most):
+    q, k, v = inputs(9, 3, H, 2, sq, most, 64, kind)
+    lengths = [most, 0, max(sq // 2, 0)]
     for b, n in enumerate(lengths):
         q[b, :, :max(sq - n, 0)] = np.nan
     got, _ = run(q, k, v, lengths, 16, kind, want={"out": (np.where(np.isnan(q), 0, attention_reference(np.nan_to_num(q), k, v, EVERY, 0, 0.125, lengths)["out"][0]),
@@ -170,30 +209,31 @@ def test_padded_queries_that_hold_nan_give_zero(kind, sq):
 
 
 @KINDS
-@pytest.mark.parametrize("sq,D", [(1, 64), (2, 20), (130, 64), (130, 200)])
+@pytest.mark.parametrize("H,sq,D,n,window", [(4, 1, 64, 200, 64), (4, 2, 20, 200, 64), (4, 130, 64, 200, 64), (4, 130, 200, 200, 64), (32, 400, 64, 700, 500),
+                                             (32, 400, 20, 700, 500)])
 @pytest.mark.parametrize("where", ["key", "value"])
-def test_visible_values_that_are_not_finite_are_as_the_formula_has_them(kind, sq, D, where):
+def test_visible_values_that_are_not_finite_are_as_the_formula_has_them(kind, H, sq, D, n, window, where):
     """NaN where the formula gives it, the same infinities, and no other row touched."""
-    q, k, v = inputs(10, 2, 4, 2, sq, 200, D, kind)
-    q = abs(q)
-    want = attention_reference(q, k, v, 64, 0, D ** -0.5, [200, 180])
+    q, k, v = inputs(10, 2, H, 2, sq, n, D, kind)
+    q, G, lengths = abs(q), H // 2, [n, n - 20]
+    want = attention_reference(q, k, v, window, 0, D ** -0.5, lengths)
     value, bound = (x.copy() for x in want["out"])
-    x = k if where == "key" else v
-    x[0, 0, 190, 3], x[1, 1, 170, 3] = np.nan, (-np.inf if where == "key" else np.inf)
-    place = {0: 200 - sq + np.arange(sq), 1: 180 - sq + np.arange(sq)}
-    sees = [(place[b] >= j) & (place[b] - j < 64) for b, j in ((0, 190), (1, 170))]
+    x, bad = k if where == "key" else v, (n - 10, n - 30)
+    x[0, 0, bad[0], 3], x[1, 1, bad[1], 3] = np.nan, (-np.inf if where == "key" else np.inf)
+    place = [m - sq + np.arange(sq) for m in lengths]
+    sees = [(place[b] >= j) & (place[b] - j < window) for b, j in enumerate(bad)]
     if where == "key":
-        value[0, :2, sees[0]] = np.nan
+        value[0, :G, sees[0]] = np.nan
         # A score of -inf has no weight: the same as without the key.
-        rows = attention_without(q, k, v, 1, 1, 170, 180, D)
-        value[1, 2:, sees[1]], bound[1, 2:, sees[1]] = rows[0][:, sees[1]].transpose(1, 0, 2), rows[1][:, sees[1]].transpose(1, 0, 2)
+        rows = attention_without(q, k, v, 1, 1, bad[1], n - 20, D, window)
+        value[1, G:, sees[1]], bound[1, G:, sees[1]] = rows[0][:, sees[1]].transpose(1, 0, 2), rows[1][:, sees[1]].transpose(1, 0, 2)
     else:
-        value[0, :2, sees[0], 3] = np.nan
-        value[1, 2:, sees[1], 3] = np.inf
-    run(q, k, v, [200, 180], 16, kind, 64, 0, want={"out": (value, bound)}, lse=False)
+        value[0, :G, sees[0], 3] = np.nan
+        value[1, G:, sees[1], 3] = np.inf
+    run(q, k, v, lengths, 16, kind, window, 0, want={"out": (value, bound)}, lse=False)
 
 
-def attention_without(q, k, v, b, head, key, n, D):
+def attention_without(q, k, v, b, head, key, n, D, window):
     """out and bound of one key head's rows with one key left out."""
     sq, G = q.shape[2], q.shape[1] // k.shape[1]
     rows = q[b, head * G:(head + 1) * G].astype(np.float64)
@@ -201,7 +241,7 @@ def attention_without(q, k, v, b, head, key, n, D):
     s = rows @ K.T * D ** -0.5
     p = (n - sq + np.arange(sq))[:, None]
     j = np.arange(n)[None]
-    s = np.where((j <= p) & (p - j < 64) & (j != key), s, -np.inf)
+    s = np.where((j <= p) & (p - j < window) & (j != key), s, -np.inf)
     e = np.exp(s - s.max(-1, keepdims=True))
     P = e / e.sum(-1, keepdims=True)
     d = (D + 8) * 2.0 ** -24 * (abs(rows) @ abs(K).T * D ** -0.5).max(-1, keepdims=True)
@@ -209,11 +249,11 @@ def attention_without(q, k, v, b, head, key, n, D):
 
 
 @KINDS
-@pytest.mark.parametrize("sq", [1, 130])
+@pytest.mark.parametrize("H,sq,most,window", [(4, 1, 200, 60), (4, 130, 200, 60), (32, 400, 700, 300)])
 @pytest.mark.parametrize("shared", [0, 32])
-def test_a_page_that_the_pool_does_not_have_makes_those_that_see_it_nan(kind, sq, shared):
-    B, lengths, window = 3, [200, 190, 185], 60
-    q, k, v = inputs(11, B, 4, 2, sq, 200, 64, kind)
+def test_a_page_that_the_pool_does_not_have_makes_those_that_see_it_nan(kind, H, sq, most, window, shared):
+    B, lengths = 3, [most, most - 10, most - 15]
+    q, k, v = inputs(11, B, H, 2, sq, most, 64, kind)
     share(k, v, shared)
     bad = {0: 10, 1: 3, 2: 11}  # page 3 of the second: before every window of one token, not of a prompt
 
@@ -232,21 +272,21 @@ def test_a_page_that_the_pool_does_not_have_makes_those_that_see_it_nan(kind, sq
 
 
 @KINDS
-@pytest.mark.parametrize("sq,D", [(1, 64), (3, 96), (150, 64), (150, 200)])
+@pytest.mark.parametrize("H,sq,D", [(4, 1, 64), (4, 3, 96), (4, 150, 64), (4, 150, 200), (64, 300, 64)])
 @pytest.mark.parametrize("size", [1e-20, 30.0, 1e4])
-def test_scores_of_any_size(kind, sq, D, size):
-    q, k, v = inputs(12, 2, 4, 2, sq, 260, D, kind, std=size)
-    run(q, k, v, [260, 200], 16, kind, 128, 2)
+def test_scores_of_any_size(kind, H, sq, D, size):
+    q, k, v = inputs(12, 2, H, 2, sq, 360, D, kind, std=size)
+    run(q, k, v, [360, 300], 16, kind, 128, 2)
 
 
 @KINDS
-@pytest.mark.parametrize("sq", [1, 100])
-def test_values_of_any_size(kind, sq):
+@pytest.mark.parametrize("H,sq", [(4, 1), (4, 100), (64, 300)])
+def test_values_of_any_size(kind, H, sq):
     """Keys beyond the products' pieces, and values near the least and the largest floats."""
-    q, k, v = inputs(13, 1, 4, 2, sq, 150, 64, kind)
-    run(q * np.float32(1e-30), held(k * np.float32(1e30), kind), v, [150], 16, kind)
-    run(q, k, held(v * np.float32(1e-36), kind), [150], 16, kind)
-    run(q, k, held(v * np.float32(1e34), kind), [150], 16, kind)
+    q, k, v = inputs(13, 1, H, 2, sq, 450, 64, kind)
+    run(q * np.float32(1e-30), held(k * np.float32(1e30), kind), v, [450], 16, kind)
+    run(q, k, held(v * np.float32(1e-36), kind), [450], 16, kind)
+    run(q, k, held(v * np.float32(1e34), kind), [450], 16, kind)
 
 
 @KINDS
@@ -256,11 +296,11 @@ def test_lengths_beyond_the_table_and_below_zero(kind):
 
 
 @KINDS
-@pytest.mark.parametrize("sq", [1, 100])
-def test_offsets_past_32_bits(kind, sq):
-    """Pools whose pages lie more than 2^32 bytes apart, in one buffer that is mostly untouched."""
+@pytest.mark.parametrize("H,sq", [(4, 1), (64, 900)])
+def test_offsets_past_32_bits(kind, H, sq):
+    """Pools that reach past 2^32 bytes and 2^31 entries, in one buffer that is mostly untouched."""
     D, page, HK = 64, 16, 2
-    q, k, v = inputs(15, 1, 4, HK, sq, 160, D, kind)
+    q, k, v = inputs(15, 1, H, HK, sq, 160, D, kind)
     size = 2 if kind == BF16 else 4
     cache = Cache(1, HK, page, D, [160], kind, "heads", k, v, extra=0)
     count, step = cache.shape[0], (1 << 32) // size // 4  # a GiB a page: offsets to 10 GiB
@@ -280,7 +320,7 @@ def test_offsets_past_32_bits(kind, sq):
 @KINDS
 def test_without_memory_for_parts(kind):
     """The parts of long sequences are for speed alone."""
-    for B, sq, shared in ((2, 1, 0), (2, 1, 320), (1, 200, 0), (33, 1, 320)):
+    for B, sq, shared in ((2, 1, 0), (2, 1, 320), (1, 200, 0), (33, 1, 880), (33, 40, 870), (2, 700, 0)):
         q, k, v = inputs(16, B, 8, 2, sq, 900, 64, kind)
         share(k, v, shared)
         Q = Placed(q)
@@ -298,10 +338,10 @@ def test_without_memory_for_parts(kind):
 
 @KINDS
 def test_the_same_bits_each_time(kind):
-    for B, sq, shared in ((5, 1, 0), (40, 1, 256), (2, 150, 0)):
-        q, k, v = inputs(17, B, 8, 2, sq, 700, 128, kind)
+    for B, sq, shared in ((5, 1, 0), (40, 1, 256), (40, 1, 1000), (40, 20, 1000), (2, 150, 0), (2, 800, 0)):
+        q, k, v = inputs(17, B, 8, 2, sq, 1100, 128, kind)
         share(k, v, shared)
-        cache = Cache(B, 2, 16, 128, [700 - 9 * i for i in range(B)], kind, "heads", k, v, shared=shared)
+        cache = Cache(B, 2, 16, 128, [1100 - 2 * i for i in range(B)], kind, "heads", k, v, shared=shared)
         Q, outs = Placed(q), []
         for _ in range(3):
             out = Placed(shape=q.shape)
