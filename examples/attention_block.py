@@ -6,7 +6,8 @@ x [batch * tokens, width] -> queries, keys and values (one product each) -> the
 norm of every head with the rotation by position -> attention over a sliding
 window and the first tokens -> the output product -> dropout -> + x.  The step's
 dropout masks come from (seed, offset) alone.  Serving computes the last token
-of a sequence against the keys and values of all of them.
+of a sequence against the keys and values of all of them: from one product's
+tensors, or from a paged cache that prompts and tokens were appended to.
 """
 from __future__ import annotations
 
@@ -68,6 +69,18 @@ class AttentionBlock:
         q = F.head_norm_rope(q, None, self.nq, None, self.cos, self.sin, start=start)
         return x + self.join(F.window_attention(q, keys, values, window=self.window, sinks=self.sinks, key_lengths=key_lengths), batch)
 
+    def serve(self, x, cache, table, lengths):
+        """The new tokens of a batch, x [batch * tokens, width], over a paged cache that they are appended to; `lengths` [batch] are
+        the sequences' tokens with the new ones."""
+        batch = len(lengths)
+        tokens = x.shape[0] // batch
+        # The tables' rows of the new tokens' places; padding in front of a sequence stands at 0.
+        places = np.maximum(np.asarray(lengths)[:, None] - tokens + np.arange(tokens), 0)
+        q, k, v = (self._heads(x @ w, batch, n) for w, n in ((self.wq, self.heads), (self.wk, self.kv_heads), (self.wv, self.kv_heads)))
+        q, k = F.head_norm_rope(q, k, self.nq, self.nk, self.cos, self.sin, positions=places)
+        F.paged_append(cache, table, lengths, k, v)
+        return x + self.join(F.paged_attention(q, cache, table, lengths, window=self.window, sinks=self.sinks), batch)
+
 
 def main() -> int:
     ap = argparse.ArgumentParser(description=__doc__.split("\n\n")[0])
@@ -92,7 +105,15 @@ def main() -> int:
         whole = block(X, 1).numpy()
         _, keys, values = block.project(X, 1)
         last = block.token(torch_rs.tensor(x[-1:], device="cuda"), keys, values, a.tokens - 1).numpy()
-    print(f"last token alone against the whole prompt: {abs(last[0] - whole[-1]).max():.2e} apart")
+        # The same from a cache of pages: all but the last token as a prompt, then that one.
+        page = 16
+        count = -(-a.tokens // page)
+        cache = F.paged_cache(count, block.kv_heads, page, block.dim)
+        table = np.random.default_rng(2).permutation(count)[None]
+        if a.tokens > 1:
+            block.serve(torch_rs.tensor(x[:-1], device="cuda"), cache, table, [a.tokens - 1])
+        paged = block.serve(torch_rs.tensor(x[-1:], device="cuda"), cache, table, [a.tokens]).numpy()
+    print(f"last token alone against the whole prompt: {abs(last[0] - whole[-1]).max():.2e} apart, from a paged cache {abs(paged[0] - whole[-1]).max():.2e}")
     return 0
 
 
