@@ -12,7 +12,9 @@ namespace trs {
 constexpr int64_t kMaxPagedTokens = (int64_t)1 << 29;  // of a sequence
 
 struct PoolView {  // [page, key head, token of the page], unit stride along dim
-    int64_t p, h, s;
+    int64_t h;
+    uint32_t p, s;
+    __device__ __forceinline__ uint64_t at(int page, int slot) const { return (uint64_t)(uint32_t)page * p + (uint64_t)(uint32_t)slot * s; }
 };
 
 // The cache as kernels see it.
@@ -45,6 +47,8 @@ inline int check_cache(const trs_paged_cache *c, int64_t batch, Pages *out) {
         for (int d = 0; d < 4; d++)
             if (l->shape[d] != c->lk.shape[d]) return set_error(TRS_E_SHAPE_MISMATCH, "key pages and value pages differ in dim %d", d);
         if (l->shape[3] > 1 && l->stride[3] != 1) return set_error(TRS_E_INVALID_ARGUMENT, "%s need a unit stride along their last dim", names[i]);
+        if (l->stride[0] > INT32_MAX || l->stride[2] > INT32_MAX)
+            return set_error(TRS_E_INDEX_OVERFLOW, "%s have a stride of 2^31 entries or more from page to page or token to token", names[i]);
         if (layout_numel(l) > 0 && !(i ? c->v : c->k)) return set_error(TRS_E_INVALID_ARGUMENT, "%s are null", names[i]);
     }
     const int64_t pages = c->lk.shape[0], page = c->lk.shape[2];
@@ -58,8 +62,8 @@ inline int check_cache(const trs_paged_cache *c, int64_t batch, Pages *out) {
     const int size = page_bytes(c);
     out->k = c->k ? (char *)c->k + c->lk.offset * size : nullptr;
     out->v = c->v ? (char *)c->v + c->lv.offset * size : nullptr;
-    out->ks = {c->lk.stride[0], c->lk.stride[1], c->lk.stride[2]};
-    out->vs = {c->lv.stride[0], c->lv.stride[1], c->lv.stride[2]};
+    out->ks = {c->lk.stride[1], (uint32_t)c->lk.stride[0], (uint32_t)c->lk.stride[2]};
+    out->vs = {c->lv.stride[1], (uint32_t)c->lv.stride[0], (uint32_t)c->lv.stride[2]};
     out->table = c->table, out->lengths = c->lengths;
     out->pages = (int32_t)pages, out->page = (int32_t)page, out->width = (int32_t)c->table_width;
     out->capacity = (int32_t)(page * c->table_width);

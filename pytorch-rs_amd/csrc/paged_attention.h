@@ -70,6 +70,26 @@ struct PagedKeys {
     __device__ __forceinline__ int first_key(int t) const { return (t < sink_tiles ? sink_first + t : first + t - sink_tiles) << SHIFT; }
 };
 
+// Pair i of a fragment's four, finite values: split_pair's pieces, the remainder behind each rounding by
+// one dot product with (-1, 0) or (0, -1), which is exact (compared bit for bit with the subtraction on
+// 2^22 pairs each of close, distant, subnormal, large and zero values), where the subtraction has to
+// widen the piece first: 7 instructions a pair, not 11.  The constants come from registers: as literals the
+// compiler takes them for the inline constant -1, which stands in both halves.
+__device__ __forceinline__ void split_weights(Splitting &x, int i, float a, float b) {
+    uint32_t low, high;
+    asm("s_mov_b32 %0, 0xbf80" : "=s"(low));
+    asm("s_mov_b32 %0, 0xbf800000" : "=s"(high));
+    const auto pack = [](float u, float v) { return __builtin_convertvector((gt_f2){u, v}, gt_bf2); };
+    const gt_bf2 first = __builtin_bit_cast(gt_bf2, low), second = __builtin_bit_cast(gt_bf2, high);
+    const gt_bf2 h = pack(a, b);
+    a = __builtin_amdgcn_fdot2_f32_bf16(h, first, a, false);
+    b = __builtin_amdgcn_fdot2_f32_bf16(h, second, b, false);
+    const gt_bf2 m = pack(a, b);
+    a = __builtin_amdgcn_fdot2_f32_bf16(m, first, a, false);
+    b = __builtin_amdgcn_fdot2_f32_bf16(m, second, b, false);
+    x.h[i] = __builtin_bit_cast(uint32_t, h), x.m[i] = __builtin_bit_cast(uint32_t, m), x.l[i] = __builtin_bit_cast(uint32_t, pack(a, b));
+}
+
 // What is the same in all lanes, where the compiler cannot tell: to scalar registers.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ int64_t uniform(int64_t x) { return (int64_t)(uint32_t)uniform((int)x) | (int64_t)uniform((int)(x >> 32)) << 32; }

@@ -141,7 +141,7 @@ struct Bf16Pages {
     __device__ __forceinline__ void add(at_f4 (&acc)[kTiles], const at_f4 (&p)[2]) const {
         Splitting w;
 #pragma unroll
-        for (int i = 0; i < 4; i++) w.pair(i, p[i >> 1][2 * (i & 1)], p[i >> 1][2 * (i & 1) + 1]);
+        for (int i = 0; i < 4; i++) split_weights(w, i, p[i >> 1][2 * (i & 1)], p[i >> 1][2 * (i & 1) + 1]);
         const Pieces x = w.done();
 #pragma unroll
         for (int u = 0; u < VU; u++)
@@ -211,7 +211,7 @@ struct Places {
 
     // The page and the token of it that a key stands in; past the last key that is read, that one's.  (An
     // entry that sees nothing has a tile none of whose keys is seen: any key that there is will do.)
-    __device__ __forceinline__ static bool find(const PagedArgs &a, int first_row_to, int owner, int j, int last, int64_t &page, int &slot) {
+    __device__ __forceinline__ static bool find(const PagedArgs &a, int first_row_to, int owner, int j, int last, int &page, int &slot) {
         const int at = max(min(j, last), 0), id = a.pages.page_of(at < first_row_to ? 0 : owner, at);
         const bool held = a.pages.holds(id);
         page = held ? id : 0, slot = a.pages.slot_of(at);
@@ -224,33 +224,33 @@ struct Places {
 #pragma unroll
             for (int h = 0; h < T::kHalves; h++) {
                 const int at = max(min(j0 + 16 * h, end & ~15), 0);
-                int64_t page;
+                int page;
                 int slot;
                 if (!find(a, first_row_to, owner, at, end, page, slot)) absent |= 1u << h;
-                k[h] = kb + page * a.pages.ks.p + slot * a.pages.ks.s;
-                v[h] = vb + page * a.pages.vs.p + slot * a.pages.vs.s;
+                k[h] = kb + a.pages.ks.at(page, slot);
+                v[h] = vb + a.pages.vs.at(page, slot);
                 last[h] = max(min(end - at, 15), 0);
             }
         }
     }
     __device__ __forceinline__ const E *k_row(const PagedArgs &a, int first_row_to, const E *kb, int h, int n) const {
-        if constexpr (ONE) return k[h] + (int64_t)min(n, last[h]) * a.pages.ks.s;
-        int64_t page;
+        if constexpr (ONE) return k[h] + (uint64_t)(uint32_t)min(n, last[h]) * a.pages.ks.s;
+        int page;
         int slot;
         find(a, first_row_to, owner, j0 + 16 * h + n, end, page, slot);
-        return kb + page * a.pages.ks.p + slot * a.pages.ks.s;
+        return kb + a.pages.ks.at(page, slot);
     }
     __device__ __forceinline__ const E *v_row(const PagedArgs &a, int first_row_to, const E *vb, int h, int n) const {
-        if constexpr (ONE) return v[h] + (int64_t)min(n, last[h]) * a.pages.vs.s;
-        int64_t page;
+        if constexpr (ONE) return v[h] + (uint64_t)(uint32_t)min(n, last[h]) * a.pages.vs.s;
+        int page;
         int slot;
         find(a, first_row_to, owner, j0 + 16 * h + n, end, page, slot);
-        return vb + page * a.pages.vs.p + slot * a.pages.vs.s;
+        return vb + a.pages.vs.at(page, slot);
     }
     // Whether the pool has the page of key n of half h.
     __device__ __forceinline__ bool held(const PagedArgs &a, int first_row_to, int h, int n) const {
         if constexpr (ONE) return !(absent >> h & 1);
-        int64_t page;
+        int page;
         int slot;
         return find(a, first_row_to, owner, j0 + 16 * h + n, end, page, slot);
     }
@@ -312,10 +312,10 @@ __device__ __forceinline__ void few_rows(const PagedArgs &a, const PagedStage &s
 #pragma unroll 1
             for (int x = 0; x < 16 * H; x++) {
                 const int j = now.keys.first_key(t) + x;
-                int64_t page;
+                int page;
                 int slot;
                 const bool held = P::find(a, first_row_to, now.owner, j, now.keys.last, page, slot);
-                const E *kp = kb + page * a.pages.ks.p + slot * a.pages.ks.s, *vp = vb + page * a.pages.vs.p + slot * a.pages.vs.s;
+                const E *kp = kb + a.pages.ks.at(page, slot), *vp = vb + a.pages.vs.at(page, slot);
                 float y = 0.f;
                 for (int c = quarter; c < a.D; c += 4) y += q[c] * a.scale2 * to_float(kp[c]);
                 y += __shfl_xor(y, 16);

@@ -157,9 +157,8 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_rows(PagedArgs a, int stage)
             const auto load = [&](int t, int id) {
                 const bool held = a.pages.holds(id);
                 missing = (uint32_t)__builtin_amdgcn_ballot_w64(!held);
-                const int64_t page = held ? id : 0;
-                const int slot = a.pages.slot_of(key_at(t));
-                const E *kp = kb + page * a.pages.ks.p + slot * a.pages.ks.s, *vp = vb + page * a.pages.vs.p + slot * a.pages.vs.s;
+                const int page = held ? id : 0, slot = a.pages.slot_of(key_at(t));
+                const E *kp = kb + a.pages.ks.at(page, slot), *vp = vb + a.pages.vs.at(page, slot);
 #pragma unroll
                 for (int q = 0; q < OWN; q++) {
                     const bool key = unit(q) < UNITS / 2;
@@ -245,7 +244,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_rows(PagedArgs a, int stage)
                     for (int n = 0; n < 2; n++) {
                         Splitting p;
 #pragma unroll
-                        for (int i = 0; i < 4; i++) p.pair(i, x[8 * n + 2 * i], x[8 * n + 2 * i + 1]);
+                        for (int i = 0; i < 4; i++) split_weights(p, i, x[8 * n + 2 * i], x[8 * n + 2 * i + 1]);
                         const Pieces y = p.done();
 #pragma unroll
                         for (int c = 0; c < NT; c++) {
@@ -270,9 +269,8 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_rows(PagedArgs a, int stage)
                     for (int k = 0; k < 32; k++) {
                         const int j = keys.first_key(t) + k, at = min(j, keys.last), page_id = page_at(at);
                         const bool held = a.pages.holds(page_id);
-                        const int64_t page = held ? page_id : 0;
-                        const int slot = a.pages.slot_of(at);
-                        const E *kp = kb + page * a.pages.ks.p + slot * a.pages.ks.s, *vp = vb + page * a.pages.vs.p + slot * a.pages.vs.s;
+                        const int page = held ? page_id : 0, slot = a.pages.slot_of(at);
+                        const E *kp = kb + a.pages.ks.at(page, slot), *vp = vb + a.pages.vs.at(page, slot);
                         float y = 0.f;
                         for (int c = half; c < a.D; c += 2) y += qp[c] * a.scale2 * as_float(kp[c]);
                         y += __shfl_xor(y, 32);

@@ -287,7 +287,7 @@ void to_rows(RopeJob &j, float *y, const trs_layout *lo) {
 }
 void to_pages(RopeJob &j, void *pool, const PoolView &v) {
     j.y = pool, j.paged = 1;
-    j.ys[0] = v.p, j.ys[1] = v.h, j.ys[2] = v.s, j.ys[3] = 1;
+    j.ys[0] = (int64_t)v.p, j.ys[1] = v.h, j.ys[2] = (int64_t)v.s, j.ys[3] = 1;
 }
 
 // Launches the jobs that have elements.
