@@ -96,6 +96,8 @@ PagedStage plan_stage(const PagedArgs &a, bool together, int from, int to, int c
     s.row_tiles = (int32_t)((rows + s.tile_rows - 1) / s.tile_rows);
     s.entries = (int32_t)(together ? s.row_tiles : (int64_t)s.row_tiles * a.batch);
     if (s.tile_rows == kFewTile) {
+        // Two waves a SIMD.  Least tiles of a wave 1, 2, 4 and 8, us: 500 keys, 8 heads of 64, bfloat16 13.3, 14.2, 16.6 and 22.2,
+        // 4000, 8 of 128 25.0, 21.3, 21.7 and 27.1, 8 sequences of 1000 21.9, 19.0, 20.4 and 27.4.
         s.least = 2;
         s.workers = std::max(1, 8 * cu_count / a.kv_heads);
     } else {

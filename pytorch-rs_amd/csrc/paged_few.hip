@@ -1,9 +1,12 @@
 // paged_few.hip -- attention over a cache in pages for few rows: single tokens of a batch.
 //
-// Bound by reading the keys and values once.  A wave takes 16 rows and streams its share
-// of the keys straight from the pages into the registers that the matrix instructions take
-// them from: no LDS, no barrier, nothing that waits for another wave.  What several waves have
-// of an entry is joined by a second launch.
+// Bound by reading the keys and values once: 32 sequences of 1640 to 8192 tokens, 8 key heads of 128,
+// bfloat16 (645 MB) 120-125 us, of which the tiles' loop reads at 6.7 TB/s and 4 us are the way to the first
+// load; 9 us for one sequence of 1000 tokens, 8 heads of 64, float32.  A wave takes 16 rows and streams its
+// share of the keys straight from the pages into the registers that the matrix instructions take
+// them from: no LDS, no barrier, nothing that waits for another wave.  (Blocks of four waves that join
+// in LDS, two blocks a CU: a batch of 64 with 60 to 512 tokens of its own 38 us, 24 so.)  What several
+// waves have of an entry is joined by a second launch, 5 us of which most is the launch.
 //
 // float32 pages: tiles of 16 keys on v_mfma_f32_16x16x4_f32, as attention_wide.h has them.
 // bfloat16 pages: tiles of 32 keys on v_mfma_f32_16x16x32_bf16.  A key is an operand as it
@@ -198,8 +201,11 @@ struct Step {
     }
 };
 
-// ONE: pages hold a multiple of 16 tokens, and no 16 keys are the first sequence's in part, so that a
-// half's keys stand in one page, and its entry of the table is read by the scalar unit.
+// Where a tile's keys stand.  ONE: pages hold a multiple of 16 tokens, and no 16 keys are the first
+// sequence's in part, so that a half's keys stand in one page, and its entry of the table is read by the
+// scalar unit.  Else every lane looks one key up and the others ask it (32 sequences of 2000 tokens, 8 key
+// heads of 128, bfloat16: pages of 16 so 54.2 us, of 8 the other way 56.0; a look-up of its own for every row a
+// lane reads takes 83).
 template <class T, bool ONE>
 struct Places {
     using E = typename T::E;
@@ -207,52 +213,46 @@ struct Places {
     int last[T::kHalves];                    // ONE: its last key that is read
     uint32_t absent;                         // ONE: halves whose page the pool does not have
 
-    int owner, j0, end;  // else: the sequence, the tile's first key and the last one that is read
+    int id, slot;  // else: the page and the token of it of key `lane` of the tile (of 16 or 32)
 
     // The page and the token of it that a key stands in; past the last key that is read, that one's.  (An
     // entry that sees nothing has a tile none of whose keys is seen: any key that there is will do.)
-    __device__ __forceinline__ static bool find(const PagedArgs &a, int first_row_to, int owner, int j, int last, int &page, int &slot) {
-        const int at = max(min(j, last), 0), id = a.pages.page_of(at < first_row_to ? 0 : owner, at);
-        const bool held = a.pages.holds(id);
-        page = held ? id : 0, slot = a.pages.slot_of(at);
-        return held;
+    __device__ __forceinline__ static int find(const PagedArgs &a, int first_row_to, int owner, int j, int last, int &slot) {
+        const int at = max(min(j, last), 0);
+        slot = a.pages.slot_of(at);
+        return a.pages.page_of(at < first_row_to ? 0 : owner, at);
     }
-    __device__ __forceinline__ Places(const PagedArgs &a, int first_row_to, const E *kb, const E *vb, const Step<T::kShift> &x) {
-        j0 = x.keys.first_key(x.t), owner = x.owner, end = x.keys.last;
+    __device__ __forceinline__ Places(const PagedArgs &a, int first_row_to, const E *kb, const E *vb, const Step<T::kShift> &x, int lane) {
+        const int j0 = x.keys.first_key(x.t), end = x.keys.last;
         if constexpr (ONE) {
             absent = 0;
 #pragma unroll
             for (int h = 0; h < T::kHalves; h++) {
-                const int at = max(min(j0 + 16 * h, end & ~15), 0);
-                int page;
-                int slot;
-                if (!find(a, first_row_to, owner, at, end, page, slot)) absent |= 1u << h;
+                const int at = max(min(j0 + 16 * h, end & ~15), 0), there = find(a, first_row_to, x.owner, at, end, slot);
+                if (!a.pages.holds(there)) absent |= 1u << h;
+                const int page = a.pages.holds(there) ? there : 0;
                 k[h] = kb + a.pages.ks.at(page, slot);
                 v[h] = vb + a.pages.vs.at(page, slot);
                 last[h] = max(min(end - at, 15), 0);
             }
+        } else {
+            id = find(a, first_row_to, x.owner, j0 + (lane & (16 * T::kHalves - 1)), end, slot);
         }
     }
-    __device__ __forceinline__ const E *k_row(const PagedArgs &a, int first_row_to, const E *kb, int h, int n) const {
+    __device__ __forceinline__ const E *k_row(const PagedArgs &a, const E *kb, int h, int n) const {
         if constexpr (ONE) return k[h] + (uint64_t)(uint32_t)min(n, last[h]) * a.pages.ks.s;
-        int page;
-        int slot;
-        find(a, first_row_to, owner, j0 + 16 * h + n, end, page, slot);
-        return kb + a.pages.ks.at(page, slot);
+        const int page = __shfl(id, 16 * h + n);
+        return kb + a.pages.ks.at(a.pages.holds(page) ? page : 0, __shfl(slot, 16 * h + n));
     }
-    __device__ __forceinline__ const E *v_row(const PagedArgs &a, int first_row_to, const E *vb, int h, int n) const {
+    __device__ __forceinline__ const E *v_row(const PagedArgs &a, const E *vb, int h, int n) const {
         if constexpr (ONE) return v[h] + (uint64_t)(uint32_t)min(n, last[h]) * a.pages.vs.s;
-        int page;
-        int slot;
-        find(a, first_row_to, owner, j0 + 16 * h + n, end, page, slot);
-        return vb + a.pages.vs.at(page, slot);
+        const int page = __shfl(id, 16 * h + n);
+        return vb + a.pages.vs.at(a.pages.holds(page) ? page : 0, __shfl(slot, 16 * h + n));
     }
     // Whether the pool has the page of key n of half h.
-    __device__ __forceinline__ bool held(const PagedArgs &a, int first_row_to, int h, int n) const {
+    __device__ __forceinline__ bool held(const PagedArgs &a, int h, int n) const {
         if constexpr (ONE) return !(absent >> h & 1);
-        int page;
-        int slot;
-        return find(a, first_row_to, owner, j0 + 16 * h + n, end, page, slot);
+        return a.pages.holds(__shfl(id, 16 * h + n));
     }
 };
 
@@ -280,9 +280,9 @@ __device__ __forceinline__ void few_rows(const PagedArgs &a, const PagedStage &s
     };
     using P = Places<T, ONE>;
     T ops;
-    P here(a, first_row_to, kb, vb, now);
-    const auto load_k = [&](const P &p) { ops.load_k([&](int h, int n) { return p.k_row(a, first_row_to, kb, h, n); }, a.D, col, quarter); };
-    const auto load_v = [&](const P &p) { ops.load_v([&](int h, int n) { return p.v_row(a, first_row_to, vb, h, n); }, a.D, col, quarter); };
+    P here(a, first_row_to, kb, vb, now, lane);
+    const auto load_k = [&](const P &p) { ops.load_k([&](int h, int n) { return p.k_row(a, kb, h, n); }, a.D, col, quarter); };
+    const auto load_v = [&](const P &p) { ops.load_v([&](int h, int n) { return p.v_row(a, vb, h, n); }, a.D, col, quarter); };
     load_k(here);
     load_v(here);
     int place = 0;
@@ -293,7 +293,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs &a, const PagedStage &s
     };
     load_q();
     advance();
-    P next(a, first_row_to, kb, vb, ahead);
+    P next(a, first_row_to, kb, vb, ahead, lane);
 
     at_f4 acc[T::kTiles];
     float most, sum;
@@ -312,9 +312,10 @@ __device__ __forceinline__ void few_rows(const PagedArgs &a, const PagedStage &s
 #pragma unroll 1
             for (int x = 0; x < 16 * H; x++) {
                 const int j = now.keys.first_key(t) + x;
-                int page;
                 int slot;
-                const bool held = P::find(a, first_row_to, now.owner, j, now.keys.last, page, slot);
+                const int id = P::find(a, first_row_to, now.owner, j, now.keys.last, slot);
+                const bool held = a.pages.holds(id);
+                const int page = held ? id : 0;
                 const E *kp = kb + a.pages.ks.at(page, slot), *vp = vb + a.pages.vs.at(page, slot);
                 float y = 0.f;
                 for (int c = quarter; c < a.D; c += 4) y += q[c] * a.scale2 * to_float(kp[c]);
@@ -384,7 +385,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs &a, const PagedStage &s
                 const int n = 4 * quarter + e;
                 const uint32_t bits = __float_as_uint(x[h][e]);
                 lowest = lowest > bits ? lowest : bits;
-                const float y = here.held(a, first_row_to, h, n) ? x[h][e] * T::kDownScale : __builtin_nanf("");
+                const float y = here.held(a, h, n) ? x[h][e] * T::kDownScale : __builtin_nanf("");
                 x[h][e] = paged_sees(a, s, place, j0 + 16 * h + n) ? y : -__builtin_inff();
                 m = __builtin_fmaxf(m, x[h][e]);
             }
@@ -417,7 +418,7 @@ __device__ __forceinline__ void few_rows(const PagedArgs &a, const PagedStage &s
         }
         here = next;
         advance();
-        next = P(a, first_row_to, kb, vb, ahead);
+        next = P(a, first_row_to, kb, vb, ahead, lane);
     }
 }
 

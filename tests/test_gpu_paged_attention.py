@@ -92,6 +92,10 @@ MANY = [
     (40, 8, 2, 30, 128, 16, [1000 - 20 * i for i in range(40)], EVERY, 0),  # 120 rows a sequence
     (4, 16, 2, 300, 64, 16, [0, 1000, 299, 5], EVERY, 0),
     (1, 5, 1, 1200, 128, 16, [1500], 1, 0),          # each query sees itself alone
+    (2, 8, 2, 700, 256, 16, [1000, 1600], EVERY, 0),
+    (1, 8, 2, 1000, 200, 16, [1300], 400, 3),
+    (1, 16, 4, 800, 150, 24, [900], EVERY, 0),
+    (1, 8, 2, 1100, 137, 10, [1200], 500, 0),
 ]
 
 
@@ -135,6 +139,7 @@ TOGETHER = [
     (33, 8, 2, 8, 128, 16, [4200 + 3 * i for i in range(33)], 4096, 3000, 5),
     (20, 8, 4, 40, 48, 16, [1600 - 20 * i for i in range(20)], 1330, EVERY, 0),
     (20, 8, 4, 100, 32, 16, [1900 + i for i in range(20)], 1330, EVERY, 0),                # many rows of both kinds
+    (12, 16, 2, 24, 256, 16, [2000 - i for i in range(12)], 1900, EVERY, 0),
     (24, 16, 2, 12, 96, 24, [2100] * 24, 2100, EVERY, 0),                                  # nothing of their own
     (34, 8, 2, 8, 20, 16, [4300 - 100 * i for i in range(34)], 4100, 2000, 40),
 ]
