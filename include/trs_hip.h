@@ -464,10 +464,11 @@ int trs_rope_axes_f32(int n, const float *const *x, const trs_layout *lx, const 
  * the page, dim], of float32 or bfloat16, with any strides but a unit one along dim
  * (one buffer may hold both).  table [batch, table_width] and lengths [batch] are int32
  * on the device, contiguous: token t of sequence b stands in page
- * table[b][t / tokens a page] at t % tokens a page, and lengths[b], taken into
- * [0, table_width * tokens a page], is the number of tokens that the sequence has, the
- * ones that a call brings among them.  Entries of the table for tokens that a call
- * neither writes nor sees are not looked at. */
+ * table[b][t / tokens a page] at t % tokens a page, and lengths[b] is the number of
+ * tokens that the sequence has, the ones that a call brings among them; one below 0
+ * counts as 0.  Entries of the table for tokens that a call neither writes nor sees are
+ * not looked at.  A row of the table holds at most 2^29 tokens, and strides from page to page
+ * and from token to token are below 2^31 entries (TRS_E_INDEX_OVERFLOW). */
 typedef struct trs_paged_cache {
     void *k, *v;
     trs_layout lk, lv;
@@ -482,7 +483,7 @@ typedef struct trs_paged_cache {
  * their pages, the keys turned on the way as trs_rope_axes_f32 turns them; with q
  * [batch, head, T, dim], its turned queries go to q_out in the same launch (q null: none).
  * Token t of sequence b stands at place lengths[b] - T + t; one before place 0 is
- * padding, of which nothing is written.  positions as above, or null for the place
+ * padding, and neither it nor one behind the last place of the table's row is written.  positions as above, or null for the place
  * itself on every axis (a padding query turns as at place 0); a pair whose position the
  * tables do not hold is NaN.  cos, sin and ltab null: nothing is turned.  Values go to
  * bfloat16 pages rounded to the nearest, ties to even.  A token whose entry of the table
@@ -496,8 +497,9 @@ int trs_paged_append_f32(const trs_paged_cache *cache, const float *k, const trs
                          int interleaved, int axes, const uint8_t *pair_axis, const int32_t *positions);
 
 /* trs_window_attention_f32 over a paged cache: q [batch, heads, Sq, dim], dim at most
- * 256, head h reads key head h / (heads / key heads).  Of a sequence of n tokens query i
- * stands at place p = n - Sq + i and sees key j where
+ * 256, head h reads key head h / (heads / key heads).  Of a sequence of n tokens (at most
+ * the table's: a greater length counts as those) query i stands at place p = n - Sq + i
+ * and sees key j where
  *     j <= p  and  (p - j < window  or  j < sinks).
  * A query that sees nothing (p < 0) gives 0 whatever it holds.  Keys j < shared of every
  * sequence are read through the table's first row, and their products are taken for
@@ -508,7 +510,10 @@ int trs_paged_append_f32(const trs_paged_cache *cache, const float *k, const trs
  * it.  window >= 1 (INT64_MAX: no window); sinks >= 0.  lse (or null) receives
  * log(sum(exp(scale q k))) as [batch, heads, Sq], -inf where nothing is seen.  Sums are
  * fp32 and their order is fixed; products as in trs_window_attention_f32, with a
- * bfloat16 key or value as it stands.  q may have any strides (one with no unit stride
+ * bfloat16 key or value as it stands.  Parts of long sequences go through a workspace
+ * from the block cache, of at most 2 parts a wave that the device holds of 16 rows, or a
+ * block of 256, and one more for every tile of rows where keys are shared; where it has
+ * none nothing is split.  q may have any strides (one with no unit stride
  * along dim is copied first, into the block cache); out needs a unit stride along dim and
  * shares no memory with anything else.  There is no gradient: trs_window_attention_f32
  * has one. */

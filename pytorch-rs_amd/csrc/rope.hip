@@ -49,15 +49,15 @@ struct RopeArgs {
 
 // A lane's token: where it stands in its sequence and in the pools.
 struct Token {
-    int place;     // below 0: padding
+    int place;     // below 0: padding; from the table's tokens on: no place
     int id, slot;  // its page; id < 0: nothing is to be written
 };
 
 __device__ __forceinline__ Token token_of(const RopeArgs &a, int b, int t) {
     Token k = {t, -1, 0};
     if (!a.appends) return k;
-    k.place = a.pages.keys_of(b) - a.tokens + t;
-    if (k.place < 0) return k;
+    k.place = max(a.pages.lengths[b], 0) - a.tokens + t;
+    if (k.place < 0 || k.place >= a.pages.capacity) return k;
     const int id = a.pages.page_of(b, k.place);
     k.id = a.pages.holds(id) ? id : -1;
     k.slot = a.pages.slot_of(k.place);
@@ -117,6 +117,7 @@ __device__ __forceinline__ Angles angles_of(const RopeArgs &a, int b, int t, con
     return g;
 }
 
+// The one rounding on the way to bfloat16 pages, of the turned fp32 value, to the nearest, ties to even.
 typedef uint32_t u2u __attribute__((ext_vector_type(2), aligned(2)));
 __device__ __forceinline__ uint32_t to_bf16(float x, float y) {
     typedef float F2 __attribute__((ext_vector_type(2)));

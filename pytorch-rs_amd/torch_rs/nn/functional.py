@@ -374,7 +374,8 @@ def paged_append(cache, table, lengths, key, value, cos=None, sin=None, *, query
 
     ``lengths`` ([batch]) are the tokens that each sequence has with the new ones: token t
     stands at place ``lengths - tokens + t``, which is also its position on every axis
-    where ``positions`` is None.  Tokens before place 0 are padding and are not written.
+    where ``positions`` is None.  Tokens before place 0 are padding; neither they nor tokens
+    behind the last place of the table's row are written.
     Records no gradient."""
     _tensor_arguments("paged_append", key=key, value=value)
     if (cos is None) != (sin is None):

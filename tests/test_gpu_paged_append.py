@@ -31,7 +31,7 @@ def run(B, HK, T, D, page, lengths, kind=F32, form="heads", pairs=None, axes=1, 
     old = cache.fetch()
     memory = [h.copy() for h in cache.host]
     capacity = cache.table.shape[1] * page
-    n = [min(max(x, 0), capacity) for x in lengths]
+    n = [max(x, 0) for x in lengths]
     place = np.array([[n[b] - T + t for t in range(T)] for b in range(B)]).reshape(B, T)
     at = np.broadcast_to(np.maximum(place, 0), (axes, B, T)) if positions is None else positions
     pairs = D // 2 if pairs is None else pairs
@@ -51,7 +51,7 @@ def run(B, HK, T, D, page, lengths, kind=F32, form="heads", pairs=None, axes=1, 
     for b in range(B):
         for t in range(T):
             p = place[b, t]
-            if p < 0:
+            if not 0 <= p < capacity:
                 continue
             page_id = cache.table[b, p // page]
             if not 0 <= page_id < cache.shape[0]:
@@ -110,6 +110,9 @@ def test_pools_and_inputs_of_any_order(form, kind, order):
 def test_padding_lengths_beyond_the_table_and_bad_pages(kind, D):
     # Sequences shorter than the call's tokens, none at all, a negative length, and one beyond the table's row.
     run(5, 2, 6, D, 4, [3, 0, -5, 1000, 6], kind, query=2, width=4)
+    # Tokens of which the table's row holds some, or just all, and a full row, which keeps what it has.
+    run(4, 2, 6, D, 4, [18, 16, 17, 2 ** 31 - 1], kind, width=4, pairs=0)
+    run(2, 2, 1, D, 4, [16, 17], kind, query=2, width=4)
 
     def damage(cache):  # pages that the pool does not have
         cache.table[0, 1], cache.table[1, 0], cache.table[1, 2] = cache.shape[0], -7, 2 ** 31 - 1

@@ -1,6 +1,6 @@
 """The paged cache as a model uses it: prompts and tokens appended, then read, through
-torch_rs and as consecutive calls, with prefixes that sequences share, on captured
-work and beside other calls."""
+torch_rs and as consecutive calls, with prefixes that sequences share, and beside
+other calls."""
 import ctypes
 import sys
 from pathlib import Path

@@ -53,6 +53,8 @@ def test_caches_that_are_refused(call, batch):
     assert call(cache(lk=lay((4, 2, 16, 8), (256, 128, 8, 2)))) == E
     assert call(cache(lk=lay((1 << 32, 2, 16, 8), (0, 0, 8, 1)), lv=lay((1 << 32, 2, 16, 8), (0, 0, 8, 1)))) == O
     assert call(cache(dim=9)) == M
+    for strides in ((1 << 31, 128, 8, 1), (256, 128, 1 << 31, 1)):
+        assert call(cache(lk=lay((4, 2, 16, 8), strides))) == O and call(cache(lv=lay((4, 2, 16, 8), strides))) == O
 
 
 def test_appending_refuses_before_it_looks_for_a_device():
