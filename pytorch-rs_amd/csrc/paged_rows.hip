@@ -8,12 +8,12 @@
 // O^T += V^T P^T as it stands.
 //
 // Bound by the card's power and by issue: 1024 tokens of two prompts over 4096, 32 heads of 128 over 8,
-// bfloat16, 310 us in the loop's passes, 1.16 PFLOP/s of bf16 products (a library product of 8192^3 reaches 1.25 on
+// bfloat16, 305-312 us, 1.16-1.19 PFLOP/s of bf16 products (a library product of 8192^3 reaches 1.25 on
 // the same card): the matrix cores are busy for half the cycles at a clock of 2.0 GHz of 2.4, and 5.5 other vector
 // instructions a matrix instruction take 35%.  Fragments read one step ahead of their products gave 376 -> 355.
 // Waves of a SIMD held in opposite phases, one multiplying while the other works out weights, took 373, blocks
 // of 128 rows, one for every tile of rows and no parts, 351 (a block brings every tile for half the rows).  The
-// same for float32 pages 590.
+// same for float32 pages 600.
 //
 // float32 pages: three bf16 pieces a float on both sides, six
 // products (attention.h).  bfloat16 pages: keys and values as they are, queries and weights in
