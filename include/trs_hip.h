@@ -513,8 +513,10 @@ int trs_paged_append_f32(const trs_paged_cache *cache, const float *k, const trs
  * bfloat16 key or value as it stands.  Parts of long sequences go through a workspace
  * from the block cache, of at most 2 parts a wave that the device holds of 16 rows, or a
  * block of 256, and one more for every tile of rows where keys are shared; where it has
- * none nothing is split.  q may have any strides (one with no unit stride
- * along dim is copied first, into the block cache); out needs a unit stride along dim and
+ * none nothing is split.  Calls that are captured into graphs on the library's stream
+ * share a workspace that is kept for them (replay them on that stream, one after another;
+ * lengths, table and tensors are read at each replay).  q may have any strides (one with no unit
+ * stride along dim is copied first, into the block cache; not in a captured call); out needs a unit stride along dim and
  * shares no memory with anything else.  There is no gradient: trs_window_attention_f32
  * has one. */
 int trs_paged_attention_f32(const float *q, const trs_layout *lq, const trs_paged_cache *cache, int64_t shared,

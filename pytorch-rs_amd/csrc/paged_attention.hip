@@ -110,8 +110,29 @@ PagedStage plan_stage(const PagedArgs &a, bool together, int from, int to, int c
     return s;
 }
 
-// Whether the stages have memory for parts; the parts are for speed alone.
-int take_parts(PagedArgs &a, void **ws) {
+// Whether the stream's work is being captured into a graph.
+int is_captured(DeviceState *dev, bool *captured) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    TRS_HIP_CHECK(hipStreamIsCapturing(dev->stream, &status), "hipStreamIsCapturing");
+    *captured = status != hipStreamCaptureStatusNone;
+    return TRS_OK;
+}
+
+// A workspace that captured calls share: their replays follow one another on the library's stream.  A
+// larger one leaves the smaller to the graphs that have it.
+int graph_workspace(DeviceState *dev, size_t bytes, void **ws) {
+    std::lock_guard<std::mutex> lock(dev->graph_mu);
+    if (bytes > dev->graph_parts_bytes) {
+        void *more = nullptr;
+        TRS_CHECK(trs_alloc(bytes, &more));
+        dev->graph_parts = more, dev->graph_parts_bytes = bytes;
+    }
+    *ws = dev->graph_parts;
+    return TRS_OK;
+}
+
+// Memory for the stages' parts.
+int take_parts(PagedArgs &a, DeviceState *dev, bool captured, void **ws) {
     size_t floats = 0, found = 0;
     for (int i = 0; i < a.stages; i++) {
         PagedStage &s = a.stage[i];
@@ -119,7 +140,8 @@ int take_parts(PagedArgs &a, void **ws) {
         floats += (size_t)(a.kv_heads * s.slots * s.tile_rows) * (size_t)(a.part_width + 2);
         found += (size_t)a.kv_heads * (size_t)s.entries;
     }
-    TRS_CHECK(trs_alloc(floats * sizeof(float) + found * sizeof(int2), ws));
+    const size_t bytes = floats * sizeof(float) + found * sizeof(int2);
+    TRS_CHECK(captured ? graph_workspace(dev, bytes, ws) : trs_alloc(bytes, ws));
     float *p = (float *)*ws;
     for (int i = 0; i < a.stages; i++) {
         PagedStage &s = a.stage[i];
@@ -135,7 +157,7 @@ int take_parts(PagedArgs &a, void **ws) {
     return TRS_OK;
 }
 
-int paged_forward(PagedArgs &a, bool bf16, DeviceState *dev) {
+int paged_forward(PagedArgs &a, bool bf16, DeviceState *dev, bool captured) {
     a.part_width = (a.D + 3) / 4 * 4;
     a.stages = 0;
     const int64_t saved = (int64_t)(a.batch - 1) * a.shared * a.kv_heads * a.D * (bf16 ? 4 : 8);
@@ -155,7 +177,7 @@ int paged_forward(PagedArgs &a, bool bf16, DeviceState *dev) {
     if (a.stages == 2 && (a.stage[0].workers == 0 || a.stage[1].workers == 0)) entry_each();
     void *ws = nullptr;
     if (a.stages && a.stage[0].workers) {
-        const int rc = take_parts(a, &ws);
+        const int rc = take_parts(a, dev, captured, &ws);
         if (rc == TRS_E_ALLOCATION_FAILED) entry_each();  // the parts are for speed alone
         else if (rc) return rc;
     }
@@ -177,7 +199,7 @@ int paged_forward(PagedArgs &a, bool bf16, DeviceState *dev) {
         TRS_LAUNCH_CHECK("paged attention join launch");
         return TRS_OK;
     };
-    const int rc = launch(), frc = ws ? trs_free(ws) : TRS_OK;
+    const int rc = launch(), frc = ws && !captured ? trs_free(ws) : TRS_OK;
     return rc ? rc : frc;
 }
 
@@ -220,6 +242,10 @@ int run_paged(const float *q, const trs_layout *lq, const trs_paged_cache *cache
     if (rows == 0) return TRS_OK;
     DeviceState *dev = device_state();
     if (!dev) return TRS_E_NO_DEVICE;
+    bool captured = false;
+    TRS_CHECK(is_captured(dev, &captured));
+    if (captured && D > 1 && lq->stride[3] != 1)
+        return set_error(TRS_E_INVALID_ARGUMENT, "query needs a unit stride along its last dim in a captured call");
     Dense dense;
     TRS_CHECK(dense.take(q, lq));
     a.q = dense.at, a.qs = dense.view;
@@ -231,7 +257,7 @@ int run_paged(const float *q, const trs_layout *lq, const trs_paged_cache *cache
     a.scale2 = scale * kLog2e;
     a.seq_rows = a.group * a.Sq;
     a.by_group = SmallDivisor((uint32_t)a.group);
-    return paged_forward(a, cache->type == TRS_PAGES_BF16, dev);
+    return paged_forward(a, cache->type == TRS_PAGES_BF16, dev, captured);
 }
 
 }  // namespace

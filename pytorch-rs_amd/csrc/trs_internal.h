@@ -45,6 +45,11 @@ struct DeviceState {
     std::multimap<size_t, void *> free_blocks;
     std::unordered_map<void *, size_t> live_blocks;
     size_t cached_bytes = 0;
+    // The workspace of attention calls that were captured into graphs, whose
+    // replays write to it long after the call: never handed to anything else.
+    std::mutex graph_mu;
+    void *graph_parts = nullptr;
+    size_t graph_parts_bytes = 0;
     // Two page-locked chunks that pipeline copies from or to pageable host
     // memory, each with the event of the last DMA that used it.
     std::mutex stage_mu;
