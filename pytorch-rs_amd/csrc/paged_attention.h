@@ -27,6 +27,7 @@ struct PagedStage {
     int32_t tile_rows;
     int32_t workers;     // of a key head; 0: one for every entry
     int32_t least;       // the least key tiles of a worker that has others beside it
+    int32_t most;        // the most key tiles of an entry
     SmallDivisor by_row_tiles;
     int64_t slots;       // of parts, a key head
     float *part_o, *part_ml;  // [key head][slot][row of the tile]: part_width floats, and (maximum, sum)

@@ -23,13 +23,24 @@ constexpr int64_t kFewPairs = 1 << 23;
 // 2 sequences over 1024 keys (4 MiB) 17.2 / 17.9 and 4096 (16 MiB) 25.7 / 22.9, 4 over 1024 (12 MiB) 17.8 / 17.9, 8 over 256 (7 MiB)
 // 16.3 / 17.3 and 1024 (28 MiB) 21.3 / 18.5; float32, 4 over 1024 (24 MiB) 24.0 / 20.5, 8 over 256 (14 MiB) 19.1 / 19.0.
 constexpr int64_t kTogetherBytes = 16 << 20;
+// A row's parts are joined by a block where a wave's lanes would have more than so many each and rows are at most
+// two a CU, us in all by waves / by blocks: one token over 14170 keys, one head of 256 53 / 24, over 4000, 8 heads of 128 21.3 / 16.5,
+// 7 sequences of 2 tokens over 7172 shared keys, float32 (112 rows) 44.5 / 28.9, 8 tokens over 1024 keys (256 rows) 25.2 / 25.3,
+// 640 rows over 288 shared keys 33.0 / 38.4, 2048 over 8192 72 / 93.
+constexpr int kBlockParts = 8;
 
 // The parts of rows, joined: a lane has four columns of a row's every `groups`-th part, `quads` lanes a part
-// (a power of two), four of its parts on their way at once; a wave 64 / (quads groups) rows.
-__global__ void __launch_bounds__(256) paged_join(PagedArgs a, int quads, int groups) {
+// (a power of two), four of its parts on their way at once; a wave 64 / (quads groups) rows.  BLOCK: the
+// waves of a block have every 16th such share of one row's parts, and the first of them joins these.
+template <bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? 1024 : 256) paged_join(PagedArgs a, int quads, int groups) {
+    __shared__ at_f4 wave_o[BLOCK ? 16 : 1][64];
+    __shared__ float2 wave_ml[BLOCK ? 16 : 1][64];
     const int64_t rows = (int64_t)a.batch * a.kv_heads * a.seq_rows;
-    const int lane = (int)threadIdx.x & 63, quad = lane & (quads - 1), group = lane / quads & (groups - 1), per = 64 / (quads * groups);
-    const int64_t first = (blockIdx.x * 4ll + (threadIdx.x >> 6)) * per + lane / (quads * groups), step = gridDim.x * 4ll * per;
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, quad = lane & (quads - 1), per = 64 / (quads * groups);
+    const int group = (lane / quads & (groups - 1)) + (BLOCK ? wave * groups : 0), apart_by = groups * (BLOCK ? 16 : 1);
+    const int64_t first = BLOCK ? (int64_t)blockIdx.x : (blockIdx.x * 4ll + wave) * per + lane / (quads * groups);
+    const int64_t step = BLOCK ? (int64_t)gridDim.x : gridDim.x * 4ll * per;
     for (int64_t at = first; at < rows; at += step) {
         const int64_t head = at / a.seq_rows;
         const int r = (int)(at - head * a.seq_rows), b = (int)(head / a.kv_heads), hk = (int)(head - (int64_t)b * a.kv_heads);
@@ -50,28 +61,36 @@ __global__ void __launch_bounds__(256) paged_join(PagedArgs a, int quads, int gr
             const int2 workers = s.found[(int64_t)hk * s.entries + entry];
             whole = a.stages == 1 && workers.x == workers.y;  // its worker wrote it
             if (whole) break;
-            for (int w0 = workers.x + group; w0 <= workers.y; w0 += 4 * groups) {
+            for (int w0 = workers.x + group; w0 <= workers.y; w0 += 4 * apart_by) {
                 float m[4], l[4];
                 at_f4 x[4];
 #pragma unroll
                 for (int p = 0; p < 4; p++) {
-                    const int w = min(w0 + p * groups, workers.y);
+                    const int w = min(w0 + p * apart_by, workers.y);
                     const int64_t part = ((int64_t)hk * s.slots + slot_of_part(a, s, w, entry, w == workers.x)) * s.tile_rows + one - tile * s.tile_rows;
                     m[p] = s.part_ml[2 * part], l[p] = s.part_ml[2 * part + 1];
                     x[p] = *(const at_f4 *)(s.part_o + part * a.part_width + d);
                 }
 #pragma unroll
                 for (int p = 0; p < 4; p++)
-                    if (w0 + p * groups <= workers.y) add(m[p], l[p], x[p]);
+                    if (w0 + p * apart_by <= workers.y) add(m[p], l[p], x[p]);
             }
         }
-        if (whole) continue;
+        if (whole) continue;  // (the same in a whole block)
         for (int apart = quads; apart < quads * groups; apart *= 2) {
             const float m = __shfl_xor(most, apart), l = __shfl_xor(sum, apart);
             at_f4 x;
 #pragma unroll
             for (int e = 0; e < 4; e++) x[e] = __shfl_xor(o[e], apart);
             add(m, l, x);
+        }
+        if constexpr (BLOCK) {
+            __syncthreads();  // the last row's have been read
+            wave_o[wave][lane] = o, wave_ml[wave][lane] = make_float2(most, sum);
+            __syncthreads();
+            if (wave != 0) continue;
+#pragma unroll 5
+            for (int w = 1; w < 16; w++) add(wave_ml[w][lane].x, wave_ml[w][lane].y, wave_o[w][lane]);
         }
         if (group != 0) continue;
         const int i = (int)a.by_group.divide((uint32_t)r);
@@ -91,21 +110,25 @@ PagedStage plan_stage(const PagedArgs &a, bool together, int from, int to, int c
     s.together = together, s.from = from, s.to = to;
     const int64_t rows = together ? (int64_t)a.batch * a.seq_rows : a.seq_rows;
     const int64_t keys = std::min<int64_t>(to - from, (int64_t)a.window + a.sinks + a.Sq);
-    const bool few = rows <= kFewRows || a.D > kPiecesDim || rows * (together ? 1 : a.batch) * a.kv_heads * keys < kFewPairs;
+    const bool pairs = rows * (together ? 1 : a.batch) * a.kv_heads * keys < kFewPairs, few = rows <= kFewRows || a.D > kPiecesDim || pairs;
     s.tile_rows = few ? kFewTile : rows <= 128 && bf16 ? 128 : 256;
     s.row_tiles = (int32_t)((rows + s.tile_rows - 1) / s.tile_rows);
     s.entries = (int32_t)(together ? s.row_tiles : (int64_t)s.row_tiles * a.batch);
     if (s.tile_rows == kFewTile) {
         // Two waves a SIMD.  Least tiles of a wave 1, 2, 4 and 8, us: 500 keys, 8 heads of 64, bfloat16 13.3, 14.2, 16.6 and 22.2,
-        // 4000, 8 of 128 25.0, 21.3, 21.7 and 27.1, 8 sequences of 1000 21.9, 19.0, 20.4 and 27.4.
+        // 4000, 8 of 128 25.0, 21.3, 21.7 and 27.1, 8 sequences of 1000 21.9, 19.0, 20.4 and 27.4.  Of wide heads one wave a
+        // SIMD is there at a time, and one for each, us with 4 waves a CU / 8: 64 rows over 6240 shared keys, heads of 256,
+        // bfloat16 30.1 / 33.6, 7 x 32 over 1838 33.8 / 41.0; the shares of many rows are evener with two: 2 x 1024 tokens of 4096, 16 heads
+        // of 256 over 4 787 / 739.
         s.least = 2;
-        s.workers = std::max(1, 8 * cu_count / a.kv_heads);
+        s.workers = std::max(1, (a.D > kPiecesDim && pairs ? 4 : 8) * cu_count / a.kv_heads);
     } else {
         s.least = 2;
         s.workers = std::max(1, cu_count * (256 / s.tile_rows) / a.kv_heads);
     }
     s.by_row_tiles = SmallDivisor((uint32_t)s.row_tiles);
     const int64_t most = (to >> (bf16 || s.tile_rows != kFewTile ? 5 : 4)) + 2;  // key tiles of an entry
+    s.most = (int32_t)most;
     if (most * s.entries >> 31) s.workers = 0;
     return s;
 }
@@ -193,9 +216,16 @@ int paged_forward(PagedArgs &a, bool bf16, DeviceState *dev, bool captured) {
         int quads = 1;
         while (quads * 4 < a.part_width) quads *= 2;
         // Waves have parts of few rows each, blocks two or three of many.
-        const int groups = a.stages && few(a.stages - 1) ? 64 / quads : 1;
-        const int64_t lanes = (int64_t)a.batch * a.kv_heads * a.seq_rows * quads * groups;
-        hipLaunchKernelGGL(paged_join, dim3((unsigned)std::min<int64_t>((lanes + 255) / 256, 1 << 22)), dim3(256), 0, dev->stream, a, quads, groups);
+        const int64_t rows = (int64_t)a.batch * a.kv_heads * a.seq_rows;
+        int64_t parts = 0;  // of a row, at most or so
+        for (int i = 0; i < a.stages; i++) parts = std::max<int64_t>(parts, std::min(a.stage[i].workers / a.stage[i].entries, a.stage[i].most / a.stage[i].least));
+        if (rows <= 2 * dev->cu_count && parts > kBlockParts * (64 / quads)) {
+            hipLaunchKernelGGL(paged_join<true>, dim3((unsigned)std::min<int64_t>(rows, 1 << 20)), dim3(1024), 0, dev->stream, a, quads, 64 / quads);
+        } else {
+            const int groups = a.stages && few(a.stages - 1) ? 64 / quads : 1;
+            const int64_t lanes = rows * quads * groups;
+            hipLaunchKernelGGL(paged_join<false>, dim3((unsigned)std::min<int64_t>((lanes + 255) / 256, 1 << 22)), dim3(256), 0, dev->stream, a, quads, groups);
+        }
         TRS_LAUNCH_CHECK("paged attention join launch");
         return TRS_OK;
     };

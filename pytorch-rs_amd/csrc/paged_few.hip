@@ -98,11 +98,18 @@ struct Bf16Pages {
         for (int j = 0; j < KJ; j++) {
             Unit<1> x;
             const int c = 32 * j + 8 * quarter;
+            if constexpr (MODE == 2) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const bool in = MODE == 0 || c + e < D;
-                const float y = row[in ? c + e : 0];
-                x.v[e] = in ? y : 0.f;
+                for (int e = 0; e < 8; e++) {
+                    const bool in = c + e < D;
+                    const float y = row[in ? c + e : 0];
+                    x.v[e] = in ? y : 0.f;
+                }
+            } else {
+                const bool in = MODE == 0 || c < D;
+                const f4u y = *(const f4u *)(row + (in ? c : 0)), z = *(const f4u *)(row + (in ? c + 4 : 0));
+#pragma unroll
+                for (int e = 0; e < 4; e++) x.v[e] = in ? y[e] : 0.f, x.v[4 + e] = in ? z[e] : 0.f;
             }
             const Pieces p = x.split(scale * kUp);
 #pragma unroll

@@ -98,9 +98,21 @@ MANY = [
     (1, 8, 2, 1100, 137, 10, [1200], 500, 0),
 ]
 
+# Few rows over so many keys that a row has tens or hundreds of parts.
+LONG = [
+    (1, 1, 1, 1, 256, 8, [7000], EVERY, 0),
+    (1, 8, 2, 2, 200, 128, [9001], EVERY, 0),
+    (2, 4, 2, 1, 128, 16, [5000, 3], EVERY, 0),
+    (3, 2, 1, 1, 64, 16, [8200, 0, 4100], 3000, 5),
+    (1, 1, 1, 1, 8, 16, [9000], EVERY, 0),
+    (1, 3, 1, 3, 33, 10, [6001], EVERY, 0),
+    (8, 8, 8, 8, 100, 16, [2600 - 300 * i for i in range(8)], EVERY, 0),  # 512 rows
+    (8, 8, 8, 9, 100, 16, [2600 - 300 * i for i in range(8)], EVERY, 0),  # and more
+]
+
 
 @KINDS
-@pytest.mark.parametrize("shape", SHAPES + MANY, ids=str)
+@pytest.mark.parametrize("shape", SHAPES + MANY + LONG, ids=str)
 def test_attention_matches_64_bits(shape, kind):
     B, H, HK, sq, D, page, lengths, window, sinks = shape
     q, k, v = inputs(sq * 7 + D, B, H, HK, sq, max(lengths), D, kind)
@@ -142,6 +154,8 @@ TOGETHER = [
     (12, 16, 2, 24, 256, 16, [2000 - i for i in range(12)], 1900, EVERY, 0),
     (24, 16, 2, 12, 96, 24, [2100] * 24, 2100, EVERY, 0),                                  # nothing of their own
     (34, 8, 2, 8, 20, 16, [4300 - 100 * i for i in range(34)], 4100, 2000, 40),
+    (7, 2, 1, 2, 128, 16, [4700 + 30 * i for i in range(7)], 4600, EVERY, 0),              # a row's parts of both kinds by the tens
+    (3, 1, 1, 1, 256, 16, [9100, 9050, 9040], 9030, EVERY, 0),
 ]
 
 
@@ -343,7 +357,7 @@ def test_without_memory_for_parts(kind):
 
 @KINDS
 def test_the_same_bits_each_time(kind):
-    for B, sq, shared in ((5, 1, 0), (40, 1, 256), (40, 1, 1000), (40, 20, 1000), (2, 150, 0), (2, 800, 0)):
+    for B, sq, shared in ((5, 1, 0), (40, 1, 256), (40, 1, 1000), (40, 20, 1000), (2, 150, 0), (2, 800, 0), (1, 1, 0)):
         q, k, v = inputs(17, B, 8, 2, sq, 1100, 128, kind)
         share(k, v, shared)
         cache = Cache(B, 2, 16, 128, [1100 - 2 * i for i in range(B)], kind, "heads", k, v, shared=shared)
