@@ -23,22 +23,24 @@ constexpr int64_t kFewPairs = 1 << 23;
 // 2 sequences over 1024 keys (4 MiB) 17.2 / 17.9 and 4096 (16 MiB) 25.7 / 22.9, 4 over 1024 (12 MiB) 17.8 / 17.9, 8 over 256 (7 MiB)
 // 16.3 / 17.3 and 1024 (28 MiB) 21.3 / 18.5; float32, 4 over 1024 (24 MiB) 24.0 / 20.5, 8 over 256 (14 MiB) 19.1 / 19.0.
 constexpr int64_t kTogetherBytes = 16 << 20;
-// A row's parts are joined by a block where a wave's lanes would have more than so many each and rows are at most
-// two a CU, us in all by waves / by blocks: one token over 14170 keys, one head of 256 53 / 24, over 4000, 8 heads of 128 21.3 / 16.5,
-// 7 sequences of 2 tokens over 7172 shared keys, float32 (112 rows) 44.5 / 28.9, 8 tokens over 1024 keys (256 rows) 25.2 / 25.3,
-// 640 rows over 288 shared keys 33.0 / 38.4, 2048 over 8192 72 / 93.
-constexpr int kBlockParts = 8;
+// A row's parts are joined by 16 waves of a block where as many have a lane's four each and rows are at most two a CU, by
+// 4 where 2 do and rows are at most four a CU; us in all with 1, 4 and 16: one token over 14170 keys, one head of 256
+// 52.7, 27.4 and 23.9, 2 over 15168, 2 heads of 200, float32 108, 50.5 and 40.4, one over 16384, 8 heads of 128 42.3, 27.2 and 25.3 and over
+// 4000 19.6, 16.0 and 16.6, over 1000, 8 of 64, float32 12.9, 12.6 and 13.3, 8 tokens over 1024 keys (256 rows) 25.3, 24.6 and 25.6,
+// 16 over 1000 (512 rows) 23.2, 23.1 and 26.1; 640 rows over 288 shared keys 32.8, 32.5 and 38.4, 1024 over 2048 35.0, 34.7 and -, 2048 over
+// 8192 71.9, 73.6 and 92.8.
 
 // The parts of rows, joined: a lane has four columns of a row's every `groups`-th part, `quads` lanes a part
-// (a power of two), four of its parts on their way at once; a wave 64 / (quads groups) rows.  BLOCK: the
-// waves of a block have every 16th such share of one row's parts, and the first of them joins these.
-template <bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 1024 : 256) paged_join(PagedArgs a, int quads, int groups) {
-    __shared__ at_f4 wave_o[BLOCK ? 16 : 1][64];
-    __shared__ float2 wave_ml[BLOCK ? 16 : 1][64];
+// (a power of two), four of its parts on their way at once; a wave 64 / (quads groups) rows.  WAVES above 1: so
+// many waves, a block, have every WAVES-th such share of one row's parts, and the first of them joins these.
+template <int WAVES>
+__global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) paged_join(PagedArgs a, int quads, int groups) {
+    constexpr bool BLOCK = WAVES > 1;
+    __shared__ at_f4 wave_o[WAVES][64];
+    __shared__ float2 wave_ml[WAVES][64];
     const int64_t rows = (int64_t)a.batch * a.kv_heads * a.seq_rows;
     const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, quad = lane & (quads - 1), per = 64 / (quads * groups);
-    const int group = (lane / quads & (groups - 1)) + (BLOCK ? wave * groups : 0), apart_by = groups * (BLOCK ? 16 : 1);
+    const int group = (lane / quads & (groups - 1)) + (BLOCK ? wave * groups : 0), apart_by = groups * WAVES;
     const int64_t first = BLOCK ? (int64_t)blockIdx.x : (blockIdx.x * 4ll + wave) * per + lane / (quads * groups);
     const int64_t step = BLOCK ? (int64_t)gridDim.x : gridDim.x * 4ll * per;
     for (int64_t at = first; at < rows; at += step) {
@@ -90,7 +92,7 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) paged_join(PagedArgs a, in
             __syncthreads();
             if (wave != 0) continue;
 #pragma unroll 5
-            for (int w = 1; w < 16; w++) add(wave_ml[w][lane].x, wave_ml[w][lane].y, wave_o[w][lane]);
+            for (int w = 1; w < WAVES; w++) add(wave_ml[w][lane].x, wave_ml[w][lane].y, wave_o[w][lane]);
         }
         if (group != 0) continue;
         const int i = (int)a.by_group.divide((uint32_t)r);
@@ -219,12 +221,15 @@ int paged_forward(PagedArgs &a, bool bf16, DeviceState *dev, bool captured) {
         const int64_t rows = (int64_t)a.batch * a.kv_heads * a.seq_rows;
         int64_t parts = 0;  // of a row, at most or so
         for (int i = 0; i < a.stages; i++) parts = std::max<int64_t>(parts, std::min(a.stage[i].workers / a.stage[i].entries, a.stage[i].most / a.stage[i].least));
-        if (rows <= 2 * dev->cu_count && parts > kBlockParts * (64 / quads)) {
-            hipLaunchKernelGGL(paged_join<true>, dim3((unsigned)std::min<int64_t>(rows, 1 << 20)), dim3(1024), 0, dev->stream, a, quads, 64 / quads);
+        const int64_t waves = parts * quads / (4 * 64);  // of four parts a lane
+        if (rows <= 2 * dev->cu_count && waves >= 16) {
+            hipLaunchKernelGGL(paged_join<16>, dim3((unsigned)rows), dim3(1024), 0, dev->stream, a, quads, 64 / quads);
+        } else if (rows <= 4 * dev->cu_count && waves >= 2) {
+            hipLaunchKernelGGL(paged_join<4>, dim3((unsigned)rows), dim3(256), 0, dev->stream, a, quads, 64 / quads);
         } else {
             const int groups = a.stages && few(a.stages - 1) ? 64 / quads : 1;
             const int64_t lanes = rows * quads * groups;
-            hipLaunchKernelGGL(paged_join<false>, dim3((unsigned)std::min<int64_t>((lanes + 255) / 256, 1 << 22)), dim3(256), 0, dev->stream, a, quads, groups);
+            hipLaunchKernelGGL(paged_join<1>, dim3((unsigned)std::min<int64_t>((lanes + 255) / 256, 1 << 22)), dim3(256), 0, dev->stream, a, quads, groups);
         }
         TRS_LAUNCH_CHECK("paged attention join launch");
         return TRS_OK;
