@@ -116,20 +116,24 @@ PagedStage plan_stage(const PagedArgs &a, bool together, int from, int to, int c
     s.tile_rows = few ? kFewTile : rows <= 128 && bf16 ? 128 : 256;
     s.row_tiles = (int32_t)((rows + s.tile_rows - 1) / s.tile_rows);
     s.entries = (int32_t)(together ? s.row_tiles : (int64_t)s.row_tiles * a.batch);
+    const int shift = bf16 || s.tile_rows != kFewTile ? 5 : 4;
+    s.least = 2;
     if (s.tile_rows == kFewTile) {
-        // Two waves a SIMD.  Least tiles of a wave 1, 2, 4 and 8, us: 500 keys, 8 heads of 64, bfloat16 13.3, 14.2, 16.6 and 22.2,
-        // 4000, 8 of 128 25.0, 21.3, 21.7 and 27.1, 8 sequences of 1000 21.9, 19.0, 20.4 and 27.4.  Of wide heads one wave a
-        // SIMD is there at a time, and one for each, us with 4 waves a CU / 8: 64 rows over 6240 shared keys, heads of 256,
-        // bfloat16 30.1 / 33.6, 7 x 32 over 1838 33.8 / 41.0; the shares of many rows are evener with two: 2 x 1024 tokens of 4096, 16 heads
-        // of 256 over 4 787 / 739.
-        s.least = 2;
+        // Two waves a SIMD, one of wide heads, which fill its registers: 64 rows over 6240 shared keys, heads of 256, bfloat16,
+        // 30.1 us with 4 waves a CU and 33.6 with 8, 7 x 32 over 1838 33.8 and 41.0; the shares of many rows are evener with 8: 2 x 1024
+        // tokens of 4096, 16 heads of 256 over 4 787 and 739.
         s.workers = std::max(1, (a.D > kPiecesDim && pairs ? 4 : 8) * cu_count / a.kv_heads);
+        // A tile a wave where that gives every SIMD one at most and a row not too many parts, else two, us with 1 and 2: 500 keys,
+        // 8 heads of 64, bfloat16 11.6 and 12.8, 1000, float32 11.6 and 12.6, 7 x 4 tokens of 432, 24 heads of 200 over 3 19.8 and 25.1; 3 x 4 of
+        // 3000, 16 heads of 128 over 2 23.3 and 18.6, 14 of 7172 shared ones, 8 heads of 128, float32 33.3 and 28.8, 16384 keys, one head of 128
+        // 19.1 and 17.6.
+        const int64_t seen = (keys >> shift) + 1;
+        if (seen <= 128 && seen * s.entries * a.kv_heads <= 4 * cu_count) s.least = 1;
     } else {
-        s.least = 2;
         s.workers = std::max(1, cu_count * (256 / s.tile_rows) / a.kv_heads);
     }
     s.by_row_tiles = SmallDivisor((uint32_t)s.row_tiles);
-    const int64_t most = (to >> (bf16 || s.tile_rows != kFewTile ? 5 : 4)) + 2;  // key tiles of an entry
+    const int64_t most = ((to - from) >> shift) + 2;  // key tiles of an entry
     s.most = (int32_t)most;
     if (most * s.entries >> 31) s.workers = 0;
     return s;
