@@ -92,7 +92,10 @@ int trs_device_info(char *name, size_t name_len, int *cu_count, int *clock_khz);
  * 2 MiB above) and trs_free returns them to it without synchronising: the
  * release is stream-ordered, so a block must not be used outside this
  * library's stream after it is freed.  Pointers not from trs_alloc are
- * released with a stream sync and hipFree. */
+ * released with a stream sync and hipFree.  While the stream is captured into
+ * a graph, in any mode, an allocation is made at once and is no part of the
+ * graph; one that the device refuses is TRS_E_ALLOCATION_FAILED, the cache keeps
+ * its blocks and the capture goes on. */
 int trs_alloc(size_t bytes, void **ptr);
 /* Test hook (no counterpart in the reference; for the tests of this
  * library's fallbacks, which nothing else can reach): after `n` more

@@ -139,14 +139,6 @@ PagedStage plan_stage(const PagedArgs &a, bool together, int from, int to, int c
     return s;
 }
 
-// Whether the stream's work is being captured into a graph.
-int is_captured(DeviceState *dev, bool *captured) {
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    TRS_HIP_CHECK(hipStreamIsCapturing(dev->stream, &status), "hipStreamIsCapturing");
-    *captured = status != hipStreamCaptureStatusNone;
-    return TRS_OK;
-}
-
 // A workspace that captured calls share: their replays follow one another on the library's stream.  A
 // larger one leaves the smaller to the graphs that have it.
 int graph_workspace(DeviceState *dev, size_t bytes, void **ws) {

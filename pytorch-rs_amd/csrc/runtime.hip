@@ -57,6 +57,17 @@ size_t round_block(size_t bytes) {
     return (bytes + g - 1) / g * g;
 }
 
+// hipMalloc, whatever is being captured: memory is no part of a graph, and in a capture that is not relaxed the
+// plain call is an error that ends the capture.
+hipError_t allocate(void **ptr, size_t bytes) {
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    const hipError_t e = hipThreadExchangeStreamCaptureMode(&mode);
+    if (e != hipSuccess) return e;
+    const hipError_t got = hipMalloc(ptr, bytes);
+    (void)hipThreadExchangeStreamCaptureMode(&mode);
+    return got;
+}
+
 // Returns every cached block to HIP after the device stream has drained.
 int release_cache(DeviceState *dev) {
     std::multimap<size_t, void *> blocks;
@@ -151,6 +162,13 @@ void merge_layout_dims(const trs_layout *in, trs_layout *out) {
     }
     m.rank = r;
     *out = m;
+}
+
+int is_captured(DeviceState *dev, bool *captured) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    TRS_HIP_CHECK(hipStreamIsCapturing(dev->stream, &status), "hipStreamIsCapturing");
+    *captured = status != hipStreamCaptureStatusNone;
+    return TRS_OK;
 }
 
 DeviceState *device_state() {
@@ -303,13 +321,16 @@ int trs_alloc(size_t bytes, void **ptr) {
                 return TRS_OK;
             }
         }
-        hipError_t e = hipMalloc(ptr, rounded);
+        hipError_t e = allocate(ptr, rounded);
         if (e != hipSuccess) {
-            // Out of memory with blocks parked in the cache: release them and retry once.
+            // Out of memory with blocks parked in the cache: release them and retry once.  (Not where the stream is
+            // captured: it cannot be waited for, and trying to would end the capture.)
             (void)hipGetLastError();
-            int rc = release_cache(dev);
+            bool captured = false;
+            int rc = is_captured(dev, &captured);
+            if (!rc && !captured) rc = release_cache(dev);
             if (rc) return rc;
-            e = hipMalloc(ptr, rounded);
+            if (!captured) e = allocate(ptr, rounded);
         }
         if (e != hipSuccess) {
             *ptr = nullptr;

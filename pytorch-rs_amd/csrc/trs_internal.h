@@ -70,6 +70,9 @@ void setup_sum_scratch(DeviceState *dev);
 // On failure returns nullptr with the error recorded.
 DeviceState *device_state();
 
+// Whether the device stream's work is being captured into a graph.
+int is_captured(DeviceState *dev, bool *captured);
+
 
 // Records a thread-local error message and returns `code`.
 int set_error(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
