@@ -117,7 +117,9 @@ int trs_debug_fail_allocs_above(size_t bytes);
  * TRS_E_INVALID_ARGUMENT. */
 int trs_debug_pointwise_grid_cap(int64_t blocks);
 int trs_free(void *ptr);
-/* Return every cached block to HIP (after draining the device stream). */
+/* Return every cached block to HIP (after draining the device stream;
+ * TRS_E_INVALID_ARGUMENT while that is captured into a graph).  Blocks that HIP
+ * does not take stay cached. */
 int trs_empty_cache(void);
 /* Bytes in live (allocated) and cached (freed, kept) blocks on the device. */
 int trs_memory_stats(size_t *live_bytes, size_t *cached_bytes);

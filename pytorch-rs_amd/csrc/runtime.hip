@@ -68,8 +68,12 @@ hipError_t allocate(void **ptr, size_t bytes) {
     return got;
 }
 
-// Returns every cached block to HIP after the device stream has drained.
+// Returns every cached block to HIP after the device stream has drained; blocks that HIP has not taken stay in the
+// cache.  Not while the stream is captured: it cannot be waited for, and trying to would end the capture.
 int release_cache(DeviceState *dev) {
+    bool captured = false;
+    TRS_CHECK(is_captured(dev, &captured));
+    if (captured) return set_error(TRS_E_INVALID_ARGUMENT, "the block cache cannot be emptied while the stream is captured");
     std::multimap<size_t, void *> blocks;
     {
         std::lock_guard<std::mutex> lock(dev->cache_mu);
@@ -77,9 +81,18 @@ int release_cache(DeviceState *dev) {
         dev->cached_bytes = 0;
     }
     if (blocks.empty()) return TRS_OK;
-    TRS_HIP_CHECK(hipStreamSynchronize(dev->stream), "cache release sync");
-    for (auto &kv : blocks) TRS_HIP_CHECK(hipFree(kv.second), "hipFree");
-    return TRS_OK;
+    int rc = TRS_OK;
+    const hipError_t e = hipStreamSynchronize(dev->stream);
+    if (e != hipSuccess) rc = hip_fail(e, "cache release sync");
+    while (!rc && !blocks.empty()) {
+        const hipError_t freed = hipFree(blocks.begin()->second);
+        if (freed != hipSuccess) rc = hip_fail(freed, "hipFree");
+        else blocks.erase(blocks.begin());
+    }
+    std::lock_guard<std::mutex> lock(dev->cache_mu);
+    for (auto &kv : blocks) dev->cached_bytes += kv.first;
+    dev->free_blocks.merge(blocks);
+    return rc;
 }
 
 }  // namespace

@@ -107,6 +107,27 @@ def test_an_allocation_that_the_device_refuses_ends_no_capture_and_drops_no_bloc
     graph.close()
 
 
+def test_the_cache_is_not_emptied_in_a_capture():
+    """Its blocks wait for the stream, which cannot be waited for: the call is refused, and the capture goes on."""
+    case = Case(4, 2, 8, 2, 1, 64, 900, F32)
+    check(case.call())
+    check(abi.lib.trs_synchronize())
+    before, got = stats(), []
+    assert before[1] > 0
+
+    def calls():
+        got.append(abi.lib.trs_empty_cache())
+        got.append(stats())
+        check(case.call())
+
+    graph = Captured(calls)
+    assert got == [abi.TRS_E_INVALID_ARGUMENT, before]
+    case.replays_right(graph)
+    graph.close()
+    check(abi.lib.trs_empty_cache())
+    assert stats()[1] == 0
+
+
 @pytest.mark.parametrize("mode", [GLOBAL, THREAD_LOCAL, RELAXED])
 @KINDS
 @SIZES
