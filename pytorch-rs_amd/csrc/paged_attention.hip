@@ -21,7 +21,10 @@ constexpr int kFewRows = 64;
 constexpr int64_t kFewPairs = 1 << 23;
 // Shared keys are worked on together where that saves so much reading, us apart / together, 8 key heads of 128: bfloat16,
 // 2 sequences over 1024 keys (4 MiB) 17.2 / 17.9 and 4096 (16 MiB) 25.7 / 22.9, 4 over 1024 (12 MiB) 17.8 / 17.9, 8 over 256 (7 MiB)
-// 16.3 / 17.3 and 1024 (28 MiB) 21.3 / 18.5; float32, 4 over 1024 (24 MiB) 24.0 / 20.5, 8 over 256 (14 MiB) 19.1 / 19.0.
+// 16.3 / 17.3 and 1024 (28 MiB) 21.3 / 18.5; float32, 4 over 1024 (24 MiB) 24.0 / 20.5, 8 over 256 (14 MiB) 19.1 / 19.0.  Of shared keys
+// a sequence reads at most what window, first tokens and new tokens leave: 64 tokens behind 8192 and 200 of their own, 32 heads,
+// bfloat16, window 16 (4 MiB) 14.4 / 18.4, 512 (126 MiB) 28.2 / 32.6, 2048 (500 MiB) 63.0 / 48.0, float32, window 64 (31 MiB)
+// 21.9 / 24.5: how many own keys a window has first stands on the device, and 512 and 64 count as more than they are.
 constexpr int64_t kTogetherBytes = 16 << 20;
 // A row's parts are joined by 16 waves of a block where as many have a lane's four each and rows are at most two a CU, by
 // 4 where 2 do and rows are at most four a CU; us in all with 1, 4 and 16: one token over 14170 keys, one head of 256
@@ -181,7 +184,8 @@ int take_parts(PagedArgs &a, DeviceState *dev, bool captured, void **ws) {
 int paged_forward(PagedArgs &a, bool bf16, DeviceState *dev, bool captured) {
     a.part_width = (a.D + 3) / 4 * 4;
     a.stages = 0;
-    const int64_t saved = (int64_t)(a.batch - 1) * a.shared * a.kv_heads * a.D * (bf16 ? 4 : 8);
+    const int64_t seen = std::min<int64_t>(a.shared, (int64_t)a.window + a.sinks + a.Sq);  // of the shared keys, by a sequence, at most
+    const int64_t saved = (int64_t)(a.batch - 1) * seen * a.kv_heads * a.D * (bf16 ? 4 : 8);
     if (saved >= kTogetherBytes && (int64_t)a.batch * a.seq_rows < (int64_t)1 << 31) {
         a.all_rows = a.batch * a.seq_rows, a.by_seq_rows = SmallDivisor((uint32_t)a.seq_rows);
         a.stage[a.stages++] = plan_stage(a, true, 0, a.shared, dev->cu_count, bf16);
