@@ -490,7 +490,8 @@ typedef struct trs_paged_cache {
  * Token t of sequence b stands at place lengths[b] - T + t; one before place 0 is
  * padding, and neither it nor one behind the last place of the table's row is written.  positions as above, or null for the place
  * itself on every axis (a padding query turns as at place 0); a pair whose position the
- * tables do not hold is NaN.  cos, sin and ltab null: nothing is turned.  Values go to
+ * tables do not hold is NaN.  cos, sin and ltab null: nothing is turned, and interleaved,
+ * axes, pair_axis and positions are not looked at.  Values go to
  * bfloat16 pages rounded to the nearest, ties to even.  A token whose entry of the table
  * is no page of the pool is not written.  Where two tokens of a call have the same place
  * in the pool, it holds entries of either.  Everything else in the pools stays as it is.

@@ -23,7 +23,7 @@ constexpr int64_t kFewPairs = 1 << 23;
 // 2 sequences over 1024 keys (4 MiB) 17.2 / 17.9 and 4096 (16 MiB) 25.7 / 22.9, 4 over 1024 (12 MiB) 17.8 / 17.9, 8 over 256 (7 MiB)
 // 16.3 / 17.3 and 1024 (28 MiB) 21.3 / 18.5; float32, 4 over 1024 (24 MiB) 24.0 / 20.5, 8 over 256 (14 MiB) 19.1 / 19.0.  Of shared keys
 // a sequence reads at most what window, first tokens and new tokens leave: 64 tokens behind 8192 and 200 of their own, 32 heads,
-// bfloat16, window 16 (4 MiB) 14.4 / 18.4, 512 (126 MiB) 28.2 / 32.6, 2048 (500 MiB) 63.0 / 48.0, float32, window 64 (31 MiB)
+// bfloat16, window 16 (4 MiB) 14.4 / 18.4, 512 (126 MiB) 28.2 / 32.6, 2048 (505 MiB) 63.0 / 48.0, float32, window 64 (32 MiB)
 // 21.9 / 24.5: how many own keys a window has first stands on the device, and 512 and 64 count as more than they are.
 constexpr int64_t kTogetherBytes = 16 << 20;
 // A row's parts are joined by 16 waves of a block where as many have a lane's four each and rows are at most two a CU, by

@@ -369,8 +369,8 @@ def _cache_arguments(op, cache, table, lengths, like):
 def paged_append(cache, table, lengths, key, value, cos=None, sin=None, *, query=None, positions=None, pair_axes=None, interleaved: bool = False):
     """Writes new tokens' keys and values [batch, key head, token, dim] to the pages that
     ``table`` ([batch, pages] integers, or an ``index_buffer``) gives, the keys turned on the
-    way as ``rope_axes`` turns them (``cos`` None: as they are); returns the turned
-    ``query`` [batch, head, token, dim], if there is one.
+    way as ``rope_axes`` turns them (``cos`` and ``sin`` None: as they are, and no argument of
+    a rotation is taken); returns the turned ``query`` [batch, head, token, dim], if there is one.
 
     ``lengths`` ([batch]) are the tokens that each sequence has with the new ones: token t
     stands at place ``lengths - tokens + t``, which is also its position on every axis
@@ -383,6 +383,10 @@ def paged_append(cache, table, lengths, key, value, cos=None, sin=None, *, query
     for name, t in (("cos", cos), ("sin", sin), ("query", query)):
         if t is not None:
             _tensor_arguments("paged_append", **{name: t})
+    if cos is None:
+        for name, given in (("positions", positions is not None), ("pair_axes", pair_axes is not None), ("interleaved", interleaved)):
+            if given:
+                raise ValueError(f"paged_append takes no {name} without tables: nothing is turned")
     table, lengths = _cache_arguments("paged_append", cache, table, lengths, key)
     positions = _indices(positions, key)
     axes, pair_axes = _pair_axes("paged_append", positions, pair_axes)
