@@ -312,13 +312,16 @@ def window_attention(query, key, value, *, window=None, sinks: int = 0, scale=No
                                float(scale), _indices(key_lengths, query))
 
 
-def _pair_axes(op, positions, pair_axes, axes=None):
+def _pair_axes(op, positions, pair_axes, tables):
     """The number of axes, and the axis of every pair as bytes (none: axis 0)."""
+    axes = None
     if positions is not None:
         axes = positions.shape[0] if len(positions.shape) == 3 else 1
     if pair_axes is None:
         return axes or 1, []
     pair_axes = [_integer(op, "pair_axes", a) for a in pair_axes]
+    if not pair_axes and len(tables.shape) == 2 and tables.shape[1]:  # (other numbers are the engine's to compare)
+        raise RuntimeError(f"{op} has axes for 0 pairs, and tables of {tables.shape[1]}")
     axes = axes or max(pair_axes, default=0) + 1
     if not 1 <= axes <= 4:
         raise ValueError(f"{op} positions have 1 to 4 axes, but got {axes}")
@@ -336,7 +339,7 @@ def rope_axes(query, key, cos, sin, *, positions=None, pair_axes=None, start: in
     ``interleaved``, (2j, 2j + 1) of the first 2 * pairs entries turn by entry j of row
     ``positions[pair_axes[j]][batch][token]``.  ``positions`` are [axes, batch, token]
     integers, or an ``index_buffer`` of that shape ([batch, token] for one axis), or None
-    for ``start + token`` on every axis; ``pair_axes`` gives each pair's axis (None: 0).
+    for ``start + token`` on every axis; ``pair_axes`` gives each pair's axis (None: 0 for all).
     ``key`` may be None, and the query alone is returned then.  Gradients reach queries and
     keys."""
     _tensor_arguments("rope_axes", query=query, cos=cos, sin=sin)
@@ -346,7 +349,7 @@ def rope_axes(query, key, cos, sin, *, positions=None, pair_axes=None, start: in
         xs.append(key)
     start = _integer("rope_axes", "start", start)
     positions = _indices(positions, query)
-    axes, pair_axes = _pair_axes("rope_axes", positions, pair_axes)
+    axes, pair_axes = _pair_axes("rope_axes", positions, pair_axes, cos)
     out = _C.rope_axes(xs, cos, sin, bool(interleaved), axes, pair_axes, start, positions)
     return out[0] if key is None else tuple(out)
 
@@ -389,7 +392,7 @@ def paged_append(cache, table, lengths, key, value, cos=None, sin=None, *, query
                 raise ValueError(f"paged_append takes no {name} without tables: nothing is turned")
     table, lengths = _cache_arguments("paged_append", cache, table, lengths, key)
     positions = _indices(positions, key)
-    axes, pair_axes = _pair_axes("paged_append", positions, pair_axes)
+    axes, pair_axes = _pair_axes("paged_append", positions, pair_axes, cos)
     return _C.paged_append(cache, table, lengths, key, value, query, cos, sin, bool(interleaved), axes, pair_axes, positions)
 
 

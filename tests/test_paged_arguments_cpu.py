@@ -17,3 +17,13 @@ def test_appending_without_tables_takes_nothing_of_a_rotation(name, value):
         F.paged_append(None, [[0]], [2], x, x, **{name: value})
     with pytest.raises(ValueError, match=f"{name} without tables"):
         F.paged_append(None, [[0]], [2], x, x, None, None, query=x, **{name: value})
+
+
+def test_no_axes_for_pairs_that_there_are():
+    """An empty list is no axes for 0 pairs, not the default for all of them."""
+    x, tables = zeros(1, 1, 2, 4), zeros(3, 2)
+    with pytest.raises(RuntimeError, match="device"):  # host tensors, and nothing before that
+        F.rope_axes(x, None, zeros(3, 0), zeros(3, 0), pair_axes=[])
+    for axes in ([], ()):
+        with pytest.raises(RuntimeError, match="rope_axes has axes for 0 pairs, and tables of 2"):
+            F.rope_axes(x, None, tables, tables, pair_axes=axes)
