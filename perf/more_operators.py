@@ -12,6 +12,12 @@
 Every case calls the C ABI of include/trs_hip.h (own) or computes the same in
 elementary torch operations (the plain form).  Queries, keys, values and outputs
 are float32, the framework's tensor type; pages hold float32 or bfloat16.
+
+The library's stream is not ordered with torch's: whoever calls run() with `own`
+waits for the device between making or changing a state with torch and the call,
+and between the call and reading its outputs or letting go of them with torch.
+Passes one behind another need no waiting between them, as long as what a pass
+takes from torch's allocator is not written by torch's own work meanwhile.
 """
 import ctypes
 import functools
@@ -242,15 +248,17 @@ def _like(t):
 
 
 def _cache(st):
-    """The cache's description, which a program keeps beside its pages."""
+    """The cache's description, which a program keeps beside its pages, table and lengths for as long as these stay where they are."""
     abi = _backend()
-    if "cache" in st:
-        return st["cache"]
     k, v = st["pages"]
-    st["cache"] = abi.PagedCache(k=k.data_ptr(), v=v.data_ptr(), lk=_layout(k.shape, k.stride()), lv=_layout(v.shape, v.stride()),
-                          type=abi.PAGES_BF16 if k.dtype == torch.bfloat16 else abi.PAGES_F32, table=st["table"].data_ptr(),
-                          table_width=st["table"].shape[1], lengths=st["lengths"].data_ptr())
-    return st["cache"]
+    table, lengths = st["table"], st["lengths"]
+    of = (k.data_ptr(), v.data_ptr(), table.data_ptr(), lengths.data_ptr(), table.shape[1], k.dtype, k.shape, k.stride(), v.stride())
+    kept = st.get("cache")
+    if kept is None or kept[0] != of:
+        kept = st["cache"] = of, abi.PagedCache(k=of[0], v=of[1], lk=_layout(k.shape, k.stride()), lv=_layout(v.shape, v.stride()),
+                                                type=abi.PAGES_BF16 if k.dtype == torch.bfloat16 else abi.PAGES_F32, table=of[2], table_width=of[4],
+                                                lengths=of[3])
+    return kept[1]
 
 
 def _rotation(st):
