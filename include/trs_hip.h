@@ -471,8 +471,9 @@ int trs_rope_axes_f32(int n, const float *const *x, const trs_layout *lx, const 
  * on the device, contiguous: token t of sequence b stands in page
  * table[b][t / tokens a page] at t % tokens a page, and lengths[b] is the number of
  * tokens that the sequence has, the ones that a call brings among them; one below 0
- * counts as 0.  Entries of the table for tokens that a call neither writes nor sees are
- * not looked at.  A row of the table holds at most 2^29 tokens, and strides from page to page
+ * counts as 0.  Entries of the table for tokens that a call neither writes nor sees may
+ * hold anything: they are read, and pages of the pool that they name too, but reach no
+ * result.  A row of the table holds at most 2^29 tokens, and strides from page to page
  * and from token to token are below 2^31 entries (TRS_E_INDEX_OVERFLOW). */
 typedef struct trs_paged_cache {
     void *k, *v;
@@ -508,20 +509,22 @@ int trs_paged_append_f32(const trs_paged_cache *cache, const float *k, const trs
  * and sees key j where
  *     j <= p  and  (p - j < window  or  j < sinks).
  * A query that sees nothing (p < 0) gives 0 whatever it holds.  Keys j < shared of every
- * sequence are read through the table's first row, and their products are taken for
- * the rows of all sequences together: the prefix that a batch has in common is read
- * once and not once a sequence (shared = 0: none; one above the table's tokens counts as
- * all of them).  A query that sees a key whose entry of the table is no page of the pool
+ * sequence are read through the table's first row (shared = 0: none; one above the table's
+ * tokens counts as all of them).  Where that saves 16 MiB of reading and there is memory
+ * for the parts, their products are taken for the rows of all sequences together: the
+ * prefix that a batch has in common is read once and not once a sequence.  A query that sees a key whose entry of the table is no page of the pool
  * gives NaN.  What stands in keys that a query does not see, NaN included, does not reach
  * it.  window >= 1 (INT64_MAX: no window); sinks >= 0.  lse (or null) receives
  * log(sum(exp(scale q k))) as [batch, heads, Sq], -inf where nothing is seen.  Sums are
  * fp32 and their order is fixed; products as in trs_window_attention_f32, with a
- * bfloat16 key or value as it stands.  Parts of long sequences go through a workspace
+ * bfloat16 key or value as it stands, and values summed ahead of the division as there.  Parts of long sequences go through a workspace
  * from the block cache, of at most 2 parts a wave that the device holds of 16 rows, or a
  * block of 256, and one more for every tile of rows where keys are shared; where it has
  * none nothing is split.  Calls that are captured into graphs on the library's stream
  * share a workspace that is kept for them (replay them on that stream, one after another;
- * lengths, table and tensors are read at each replay).  q may have any strides (one with no unit
+ * lengths, table and tensors are read at each replay).  One that needs more than the calls
+ * before it takes a larger one beside theirs; since graphs that use them may live, none is
+ * given back before the process ends, by trs_empty_cache neither.  q may have any strides (one with no unit
  * stride along dim is copied first, into the block cache; not in a captured call); out needs a unit stride along dim and
  * shares no memory with anything else.  There is no gradient: trs_window_attention_f32
  * has one. */

@@ -1,8 +1,8 @@
 // paged_few.hip -- attention over a cache in pages for few rows: single tokens of a batch.
 //
 // Bound by reading the keys and values once: 32 sequences of 1640 to 8192 tokens, 8 key heads of 128,
-// bfloat16 (645 MB) 120-125 us, of which the tiles' loop reads at 6.7 TB/s and 4 us are the way to the first
-// load; 7 to 9 us for one sequence of 1000 tokens, 8 heads of 64, float32.  A wave takes 16 rows and streams its
+// bfloat16 (645 MB) 120-125 us; of calls over 4096, 8192 and 16384 keys each (104, 187 and 358 us) the keys added are
+// read at 6.3-6.4 TB/s, and 17 to 20 us are the way in and out, joining's 5 among them; 7 to 9 us for one sequence of 1000 tokens, 8 heads of 64, float32.  A wave takes 16 rows and streams its
 // share of the keys straight from the pages into the registers that the matrix instructions take
 // them from: no LDS, no barrier, nothing that waits for another wave.  (Blocks of four waves that join
 // in LDS, two blocks a CU: a batch of 64 with 60 to 512 tokens of its own 38 us, 24 so.)  What several

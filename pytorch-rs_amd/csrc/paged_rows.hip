@@ -8,7 +8,7 @@
 // O^T += V^T P^T as it stands.
 //
 // Bound by the card's power and by issue: 1024 tokens of two prompts over 4096, 32 heads of 128 over 8,
-// bfloat16, 305-317 us by card, 1.14-1.19 PFLOP/s of bf16 products (a library product of 8192^3 reaches 1.25 on
+// bfloat16, 313-327 us back to back, 1.10-1.16 PFLOP/s of bf16 products (a library product of 8192^3 reaches 1.31 on
 // the same card): the matrix cores are busy for half the cycles at a clock of 2.0 GHz of 2.4, and 5.5 other vector
 // instructions a matrix instruction take 35%.  Fragments read one step ahead of their products gave 376 -> 355.
 // Waves of a SIMD held in opposite phases, one multiplying while the other works out weights, took 373, blocks

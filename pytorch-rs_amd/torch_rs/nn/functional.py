@@ -400,9 +400,9 @@ def paged_attention(query, cache, table, lengths, *, window=None, sinks: int = 0
     """``window_attention`` of ``query`` [batch, heads, tokens, dim] over a paged cache.
 
     The last query of a sequence stands at its last token, ``lengths`` of ``table``'s
-    (see ``paged_append``).  The first ``shared`` tokens of every sequence are read
-    through the table's first row, once for the whole batch: a prefix that all have in
-    common.  Records no gradient."""
+    (see ``paged_append``).  The first ``shared`` tokens of every sequence, a prefix that
+    all have in common, are read through the table's first row: once for the whole batch
+    where that saves enough reading.  Records no gradient."""
     _tensor_arguments("paged_attention", query=query)
     table, lengths = _cache_arguments("paged_attention", cache, table, lengths, query)
     window = None if window is None else _integer("paged_attention", "window", window)
